@@ -168,9 +168,14 @@ def run(s):
     return {"out": out, "k_codes": s.k_codes, "k_pairs": s.k_pairs, "v_codes": s.v_codes, "v_pairs": s.v_pairs}
 
 
+def _over(x, n):
+    """x / n, rounded once (by a number of the host, torch multiplies by its reciprocal)."""
+    return x / x.new_full((), n)
+
+
 def _plain_product(s):
     x = s.x.float()
-    scale = x.abs().amax(1, keepdim=True) / 127
+    scale = _over(x.abs().amax(1, keepdim=True), 127)
     codes = torch.where(scale > 0, (x / scale).round(), 0)
     y = (codes @ s.codes.float().t()) * (scale * s.scales)
     if s.bias is not None:
@@ -187,7 +192,7 @@ def _word_shifts(device):
 def _plain_write(x, codes, pairs, view):
     x = x.float()
     zero = x.amin(-1, keepdim=True).to(torch.bfloat16).float()
-    scale = ((x.amax(-1, keepdim=True) - zero) / 15).to(torch.bfloat16).float()
+    scale = _over(x.amax(-1, keepdim=True) - zero, 15).to(torch.bfloat16).float()
     c = torch.where(scale > 0, ((x - zero) / scale).round().clamp(0, 15), 0).int()
     words = (c.unflatten(-1, (-1, 8)) << _word_shifts(x.device)).sum(-1).int()          # (the terms share no bit)
     page, slot = (view.slot_mapping // view.page_size).long(), (view.slot_mapping % view.page_size).long()
@@ -251,7 +256,7 @@ def exact(case, seed):
         # the codes are defined by 32-bit operations; everything after them is exact
         x = s.x.to(torch.float32)
         top = torch.maximum(x.amax(1), -x.amin(1))
-        step = torch.div(top, torch.tensor(127.0, device=x.device))
+        step = torch.div(top, torch.full_like(top, 127.0))
         codes = torch.nan_to_num(torch.div(x, step[:, None])).round().double()
         y = torch.einsum("mk,nk->mn", codes, s.codes.double()) * step.double()[:, None] * s.scales.double()
         return y if s.bias is None else y + s.bias.double()
@@ -259,7 +264,8 @@ def exact(case, seed):
     tensors = {}
     for name, x in (("k", s.k.float()), ("v", s.v.float())):
         low = x.min(-1).values.bfloat16()
-        step = ((x.max(-1).values - low.float()) / 15).bfloat16()
+        span = x.max(-1).values - low.float()
+        step = torch.div(span, torch.full_like(span, 15.0)).bfloat16()
         c = torch.div(x - low.float()[..., None], step.float()[..., None]).nan_to_num().round().clamp(0, 15).to(torch.uint8)
         c = c.unflatten(-1, (-1, 8))[..., order].flatten(-2)
         codes, pairs = getattr(s, name + "_codes").clone(), getattr(s, name + "_pairs").clone()
