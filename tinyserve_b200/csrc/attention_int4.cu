@@ -1,0 +1,395 @@
+// A paged cache held in 4 bits: the write of a step's keys and values, and attention over it.
+//
+// A key or value head of a token is D codes of 4 bits and a pair (scale, zero) of bfloat16: with everything in 32 bits,
+//   zero = bfloat16(min x), scale = bfloat16((max x - zero) / 15), code = round((x - zero) / scale), halves to even, within 0 .. 15;
+// a code stands for zero + code * scale.  The codes are taken against the rounded pair, so that the pair's own rounding costs
+// at most a clamped end of the range.  A row that holds an infinity or a NaN, or whose range passes the largest
+// 32-bit number, gets a pair of NaN: whoever attends to it gets NaN, as from a cache of whole numbers.
+//
+// Eight codes fill a 32-bit word: even columns in its lower half, odd ones in its upper half, the first in the lowest bits.
+// One shift and one AND-OR then make a pair of neighbouring columns as two bfloat16 (see `codes2` in the kernels below).
+// Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
+// a token for heads of 128 where bfloat16 takes 256.
+#include "common.cuh"
+
+#ifndef TS_HEAD_DIM
+#error "compile with -DTS_HEAD_DIM=<head size, a multiple of 16 up to 512>"
+#endif
+
+TS_DEFINE_LAST_ERROR()
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr int D = TS_HEAD_DIM;
+static_assert(D % 16 == 0 && D >= 16 && D <= 512, "head sizes are multiples of 16 up to 512");
+constexpr int W = D / 8;                     // words of a row
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float pair_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float pair_zero(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+// where column i of a word's eight stands
+__host__ __device__ constexpr int shift_of(int i) { return (i >> 1) * 4 + (i & 1) * 16; }
+
+// ------------------------------------------------------------------------------------------ write
+struct WriteParams {
+  const void *k, *v;                         // [T, Hkv, D], columns contiguous
+  long long k_row, k_head, v_row, v_head;    // strides in elements
+  uint32_t *kc, *vc;                         // codes, W words a row
+  uint32_t *kp, *vp;                         // pairs
+  const int* slot_mapping;                   // [T]: page * page_size + slot, < 0: not written
+  int T, Hkv, page_shift;
+  long long slots;                           // of the pool
+};
+constexpr int LANES = W >= 32 ? 32 : (W > 16 ? 32 : (W > 8 ? 16 : (W > 4 ? 8 : (W > 2 ? 4 : 2))));    // a row's lanes: a power of two
+constexpr int WORDS = (W + LANES - 1) / LANES;                                                        // words of a lane
+constexpr int WRITE_THREADS = 128;
+
+template <typename T>
+__device__ __forceinline__ void load8_any(const T* p, float (&x)[8], bool vec) {
+  if (vec) {
+    load8<T>(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+  }
+}
+
+// LANES lanes bring one row (token, key or value, head) to its slot
+template <typename T>
+__global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams p, bool vec) {
+  pdl_trigger();
+  pdl_wait();
+  const long long row = (long long)blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES;
+  const bool live = row < 2LL * p.T * p.Hkv;
+  const int head = (int)(row % p.Hkv), which = (int)(row / p.Hkv & 1), t = live ? (int)(row / p.Hkv >> 1) : 0;
+  const T* src = which ? static_cast<const T*>(p.v) + t * p.v_row + head * p.v_head : static_cast<const T*>(p.k) + t * p.k_row + head * p.k_head;
+  float x[WORDS][8];
+  float lo = INFINITY, hi = -INFINITY;
+  int bad = 0;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int word = lane + w * LANES;
+    if (live && word < W) {
+      load8_any<T>(src + word * 8, x[w], vec);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        lo = fminf(lo, x[w][i]);
+        hi = fmaxf(hi, x[w][i]);
+        bad |= !(fabsf(x[w][i]) <= 3.402823466e38f);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+  }
+  if (!live) return;
+  const int slot = p.slot_mapping[t];
+  if (slot < 0) return;
+  if (slot >= p.slots) {
+    if (lane == 0) ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_CACHE_SLOT);
+    return;
+  }
+  const bf16 zero16 = __float2bfloat16_rn(lo);
+  const float zero = __bfloat162float(zero16);
+  const bf16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, zero), 15.f));
+  const float scale = __bfloat162float(scale16);
+  bad |= !(fabsf(scale) <= 3.402823466e38f) || !(fabsf(zero) <= 3.402823466e38f);
+  const size_t at = (((size_t)(slot >> p.page_shift) * p.Hkv + head) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int word = lane + w * LANES;
+    if (word >= W) continue;
+    uint32_t bits = 0;
+    if (!bad && scale > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[w][i], zero), scale)), 0.f), 15.f);
+        bits |= (uint32_t)c << shift_of(i);
+      }
+    }
+    (which ? p.vc : p.kc)[at * W + word] = bits;
+  }
+  if (lane == 0) {
+    const uint32_t s = bad ? 0x7fc0u : (scale > 0.f ? __bfloat16_as_ushort(scale16) : 0u), z = bad ? 0x7fc0u : __bfloat16_as_ushort(zero16);
+    (which ? p.vp : p.kp)[at] = s | z << 16;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ attention
+struct Int4Params {
+  const void* q;                             // [T, H, D], columns contiguous
+  long long q_row, q_head;                   // strides in elements
+  void* out;                                 // [T, H, D]
+  const uint32_t *kc, *vc;                   // codes
+  const uint32_t *kp, *vp;                   // pairs
+  const int* block_table;                    // [B, table_stride], max_blocks used
+  const int* cu_q;                           // [B + 1]
+  const int* kv_lens;                        // [B]
+  int T, B, H, Hkv, page_shift, max_blocks, table_stride, num_pages;
+  float scale;
+  int window;
+  float softcap;
+  const float* sinks;                        // [H] or null: one more term exp(sinks[h]) in head h's sum
+  int splits;                                // key ranges; > 1: partial results for the combine kernel
+  float *part_o, *part_ml;                   // [T * H][splits][D], [T * H][splits][2] (maximum in the log2 domain, sum)
+};
+
+// the request that row t belongs to: the first b with cu_q[b + 1] > t (requests may be empty), -1 behind the last
+__device__ __forceinline__ int request_of(const int* cu_q, int B, int t) {
+  if (t >= cu_q[B]) return -1;
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu_q[mid + 1] > t) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+// row of key j of a request in the cache; a page number outside the pool is reported and read as page 0
+__device__ __forceinline__ size_t cache_row(const Int4Params& p, const int* bt, int kvh, int j) {
+  int page = bt[j >> p.page_shift];
+  if ((unsigned)page >= (unsigned)p.num_pages) {
+    ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_PAGE);
+    page = 0;
+  }
+  return (((size_t)page * p.Hkv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1));
+}
+__device__ __forceinline__ float capped(const Int4Params& p, float s) { return p.softcap > 0.f ? p.softcap * tanhf(s / p.softcap) : s; }
+
+// The 32-bit form (and head sizes that the tensor-core kernel does not take): a block is one token's heads of one key head, up to eight
+// at a time, and a range of its keys.  A thread makes the scores of one key of a tile of 128 for all its heads, so that a
+// row of codes is read once; for P V a thread holds eight columns of all heads and walks every KG-th key.
+constexpr int SIMT_THREADS = 128, SIMT_KEYS = 128, SIMT_HEADS = 8, KG = SIMT_THREADS / W;
+
+template <typename T>
+__global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p) {
+  __shared__ __align__(16) float qs[SIMT_HEADS][D];
+  __shared__ float qsum[SIMT_HEADS], alpha[SIMT_HEADS], ml[SIMT_HEADS][2];
+  __shared__ float prob[SIMT_HEADS][SIMT_KEYS];
+  __shared__ size_t key_row[SIMT_KEYS];
+  __shared__ uint32_t v_pair[SIMT_KEYS];
+  __shared__ __align__(16) float red[SIMT_THREADS * 8];
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.H / p.Hkv, head_tiles = (G + SIMT_HEADS - 1) / SIMT_HEADS;
+  const int kvh = blockIdx.y / head_tiles, g0 = blockIdx.y % head_tiles * SIMT_HEADS, split = blockIdx.z;
+  const int nh = min(SIMT_HEADS, G - g0), h0 = kvh * G + g0;
+  const int b = request_of(p.cu_q, p.B, t);
+  if (b < 0) return;
+  const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
+  const int pos = kv_len - (p.cu_q[b + 1] - t);
+  const int j_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0, j_hi = max(pos + 1, j_lo);
+  const int tiles = (j_hi - j_lo + SIMT_KEYS - 1) / SIMT_KEYS, per = (tiles + p.splits - 1) / p.splits;
+  const int* bt = p.block_table + (size_t)b * p.table_stride;
+
+  for (int i = tid; i < SIMT_HEADS * D; i += SIMT_THREADS) {
+    const int h = i / D, d = i % D;
+    qs[h][d] = h < nh ? to_f32<T>(static_cast<const T*>(p.q)[t * p.q_row + (h0 + h) * p.q_head + d]) : 0.f;
+  }
+  if (tid < SIMT_HEADS) { ml[tid][0] = -INFINITY; ml[tid][1] = 0.f; }
+  __syncthreads();
+  for (int h = warp; h < SIMT_HEADS; h += 4) {
+    float s = 0.f;
+    for (int d = lane; d < D; d += 32) s += qs[h][d];
+    s = warp_sum(s);
+    if (lane == 0) qsum[h] = s;
+  }
+  float o[SIMT_HEADS][8];
+#pragma unroll
+  for (int h = 0; h < SIMT_HEADS; ++h)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[h][i] = 0.f;
+  const int word = tid % W, kg = tid / W;
+  __syncthreads();
+
+  for (int tile = split * per; tile < min(tiles, (split + 1) * per); ++tile) {
+    const int j0 = j_lo + tile * SIMT_KEYS, j = j0 + tid, n = min(SIMT_KEYS, j_hi - j0);
+    if (tid < n) {
+      const size_t row = cache_row(p, bt, kvh, j);
+      key_row[tid] = row;
+      v_pair[tid] = p.vp[row];
+      const uint32_t kpair = p.kp[row];
+      const float ks = pair_scale(kpair), kz = pair_zero(kpair);
+      float acc[SIMT_HEADS] = {};
+#pragma unroll 2
+      for (int w = 0; w < W; ++w) {
+        const uint32_t bits = p.kc[row * W + w];
+        float c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = (float)((bits >> shift_of(i)) & 15u);
+#pragma unroll
+        for (int h = 0; h < SIMT_HEADS; ++h) {
+          const float4 a = *reinterpret_cast<const float4*>(&qs[h][w * 8]), e = *reinterpret_cast<const float4*>(&qs[h][w * 8 + 4]);
+          acc[h] = fmaf(a.x, c[0], fmaf(a.y, c[1], fmaf(a.z, c[2], fmaf(a.w, c[3], acc[h]))));
+          acc[h] = fmaf(e.x, c[4], fmaf(e.y, c[5], fmaf(e.z, c[6], fmaf(e.w, c[7], acc[h]))));
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < SIMT_HEADS; ++h) prob[h][tid] = capped(p, fmaf(ks, acc[h], kz * qsum[h]) * p.scale) * LOG2E;
+    }
+    __syncthreads();
+    for (int h = warp; h < nh; h += 4) {
+      float s[SIMT_KEYS / 32], m = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < SIMT_KEYS / 32; ++i) {
+        s[i] = lane + 32 * i < n ? prob[h][lane + 32 * i] : -INFINITY;
+        m = fmaxf(m, s[i]);
+      }
+      const float before = ml[h][0];
+      m = fmaxf(warp_max(m), before);
+      const float base = m == -INFINITY ? 0.f : m;          // (every score -infinity or NaN: nothing to subtract)
+#pragma unroll
+      for (int i = 0; i < SIMT_KEYS / 32; ++i) {
+        s[i] = exp2f(s[i] - base);
+        sum += s[i];
+        prob[h][lane + 32 * i] = s[i];
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) {
+        const float a = exp2f(before - base);
+        alpha[h] = a;
+        ml[h][0] = m;
+        ml[h][1] = ml[h][1] * a + sum;
+      }
+    }
+    __syncthreads();
+    if (kg < KG) {
+#pragma unroll
+      for (int h = 0; h < SIMT_HEADS; ++h)
+        if (h < nh) {
+          const float a = alpha[h];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[h][i] *= a;
+        }
+      for (int key = kg; key < n; key += KG) {
+        const uint32_t bits = p.vc[key_row[key] * W + word];
+        const float vs = pair_scale(v_pair[key]), vz = pair_zero(v_pair[key]);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaf((float)((bits >> shift_of(i)) & 15u), vs, vz);
+#pragma unroll
+        for (int h = 0; h < SIMT_HEADS; ++h)
+          if (h < nh) {
+            const float pr = prob[h][key];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[h][i] = fmaf(pr, v[i], o[h][i]);
+          }
+      }
+    }
+    __syncthreads();
+  }
+
+  for (int h = 0; h < nh; ++h) {
+    // (o[h] with a constant h: registers)
+    if (kg < KG) {
+#pragma unroll
+      for (int hh = 0; hh < SIMT_HEADS; ++hh)
+        if (hh == h) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) red[kg * D + word * 8 + i] = o[hh][i];
+        }
+    }
+    __syncthreads();
+    const size_t row = (size_t)t * p.H + h0 + h;
+    float m = ml[h][0], l = ml[h][1], a = 1.f;
+    if (p.splits == 1 && p.sinks != nullptr) {
+      const float sink = p.sinks[h0 + h] * LOG2E, top = fmaxf(m, sink);
+      a = m == -INFINITY ? 0.f : exp2f(m - top);
+      l = l * a + exp2f(sink - top);
+    }
+    for (int d = tid; d < D; d += SIMT_THREADS) {
+      float sum = 0.f;
+      for (int k = 0; k < KG; ++k) sum += red[k * D + d];
+      if (p.splits == 1) {
+        static_cast<T*>(p.out)[row * D + d] = from_f32<T>(l == 0.f ? 0.f : sum * a / l);
+      } else {
+        p.part_o[(row * p.splits + split) * D + d] = sum;
+      }
+    }
+    if (p.splits > 1 && tid == 0) {
+      p.part_ml[(row * p.splits + split) * 2] = m;
+      p.part_ml[(row * p.splits + split) * 2 + 1] = l;
+    }
+    __syncthreads();
+  }
+}
+
+// out[row] = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the key ranges of a row (token, head)
+template <typename T>
+__global__ void int4_combine_kernel(Int4Params p) {
+  pdl_trigger();
+  pdl_wait();
+  const size_t row = blockIdx.x;
+  if ((int)(row / p.H) >= p.cu_q[p.B]) return;
+  const float* ml = p.part_ml + row * p.splits * 2;
+  float m = p.sinks ? p.sinks[row % p.H] * LOG2E : -INFINITY;
+  const float sink = m;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[2 * s]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = p.sinks ? exp2f(sink - base) : 0.f;
+  for (int s = 0; s < p.splits; ++s) l += exp2f(ml[2 * s] - base) * ml[2 * s + 1];
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float sum = 0.f;
+    for (int s = 0; s < p.splits; ++s) sum += exp2f(ml[2 * s] - base) * p.part_o[(row * p.splits + s) * D + d];
+    static_cast<T*>(p.out)[row * D + d] = from_f32<T>(l == 0.f ? 0.f : sum / l);
+  }
+}
+
+int shift_of_page(int page_size) {
+  for (int s = 0; s < 20; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+
+template <typename T>
+int attend_simt(const Int4Params& p, cudaStream_t stream) {
+  const int G = p.H / p.Hkv, head_tiles = (G + SIMT_HEADS - 1) / SIMT_HEADS;
+  TS_REQUIRE(p.Hkv * head_tiles <= 65535 && p.splits <= 65535, "int4_attention: grid out of range");
+  TS_LAUNCH("int4_attention", int4_attend_kernel<T>, dim3(p.T, p.Hkv * head_tiles, p.splits), dim3(SIMT_THREADS), 0, stream, p);
+  if (p.splits > 1)
+    TS_LAUNCH("int4_attention (combine)", int4_combine_kernel<T>, dim3((unsigned)(p.T * p.H)), dim3(D < 128 ? D : 128), 0, stream, p);
+  return 0;
+}
+
+}  // namespace
+
+// k, v [T, Hkv, D] (strides in elements, columns contiguous) to the slots of slot_mapping [T] (< 0: skipped; slots are distinct)
+TS_EXPORT int ts_int4_kvwrite(int dtype, const void* k, const void* v, long long k_row, long long k_head, long long v_row, long long v_head,
+                              int T, int Hkv, void* k_codes, void* k_pairs, void* v_codes, void* v_pairs, const int* slot_mapping,
+                              int page_size, int num_pages, cudaStream_t stream) {
+  const int shift = shift_of_page(page_size);
+  TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_kvwrite: unknown dtype %d", dtype);
+  TS_REQUIRE(T > 0 && Hkv > 0 && shift >= 0 && num_pages > 0, "int4_kvwrite: %d tokens, %d heads, pages of %d", T, Hkv, page_size);
+  TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 3) == 0, "int4_kvwrite: the cache is not aligned to words");
+  const int e = dtype == TS_F32 ? 4 : 2;
+  const bool vec = ((((uintptr_t)k | (uintptr_t)v) | (uintptr_t)((k_row | k_head | v_row | v_head) * e)) & 15) == 0;
+  WriteParams p = {k, v, k_row, k_head, v_row, v_head, (uint32_t*)k_codes, (uint32_t*)v_codes, (uint32_t*)k_pairs, (uint32_t*)v_pairs,
+                   slot_mapping, T, Hkv, shift, (long long)num_pages << shift};
+  const long long rows = 2LL * T * Hkv, per = WRITE_THREADS / LANES, blocks = (rows + per - 1) / per;
+  TS_REQUIRE(blocks < (1LL << 31), "int4_kvwrite: too many rows");
+  if (dtype == TS_F32) TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<float>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, vec);
+  else TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<bf16>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, vec);
+  return 0;
+}
+
+// q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml.
+TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
+                                const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
+                                int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
+                                int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, cudaStream_t stream) {
+  const int shift = shift_of_page(page_size);
+  TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_attention: unknown dtype %d", dtype);
+  TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
+             T, B, H, Hkv, page_size);
+  TS_REQUIRE((long long)T * H < (1LL << 31), "int4_attention: too many rows");
+  TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml)), "int4_attention: key ranges need their scratch");
+  Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
+                  block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
+                  splits, part_o, part_ml};
+  return dtype == TS_F32 ? attend_simt<float>(p, stream) : attend_simt<bf16>(p, stream);
+}

@@ -1,0 +1,352 @@
+// Matrix products in 8-bit integers: y[m, n] = (sum_k cx[m, k] cw[n, k]) sx[m] sw[n] (+ bias[n]).
+//
+// Rows of x (tokens) and of W (output channels) are held as codes of 8 bits and one 32-bit scale each:
+//   scale = max |row| / 127, code = round(row / scale), halves to even; both operations in 32 bits.
+// A row of zeros has scale 0 and codes 0; a row that holds an infinity or a NaN has scale NaN, and its products are NaN.
+// The sums are exact: the tensor core adds products of 8-bit numbers in 32-bit integers (K up to 131,072: 127 * 127 * K < 2^31),
+// so cutting K never changes a result, and the scales are applied once, in 32 bits.
+//
+// The product has the roles of gemm_tcgen05.cu: 128 rows of W are the M side of tcgen05.mma (kind::i8), TILE_T tokens its N side; a
+// slice of K of 128 codes is 128 bytes, one swizzle row, so that shared memory, the TMA boxes and the four MMAs of a slice (32 bytes of
+// K each) are those of 64 bfloat16.  K is cut over the blocks of a cluster, which add their integer sums through distributed shared
+// memory: no scratch, no counters, nothing that two launches could share.
+#include "tcgen05.cuh"
+
+TS_DEFINE_LAST_ERROR()
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+// ------------------------------------------------------------------------------------------ rows to 8 bits
+constexpr int QUANT_THREADS = 256;
+
+struct QuantParams {
+  const void* x;        // [M, K], leading dimension ldx
+  signed char* codes;   // [M, K], leading dimension ldq (a multiple of 16)
+  float* scales;        // [M]
+  long long ldx, ldq;
+  int K;
+};
+
+__device__ __forceinline__ int code_of(float x, float scale) {
+  return (int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f);
+}
+
+// a block a row: the largest magnitude, then the codes (the second read comes from the caches)
+template <typename T>
+__global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParams p, bool vec) {
+  __shared__ float tops[QUANT_THREADS / 32];
+  __shared__ int bads[QUANT_THREADS / 32];
+  // The trigger comes behind the wait: what the kernel after this one reads before its own wait (the codes of the weights) is
+  // then complete, whoever wrote it.
+  pdl_wait();
+  pdl_trigger();
+  const size_t m = blockIdx.x;
+  const T* x = static_cast<const T*>(p.x) + m * p.ldx;
+  signed char* out = p.codes + m * p.ldq;
+  const int n8 = vec ? p.K / 8 : 0;
+  float top = 0.f;
+  int bad = 0;
+  for (int i = threadIdx.x; i < n8; i += QUANT_THREADS) {
+    float v[8];
+    load8<T>(x + i * 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top = fmaxf(top, fabsf(v[e]));
+      bad |= !(fabsf(v[e]) <= 3.402823466e38f);
+    }
+  }
+  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += QUANT_THREADS) {
+    const float v = to_f32<T>(x[i]);
+    top = fmaxf(top, fabsf(v));
+    bad |= !(fabsf(v) <= 3.402823466e38f);
+  }
+  top = warp_max(top);
+  bad = __any_sync(0xffffffffu, bad);
+  if ((threadIdx.x & 31) == 0) { tops[threadIdx.x >> 5] = top; bads[threadIdx.x >> 5] = bad; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < QUANT_THREADS / 32; ++w) { top = fmaxf(top, tops[w]); bad |= bads[w]; }
+  const float scale = __fdiv_rn(top, 127.f);
+  const bool zero = bad || !(scale > 0.f);
+  if (threadIdx.x == 0) p.scales[m] = bad ? __int_as_float(0x7fc00000) : scale;
+  for (int i = threadIdx.x; i < n8; i += QUANT_THREADS) {
+    float v[8];
+    load8<T>(x + i * 8, v);
+    uint32_t w[2] = {0u, 0u};
+    if (!zero) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(code_of(v[e], scale) & 255) << (8 * (e & 3));
+    }
+    *reinterpret_cast<uint2*>(out + i * 8) = make_uint2(w[0], w[1]);
+  }
+  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += QUANT_THREADS)
+    out[i] = zero ? 0 : (signed char)code_of(to_f32<T>(x[i]), scale);
+}
+
+// ------------------------------------------------------------------------------------------ the product
+constexpr int TILE_N = 128;          // weight rows of a block (MMA M)
+constexpr int BK = 128;              // codes of a stage: 128 bytes, one swizzle row
+constexpr int K_STEPS = BK / 32;     // MMAs of a stage
+constexpr int THREADS = 128;         // warp 0 loads, warp 1 issues, all four do the epilogue
+constexpr int W_STAGE_BYTES = TILE_N * BK;
+constexpr int MAX_SPLITS = 8;
+
+struct I8Params {
+  void* out;            // [M, ldc] bfloat16 or float
+  const float* sx;      // [M]
+  const float* sw;      // [N]
+  VecParam bias;        // [N]; ptr null: none
+  long long ldc;
+  int M, N, K, splits, out_f32;
+  int w_ready;          // nobody that may still run writes the codes of W: they are fetched before the dependency wait
+};
+
+// instruction descriptor: signed 8-bit x signed 8-bit -> 32-bit integers, both operands K-major, M = 128, N = tile_t
+__host__ __device__ constexpr uint32_t instr_desc(int tile_t) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(tile_t >> 3) << 17) | (static_cast<uint32_t>(TILE_N >> 4) << 24);
+}
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_load8_int(uint32_t addr, int (&v)[8]) {
+  float f[8];
+  tmem_load8(addr, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __float_as_int(f[i]);
+}
+
+template <int TILE_T> struct Cfg {
+  static constexpr int STAGE_BYTES = W_STAGE_BYTES + TILE_T * BK;
+  static constexpr int RING = 110 * 1024;                     // two blocks share an SM
+  static constexpr int STAGES = RING / STAGE_BYTES > 6 ? 6 : RING / STAGE_BYTES;
+  static constexpr int TMEM_COLS = TILE_T < 32 ? 32 : TILE_T;
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 256;
+  static_assert(STAGES >= 3 && STAGES * STAGE_BYTES >= TILE_T * TILE_N * 4, "the ring holds the block's sums");
+};
+
+template <int TILE_T>
+__global__ void __launch_bounds__(THREADS, 2)
+gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ I8Params p) {
+  using C = Cfg<TILE_T>;
+  extern __shared__ char smem_raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* ctrl = smem + (size_t)C::STAGES * C::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ctrl);            // [STAGES]
+  uint64_t* empty = full + C::STAGES;                            // [STAGES]
+  uint64_t* accum = empty + C::STAGES;                           // [1]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int n_tile = blockIdx.x, t_tile = blockIdx.y, split = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kb_total = (p.K + BK - 1) / BK, per = (kb_total + p.splits - 1) / p.splits;
+  const int kb0 = split * per, nkb = max(0, min(kb_total, kb0 + per) - kb0);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(accum), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                 ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)C::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  pdl_trigger();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (threadIdx.x == 0) {
+    // loader: one slice of K per stage
+    if (!p.w_ready) pdl_wait();
+    const int pre = min(nkb, C::STAGES);
+    for (int i = 0; i < pre; ++i) {
+      const uint32_t bar = smem_u32(&full[i]);
+      mbar_expect_tx(bar, C::STAGE_BYTES);
+      tma_load_2d(smem_u32(smem + (size_t)i * C::STAGE_BYTES), &map_w, bar, (kb0 + i) * BK, n_tile * TILE_N);
+    }
+    pdl_wait();
+    for (int i = 0; i < pre; ++i)
+      tma_load_2d(smem_u32(smem + (size_t)i * C::STAGE_BYTES + W_STAGE_BYTES), &map_x, smem_u32(&full[i]), (kb0 + i) * BK, t_tile * TILE_T);
+    int armed = pre;
+    for (int i = pre; i < nkb; ++i) {
+      const int s = i % C::STAGES;
+      if (!mbar_wait(smem_u32(&empty[s]), ((i / C::STAGES) & 1) ^ 1, abort_flag)) break;
+      const uint32_t bar = smem_u32(&full[s]);
+      mbar_expect_tx(bar, C::STAGE_BYTES);
+      char* stage = smem + (size_t)s * C::STAGE_BYTES;
+      tma_load_2d(smem_u32(stage), &map_w, bar, (kb0 + i) * BK, n_tile * TILE_N);
+      tma_load_2d(smem_u32(stage + W_STAGE_BYTES), &map_x, bar, (kb0 + i) * BK, t_tile * TILE_T);
+      armed = i + 1;
+    }
+    if (*abort_flag) {
+      // let the copies that are still in flight land before the block goes away
+      for (int i = max(0, armed - C::STAGES); i < armed; ++i) {
+        const uint32_t bar = smem_u32(&full[i % C::STAGES]);
+        for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(bar, (i / C::STAGES) & 1); ++w) {}
+      }
+    }
+  } else if (warp == 1 && elect_one()) {
+    pdl_wait();
+    const uint32_t idesc = instr_desc(TILE_T);
+    const uint64_t desc0 = smem_desc(smem_u32(smem));
+    bool ok = true;
+    for (int i = 0; i < nkb && ok; ++i) {
+      const int s = i % C::STAGES;
+      ok = mbar_spin_wait(smem_u32(&full[s]), (i / C::STAGES) & 1, abort_flag);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const uint64_t ad = desc0 + (uint64_t)s * (C::STAGE_BYTES >> 4), bd = ad + (W_STAGE_BYTES >> 4);
+#pragma unroll
+      for (int k = 0; k < K_STEPS; ++k) umma_i8(tmem_base, ad + 2 * k, bd + 2 * k, idesc, i > 0 || k > 0 ? 1u : 0u);
+      tcgen05_commit(smem_u32(&empty[s]));
+    }
+    if (ok && nkb > 0) tcgen05_commit(smem_u32(accum));
+  } else {
+    pdl_wait();
+  }
+  __syncthreads();
+
+  // epilogue: lane = weight row, columns = tokens
+  bool have = nkb > 0;
+  if (have) have = mbar_spin_wait(smem_u32(accum), 0, abort_flag);
+  have = __all_sync(0xffffffffu, have);      // tcgen05.ld is warp-wide: decide per warp
+  tcgen05_fence_after();
+  const int n = n_tile * TILE_N + threadIdx.x, t0 = t_tile * TILE_T;
+  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+  const float sw = n < p.N ? p.sw[n] : 0.f;
+  const float bn = p.bias.ptr != nullptr && n < p.N ? p.bias[n] : 0.f;
+  auto put = [&](int m, int sum) {
+    float y = (float)sum * (p.sx[m] * sw) + bn;
+    if (p.out_f32) static_cast<float*>(p.out)[m * p.ldc + n] = y;
+    else static_cast<bf16*>(p.out)[m * p.ldc + n] = __float2bfloat16_rn(y);
+  };
+  if (p.splits == 1) {
+#pragma unroll 1
+    for (int c = 0; c < TILE_T && t0 + c < p.M; c += 8) {
+      int v[8] = {};
+      if (have) tmem_load8_int(taddr + c, v);
+      if (n < p.N) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t0 + c + i < p.M) put(t0 + c + i, v[i]);
+      }
+    }
+  } else {
+    // every block of the cluster leaves its sums in its shared memory (the ring is idle); rank r then owns the tokens r, r + splits, ..
+    int* red = reinterpret_cast<int*>(smem);               // [TILE_T][TILE_N]
+#pragma unroll 1
+    for (int c = 0; c < TILE_T; c += 8) {
+      int v[8] = {};
+      if (have) tmem_load8_int(taddr + c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) red[(c + i) * TILE_N + threadIdx.x] = v[i];
+    }
+    cluster_arrive();
+    cluster_wait();
+    for (int j = split; j < TILE_T && t0 + j < p.M; j += p.splits) {
+      int sum = 0;
+#pragma unroll
+      for (int s = 0; s < MAX_SPLITS; ++s)
+        if (s < p.splits) sum += __float_as_int(cluster_load_f32(reinterpret_cast<const float*>(red) + j * TILE_N + threadIdx.x, s));
+      if (n < p.N) put(t0 + j, sum);
+    }
+    // no block leaves while a peer may still read its shared memory
+    cluster_arrive();
+    cluster_wait();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"((uint32_t)C::TMEM_COLS) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------- host side
+// rows x K codes with leading dimension ld; boxes of box_rows x 128
+bool make_map(CUtensorMap* map, const void* base, long long rows, long long K, long long ld, int box_rows) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {BK, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int TILE_T>
+int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, cudaStream_t stream) {
+  const cudaError_t set = cudaFuncSetAttribute(gemm_i8_kernel<TILE_T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<TILE_T>::SMEM);
+  if (set != cudaSuccess) return ts_fail("gemm_int8: %s", cudaGetErrorString(set));
+  const dim3 grid((p.N + TILE_N - 1) / TILE_N, (p.M + TILE_T - 1) / TILE_T, p.splits);
+  const cudaError_t e = ts_launch_cluster(gemm_i8_kernel<TILE_T>, grid, dim3(THREADS), Cfg<TILE_T>::SMEM, stream, dim3(1, 1, p.splits), map_w, map_x, p);
+  if (e != cudaSuccess) return ts_fail("gemm_int8 (clusters of %d): %s", p.splits, cudaGetErrorString(e));
+  return 0;
+}
+
+int tile_tokens(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
+
+int quantize(int dtype, const void* x, long long ldx, void* codes, long long ldq, float* scales, int M, int K, cudaStream_t stream) {
+  const int e = dtype == TS_F32 ? 4 : 2;
+  const bool vec = (((uintptr_t)x | (uintptr_t)(ldx * e)) & 15) == 0 && (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
+  const QuantParams p = {x, static_cast<signed char*>(codes), scales, ldx, ldq, K};
+  if (dtype == TS_F32) TS_LAUNCH("quantize_rows", quantize_rows_kernel<float>, dim3(M), dim3(QUANT_THREADS), 0, stream, p, vec);
+  else TS_LAUNCH("quantize_rows", quantize_rows_kernel<bf16>, dim3(M), dim3(QUANT_THREADS), 0, stream, p, vec);
+  return 0;
+}
+
+}  // namespace
+
+// 1 if a block ever gave up on a wait since the library was loaded (reads device memory: syncs)
+TS_EXPORT int ts_gemm_int8_error() {
+  int flag = 0;
+  if (cudaMemcpyFromSymbol(&flag, g_error_flag, sizeof(int)) != cudaSuccess) return -1;
+  return flag;
+}
+
+// codes [M, K] (leading dimension ldq) and scales [M] of the rows of x [M, K] (ldx)
+TS_EXPORT int ts_quantize_rows(int dtype, const void* x, long long ldx, void* codes, long long ldq, float* scales, int M, int K, cudaStream_t stream) {
+  TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "quantize_rows: unknown dtype %d", dtype);
+  TS_REQUIRE(M > 0 && K > 0, "quantize_rows: empty operand");
+  return quantize(dtype, x, ldx, codes, ldq, scales, M, K, stream);
+}
+
+// out [M, N] (ldc; float where out_f32, else bfloat16) from codes and scales of x and w (leading dimensions multiples of 16).
+// x_dtype >= 0: x is a tensor of that type (leading dimension ldx) whose rows are brought to cx, sx first; -1: cx and sx are given.
+// w_constant: nobody that may still run writes w (with x_dtype >= 0 the first launch sees to that).
+TS_EXPORT int ts_gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, long long ldcx, float* sx, const void* cw, long long ldw,
+                           const float* sw, const void* bias, int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K,
+                           int splits, int w_constant, cudaStream_t stream) {
+  TS_REQUIRE(M > 0 && N > 0 && K > 0 && K <= 131072, "gemm_int8: M=%d N=%d K=%d (K up to 131072: the sums are 32-bit integers)", M, N, K);
+  TS_REQUIRE((ldcx | ldw) % 16 == 0 && (((uintptr_t)cx | (uintptr_t)cw) & 15) == 0, "gemm_int8: rows of codes begin on 16 bytes");
+  TS_REQUIRE(splits >= 1 && splits <= MAX_SPLITS, "gemm_int8: splits out of range");
+  const int tile_t = tile_tokens(M);
+  TS_REQUIRE((M + tile_t - 1) / tile_t <= 65535, "gemm_int8: too many rows");
+  if (x_dtype >= 0) {
+    TS_REQUIRE(x_dtype == TS_F32 || x_dtype == TS_BF16, "gemm_int8: unknown dtype %d", x_dtype);
+    const int rc = quantize(x_dtype, x, ldx, cx, ldcx, sx, M, K, stream);
+    if (rc != 0) return rc;
+  }
+  CUtensorMap map_w, map_x;
+  TS_REQUIRE(make_map(&map_w, cw, N, K, ldw, TILE_N) && make_map(&map_x, cx, M, K, ldcx, tile_t), "gemm_int8: cuTensorMapEncodeTiled failed");
+  const I8Params p = {out, sx, sw, VecParam{bias, bias_f32}, ldc, M, N, K, splits, out_f32, x_dtype >= 0 || w_constant};
+  switch (tile_t) {
+    case 16: return launch<16>(map_w, map_x, p, stream);
+    case 32: return launch<32>(map_w, map_x, p, stream);
+    case 64: return launch<64>(map_w, map_x, p, stream);
+    default: return launch<128>(map_w, map_x, p, stream);
+  }
+}

@@ -647,16 +647,34 @@ def _streams():
     return build.load_unit("streams.cu")
 
 
+def _gemm_int8():
+    return build.load_unit("gemm_int8.cu")
+
+
+def _attention_int4(head_dim: int):
+    if head_dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"head size {head_dim} is not supported: attention takes multiples of 16 "
+                         f"up to {SUPPORTED_HEAD_DIMS[-1]}")
+    return build.load_unit("attention_int4.cu", {"TS_HEAD_DIM": head_dim})
+
+
+def gemm_int8_error() -> int:
+    """1 if a block of the 8-bit product ever gave up on a wait (synchronises)."""
+    return _gemm_int8().ts_gemm_int8_error()
+
+
 def units_for(head_dims, key_dims=(), delta_dims=()) -> list:
     """The (source, defines) units a model with these attention head sizes, these key sizes of
     its matrix-state mixers and these of its delta-rule mixers needs."""
     units = [("elementwise.cu", {}), ("gemm_simt.cu", {}), ("gemm_tcgen05.cu", {}), ("gemm_pair_tcgen05.cu", {}),
-             ("gemv_mma.cu", {}), ("sampler.cu", {}), ("latent_moe.cu", {}), ("sequence.cu", {}), ("streams.cu", {})]
+             ("gemv_mma.cu", {}), ("sampler.cu", {}), ("latent_moe.cu", {}), ("sequence.cu", {}), ("streams.cu", {}),
+             ("gemm_int8.cu", {})]
     units += [("attention_simt.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims))]
     units += [("attention_mma.cu", _mma_defines(d)) for d in sorted(set(head_dims))
               if d <= MMA_MAX_HEAD_DIM]
     units += [("attention_tcgen05.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims))
               if d in TCGEN05_HEAD_DIMS]
+    units += [("attention_int4.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims))]
     units += [("linear_attention.cu", {"TS_KEY_DIM": d}) for d in sorted(set(key_dims))]
     units += [("delta_rule.cu", {"TS_KEY_DIM": d}) for d in sorted(set(delta_dims))]
     return units
@@ -861,7 +879,7 @@ def activated_linear(x, weight, activation, constant_weight=False):
     """act(x @ weight^T) [M, N]: in the tcgen05 product's epilogue for up to TCGEN05_MAX_TOKENS bfloat16 rows,
     else the product followed by the activation in place.  ``constant_weight``: as for ``linear``."""
     x = materialize(x)
-    if x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and activation in PLAIN_ACTIVATIONS and _tcgen05_ok(x, weight):
+    if not isinstance(weight, Int8Rows) and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and activation in PLAIN_ACTIVATIONS and _tcgen05_ok(x, weight):
         _cuda(x, weight)
         return _linear_tcgen05(x, weight, False, plain=PLAIN_ACTIVATIONS[activation])
     return plain_activation_(linear(x, weight, constant_weight=constant_weight), activation)
@@ -1083,7 +1101,13 @@ def paged_attention(q, k_cache, v_cache, view, ctx, scale, window=0, num_splits=
     q [T, H, D]; caches [pages, Hkv, page_size, D]; ``view`` a GroupView; ``ctx`` gives cu_q,
     kv_lens and the batch's maxima.  bfloat16 runs on the tensor cores (a decode kernel when
     every request brings one token, else a prefill kernel); float32 on the 32-bit kernel.
-    ``backend`` overrides ``attention_backend`` (tests run the slower kernels at every size)."""
+    ``backend`` overrides ``attention_backend`` (tests run the slower kernels at every size).
+    The caches may be ``Int4Pages`` (4 bits; a window, sinks and a soft cap, none of the other forms)."""
+    if isinstance(k_cache, Int4Pages) or isinstance(v_cache, Int4Pages):
+        if keep_first or chunk or slopes is not None or turn is not None:
+            raise ValueError("paged_attention: a 4-bit cache takes a window, sinks and a soft cap; kept first keys, chunks, slopes and "
+                             "turned values need a cache of whole numbers")
+        return _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_splits, backend, sinks, softcap)
     _cuda(q, k_cache, v_cache)
     T, H, D = q.shape
     Hkv = k_cache.shape[1]
@@ -1237,11 +1261,15 @@ def linear(x, weight, bias=None, out_float32=False, allow_partials=False, allow_
     result may be a SplitPartials (the caller hands it to add_rmsnorm, qk_norm_rope_kvwrite, or
     calls materialize); with ``allow_pending`` a PendingProduct (for add_rmsnorm, or materialize).
     x may be the ScaledRows that add_rmsnorm returned.
+    ``weight`` may be an ``Int8Rows``: the rows of x are then brought to 8 bits too (or x is an Int8Rows already), and the
+    result is a plain tensor of x's type (of bfloat16 for an Int8Rows), or float32 with ``out_float32``.
     ``constant_weight``: no kernel that may still run writes ``weight`` (a model's weights).  A float32 product
     then fetches its first tiles of it while the kernels before it still run; without, the weight may be the
     result of the product before.  The bfloat16 products of this package always fetch them so: a
     bfloat16 weight that was computed on the device needs a synchronisation before its first product."""
     scale = None
+    if isinstance(weight, Int8Rows) or isinstance(x, Int8Rows):
+        return _linear_int8(x, weight, bias, out_float32, constant_weight)
     if isinstance(x, ScaledRows):
         scale, x = x, x.data
     _cuda(x, weight, bias)
@@ -2328,7 +2356,7 @@ def linear_beside(groups):
     rows = [h.data if isinstance(h, ScaledRows) else h for h, _ in flat]
     scaled = [h for h, _ in flat if isinstance(h, ScaledRows)]
     M, K = rows[0].shape
-    one = (1 < len(flat) <= BESIDE_MAX_PRODUCTS and M <= TCGEN05_MAX_TOKENS
+    one = (1 < len(flat) <= BESIDE_MAX_PRODUCTS and M <= TCGEN05_MAX_TOKENS and not any(isinstance(p.weight, Int8Rows) for _, p in flat)
            and all(r.dtype == torch.bfloat16 and tuple(r.shape) == (M, K) and _tcgen05_ok(r, p.weight) for r, (_, p) in zip(rows, flat))
            and (not scaled or (len(scaled) == len(flat) and M <= FUSED_MAX_TOKENS
                                and all(h.sumsq is scaled[0].sumsq and h.eps == scaled[0].eps for h in scaled))))
@@ -2530,4 +2558,221 @@ def delta_rule(q, k, v, gate, logits, bias, rate, state, ctx, num_heads, key_dim
         _ptr(ctx.cu_q), c_int(ctx.num_requests), c_int(longest), c_int(T), _ptr(norm_weight), c_int(_f32(norm_weight)), c_float(eps),
         _ptr(out), c_longlong(out.stride(0)), _ptr(raw), c_int(H), c_int(value_dim), c_int(qk_group), c_int(tile), _ptr(groups), _stream()),
         1 + int(spread) + int(tile > 0))
+    return out
+
+
+# ----------------------------------------------------------------------------- fewer bits
+class Int8Rows:
+    """Rows of a matrix in 8 bits: ``codes`` int8 [R, K] (rows that begin on 16 bytes: a leading dimension that is a multiple
+    of 16) and ``scales`` float32 [R]; row r stands for codes[r] * scales[r].  ``quantize_rows`` makes them, for the weights of a
+    product as for its tokens: scale = max |row| / 127, code = round(row / scale), halves to even, both in 32 bits."""
+    __slots__ = ("codes", "scales", "shape")
+    dtype = torch.int8
+
+    def __init__(self, codes, scales):
+        if codes.dtype != torch.int8 or codes.dim() != 2 or scales.dtype != torch.float32 or scales.shape != codes.shape[:1]:
+            raise TypeError("Int8Rows: codes are int8 [R, K] and scales float32 [R], got "
+                            f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+        if (codes.shape[1] > 1 and codes.stride(1) != 1) or codes.stride(0) % 16 or codes.data_ptr() % 16 or not scales.is_contiguous():
+            raise ValueError("Int8Rows: a row of codes lies in one run that begins on 16 bytes (a leading dimension that is a "
+                             "multiple of 16), and the scales are contiguous")
+        self.codes, self.scales, self.shape = codes, scales, tuple(codes.shape)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def float(self):
+        """The values that the codes stand for."""
+        return self.codes.float() * self.scales[:, None]
+
+
+#: the sums of an 8-bit product are 32-bit integers: 127 * 127 * K stays below 2^31
+INT8_MAX_K = 131072
+
+
+def _here(what, *tensors):
+    """Operands lie on the current device: the launch goes to its current stream."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != here):
+            if not t.is_cuda:
+                raise RuntimeError("kernel operands must be CUDA tensors: there is no CPU path")
+            raise RuntimeError(f"{what}: an operand lies on {t.device}, the current device is cuda:{here}")
+
+
+def _quantizable(x, what):
+    if x.dim() != 2 or x.dtype not in _DTYPE:
+        raise TypeError(f"{what}: rows are float32 or bfloat16 [R, K], got {x.dtype} {tuple(x.shape)}")
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        raise ValueError(f"{what}: a row lies in one run (stride 1 along K), got strides {x.stride()}")
+    if not 0 < x.shape[1] <= INT8_MAX_K:
+        raise ValueError(f"{what}: K is 1 to {INT8_MAX_K} (sums of products of 8-bit numbers in 32 bits), got {x.shape[1]}")
+
+
+def quantize_rows(x) -> Int8Rows:
+    """The rows of x (float32 or bfloat16 [R, K], rows contiguous) in 8 bits.  A row of zeros has scale 0; one that holds an infinity or a NaN
+    has scale NaN."""
+    x = materialize(x)
+    _quantizable(x, "quantize_rows")
+    _here("quantize_rows", x)
+    M, K = x.shape
+    codes = torch.empty(M, -(-K // 16) * 16, dtype=torch.int8, device=x.device)[:, :K]
+    scales = torch.empty(M, dtype=torch.float32, device=x.device)
+    if M:
+        lib = _gemm_int8()
+        _check(lib, lib.ts_quantize_rows(c_int(_dt(x)), _ptr(x), c_longlong(x.stride(0)), _ptr(codes), c_longlong(codes.stride(0)), _ptr(scales),
+                                         c_int(M), c_int(K), _stream()))
+    return Int8Rows(codes, scales)
+
+
+def int8_splits(M, N, K):
+    """Cuts along K of the 8-bit product: a product with few row tiles fills the places of two blocks an SM, with at
+    least two slices of 128 a cut; the cuts of a tile are a cluster of up to 8 blocks."""
+    tile_t = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
+    tiles = -(-N // 128) * -(-M // tile_t)
+    slices = -(-K // 128)
+    splits = max(1, min(2 * num_sms() // tiles, slices // 2, 8))
+    return -(-slices // -(-slices // splits))           # no cut without a slice
+
+
+def _linear_int8(x, weight, bias, out_float32, constant_weight):
+    if not isinstance(weight, Int8Rows):
+        raise TypeError("linear: rows in 8 bits need a weight in 8 bits (quantize_rows)")
+    N, K = weight.shape
+    given = isinstance(x, Int8Rows)
+    if not given:
+        x = materialize(x)
+        _quantizable(x, "linear")
+    if x.shape[1] != K:
+        raise ValueError(f"linear: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in _DTYPE or not bias.is_contiguous()):
+        raise ValueError(f"linear: bias {bias.dtype} {tuple(bias.shape)} does not fit {N} outputs (float32 or bfloat16, contiguous)")
+    M = x.shape[0]
+    device = weight.codes.device
+    dtype = torch.float32 if out_float32 else torch.bfloat16 if given else x.dtype
+    _here("linear", x.codes if given else x, weight.codes, weight.scales, x.scales if given else None, bias)
+    out = torch.empty(M, N, dtype=dtype, device=device)
+    if M == 0 or N == 0:
+        return out
+    if given:
+        cx, ldcx, sx = c_void_p(x.codes.data_ptr()), x.codes.stride(0), c_void_p(x.scales.data_ptr())
+        xp, ldx, xt = c_void_p(0), 0, -1
+    else:
+        ldcx = -(-K // 16) * 16
+        scratch = torch.empty(M * (ldcx + 4), dtype=torch.uint8, device=device)
+        cx, sx = c_void_p(scratch.data_ptr()), c_void_p(scratch.data_ptr() + M * ldcx)
+        xp, ldx, xt = c_void_p(x.data_ptr()), x.stride(0), _DTYPE[x.dtype]
+    lib = _gemm_int8()
+    _check(lib, lib.ts_gemm_int8(
+        c_int(xt), xp, c_longlong(ldx), cx, c_longlong(ldcx), sx, c_void_p(weight.codes.data_ptr()), c_longlong(weight.codes.stride(0)),
+        c_void_p(weight.scales.data_ptr()), _ptr(bias), c_int(_DTYPE[bias.dtype] == 0 if bias is not None else 0), c_void_p(out.data_ptr()),
+        c_longlong(N), c_int(1 if dtype == torch.float32 else 0), c_int(M), c_int(N), c_int(K), c_int(int8_splits(M, N, K)),
+        c_int(1 if constant_weight else 0), _stream()), 1 if given else 2)
+    return out
+
+
+class Int4Pages:
+    """One of the caches (keys or values) in 4 bits: ``codes`` uint8 [pages, kv heads, slots, D / 2] and ``pairs`` bfloat16 [pages, kv
+    heads, slots, 2], both contiguous.  A head of a token with pair (scale, zero) stands for zero + code * scale; eight codes fill a
+    32-bit word, even columns in its lower half, odd ones in its upper half, the first in the lowest bits.  ``int4_kvwrite`` fills it."""
+    __slots__ = ("codes", "pairs", "shape")
+
+    def __init__(self, codes, pairs):
+        if codes.dtype != torch.uint8 or codes.dim() != 4 or pairs.dtype != torch.bfloat16 or pairs.shape != codes.shape[:3] + (2,):
+            raise TypeError("Int4Pages: codes are uint8 [pages, heads, slots, D / 2] and pairs bfloat16 [pages, heads, slots, 2], got "
+                            f"{codes.dtype} {tuple(codes.shape)} and {pairs.dtype} {tuple(pairs.shape)}")
+        if not codes.is_contiguous() or not pairs.is_contiguous() or codes.data_ptr() % 16 or pairs.data_ptr() % 16:
+            raise ValueError("Int4Pages: codes and pairs are contiguous and begin on 16 bytes")
+        pages, heads, slots, half = codes.shape
+        self.codes, self.pairs, self.shape = codes, pairs, (pages, heads, slots, 2 * half)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _int4_caches(what, k_cache, v_cache, page):
+    if not isinstance(k_cache, Int4Pages) or not isinstance(v_cache, Int4Pages) or k_cache.shape != v_cache.shape:
+        raise TypeError(f"{what}: keys and values are both Int4Pages of one shape")
+    if page != k_cache.shape[2] or page & (page - 1):
+        raise ValueError(f"{what}: pages of {page} tokens on a cache with pages of {k_cache.shape[2]} (a power of two)")
+
+
+def _int32_row(what, t, name, n):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
+        raise TypeError(f"{what}: {name} is int32 [{n}], contiguous, got {t.dtype} {tuple(t.shape)}")
+
+
+def int4_kvwrite(k, v, k_cache, v_cache, slot_mapping):
+    """Brings a step's keys and values (float32 or bfloat16 [T, kv heads, D], columns contiguous) to their slots (int32 [T]: page *
+    page size + slot; < 0: not written; no slot twice) of a 4-bit cache.  For every head of a token, in 32 bits: zero =
+    bfloat16(min), scale = bfloat16((max - zero) / 15), code = round((x - zero) / scale), halves to even, within 0 and 15; a row with an
+    infinity or a NaN gets a pair of NaN."""
+    what = "int4_kvwrite"
+    _int4_caches(what, k_cache, v_cache, k_cache.shape[2] if isinstance(k_cache, Int4Pages) else 0)
+    pages, heads, page, D = k_cache.shape
+    for x in (k, v):
+        if x.dim() != 3 or x.dtype not in _DTYPE or x.dtype != k.dtype or tuple(x.shape) != (k.shape[0], heads, D):
+            raise TypeError(f"{what}: keys and values are float32 or bfloat16 [T, {heads}, {D}], got {x.dtype} {tuple(x.shape)}")
+        if x.stride(2) != 1:
+            raise ValueError(f"{what}: a head lies in one run, got strides {x.stride()}")
+    T = k.shape[0]
+    _int32_row(what, slot_mapping, "slot_mapping", T)
+    _here(what, k, v, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping)
+    lib = _attention_int4(D)
+    if T == 0:
+        return
+    _check(lib, lib.ts_int4_kvwrite(
+        c_int(_DTYPE[k.dtype]), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), c_longlong(k.stride(0)), c_longlong(k.stride(1)),
+        c_longlong(v.stride(0)), c_longlong(v.stride(1)), c_int(T), c_int(heads), c_void_p(k_cache.codes.data_ptr()),
+        c_void_p(k_cache.pairs.data_ptr()), c_void_p(v_cache.codes.data_ptr()), c_void_p(v_cache.pairs.data_ptr()),
+        c_void_p(slot_mapping.data_ptr()), c_int(page), c_int(pages), _stream()))
+
+
+def int4_attention_splits(blocks, max_kv_len):
+    """Key ranges of the 32-bit kernel over a 4-bit cache: four blocks an SM, two tiles of 128 keys a range at least."""
+    return max(1, min(-(-4 * num_sms() // blocks), max_kv_len // 256, 32))
+
+
+def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_splits, backend, sinks, softcap):
+    what = "paged_attention"
+    _int4_caches(what, k_cache, v_cache, view.page_size)
+    pages, Hkv, page, D = k_cache.shape
+    if q.dim() != 3 or q.dtype not in _DTYPE or q.shape[2] != D or q.shape[1] % Hkv:
+        raise TypeError(f"{what}: queries are float32 or bfloat16 [T, H, {D}] with H a multiple of {Hkv}, got {q.dtype} {tuple(q.shape)}")
+    if q.stride(2) != 1:
+        raise ValueError(f"{what}: a head lies in one run, got strides {q.stride()}")
+    T, H = q.shape[:2]
+    B = ctx.num_requests
+    window, softcap = int(window or 0), float(softcap or 0.0)
+    if window < 0 or softcap < 0:
+        raise ValueError(f"{what}: a window and a soft cap are positive (0: none)")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous()):
+        raise TypeError(f"{what}: sinks are float32 [heads] on the device")
+    table = view.block_table
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < B or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise TypeError(f"{what}: the block table is int32 [requests, blocks], rows contiguous, got {table.dtype} {tuple(table.shape)}")
+    _int32_row(what, ctx.cu_q, "cu_q", B + 1)
+    _int32_row(what, ctx.kv_lens, "kv_lens", B)
+    if backend not in (None, "simt"):
+        raise ValueError(f"attention backend {backend!r} does not take {q.dtype}, head size {D} and a 4-bit cache")
+    _here(what, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, table, ctx.cu_q, ctx.kv_lens, sinks)
+    out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+    lib = _attention_int4(D)
+    if T == 0 or B == 0:
+        return out
+    span = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
+    if num_splits is None:
+        num_splits = int4_attention_splits(T * Hkv * -(-(H // Hkv) // 8), span)
+    part_o = part_ml = None
+    if num_splits > 1:
+        part_o = torch.empty(T * H * num_splits * D, dtype=torch.float32, device=q.device)
+        part_ml = torch.empty(T * H * num_splits * 2, dtype=torch.float32, device=q.device)
+    _check(lib, lib.ts_int4_attention(
+        c_int(_DTYPE[q.dtype]), c_void_p(q.data_ptr()), c_longlong(q.stride(0)), c_longlong(q.stride(1)), c_void_p(out.data_ptr()),
+        c_void_p(k_cache.codes.data_ptr()), c_void_p(k_cache.pairs.data_ptr()), c_void_p(v_cache.codes.data_ptr()),
+        c_void_p(v_cache.pairs.data_ptr()), c_void_p(table.data_ptr()), c_void_p(ctx.cu_q.data_ptr()), c_void_p(ctx.kv_lens.data_ptr()),
+        c_int(T), c_int(B), c_int(H), c_int(Hkv), c_int(page), c_int(table.shape[1]), c_int(table.stride(0)), c_int(pages), c_float(scale),
+        c_int(window), c_float(softcap), _ptr(sinks), c_int(num_splits), _ptr(part_o), _ptr(part_ml), _stream()), 1 if num_splits == 1 else 2)
     return out
