@@ -103,3 +103,42 @@ def test_attention():
                              (dict(ctx=other(ctx, kv_lens=torch.zeros(2))), TypeError, "kv_lens"), (dict(backend="tcgen05x"), ValueError, "backend"), (dict(), RuntimeError, "no CPU path")):
         with pytest.raises(error, match=match):
             call(**kw)
+
+
+def test_engine_options():
+    from tinyserve_b200.config.engine_config import EngineConfig
+    cfg = EngineConfig(model="", weight_dtype="int8", kv_cache_dtype="int4")
+    assert (cfg.weight_dtype, cfg.kv_cache_dtype, EngineConfig(model="").weight_dtype, EngineConfig(model="").kv_cache_dtype) == ("int8", "int4", "auto", "auto")
+    for kw in (dict(weight_dtype="int4"), dict(kv_cache_dtype="int8")):
+        with pytest.raises(ValueError, match="must be one of"):
+            EngineConfig(model="", **kw)
+
+
+def test_models_with_a_4_bit_cache():
+    from helpers import tiny_config
+    from tinyserve_b200.parts.model import build_model
+    model = build_model(tiny_config("C"), "int4")
+    assert [g.kind for g in model.cache_groups] == ["full", "window"]
+    for spec in model.cache_groups:
+        assert [(t.name, t.heads, t.width, t.dtype) for t in spec.tensors] == [("k", 2, 24, "uint8"), ("k_pairs", 2, 2, "bfloat16"), ("v", 2, 24, "uint8"), ("v_pairs", 2, 2, "bfloat16")]
+        assert spec.bytes_per_token(2) == spec.bytes_per_token(4) == 2 * 2 * (24 + 4)
+    plain = build_model(tiny_config("C"))
+    assert [spec.bytes_per_token(4) for spec in plain.cache_groups] == [2 * 2 * 48 * 4] * 2
+
+
+def test_models_that_cannot():
+    from delilorn_configs import DELILORN_TINY, delilorn_config
+    from tinyserve_b200.parts.model import build_model
+    for name in DELILORN_TINY:
+        config = delilorn_config(name)
+        build_model(config)
+        with pytest.raises(ValueError, match="4 bits|4-bit"):
+            build_model(config, "int4")
+
+
+def test_which_matrices_may_be_held_in_8_bits():
+    from helpers import tiny_config
+    from tinyserve_b200.parts.model import build_model
+    model = build_model(tiny_config("B"))
+    names = {f"{part.path}.{name}" for part in model.named_parts() for name, spec in part.param_specs().items() if spec.int8}
+    assert names == {f"model.layers.{i}.{n}" for i in range(3) for n in ("self_attn.qkv_proj.weight", "self_attn.o_proj.weight", "mlp.gate_up_proj.weight", "mlp.down_proj.weight")}

@@ -3,7 +3,7 @@ and the state-slot tensors.
 
 Layout of a cache tensor: [entry, page, head, slot, width], so the share of one head in one page
 is one contiguous run of page_size * width elements (attention: "k" and "v" of kv_heads heads of
-head_dim; a mixer may keep other tensors, see ``parts.CacheSpec``).  tinyserve keeps
+head_dim; a mixer may keep other tensors, and tensors of another element type, see ``parts.CacheSpec``).  tinyserve keeps
 [2, page, slot, kv_head, head_dim] per layer (serve.py:1791-1796)."""
 from __future__ import annotations
 
@@ -11,19 +11,25 @@ from dataclasses import dataclass
 
 import torch
 
+from ..kernels import ops
+
 
 @dataclass
 class CacheEntry:
     group: int
     tensors: dict        # name -> [page, head, slot, width]
 
-    @property
-    def k(self) -> torch.Tensor:
-        return self.tensors["k"]
+    def __post_init__(self):
+        # keys and values in 4 bits: codes and pairs travel together
+        self._packed = {name: ops.Int4Pages(self.tensors[name], self.tensors[f"{name}_pairs"]) for name in ("k", "v") if f"{name}_pairs" in self.tensors}
 
     @property
-    def v(self) -> torch.Tensor:
-        return self.tensors["v"]
+    def k(self):
+        return self._packed.get("k") or self.tensors["k"]
+
+    @property
+    def v(self):
+        return self._packed.get("v") or self.tensors["v"]
 
 
 class DeviceCache:
@@ -33,7 +39,8 @@ class DeviceCache:
         self.pools = []          # per group: {tensor name: [entry, page, head, slot, width]}
         for spec, entries, pages in zip(model.cache_groups, model.group_sizes, counts):
             self.pools.append({t.name: torch.zeros(entries, pages, t.heads, page_size, t.width,
-                                                   dtype=dtype, device=device) for t in spec.tensors})
+                                                   dtype=getattr(torch, t.dtype) if t.dtype else dtype, device=device)
+                               for t in spec.tensors})
         self.entries = [CacheEntry(info.group, {name: pool[info.index_in_group]
                                                 for name, pool in self.pools[info.group].items()})
                         for info in model.cache_entries]
@@ -42,7 +49,7 @@ class DeviceCache:
 
     @staticmethod
     def bytes_per_page(model, page_size: int, element_size: int) -> list:
-        return [n * spec.elements_per_token() * page_size * element_size
+        return [n * spec.bytes_per_token(element_size) * page_size
                 for spec, n in zip(model.cache_groups, model.group_sizes)]
 
     def zero_state(self, slots) -> None:

@@ -1,6 +1,6 @@
 """Engine options.  Names and meanings follow tinyserve's ``Config`` dataclass and
 its command line (serve.py:76-122, 3098-3142) where it has them; ``dtype``,
-``num_blocks`` and ``block_size`` are this engine's own."""
+``weight_dtype``, ``kv_cache_dtype``, ``num_blocks`` and ``block_size`` are this engine's own."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -9,6 +9,8 @@ from dataclasses import dataclass
 #: what ``check_indices`` is when an engine is configured without saying (tests switch it on)
 CHECK_INDICES_DEFAULT = False
 
+WEIGHT_DTYPES = ("auto", "int8")
+KV_CACHE_DTYPES = ("auto", "int4")
 DTYPE_NAMES = {"bfloat16": "bfloat16", "bf16": "bfloat16", "float32": "float32", "fp32": "float32"}
 
 
@@ -28,6 +30,11 @@ class EngineConfig:
     # debug pass: check every index buffer of every step on the host before it is uploaded, and
     # again on the device before the kernels run (the stand-in for a memory checker)
     check_indices: bool = None
+    # "auto": the matrices that only products read are held in ``dtype``; "int8": in 8-bit integers with a scale per output channel
+    # (the rows they meet are brought to 8 bits too, a scale per token)
+    weight_dtype: str = "auto"
+    # "auto": keys and values are cached in ``dtype``; "int4": in 4 bits with a scale and a zero per head of a token
+    kv_cache_dtype: str = "auto"
 
     def __post_init__(self):
         if self.check_indices is None:
@@ -35,6 +42,9 @@ class EngineConfig:
         if self.dtype not in DTYPE_NAMES:
             raise ValueError(f"dtype must be one of {sorted(DTYPE_NAMES)}, got {self.dtype!r}")
         self.dtype = DTYPE_NAMES[self.dtype]
+        for name, known in (("weight_dtype", WEIGHT_DTYPES), ("kv_cache_dtype", KV_CACHE_DTYPES)):
+            if getattr(self, name) not in known:
+                raise ValueError(f"{name} must be one of {list(known)}, got {getattr(self, name)!r}")
         if self.block_size == 0:
             # tinyserve's pages hold 16 tokens (serve.py:114-115).  Pages of 64 let the decode kernel
             # fetch whole pages by TMA and the prefill kernel walk fewer of them (measured on B200 at

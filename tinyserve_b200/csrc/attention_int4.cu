@@ -55,50 +55,41 @@ __device__ __forceinline__ void load8_any(const T* p, float (&x)[8], bool vec) {
   }
 }
 
-// LANES lanes bring one row (token, key or value, head) to its slot
-template <typename T>
-__global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams p, bool vec) {
-  pdl_trigger();
-  pdl_wait();
-  const long long row = (long long)blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES;
-  const int lane = threadIdx.x % LANES;
-  const bool live = row < 2LL * p.T * p.Hkv;
-  const int head = (int)(row % p.Hkv), which = (int)(row / p.Hkv & 1), t = live ? (int)(row / p.Hkv >> 1) : 0;
-  const T* src = which ? static_cast<const T*>(p.v) + t * p.v_row + head * p.v_head : static_cast<const T*>(p.k) + t * p.k_row + head * p.k_head;
-  float x[WORDS][8];
+// What the LANES lanes of a row have of it: minimum, maximum, anything that is not finite
+struct RowRange {
   float lo = INFINITY, hi = -INFINITY;
   int bad = 0;
+  __device__ __forceinline__ void add(const float (&x)[8]) {
 #pragma unroll
-  for (int w = 0; w < WORDS; ++w) {
-    const int word = lane + w * LANES;
-    if (live && word < W) {
-      load8_any<T>(src + word * 8, x[w], vec);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[w][i]);
-        hi = fmaxf(hi, x[w][i]);
-        bad |= !(fabsf(x[w][i]) <= 3.402823466e38f);
-      }
+    for (int i = 0; i < 8; ++i) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+      bad |= !(fabsf(x[i]) <= 3.402823466e38f);
     }
   }
+  __device__ __forceinline__ void join() {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    }
   }
-  if (!live) return;
+};
+
+// a row that its LANES lanes hold, to the slot of its token
+__device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)[WORDS][8], RowRange r, int which, int head, int t, int lane) {
   const int slot = p.slot_mapping[t];
   if (slot < 0) return;
   if (slot >= p.slots) {
     if (lane == 0) ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_CACHE_SLOT);
     return;
   }
-  const bf16 zero16 = __float2bfloat16_rn(lo);
+  const bf16 zero16 = __float2bfloat16_rn(r.lo);
   const float zero = __bfloat162float(zero16);
-  const bf16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, zero), 15.f));
+  const bf16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(r.hi, zero), 15.f));
   const float scale = __bfloat162float(scale16);
-  bad |= !(fabsf(scale) <= 3.402823466e38f) || !(fabsf(zero) <= 3.402823466e38f);
+  const bool bad = r.bad || !(fabsf(scale) <= 3.402823466e38f) || !(fabsf(zero) <= 3.402823466e38f);
   const size_t at = (((size_t)(slot >> p.page_shift) * p.Hkv + head) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
 #pragma unroll
   for (int w = 0; w < WORDS; ++w) {
@@ -118,6 +109,125 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams
     const uint32_t s = bad ? 0x7fc0u : (scale > 0.f ? __bfloat16_as_ushort(scale16) : 0u), z = bad ? 0x7fc0u : __bfloat16_as_ushort(zero16);
     (which ? p.vp : p.kp)[at] = s | z << 16;
   }
+}
+
+// LANES lanes bring one row (token, key or value, head) to its slot
+template <typename T>
+__global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams p, bool vec) {
+  pdl_trigger();
+  pdl_wait();
+  const long long row = (long long)blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES;
+  const bool live = row < 2LL * p.T * p.Hkv;
+  const int head = (int)(row % p.Hkv), which = (int)(row / p.Hkv & 1), t = live ? (int)(row / p.Hkv >> 1) : 0;
+  const T* src = which ? static_cast<const T*>(p.v) + t * p.v_row + head * p.v_head : static_cast<const T*>(p.k) + t * p.k_row + head * p.k_head;
+  float x[WORDS][8];
+  RowRange r;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int word = lane + w * LANES;
+    if (live && word < W) {
+      load8_any<T>(src + word * 8, x[w], vec);
+      r.add(x[w]);
+    }
+  }
+  r.join();
+  if (live) store_row(p, x, r, which, head, t, lane);
+}
+
+// The same behind a fused projection: qkv [T, (H + 2 Hkv) D] -> q [T, H, D] and the cache.  Heads of q and k are divided by their root
+// mean square (with weights; has_norm) and turned to their token's position; keys are rounded to T, as a cache
+// of T would hold them, and then brought to 4 bits.
+struct RopeParams {
+  const void* qkv;
+  void* q;
+  const int* positions;
+  const float *cos, *sin;                    // [positions, rot / 2]; null: no rotation
+  int rot, interleaved;
+  VecParam qw, kw;
+  int has_norm;
+  float eps;
+  int H;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteParams p, RopeParams rp, bool vec) {
+  __shared__ float stage[WRITE_THREADS / LANES][D];
+  pdl_trigger();
+  pdl_wait();
+  const int heads = rp.H + 2 * p.Hkv, lane = threadIdx.x % LANES;
+  const long long row = (long long)blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES;
+  const bool live = row < (long long)p.T * heads;
+  const int t = live ? (int)(row / heads) : 0, head = live ? (int)(row % heads) : 0;
+  const bool is_q = head < rp.H, is_v = head >= rp.H + p.Hkv;
+  const T* src = static_cast<const T*>(rp.qkv) + ((size_t)t * heads + head) * D;
+  float x[WORDS][8], sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int word = lane + w * LANES;
+    if (live && word < W) {
+      load8_any<T>(src + word * 8, x[w], vec);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[w][i], x[w][i], sum);
+    }
+  }
+  if (rp.has_norm) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float rstd = rsqrtf(sum / (float)D + rp.eps);
+    const VecParam wt = is_q ? rp.qw : rp.kw;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int word = lane + w * LANES;
+      if (live && !is_v && word < W) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[w][i] = x[w][i] * rstd * wt[word * 8 + i];
+      }
+    }
+  }
+  if (rp.cos != nullptr) {
+    float* mine = stage[threadIdx.x / LANES];
+    const int half = rp.rot >> 1;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int word = lane + w * LANES;
+      if (live && !is_v && word < W) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[word * 8 + i] = x[w][i];
+      }
+    }
+    __syncwarp();
+    const size_t angles = live && !is_v ? (size_t)rp.positions[t] * half : 0;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int word = lane + w * LANES;
+      if (live && !is_v && word < W) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int d = word * 8 + i;
+          if (d >= rp.rot) continue;
+          const int j = rp.interleaved ? d >> 1 : (d < half ? d : d - half);
+          const bool first = rp.interleaved ? (d & 1) == 0 : d < half;
+          const float mate = mine[rp.interleaved ? d ^ 1 : (first ? d + half : d - half)];
+          const float c = rp.cos[angles + j], s = rp.sin[angles + j];
+          x[w][i] = first ? x[w][i] * c - mate * s : x[w][i] * c + mate * s;
+        }
+      }
+    }
+  }
+  RowRange r;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int word = lane + w * LANES;
+    if (live && word < W) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[w][i] = to_f32<T>(from_f32<T>(x[w][i]));
+      r.add(x[w]);
+      if (is_q) store8<T>(static_cast<T*>(rp.q) + ((size_t)t * rp.H + head) * D + word * 8, x[w]);
+    }
+  }
+  r.join();
+  if (live && !is_q && p.slot_mapping != nullptr) store_row(p, x, r, is_v ? 1 : 0, is_v ? head - rp.H - p.Hkv : head - rp.H, t, lane);
 }
 
 // ------------------------------------------------------------------------------------------ attention
@@ -374,6 +484,30 @@ TS_EXPORT int ts_int4_kvwrite(int dtype, const void* k, const void* v, long long
   TS_REQUIRE(blocks < (1LL << 31), "int4_kvwrite: too many rows");
   if (dtype == TS_F32) TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<float>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, vec);
   else TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<bf16>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, vec);
+  return 0;
+}
+
+// qkv [T, (H + 2 Hkv) D] contiguous -> q [T, H, D] and, with a slot_mapping, the cache; see RopeParams.  rot 0: no rotation, q_weight null: no norm.
+TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const int* positions, const float* cos, const float* sin, int rot,
+                                   int interleaved, const void* q_weight, const void* k_weight, int weight_f32, float eps, int T, int H, int Hkv,
+                                   void* k_codes, void* k_pairs, void* v_codes, void* v_pairs, const int* slot_mapping, int page_size,
+                                   int num_pages, cudaStream_t stream) {
+  const int shift = shift_of_page(page_size);
+  TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_rope_kvwrite: unknown dtype %d", dtype);
+  TS_REQUIRE(T > 0 && H > 0 && Hkv > 0 && shift >= 0 && num_pages > 0, "int4_rope_kvwrite: %d tokens, %d and %d heads, pages of %d", T, H, Hkv, page_size);
+  TS_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0 && (rot == 0 || (cos && sin && positions)), "int4_rope_kvwrite: a rotation over %d of %d columns", rot, D);
+  TS_REQUIRE((q_weight == nullptr) == (k_weight == nullptr), "int4_rope_kvwrite: q and k norm weights come together");
+  TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 3) == 0 && ((uintptr_t)q & 15) == 0, "int4_rope_kvwrite: the cache or q is not aligned");
+  const bool vec = ((uintptr_t)qkv & 15) == 0;
+  WriteParams p = {};
+  p.kc = (uint32_t*)k_codes; p.vc = (uint32_t*)v_codes; p.kp = (uint32_t*)k_pairs; p.vp = (uint32_t*)v_pairs;
+  p.slot_mapping = slot_mapping; p.T = T; p.Hkv = Hkv; p.page_shift = shift; p.slots = (long long)num_pages << shift;
+  const RopeParams rp = {qkv, q, positions, rot ? cos : nullptr, sin, rot, interleaved, VecParam{q_weight, weight_f32}, VecParam{k_weight, weight_f32},
+                         q_weight != nullptr, eps, H};
+  const long long rows = (long long)T * (H + 2 * Hkv), per = WRITE_THREADS / LANES, blocks = (rows + per - 1) / per;
+  TS_REQUIRE(blocks < (1LL << 31), "int4_rope_kvwrite: too many rows");
+  if (dtype == TS_F32) TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<float>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, rp, vec);
+  else TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<bf16>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, rp, vec);
   return 0;
 }
 

@@ -1,6 +1,6 @@
 """Command line in tinyserve's manner: ``python -m tinyserve_b200 generate --model DIR
 --prompt "..."`` (serve.py:3098-3155).  Options that tinyserve has keep its names and
-meanings; ``--dtype``, ``--block-size``, ``--num-blocks``, ``--prompt-ids``, ``--ignore-eos``,
+meanings; ``--dtype``, ``--weight-dtype``, ``--kv-cache-dtype``, ``--block-size``, ``--num-blocks``, ``--prompt-ids``, ``--ignore-eos``,
 ``--top-p``, ``--top-k`` and the ``random-weights`` command are this engine's own.  The
 ``serve`` command (HTTP) is not part of this engine."""
 from __future__ import annotations
@@ -8,6 +8,8 @@ from __future__ import annotations
 import argparse
 import json
 import sys
+
+from ..config.engine_config import KV_CACHE_DTYPES, WEIGHT_DTYPES
 
 
 def _ids(text: str) -> list:
@@ -40,6 +42,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--no-cuda-graphs", action="store_true")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--weight-dtype", choices=WEIGHT_DTYPES, default="auto", help="int8: products in 8-bit integers, a scale per output channel and per token")
+    ap.add_argument("--kv-cache-dtype", choices=KV_CACHE_DTYPES, default="auto", help="int4: keys and values in 4 bits, a scale and a zero per head of a token")
     ap.add_argument("--block-size", type=int, default=0, help="tokens per cache page (0: 64 from 2,048 tokens of context on, else 16)")
     ap.add_argument("--num-blocks", type=int, default=0, help="cache pages per group (0: from memory)")
     # random-weights
@@ -74,7 +78,8 @@ def main(argv=None) -> int:
     llm = LLM(a.model, dtype=a.dtype, max_model_len=a.max_model_len, max_num_seqs=a.max_num_seqs,
               max_num_batched_tokens=a.max_num_batched_tokens,
               gpu_memory_utilization=a.gpu_memory_utilization, use_cuda_graphs=not a.no_cuda_graphs,
-              seed=a.seed, block_size=a.block_size, num_blocks=a.num_blocks, verbose=True)
+              seed=a.seed, block_size=a.block_size, num_blocks=a.num_blocks, weight_dtype=a.weight_dtype,
+              kv_cache_dtype=a.kv_cache_dtype, verbose=True)
     params = SamplingParams(temperature=a.temperature, top_p=a.top_p, top_k=a.top_k,
                             max_tokens=a.max_tokens, repetition_penalty=a.repetition_penalty,
                             repeat_last_n=a.repeat_last_n, ignore_eos=a.ignore_eos)

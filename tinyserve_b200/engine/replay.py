@@ -28,14 +28,16 @@ class TraceError(ValueError):
 
 
 def make_runner(model_dir: str, dtype: str, max_tokens: int, block_size: int = DEFAULT_PAGE_SIZE,
-                max_live: int = DEFAULT_MAX_LIVE, num_blocks: int = 0, use_cuda_graphs: bool = False):
+                max_live: int = DEFAULT_MAX_LIVE, num_blocks: int = 0, use_cuda_graphs: bool = False,
+                weight_dtype: str = "auto", kv_cache_dtype: str = "auto"):
     from ..config.engine_config import EngineConfig
     from .runner import ModelRunner
     unit = max(ROUND_TOKENS, block_size)
     capacity = -(-max_tokens // unit) * unit
     cfg = EngineConfig(model=model_dir, dtype=dtype, max_model_len=capacity, block_size=block_size,
                        max_num_seqs=max_live, max_num_batched_tokens=capacity,
-                       num_blocks=num_blocks or capacity // block_size, use_cuda_graphs=use_cuda_graphs)
+                       num_blocks=num_blocks or capacity // block_size, use_cuda_graphs=use_cuda_graphs,
+                       weight_dtype=weight_dtype, kv_cache_dtype=kv_cache_dtype)
     runner = ModelRunner(cfg)
     if use_cuda_graphs:
         runner.capture_decode_graphs()
@@ -95,6 +97,7 @@ def replay(runner, lines, out_dir: str, report=print) -> int:
 
 def main(argv=None) -> int:
     import argparse
+    from ..config.engine_config import KV_CACHE_DTYPES, WEIGHT_DTYPES
     ap = argparse.ArgumentParser(prog="trace_run", description=__doc__.split("\n\n")[0])
     ap.add_argument("--model", required=True, help="folder with config.json and model.safetensors")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
@@ -107,9 +110,11 @@ def main(argv=None) -> int:
                     help="cache pages per group (default: --max-tokens worth of pages)")
     ap.add_argument("--cuda-graphs", action="store_true",
                     help="replay captured graphs for steps of single tokens, as serving does")
+    ap.add_argument("--weight-dtype", choices=WEIGHT_DTYPES, default="auto")
+    ap.add_argument("--kv-cache-dtype", choices=KV_CACHE_DTYPES, default="auto")
     args = ap.parse_args(argv)
     runner = make_runner(args.model, args.dtype, args.max_tokens, args.block_size, args.max_live,
-                         args.num_blocks, args.cuda_graphs)
+                         args.num_blocks, args.cuda_graphs, args.weight_dtype, args.kv_cache_dtype)
 
     def report(msg):
         sys.stdout.write(msg + "\n")

@@ -67,11 +67,11 @@ class ModelRunner:
         self.device = torch.device(cfg.device)
         self.dtype = _TORCH_DTYPES[cfg.dtype]
         self.model_config = model_config or load_model_config(cfg.model)
-        self.model = build_model(self.model_config)
+        self.model = build_model(self.model_config, cfg.kv_cache_dtype)
         if random_weights:
-            self.weight_bytes = fill_random_on_device(self.model, self.dtype, self.device, cfg.seed)
+            self.weight_bytes = fill_random_on_device(self.model, self.dtype, self.device, cfg.seed, cfg.weight_dtype)
         else:
-            self.weight_bytes = load_weights(self.model, cfg.model, self.dtype, self.device)
+            self.weight_bytes = load_weights(self.model, cfg.model, self.dtype, self.device, cfg.weight_dtype)
         self.model.prepare(_Runtime(self.device, cfg.max_model_len, self.dtype))
         self.page_size = cfg.block_size
         self.max_blocks = -(-cfg.max_model_len // self.page_size)

@@ -889,7 +889,10 @@ def qk_norm_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rota
                          q_weight=None, k_weight=None, eps=0.0, k_cache=None, v_cache=None,
                          slot_mapping=None, page_size=0):
     """Per-head norm of q and k, rotary encoding, q to a [T, H, D] tensor (returned), k and v
-    to the cache slots of ``slot_mapping`` (None: nothing is written)."""
+    to the cache slots of ``slot_mapping`` (None: nothing is written).  The caches may be ``Int4Pages``."""
+    if isinstance(k_cache, Int4Pages) or isinstance(v_cache, Int4Pages):
+        return _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary, q_weight, k_weight, eps, k_cache, v_cache,
+                                  slot_mapping, page_size)
     parts, dtype = _NO_PARTIALS, qkv.dtype
     if isinstance(qkv, SplitPartials):
         if head_dim % 2:
@@ -1216,7 +1219,7 @@ def attention_from_qkv(qkv, positions, num_heads, num_kv_heads, head_dim, rotary
     H, Hkv, D = num_heads, num_kv_heads, head_dim
     plain = isinstance(qkv, torch.Tensor)
     # (up to FUSED_MAX_TOKENS requests: measured, at 64 the separate kernel is 4 % of the step faster)
-    fused = (fused and write_cache and dtype == torch.bfloat16 and ctx.max_q_len == 1
+    fused = (fused and write_cache and dtype == torch.bfloat16 and ctx.max_q_len == 1 and not isinstance(k_cache, Int4Pages)
              and qkv.shape[0] <= FUSED_MAX_TOKENS
              and D in SUPPORTED_HEAD_DIMS and D <= MMA_MAX_HEAD_DIM
              and rotary is not None and rotary.rotary_dim == D and not rotary.interleaved
@@ -2682,9 +2685,9 @@ class Int4Pages:
         if codes.dtype != torch.uint8 or codes.dim() != 4 or pairs.dtype != torch.bfloat16 or pairs.shape != codes.shape[:3] + (2,):
             raise TypeError("Int4Pages: codes are uint8 [pages, heads, slots, D / 2] and pairs bfloat16 [pages, heads, slots, 2], got "
                             f"{codes.dtype} {tuple(codes.shape)} and {pairs.dtype} {tuple(pairs.shape)}")
-        if not codes.is_contiguous() or not pairs.is_contiguous() or codes.data_ptr() % 16 or pairs.data_ptr() % 16:
-            raise ValueError("Int4Pages: codes and pairs are contiguous and begin on 16 bytes")
         pages, heads, slots, half = codes.shape
+        if not codes.is_contiguous() or not pairs.is_contiguous() or codes.data_ptr() % (4 if half % 16 else 16) or pairs.data_ptr() % 4:
+            raise ValueError("Int4Pages: codes and pairs are contiguous; codes begin on 16 bytes (on 4 where a row is no multiple of 16), pairs on 4")
         self.codes, self.pairs, self.shape = codes, pairs, (pages, heads, slots, 2 * half)
 
     @property
@@ -2728,6 +2731,37 @@ def int4_kvwrite(k, v, k_cache, v_cache, slot_mapping):
         c_longlong(v.stride(0)), c_longlong(v.stride(1)), c_int(T), c_int(heads), c_void_p(k_cache.codes.data_ptr()),
         c_void_p(k_cache.pairs.data_ptr()), c_void_p(v_cache.codes.data_ptr()), c_void_p(v_cache.pairs.data_ptr()),
         c_void_p(slot_mapping.data_ptr()), c_int(page), c_int(pages), _stream()))
+
+
+def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary, q_weight, k_weight, eps, k_cache, v_cache, slot_mapping, page_size):
+    what = "qk_norm_rope_kvwrite"
+    qkv = materialize(qkv)
+    H, Hkv, D = num_heads, num_kv_heads, head_dim
+    _int4_caches(what, k_cache, v_cache, page_size)
+    if k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+        raise TypeError(f"{what}: {Hkv} heads of {D} on a cache of {k_cache.shape[1]} heads of {k_cache.shape[3]}")
+    if qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hkv) * D or qkv.dtype not in _DTYPE or not qkv.is_contiguous():
+        raise ValueError("qkv must be [T, (H + 2 Hkv) * D], contiguous, float32 or bfloat16")
+    if (q_weight is None) != (k_weight is None) or (q_weight is not None and q_weight.dtype != k_weight.dtype):
+        raise TypeError("q and k norm weights come together and have one dtype")
+    T = qkv.shape[0]
+    if slot_mapping is not None:
+        _int32_row(what, slot_mapping, "slot_mapping", T)
+    if rotary is not None:
+        _int32_row(what, positions, "positions", T)
+    cos, sin = (rotary.cos, rotary.sin) if rotary is not None else (None, None)
+    _here(what, qkv, positions, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping, cos, sin, q_weight, k_weight)
+    q = torch.empty(T, H, D, dtype=qkv.dtype, device=qkv.device)
+    lib = _attention_int4(D)
+    if T == 0:
+        return q
+    _check(lib, lib.ts_int4_rope_kvwrite(
+        c_int(_DTYPE[qkv.dtype]), _ptr(qkv), _ptr(q), _ptr(positions), _ptr(cos), _ptr(sin), c_int(rotary.rotary_dim if rotary is not None else 0),
+        c_int(int(rotary.interleaved) if rotary is not None else 0), _ptr(q_weight), _ptr(k_weight),
+        c_int(_vec_flag(q_weight, qkv.dtype) if q_weight is not None else 0), c_float(eps), c_int(T), c_int(H), c_int(Hkv),
+        _ptr(k_cache.codes), _ptr(k_cache.pairs), _ptr(v_cache.codes), _ptr(v_cache.pairs), _ptr(slot_mapping), c_int(page_size),
+        c_int(k_cache.shape[0]), _stream()))
+    return q
 
 
 def int4_attention_splits(blocks, max_kv_len):

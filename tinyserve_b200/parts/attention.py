@@ -47,12 +47,14 @@ head's values; with lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + d (four learned v
 elements, one number per layer, made once in 32-bit) the head's output is
 o = a_1 - lambda a_2, divided by sqrt(mean(o^2) + e) over its value columns and multiplied by 1 - d.
 The attention kernels run it as 2 H query heads on 2 G key heads that read G value heads (key
-head i reads value head i / 2); ``ops.map_difference`` then combines the pairs."""
+head i reads value head i / 2); ``ops.map_difference`` then combines the pairs.
+
+``cache_bits`` = 4 (the plain form only): keys and values are kept in 4 bits (``ops.Int4Pages``)."""
 from __future__ import annotations
 
 from ..kernels import ops
 from .base import (CacheSpec, Mixer, ParamSpec, Source, StateSpec, build_norm, build_position_encoding,
-                   register_mixer)
+                   int4_cache_tensors, register_mixer)
 
 
 DEFAULT_NAMES = {"q": "q_proj", "k": "k_proj", "v": "v_proj", "o": "o_proj", "q_norm": "q_norm", "k_norm": "k_norm",
@@ -68,7 +70,7 @@ class Attention(Mixer):
                  position=None, window=0, scale=None, names=None, value_dim=None, unit_norm_eps=None,
                  head_gate=False, keep_first=0, joint_norm=False, norm_eps=0.0, chunk=0, distance_slopes=None,
                  sinks=False, out_gate=False, softcap=0.0, differential=None, conv_taps=0, query_factor=False,
-                 sink_score=None, value_rotation=None, borrows_kv=False, out_bias=False, tied_values=False):
+                 sink_score=None, value_rotation=None, borrows_kv=False, out_bias=False, tied_values=False, cache_bits=0):
         super().__init__()
         self.names = dict(DEFAULT_NAMES, **(names or {}))
         if num_heads % num_kv_heads:
@@ -132,6 +134,12 @@ class Attention(Mixer):
                              "gate come without a weighted per-head q/k norm")
         if self.joint_norm and self.unit_norm_eps is not None:
             raise ValueError("attention: the norm over all heads comes without the unit norm")
+        self.cache_bits = int(cache_bits or 0)
+        if self.cache_bits not in (0, 4):
+            raise ValueError(f"attention: a cache of the engine's element type (0) or of 4 bits, got {cache_bits}")
+        if self.cache_bits and self.general:
+            raise ValueError("attention: a 4-bit cache comes with the plain form only (per-head norm, rotation and a window; head sizes that "
+                             "are multiples of 16)")
         self.slopes = self.sinks = None
         widest = max(head_dim, self.value_dim)
         self.stored_dim = -(-widest // 16) * 16 if self.general else head_dim
@@ -166,8 +174,8 @@ class Attention(Mixer):
             rows += ((nm["gate"], q + kv + vs, q + kv + vs + self.gate_size),)
         specs = {
             "qkv_proj.weight": ParamSpec((q + kv + vs + self.gate_size, self.hidden_size), sources=tuple(
-                Source(f"{n}.weight", a, b) for n, a, b in rows)),
-            "o_proj.weight": ParamSpec((self.hidden_size, self.num_heads * self.value_dim),
+                Source(f"{n}.weight", a, b) for n, a, b in rows), int8=True),
+            "o_proj.weight": ParamSpec((self.hidden_size, self.num_heads * self.value_dim), int8=True,
                                        sources=(Source(f"{nm['o']}.weight", 0, self.hidden_size),)),
         }
         if self.bias:
@@ -229,6 +237,8 @@ class Attention(Mixer):
             tensors = (CacheTensor("k", self.num_kv_heads * self.maps, self.stored_dim), CacheTensor("v", self.num_kv_heads, self.stored_dim))
             return CacheSpec(kind, self.num_kv_heads * self.maps, self.stored_dim, self.window, tensors=tensors,
                              keep_first=self.keep_first)
+        if self.cache_bits:
+            return CacheSpec(kind, self.num_kv_heads, self.stored_dim, self.window, tensors=int4_cache_tensors(self.num_kv_heads, self.stored_dim))
         return CacheSpec(kind, self.num_kv_heads, self.stored_dim, self.window, keep_first=self.keep_first)
 
     def state_spec(self):
@@ -240,6 +250,7 @@ class Attention(Mixer):
         return self.chunk > 0 or self.slope_values is not None
 
     accepts_scaled_rows = True
+    takes_cache_bits = True
 
     def work_tile_queries(self, dtype, page_size):
         return ops.prefill_tile_queries(dtype, self.num_heads * self.maps, self.num_kv_heads * self.maps, self.stored_dim,

@@ -39,6 +39,8 @@ class ParamSpec:
     (default: one tensor of the same name and shape).  ``interleave_halves`` = b > 0: after the
     sources are placed, the rows of the first and the second half alternate in blocks of b rows
     (first-half rows [0, b), second-half rows [0, b), first-half rows [b, 2b), ...).
+    ``int8``: the matrix only ever goes to ``ops.linear`` and its kin as their weight, so that an engine
+    with 8-bit weights may bind it as ``ops.Int8Rows``.
     """
 
     shape: tuple
@@ -46,6 +48,7 @@ class ParamSpec:
     init: str = "normal"
     sources: tuple = ()
     interleave_halves: int = 0
+    int8: bool = False
 
 
 def interleave_halves(tensor, block: int):
@@ -60,11 +63,18 @@ def interleave_halves(tensor, block: int):
 
 @dataclass(frozen=True)
 class CacheTensor:
-    """One tensor that a mixer keeps per token: ``heads`` vectors of ``width`` elements."""
+    """One tensor that a mixer keeps per token: ``heads`` vectors of ``width`` elements, of the engine's
+    element type or of ``dtype``."""
 
     name: str
     heads: int
     width: int
+    dtype: str = ""
+
+    def bytes_per_token(self, element_size: int) -> int:
+        """``element_size``: of the engine's element type."""
+        size = {"": element_size, "uint8": 1, "bfloat16": 2, "float32": 4}[self.dtype]
+        return self.heads * self.width * size
 
 
 @dataclass(frozen=True)
@@ -91,6 +101,15 @@ class CacheSpec:
 
     def elements_per_token(self) -> int:
         return sum(t.heads * t.width for t in self.tensors)
+
+    def bytes_per_token(self, element_size: int) -> int:
+        return sum(t.bytes_per_token(element_size) for t in self.tensors)
+
+
+def int4_cache_tensors(num_kv_heads: int, head_dim: int) -> tuple:
+    """Keys and values in 4 bits (``kernels.ops.Int4Pages``): codes, two a byte, and a pair (scale, zero) per head."""
+    return tuple(t for name in ("k", "v") for t in (CacheTensor(name, num_kv_heads, head_dim // 2, "uint8"),
+                                                    CacheTensor(f"{name}_pairs", num_kv_heads, 2, "bfloat16")))
 
 
 @dataclass(frozen=True)
@@ -182,6 +201,8 @@ class PositionEncoding(Part):
 
 class Mixer(Part):
     tree_name = "mixer"
+    #: the mixer takes the parameter ``cache_bits`` (4: its cache is a pair of ``ops.Int4Pages``)
+    takes_cache_bits = False
     #: forward hands h to ops.linear only (never reads it itself), so h may be a ScaledRows
     accepts_scaled_rows = False
 

@@ -38,9 +38,9 @@ class GatedMLP(FeedForward):
         return {
             "gate_up_proj.weight": ParamSpec((2 * i, self.hidden_size), sources=(
                 Source(f"{nm['gate']}.weight", 0, i), Source(f"{nm['up']}.weight", i, 2 * i)),
-                interleave_halves=self.block),
+                interleave_halves=self.block, int8=True),
             "down_proj.weight": ParamSpec((self.hidden_size, i), sources=(
-                Source(f"{nm['down']}.weight", 0, self.hidden_size),)),
+                Source(f"{nm['down']}.weight", 0, self.hidden_size),), int8=True),
         }
 
     accepts_scaled_rows = True
@@ -67,9 +67,9 @@ class PolyNormMLP(FeedForward):
         i, n, nm = self.intermediate_size, self.hidden_size, self.names
         # (the biases and coefficients drawn so that losing one shows in the random-weights mode)
         return {
-            "up_proj.weight": ParamSpec((i, n), sources=(Source(f"{nm['up']}.weight", 0, i),)),
+            "up_proj.weight": ParamSpec((i, n), sources=(Source(f"{nm['up']}.weight", 0, i),), int8=True),
             "up_proj.bias": ParamSpec((i,), role="vector", init="around_zero", sources=(Source(f"{nm['up']}.bias", 0, i),)),
-            "down_proj.weight": ParamSpec((n, i), sources=(Source(f"{nm['down']}.weight", 0, n),)),
+            "down_proj.weight": ParamSpec((n, i), sources=(Source(f"{nm['down']}.weight", 0, n),), int8=True),
             "down_proj.bias": ParamSpec((n,), role="vector", init="around_zero", sources=(Source(f"{nm['down']}.bias", 0, n),)),
             "act": ParamSpec((4,), role="vector", init="wide", sources=(Source(nm["act"], 0, 4),)),
         }
@@ -102,8 +102,8 @@ class PlainMLP(FeedForward):
 
     def param_specs(self):
         i, n, nm = self.intermediate_size, self.hidden_size, self.names
-        return {"up_proj.weight": ParamSpec((i, n), sources=(Source(f"{nm['up']}.weight", 0, i),)),
-                "down_proj.weight": ParamSpec((n, i), sources=(Source(f"{nm['down']}.weight", 0, n),))}
+        return {"up_proj.weight": ParamSpec((i, n), sources=(Source(f"{nm['up']}.weight", 0, i),), int8=True),
+                "down_proj.weight": ParamSpec((n, i), sources=(Source(f"{nm['down']}.weight", 0, n),), int8=True)}
 
     def forward(self, h, ctx):
         return ops.linear(ops.activated_linear(h, self.w["up_proj.weight"], self.activation, constant_weight=True), self.w["down_proj.weight"],

@@ -6,11 +6,12 @@ residual add with the final norm; logits = hidden @ W.T with W the embedding tab
 through the final norm and the vocabulary projection, and logits are returned in 32-bit."""
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
-from ..config.model_config import ModelConfig, ModelSpec
+from ..config.model_config import ModelConfig, ModelSpec, PartSpec
 from ..kernels import ops
-from .base import CacheSpec, ParamSpec, Part, StateSpec, build_norm, build_position_encoding, build_stream_op
+from .base import (MIXERS, CacheSpec, ParamSpec, Part, StateSpec, build_mixer, build_norm, build_position_encoding,
+                   build_stream_op)
 from .block import add_and_norm, build_block
 
 
@@ -194,7 +195,28 @@ class DecoderModel(Part):
         return logits
 
 
-def build_model(config: ModelConfig) -> DecoderModel:
+def with_int4_cache(spec: ModelSpec) -> ModelSpec:
+    """``spec`` with every cache of keys and values in 4 bits.  All mixers that keep something per token have to be able to."""
+    layers = [replace(layer, mixer=PartSpec(layer.mixer.kind, dict(layer.mixer.params, cache_bits=4)))
+              if getattr(MIXERS.get(layer.mixer.kind), "takes_cache_bits", False) else layer for layer in spec.layers]
+    kept = 0
+    for i, layer in enumerate(layers):
+        try:
+            cache = build_mixer(layer.mixer).cache_spec()
+        except ValueError as e:
+            raise ValueError(f"layer {i} cannot keep its keys and values in 4 bits: {e}") from None
+        if cache is not None:
+            if not any(t.name == "k_pairs" for t in cache.tensors):
+                raise ValueError(f"layer {i} cannot keep its cache in 4 bits: the mixer {layer.mixer.kind!r} has no such form")
+            kept += 1
+    if not kept:
+        raise ValueError("no layer of the model keeps keys and values: there is no cache to hold in 4 bits")
+    return replace(spec, layers=tuple(layers))
+
+
+def build_model(config: ModelConfig, kv_cache_dtype: str = "auto") -> DecoderModel:
     """From an architecture's configuration to a model made of parts: the configuration names
-    the parts, layer by layer, and the run order; nothing else of it reaches the parts."""
-    return DecoderModel(config.model_spec())
+    the parts, layer by layer, and the run order; nothing else of it reaches the parts.
+    ``kv_cache_dtype`` "int4": keys and values are cached in 4 bits."""
+    spec = config.model_spec()
+    return DecoderModel(with_int4_cache(spec) if kv_cache_dtype == "int4" else spec)

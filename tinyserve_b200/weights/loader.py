@@ -22,6 +22,7 @@ from dataclasses import dataclass
 import torch
 from safetensors import safe_open
 
+from ..kernels import ops
 from ..parts.base import ParamSpec, Source, interleave_halves
 
 
@@ -127,8 +128,17 @@ def check_checkpoint(model, index, duplicates=()):
     return expected
 
 
-def load_weights(model, model_dir: str, dtype: torch.dtype, device) -> int:
-    """Fill every part of ``model`` from ``model_dir``; returns the bytes placed."""
+def held(spec: ParamSpec, tensor, weight_dtype: str):
+    """A parameter as the engine holds it: with ``weight_dtype`` "int8" the matrices that only products read are brought to 8
+    bits, row by row.  Returns (what the part binds, its bytes)."""
+    if weight_dtype == "int8" and spec.int8:
+        rows = ops.quantize_rows(tensor)
+        return rows, rows.codes.numel() + 4 * rows.scales.numel()
+    return tensor, tensor.numel() * tensor.element_size()
+
+
+def load_weights(model, model_dir: str, dtype: torch.dtype, device, weight_dtype: str = "auto") -> int:
+    """Fill every part of ``model`` from ``model_dir``; returns the bytes placed.  ``weight_dtype``: see ``held``."""
     index, duplicates = _index_folder(model_dir)
     expected = check_checkpoint(model, index, duplicates)
     by_param = {}
@@ -150,8 +160,9 @@ def load_weights(model, model_dir: str, dtype: torch.dtype, device) -> int:
                 dst.copy_(src.to(pdtype) if src.dtype != pdtype else src)
             if spec.interleave_halves:
                 param = interleave_halves(param, spec.interleave_halves).contiguous()
+            param, size = held(spec, param, weight_dtype)
             tensors.setdefault(id(part), (part, {}))[1][local] = param
-            total += param.numel() * param.element_size()
+            total += size
     finally:
         handles.clear()
     for part, bound in tensors.values():

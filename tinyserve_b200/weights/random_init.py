@@ -13,7 +13,7 @@ import os
 import torch
 from safetensors.torch import save_file
 
-from .loader import expected_tensors
+from .loader import expected_tensors, held
 
 _STORE = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
@@ -66,8 +66,8 @@ def write_random_model(config, out_dir: str, seed: int = 0, store_dtype: str = "
     return out_dir
 
 
-def fill_random_on_device(model, dtype: torch.dtype, device, seed: int = 0) -> int:
-    """Give every part of ``model`` random tensors made on ``device``; returns bytes."""
+def fill_random_on_device(model, dtype: torch.dtype, device, seed: int = 0, weight_dtype: str = "auto") -> int:
+    """Give every part of ``model`` random tensors made on ``device``; returns bytes.  ``weight_dtype``: as for ``load_weights``."""
     gen = torch.Generator(device=device)
     gen.manual_seed(int(seed))
     total = 0
@@ -78,7 +78,7 @@ def fill_random_on_device(model, dtype: torch.dtype, device, seed: int = 0) -> i
                 value = torch.zeros(spec.shape, dtype=torch.int32, device=device)
             else:
                 value = _draw(spec.init, spec.shape, gen, device).to(dtype)
-            bound[local] = value
-            total += value.numel() * value.element_size()
+            bound[local], size = held(spec, value, weight_dtype)
+            total += size
         part.bind(bound)
     return total
