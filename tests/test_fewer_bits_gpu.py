@@ -228,7 +228,7 @@ LENGTHS = {"one": [(1, 1)], "decode": [(1, 1), (1, 64), (1, 65), (1, 700)], "lon
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("H,Hkv,D,page", [(4, 4, 16, 8), (8, 2, 128, 64), (14, 2, 64, 16), (3, 3, 96, 1), (20, 1, 256, 32), (2, 1, 512, 16)])
+@pytest.mark.parametrize("H,Hkv,D,page", [(4, 4, 16, 8), (8, 2, 128, 64), (14, 2, 64, 16), (3, 3, 96, 1), (20, 1, 256, 32), (2, 1, 512, 16), (9, 1, 32, 64), (32, 8, 128, 16), (5, 1, 160, 64), (2, 1, 224, 16)])
 @pytest.mark.parametrize("name", sorted(LENGTHS))
 def test_attention(dtype, H, Hkv, D, page, name):
     from tinyserve_b200.kernels import ops
@@ -238,8 +238,9 @@ def test_attention(dtype, H, Hkv, D, page, name):
     sinks = torch.randn(H, device="cuda")
     for window, softcap, sink, splits in ((0, 0.0, None, None), (0, 0.0, None, 3), (50, 0.0, sinks, None), (1, 2.0, None, None), (100, 5.0, sinks, 12)):
         want, top, span = attention(q, lengths, ks, vs, D ** -0.5, window, softcap, sink)
-        out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, window, sinks=sink, softcap=softcap, num_splits=splits)
-        assert ((out.double() - want).abs() <= allowed(dtype, want, top, span, D, max(m for _, m in lengths))).all(), (window, softcap, splits)
+        for backend in {ops.int4_attention_backend(dtype, D), "simt"}:
+            out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, window, sinks=sink, softcap=softcap, num_splits=splits, backend=backend)
+            assert ((out.double() - want).abs() <= allowed(dtype, want, top, span, D, max(m for _, m in lengths))).all(), (window, softcap, splits, backend)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -450,6 +450,407 @@ __global__ void int4_combine_kernel(Int4Params p) {
   }
 }
 
+#if TS_HEAD_DIM % 32 == 0 && TS_HEAD_DIM <= 256
+#define TS_INT4_MMA 1
+// ------------------------------------------------------------------------------------------ attention on the tensor cores
+// bfloat16 queries.  A block is up to 8 NT columns = (query, head) pairs of one key head, and a range of its keys; every warp walks keys of its
+// own, 32 at a time, through a ring of shared memory that nobody else touches (cp.async, no barriers in the loop):
+//   S^T = K Q^T with the keys as the rows of m16n8k16, P^T brought to the next operand's layout by movmatrix, O^T += V^T P^T with the columns
+//   of the values as rows.  A code c enters the tensor core as the bfloat16 number 16 + c, which is one shift and one AND-OR for two
+//   codes (c in the upper mantissa bits under the exponent of 16): no conversion, no multiplication.  Scales and zeros are per
+//   key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.(16 + c)) + (z - 16 s) sum(q), and for values with p' = bfloat16(p s):
+//   sum p v = sum p' (16 + c) + sum (p z - 16 p'), the second a number per column that every column of the output gets.  (p' is rounded
+//   before both sums, so that the 16 cancels exactly.)
+// A thread's four rows of K (or V) in a group of 16 keys lie 4 keys apart, for loads without bank conflicts; keys are stored in the order
+// in which the rows of the MMA name them.
+constexpr int MMA_WARPS = 8, STEP = 32, RING = 3;
+constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
+constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;
+constexpr float FOUR = 16.f;                                       // what a code's bfloat16 is above it
+
+template <int NT> struct MmaCfg {
+  static constexpr int NC = 8 * NT;
+  static constexpr int Q_BYTES = (D / 16) * NT * 32 * 8;
+  static constexpr int RING_BYTES = MMA_WARPS * RING * STAGE_BYTES;
+  static constexpr int MERGE_BYTES = MMA_WARPS * NC * (D + 3) * 4;
+  static constexpr int SMEM = Q_BYTES + (RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES);
+  static constexpr bool Q_REGS = NT == 1 && D <= 128;              // the queries' operands stay in registers
+  static constexpr int BLOCKS = Q_REGS ? 2 : 1;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t b;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(b) : "r"(a));
+  return b;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// codes number e (0 .. 3) of both halves of a word as two bfloat16 numbers 16 + c
+template <int E>
+__device__ __forceinline__ uint32_t codes2(uint32_t word) {
+  const uint32_t moved = E == 0 ? word << 3 : word >> (4 * E - 3);
+  return (moved & 0x00780078u) | 0x41804180u;
+}
+// where key k (0 .. 15) of a group stands among the MMA's rows: thread t of a quad reads keys t, t + 4, t + 8, t + 12 as its rows
+// 2t, 2t + 1, 2t + 8, 2t + 9
+__device__ __forceinline__ int row_of_key(int k) { return (k & 8) | (k & 3) << 1 | (k >> 2 & 1); }
+__device__ __forceinline__ int key_of_row(int r) { return (r & 8) | (r >> 1 & 3) | (r & 1) << 2; }
+// 16-byte piece c of a value row stands here: rows whose reads meet are spread over the banks
+__device__ __forceinline__ int v_piece(int row, int c) {
+  if (D == 128) return c ^ (row >> 1 & 1) << 1;
+  if (D == 256) return c ^ (row & 3) << 1;
+  return c;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_kernel(Int4Params p) {
+  using C = MmaCfg<NT>;
+  extern __shared__ __align__(16) char smem[];
+  uint2* qf_s = reinterpret_cast<uint2*>(smem);                    // [D / 16][NT][32 lanes]
+  char* work = smem + C::Q_BYTES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_trigger();
+  pdl_wait();
+  const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
+  const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC, b = blockIdx.z;
+  const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
+  const int nc = min(C::NC, q_len * G - c0);                       // columns of this block
+  if (nc <= 0) return;
+  const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
+  const int pos0 = kv_len - q_len;                                 // position of the request's first query of this step
+  const int* bt = p.block_table + (size_t)b * p.table_stride;
+  const int first = pos0 + c0 / G, last = pos0 + (c0 + nc - 1) / G;
+  const int j_lo = p.window > 0 ? max(0, first - p.window + 1) : 0, j_hi = max(last + 1, 0);
+  const int step0 = j_lo / STEP, steps = max(0, (j_hi + STEP - 1) / STEP - step0), per = (steps + p.splits - 1) / p.splits;
+  const int s_end = min(steps, (split + 1) * per);
+
+  // the queries as B operands: row (query, head) c, columns 4 (s % 2) .. + 3 of word t KW + s / 2
+  for (int i = threadIdx.x; i < (D / 16) * NT * 32; i += MMA_WARPS * 32) {
+    const int l = i & 31, nt = (i >> 5) % NT, s = (i >> 5) / NT, c = nt * 8 + (l >> 2);
+    uint2 v = make_uint2(0u, 0u);
+    if (c < nc) {
+      const int r = c0 + c;
+      const bf16* src = static_cast<const bf16*>(p.q) + (q_begin + r / G) * p.q_row + (kvh * G + r % G) * p.q_head + ((l & 3) * KW + (s >> 1)) * 8 + 4 * (s & 1);
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+      if (((reinterpret_cast<uintptr_t>(src)) & 7) == 0) v = *reinterpret_cast<const uint2*>(src);
+      else v = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+    }
+    qf_s[i] = v;
+  }
+
+  char* ring = work + warp * RING * STAGE_BYTES;
+  auto fetch = [&](int s, int stage) {
+    char* at = ring + stage * STAGE_BYTES;
+    const int j0 = (step0 + s) * STEP;
+    const bool one_page = p.page_shift >= 5;
+    size_t base = 0;
+    if (one_page) base = cache_row(p, bt, kvh, j0);
+    auto row_at = [&](int r) { return one_page ? base + r : (j0 + r < j_hi ? cache_row(p, bt, kvh, j0 + r) : 0); };
+    constexpr int CH = ROW_BYTES / 16;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int idx = lane + 32 * i, r = idx / CH, c = idx % CH;
+      const bool valid = j0 + r < j_hi;
+      const size_t row = row_at(r);
+      cp_async16(smem_u32(at + ((r & 16) + row_of_key(r & 15)) * ROW_BYTES + c * 16), reinterpret_cast<const char*>(p.kc) + row * ROW_BYTES + c * 16, valid);
+      cp_async16(smem_u32(at + STEP * ROW_BYTES + r * ROW_BYTES + v_piece(r, c) * 16), reinterpret_cast<const char*>(p.vc) + row * ROW_BYTES + c * 16, valid);
+    }
+    const size_t row = row_at(lane);
+    cp_async4(smem_u32(at + 2 * STEP * ROW_BYTES + lane * 4), p.kp + row, j0 + lane < j_hi);
+    cp_async4(smem_u32(at + 2 * STEP * ROW_BYTES + STEP * 4 + lane * 4), p.vp + row, j0 + lane < j_hi);
+  };
+  const int mine = split * per + warp;
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) {
+    if (mine + i * MMA_WARPS < s_end) fetch(mine + i * MMA_WARPS, i);
+    asm volatile("cp.async.commit_group;\n" ::);
+  }
+  __syncthreads();
+  uint2 qf[C::Q_REGS ? D / 16 : 1];
+  float qsum[NT][2];                                               // of columns 2t and 2t + 1
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const uint2 v = qf_s[(s * NT + nt) * 32 + lane];
+      if (C::Q_REGS) qf[C::Q_REGS ? s : 0] = v;
+      sum += pair_scale(v.x) + pair_zero(v.x) + pair_scale(v.y) + pair_zero(v.y);       // (the halves of a word as numbers)
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    qsum[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+    qsum[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+  }
+  int pos[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = nt * 8 + 2 * t + i;
+      pos[nt][i] = c < nc ? pos0 + (c0 + c) / G : -1;
+    }
+  const int all_from = p.window > 0 ? max(0, last - p.window + 1) : 0;       // keys from here to `first` are seen by every column
+  const float scale2 = p.scale * LOG2E;
+
+  float o[D / 16][NT][4], m[NT][2], l[NT][2], z[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { m[nt][i] = -INFINITY; l[nt][i] = z[nt][i] = 0.f; }
+  }
+
+  int stage = 0;
+#pragma unroll 1
+  for (int s = mine; s < s_end; s += MMA_WARPS) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(RING - 2));
+    __syncwarp();
+    {
+      const int ahead = s + (RING - 1) * MMA_WARPS;
+      if (ahead < s_end) fetch(ahead, stage == 0 ? RING - 1 : stage - 1);
+      asm volatile("cp.async.commit_group;\n" ::);
+    }
+    const char* ks = ring + stage * STAGE_BYTES;
+    const char* vs = ks + STEP * ROW_BYTES;
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(vs + STEP * ROW_BYTES);
+    const uint32_t* vp = kp + STEP;
+    stage = stage == RING - 1 ? 0 : stage + 1;
+    const int j0 = (step0 + s) * STEP;
+
+    float sc[2][NT][4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[kb][nt][e] = 0.f;
+      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(ks + (kb * 16 + g) * ROW_BYTES) + t * KW;
+      const uint32_t* r1 = r0 + 8 * ROW_BYTES / 4;
+      uint32_t w0[KW], w1[KW];
+      if constexpr (KW % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < KW; i += 4) {
+          *reinterpret_cast<uint4*>(w0 + i) = *reinterpret_cast<const uint4*>(r0 + i);
+          *reinterpret_cast<uint4*>(w1 + i) = *reinterpret_cast<const uint4*>(r1 + i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KW; ++i) { w0[i] = r0[i]; w1[i] = r1[i]; }
+      }
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        const uint32_t a[2][4] = {{codes2<0>(w0[i]), codes2<0>(w1[i]), codes2<1>(w0[i]), codes2<1>(w1[i])},
+                                  {codes2<2>(w0[i]), codes2<2>(w1[i]), codes2<3>(w0[i]), codes2<3>(w1[i])}};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint2 q = C::Q_REGS ? qf[C::Q_REGS ? 2 * i + h : 0] : qf_s[((2 * i + h) * NT + nt) * 32 + lane];
+            mma_bf16(sc[kb][nt], a[h][0], a[h][1], a[h][2], a[h][3], q.x, q.y);
+          }
+      }
+    }
+    // scores; this thread's keys are those of rows g and g + 8 of both groups
+    const bool inner = j0 >= all_from && j0 + STEP - 1 <= first;
+    float vscale[2][2], vzero[2][2], top[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) top[nt][i] = m[nt][i];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = kb * 16 + key_of_row(g) + 8 * h;
+        const uint32_t kpair = kp[key], vpair = vp[key];
+        const float a = pair_scale(kpair) * scale2, bq = (pair_zero(kpair) - FOUR * pair_scale(kpair)) * scale2;
+        vscale[kb][h] = pair_scale(vpair);
+        vzero[kb][h] = pair_zero(vpair);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x = fmaf(a, sc[kb][nt][2 * h + i], bq * qsum[nt][i]);
+            if (p.softcap > 0.f) x = p.softcap * tanhf(x / (p.softcap * LOG2E)) * LOG2E;
+            if (!inner && (j0 + key > pos[nt][i] || (p.window > 0 && j0 + key <= pos[nt][i] - p.window))) x = -INFINITY;
+            sc[kb][nt][2 * h + i] = x;
+            top[nt][i] = fmaxf(top[nt][i], x);
+          }
+      }
+    bool moved = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
+        moved |= top[nt][i] > m[nt][i];
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float f = m[nt][i] == -INFINITY ? 0.f : ex2(m[nt][i] - top[nt][i]);
+          m[nt][i] = top[nt][i];
+          l[nt][i] *= f;
+          z[nt][i] *= f;
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= f; o[mt][nt][2 + i] *= f; }
+        }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float ps[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float x = sc[kb][nt][2 * h + i];
+            const bool seen = x != -INFINITY;                       // (a NaN stays)
+            const float pr = seen ? ex2(x - m[nt][i]) : 0.f;
+            l[nt][i] += pr;
+            ps[i] = seen ? pr * vscale[kb][h] : 0.f;
+            z[nt][i] += seen ? pr * vzero[kb][h] : 0.f;
+          }
+          const __nv_bfloat162 two = __floats2bfloat162_rn(ps[0], ps[1]);
+          const uint32_t bits = *reinterpret_cast<const uint32_t*>(&two);
+          z[nt][0] = fmaf(-FOUR, pair_scale(bits), z[nt][0]);
+          z[nt][1] = fmaf(-FOUR, pair_zero(bits), z[nt][1]);
+          pb[nt][h] = transposed(bits);
+        }
+      // values: 16-bit units g UNITS .. of keys t, t + 4, t + 8, t + 12 of the group
+      uint32_t u[4][(UNITS + 1) / 2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = kb * 16 + t + 4 * q;
+        const char* at = vs + row * ROW_BYTES;
+        if constexpr (UNITS == 4) {
+          const uint2 x = *reinterpret_cast<const uint2*>(at + v_piece(row, g >> 1) * 16 + (g & 1) * 8);
+          u[q][0] = x.x; u[q][1] = x.y;
+        } else if constexpr (UNITS == 8) {
+          const uint4 x = *reinterpret_cast<const uint4*>(at + v_piece(row, g) * 16);
+          u[q][0] = x.x; u[q][1] = x.y; u[q][2] = x.z; u[q][3] = x.w;
+        } else if constexpr (UNITS % 2 == 0) {
+#pragma unroll
+          for (int i = 0; i < UNITS / 2; ++i) u[q][i] = reinterpret_cast<const uint32_t*>(at)[g * (UNITS / 2) + i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < UNITS; ++i) {
+            const uint32_t x = reinterpret_cast<const uint16_t*>(at)[g * UNITS + i];
+            u[q][i / 2] = i % 2 ? u[q][i / 2] | x << 16 : x;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) {
+        const uint32_t x0 = __byte_perm(u[0][i / 2], u[1][i / 2], i % 2 ? 0x7632 : 0x5410), x1 = __byte_perm(u[2][i / 2], u[3][i / 2], i % 2 ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_bf16(o[2 * i][nt], codes2<0>(x0), codes2<1>(x0), codes2<0>(x1), codes2<1>(x1), pb[nt][0], pb[nt][1]);
+          mma_bf16(o[2 * i + 1][nt], codes2<2>(x0), codes2<3>(x0), codes2<2>(x1), codes2<3>(x1), pb[nt][0], pb[nt][1]);
+        }
+      }
+    }
+  }
+
+  // the warps' results meet in shared memory
+  asm volatile("cp.async.wait_group 0;\n" ::);
+  __syncthreads();
+  float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][D]
+  float* sm_ml = sm_o + MMA_WARPS * C::NC * D;                     // [warp][column][3]
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], d);
+        z[nt][i] += __shfl_xor_sync(0xffffffffu, z[nt][i], d);
+      }
+      const int c = nt * 8 + 2 * t + i;
+      if (g == 0) {
+        sm_ml[(warp * C::NC + c) * 3] = m[nt][i];
+        sm_ml[(warp * C::NC + c) * 3 + 1] = l[nt][i];
+        sm_ml[(warp * C::NC + c) * 3 + 2] = z[nt][i];
+      }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int unit = g * UNITS + u, d = 8 * (unit >> 1) + (unit & 1);
+        float* dst = sm_o + (warp * C::NC + c) * D + d;
+        dst[0] = o[2 * u][nt][i];
+        dst[2] = o[2 * u][nt][2 + i];
+        dst[4] = o[2 * u + 1][nt][i];
+        dst[6] = o[2 * u + 1][nt][2 + i];
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nc * D; i += MMA_WARPS * 32) {
+    const int c = i / D, d = i % D, r = c0 + c, head = kvh * G + r % G;
+    const size_t row = (size_t)(q_begin + r / G) * p.H + head;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < MMA_WARPS; ++w) top = fmaxf(top, sm_ml[(w * C::NC + c) * 3]);
+    const bool sink = p.splits == 1 && p.sinks != nullptr;
+    const float sink2 = sink ? p.sinks[head] * LOG2E : -INFINITY;
+    top = fmaxf(top, sink2);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, total = sink ? ex2(sink2 - base) : 0.f;
+#pragma unroll
+    for (int w = 0; w < MMA_WARPS; ++w) {
+      const float* ml = sm_ml + (w * C::NC + c) * 3;
+      const float f = ml[0] == -INFINITY ? 0.f : ex2(ml[0] - base);
+      total += (ml[1] == 0.f ? 0.f : f * ml[1]);
+      sum += f * (sm_o[(w * C::NC + c) * D + d] + ml[2]);
+    }
+    if (p.splits == 1) {
+      static_cast<bf16*>(p.out)[row * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : sum / total);
+    } else {
+      p.part_o[(row * p.splits + split) * D + d] = sum;
+      if (d == 0) {
+        p.part_ml[(row * p.splits + split) * 2] = top;
+        p.part_ml[(row * p.splits + split) * 2 + 1] = total;
+      }
+    }
+  }
+}
+
+template <int NT>
+int attend_mma(const Int4Params& p, int max_q_len, cudaStream_t stream) {
+  using C = MmaCfg<NT>;
+  const cudaError_t set = cudaFuncSetAttribute(int4_mma_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (set != cudaSuccess) return ts_fail("int4_attention: %s", cudaGetErrorString(set));
+  const int G = p.H / p.Hkv;
+  const long long tiles = ((long long)max_q_len * G + C::NC - 1) / C::NC * p.Hkv;
+  TS_REQUIRE(tiles <= 65535 && p.B <= 65535, "int4_attention: grid out of range");
+  TS_LAUNCH("int4_attention", int4_mma_kernel<NT>, dim3(p.splits, (unsigned)tiles, p.B), dim3(MMA_WARPS * 32), C::SMEM, stream, p);
+  if (p.splits > 1)
+    TS_LAUNCH("int4_attention (combine)", int4_combine_kernel<bf16>, dim3((unsigned)(p.T * p.H)), dim3(D < 128 ? D : 128), 0, stream, p);
+  return 0;
+}
+#endif
+
 int shift_of_page(int page_size) {
   for (int s = 0; s < 20; ++s)
     if (page_size == 1 << s) return s;
@@ -511,11 +912,13 @@ TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const in
   return 0;
 }
 
-// q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml.
+// q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
+// steps of 32 up to 256; 16 columns up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.
 TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
                                 const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
                                 int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
-                                int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, cudaStream_t stream) {
+                                int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, int max_q_len,
+                                int columns, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_attention: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
@@ -525,5 +928,15 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
   Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
                   block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
                   splits, part_o, part_ml};
+  if (columns > 0) {
+#ifdef TS_INT4_MMA
+    TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0, "int4_attention: the tensor-core kernel takes bfloat16 queries");
+    if (columns == 8) return attend_mma<1>(p, max_q_len, stream);
+#if TS_HEAD_DIM <= 128
+    if (columns == 16) return attend_mma<2>(p, max_q_len, stream);
+#endif
+#endif
+    return ts_fail("int4_attention: no tensor-core kernel for heads of %d and %d columns", D, columns);
+  }
   return dtype == TS_F32 ? attend_simt<float>(p, stream) : attend_simt<bf16>(p, stream);
 }

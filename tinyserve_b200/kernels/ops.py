@@ -2764,6 +2764,17 @@ def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary
     return q
 
 
+def int4_attention_backend(dtype, head_dim) -> str:
+    """Which kernel attends over a 4-bit cache: "mma" (tensor cores: bfloat16 heads in steps of 32 up to 256) or "simt"."""
+    return "mma" if dtype == torch.bfloat16 and head_dim % 32 == 0 and head_dim <= 256 else "simt"
+
+
+def int4_decode_splits(blocks, max_kv_len):
+    """Key ranges of the tensor-core kernel over a 4-bit cache: two blocks an SM; a range has a step of 32 keys for each of its
+    eight warps."""
+    return max(1, min(2 * num_sms() // blocks, -(-max_kv_len // 256), 32))
+
+
 def int4_attention_splits(blocks, max_kv_len):
     """Key ranges of the 32-bit kernel over a 4-bit cache: four blocks an SM, two tiles of 128 keys a range at least."""
     return max(1, min(-(-4 * num_sms() // blocks), max_kv_len // 256, 32))
@@ -2789,16 +2800,25 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         raise TypeError(f"{what}: the block table is int32 [requests, blocks], rows contiguous, got {table.dtype} {tuple(table.shape)}")
     _int32_row(what, ctx.cu_q, "cu_q", B + 1)
     _int32_row(what, ctx.kv_lens, "kv_lens", B)
-    if backend not in (None, "simt"):
+    chosen = int4_attention_backend(q.dtype, D)
+    if backend not in (None, chosen, "simt"):
         raise ValueError(f"attention backend {backend!r} does not take {q.dtype}, head size {D} and a 4-bit cache")
+    chosen = backend or chosen
     _here(what, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, table, ctx.cu_q, ctx.kv_lens, sinks)
     out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
     lib = _attention_int4(D)
     if T == 0 or B == 0:
         return out
     span = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
+    columns = 0
+    if chosen == "mma":
+        rows = ctx.max_q_len * (H // Hkv)
+        columns = 16 if rows > 8 and D <= 128 else 8
+        if -(-rows // columns) * Hkv > 65535 or B > 65535:
+            columns = 0
     if num_splits is None:
-        num_splits = int4_attention_splits(T * Hkv * -(-(H // Hkv) // 8), span)
+        num_splits = (int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else
+                      int4_attention_splits(T * Hkv * -(-(H // Hkv) // 8), span))
     part_o = part_ml = None
     if num_splits > 1:
         part_o = torch.empty(T * H * num_splits * D, dtype=torch.float32, device=q.device)
@@ -2808,5 +2828,6 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         c_void_p(k_cache.codes.data_ptr()), c_void_p(k_cache.pairs.data_ptr()), c_void_p(v_cache.codes.data_ptr()),
         c_void_p(v_cache.pairs.data_ptr()), c_void_p(table.data_ptr()), c_void_p(ctx.cu_q.data_ptr()), c_void_p(ctx.kv_lens.data_ptr()),
         c_int(T), c_int(B), c_int(H), c_int(Hkv), c_int(page), c_int(table.shape[1]), c_int(table.stride(0)), c_int(pages), c_float(scale),
-        c_int(window), c_float(softcap), _ptr(sinks), c_int(num_splits), _ptr(part_o), _ptr(part_ml), _stream()), 1 if num_splits == 1 else 2)
+        c_int(window), c_float(softcap), _ptr(sinks), c_int(num_splits), _ptr(part_o), _ptr(part_ml), c_int(ctx.max_q_len),
+        c_int(columns), _stream()), 1 if num_splits == 1 else 2)
     return out
