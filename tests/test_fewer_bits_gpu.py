@@ -261,21 +261,24 @@ def test_rows_without_keys_and_behind_the_last(dtype):
     assert ops.paged_attention(q[:0], kc, vc, view, ctx, 0.125).shape == (0, 4, 64)
 
 
-def test_non_finite_rows_reach_who_sees_them():
+@pytest.mark.parametrize("H", [8, 6, 2])
+@pytest.mark.parametrize("window", [0, 2])
+def test_non_finite_rows_reach_who_sees_them(H, window):
     from tinyserve_b200.kernels import ops
     lengths = [(3, 90), (1, 5)]
     ctx, view, kc, vc, ks, vs = batch(lengths, 2, 128, 16, torch.bfloat16)
-    q = torch.randn(4, 8, 128, device="cuda").bfloat16()
-    clean = ops.paged_attention(q, kc, vc, view, ctx, 0.1)
+    q = torch.randn(4, H, 128, device="cuda").bfloat16()
+    clean = ops.paged_attention(q, kc, vc, view, ctx, 0.1, window)
     j = 88                                     # the last query but one sees it, the first does not
     page = int(view.block_table[0, j // 16])
     for c in (kc, vc):
         keep = c.pairs.clone()
         c.pairs[page, 1, j % 16] = math.nan
-        out = ops.paged_attention(q, kc, vc, view, ctx, 0.1)
+        out = ops.paged_attention(q, kc, vc, view, ctx, 0.1, window)
         c.pairs.copy_(keep)
-        assert torch.equal(out[0], clean[0]) and torch.equal(out[3], clean[3]) and torch.equal(out[:, :4], clean[:, :4])
-        assert out[1:3, 4:].isnan().all()
+        assert torch.equal(out[0], clean[0]) and torch.equal(out[3], clean[3]) and torch.equal(out[:, :H // 2], clean[:, :H // 2])
+        assert out[1:3, H // 2:].isnan().all()
+    assert ops.int4_attention_error(128) == 0
 
 
 def test_pages_outside_the_pool_are_reported():

@@ -10,7 +10,7 @@
 // One shift and one AND-OR then make a pair of neighbouring columns as two bfloat16 (see `codes2` in the kernels below).
 // Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
 // a token for heads of 128 where bfloat16 takes 256.
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 #ifndef TS_HEAD_DIM
 #error "compile with -DTS_HEAD_DIM=<head size, a multiple of 16 up to 512>"
@@ -97,10 +97,15 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
     if (word >= W) continue;
     uint32_t bits = 0;
     if (!bad && scale > 0.f) {
+      // the quotient rounded to 32 bits decides; the product with the reciprocal is off by 3 roundings of at most 16, so a division is
+      // only made next to a half, and where the reciprocal could overflow
+      const float inverse = 1.f / scale;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[w][i], zero), scale)), 0.f), 15.f);
-        bits |= (uint32_t)c << shift_of(i);
+        const float y = __fsub_rn(x[w][i], zero);
+        float r = y * inverse;
+        if (fabsf(fabsf(r - rintf(r)) - 0.5f) < 1e-4f || !(scale > 1e-30f)) r = __fdiv_rn(y, scale);
+        bits |= (uint32_t)fminf(fmaxf(rintf(r), 0.f), 15.f) << shift_of(i);
       }
     }
     (which ? p.vc : p.kc)[at * W + word] = bits;
@@ -454,19 +459,17 @@ __global__ void int4_combine_kernel(Int4Params p) {
 #define TS_INT4_MMA 1
 // ------------------------------------------------------------------------------------------ attention on the tensor cores
 // bfloat16 queries.  A block is up to 8 NT columns = (query, head) pairs of one key head, and a range of its keys; every warp walks keys of its
-// own, 32 at a time, through a ring of shared memory that nobody else touches (cp.async, no barriers in the loop):
+// own, 32 at a time, through a ring of shared memory that nobody else touches (bulk copies by runs of a page, no block barriers in the loop):
 //   S^T = K Q^T with the keys as the rows of m16n8k16, P^T brought to the next operand's layout by movmatrix, O^T += V^T P^T with the columns
 //   of the values as rows.  A code c enters the tensor core as the bfloat16 number 16 + c, which is one shift and one AND-OR for two
 //   codes (c in the upper mantissa bits under the exponent of 16): no conversion, no multiplication.  Scales and zeros are per
 //   key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.(16 + c)) + (z - 16 s) sum(q), and for values with p' = bfloat16(p s):
 //   sum p v = sum p' (16 + c) + sum (p z - 16 p'), the second a number per column that every column of the output gets.  (p' is rounded
 //   before both sums, so that the 16 cancels exactly.)
-// A thread's four rows of K (or V) in a group of 16 keys lie 4 keys apart, for loads without bank conflicts; keys are stored in the order
-// in which the rows of the MMA name them.
 constexpr int MMA_WARPS = 8, STEP = 32, RING = 3;
 constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
-constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;
-constexpr float FOUR = 16.f;                                       // what a code's bfloat16 is above it
+constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;   // codes of K and V, pairs of K and V
+constexpr float ABOVE = 16.f;                                      // what a code's bfloat16 is above it
 
 template <int NT> struct MmaCfg {
   static constexpr int NC = 8 * NT;
@@ -478,12 +481,9 @@ template <int NT> struct MmaCfg {
   static constexpr int BLOCKS = Q_REGS ? 2 : 1;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+// bytes (a multiple of 16) of global memory to shared memory, counted by a barrier
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -503,26 +503,31 @@ __device__ __forceinline__ float ex2(float x) {
 template <int E>
 __device__ __forceinline__ uint32_t codes2(uint32_t word) {
   const uint32_t moved = E == 0 ? word << 3 : word >> (4 * E - 3);
-  return (moved & 0x00780078u) | 0x41804180u;
+  uint32_t two;
+  // (written out: the compiler makes two instructions of an AND and an OR with constants, and these pipes bound the kernel)
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(two) : "r"(moved), "r"(0x00780078u), "r"(0x41804180u));
+  return two;
 }
-// where key k (0 .. 15) of a group stands among the MMA's rows: thread t of a quad reads keys t, t + 4, t + 8, t + 12 as its rows
-// 2t, 2t + 1, 2t + 8, 2t + 9
-__device__ __forceinline__ int row_of_key(int k) { return (k & 8) | (k & 3) << 1 | (k >> 2 & 1); }
+// Where a running maximum starts: below every score, and finite, so that nothing subtracts infinities.  It moves only when a score passes it by
+// more than SLACK (a power of two): probabilities up to 2^SLACK do no harm in 32-bit sums, and most steps then rescale nothing.
+constexpr float LOWEST = -3e38f, SLACK = 8.f;
+// Row r of the 16 that an MMA reads of K is this key of the group: thread t of a quad then finds its columns of V^T (rows 2t, 2t + 1, 2t + 8,
+// 2t + 9) in keys t, t + 4, t + 8, t + 12, and the eight lanes whose reads of K meet read neighbouring keys' halves of a bank line
 __device__ __forceinline__ int key_of_row(int r) { return (r & 8) | (r >> 1 & 3) | (r & 1) << 2; }
-// 16-byte piece c of a value row stands here: rows whose reads meet are spread over the banks
-__device__ __forceinline__ int v_piece(int row, int c) {
-  if (D == 128) return c ^ (row >> 1 & 1) << 1;
-  if (D == 256) return c ^ (row & 3) << 1;
-  return c;
-}
 
 template <int NT>
 __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_kernel(Int4Params p) {
   using C = MmaCfg<NT>;
   extern __shared__ __align__(16) char smem[];
+  __shared__ uint64_t full[MMA_WARPS][RING];
+  __shared__ volatile int abort_flag;
   uint2* qf_s = reinterpret_cast<uint2*>(smem);                    // [D / 16][NT][32 lanes]
   char* work = smem + C::Q_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (lane < RING) mbar_init(smem_u32(&full[warp][lane]), 1);
+  if (threadIdx.x == 0) abort_flag = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  __syncthreads();
   pdl_trigger();
   pdl_wait();
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
@@ -538,6 +543,31 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   const int step0 = j_lo / STEP, steps = max(0, (j_hi + STEP - 1) / STEP - step0), per = (steps + p.splits - 1) / p.splits;
   const int s_end = min(steps, (split + 1) * per);
 
+  char* ring = work + warp * RING * STAGE_BYTES;
+  // A step's 32 keys lie in whole or in runs of a page; every run is four copies (codes and pairs of K and V) by a lane of its own.  A run
+  // that starts behind the last key is not fetched, and what its place holds is masked.
+  const int run_shift = min(p.page_shift, 5), runs = STEP >> run_shift, run_keys = 1 << run_shift;
+  auto fetch = [&](int s, int stage) {
+    const int j = (step0 + s) * STEP + (lane << run_shift);
+    const bool mine = lane < runs && j < j_hi;
+    const uint32_t bar = smem_u32(&full[warp][stage]);
+    const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
+    if (lane == 0) mbar_expect_tx(bar, n * (STAGE_BYTES >> (5 - run_shift)));
+    __syncwarp();
+    if (mine) {
+      const size_t row = cache_row(p, bt, kvh, j);
+      const uint32_t at = smem_u32(ring) + stage * STAGE_BYTES, code_bytes = ROW_BYTES << run_shift, first_row = lane << run_shift;
+      bulk_copy(at + first_row * ROW_BYTES, reinterpret_cast<const char*>(p.kc) + row * ROW_BYTES, code_bytes, bar);
+      bulk_copy(at + (STEP + first_row) * ROW_BYTES, reinterpret_cast<const char*>(p.vc) + row * ROW_BYTES, code_bytes, bar);
+      bulk_copy(at + 2 * STEP * ROW_BYTES + first_row * 4, p.kp + row, run_keys * 4, bar);
+      bulk_copy(at + 2 * STEP * ROW_BYTES + (STEP + first_row) * 4, p.vp + row, run_keys * 4, bar);
+    }
+  };
+  const int mine = split * per + warp;
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i)
+    if (mine + i * MMA_WARPS < s_end) fetch(mine + i * MMA_WARPS, i);
+
   // the queries as B operands: row (query, head) c, columns 4 (s % 2) .. + 3 of word t KW + s / 2
   for (int i = threadIdx.x; i < (D / 16) * NT * 32; i += MMA_WARPS * 32) {
     const int l = i & 31, nt = (i >> 5) % NT, s = (i >> 5) / NT, c = nt * 8 + (l >> 2);
@@ -550,34 +580,6 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       else v = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
     }
     qf_s[i] = v;
-  }
-
-  char* ring = work + warp * RING * STAGE_BYTES;
-  auto fetch = [&](int s, int stage) {
-    char* at = ring + stage * STAGE_BYTES;
-    const int j0 = (step0 + s) * STEP;
-    const bool one_page = p.page_shift >= 5;
-    size_t base = 0;
-    if (one_page) base = cache_row(p, bt, kvh, j0);
-    auto row_at = [&](int r) { return one_page ? base + r : (j0 + r < j_hi ? cache_row(p, bt, kvh, j0 + r) : 0); };
-    constexpr int CH = ROW_BYTES / 16;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int idx = lane + 32 * i, r = idx / CH, c = idx % CH;
-      const bool valid = j0 + r < j_hi;
-      const size_t row = row_at(r);
-      cp_async16(smem_u32(at + ((r & 16) + row_of_key(r & 15)) * ROW_BYTES + c * 16), reinterpret_cast<const char*>(p.kc) + row * ROW_BYTES + c * 16, valid);
-      cp_async16(smem_u32(at + STEP * ROW_BYTES + r * ROW_BYTES + v_piece(r, c) * 16), reinterpret_cast<const char*>(p.vc) + row * ROW_BYTES + c * 16, valid);
-    }
-    const size_t row = row_at(lane);
-    cp_async4(smem_u32(at + 2 * STEP * ROW_BYTES + lane * 4), p.kp + row, j0 + lane < j_hi);
-    cp_async4(smem_u32(at + 2 * STEP * ROW_BYTES + STEP * 4 + lane * 4), p.vp + row, j0 + lane < j_hi);
-  };
-  const int mine = split * per + warp;
-#pragma unroll
-  for (int i = 0; i < RING - 1; ++i) {
-    if (mine + i * MMA_WARPS < s_end) fetch(mine + i * MMA_WARPS, i);
-    asm volatile("cp.async.commit_group;\n" ::);
   }
   __syncthreads();
   uint2 qf[C::Q_REGS ? D / 16 : 1];
@@ -615,34 +617,31 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) { m[nt][i] = -INFINITY; l[nt][i] = z[nt][i] = 0.f; }
+    for (int i = 0; i < 2; ++i) { m[nt][i] = LOWEST; l[nt][i] = z[nt][i] = 0.f; }
   }
 
-  int stage = 0;
+  int stage = 0, waits = 0;
+  bool ok = true;
 #pragma unroll 1
   for (int s = mine; s < s_end; s += MMA_WARPS) {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(RING - 2));
-    __syncwarp();
+    ok = mbar_wait(smem_u32(&full[warp][stage]), waits & 1, &abort_flag);
+    ok = __all_sync(0xffffffffu, ok);          // (and everybody has read what the stage before this one held)
+    if (!ok) break;
     {
       const int ahead = s + (RING - 1) * MMA_WARPS;
       if (ahead < s_end) fetch(ahead, stage == 0 ? RING - 1 : stage - 1);
-      asm volatile("cp.async.commit_group;\n" ::);
     }
     const char* ks = ring + stage * STAGE_BYTES;
     const char* vs = ks + STEP * ROW_BYTES;
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(vs + STEP * ROW_BYTES);
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(vs + STEP * ROW_BYTES) + key_of_row(g);
     const uint32_t* vp = kp + STEP;
-    stage = stage == RING - 1 ? 0 : stage + 1;
+    if (stage == RING - 1) { stage = 0; ++waits; } else ++stage;
     const int j0 = (step0 + s) * STEP;
 
     float sc[2][NT][4];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[kb][nt][e] = 0.f;
-      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(ks + (kb * 16 + g) * ROW_BYTES) + t * KW;
+      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(ks + (kb * 16 + key_of_row(g)) * ROW_BYTES) + t * KW;
       const uint32_t* r1 = r0 + 8 * ROW_BYTES / 4;
       uint32_t w0[KW], w1[KW];
       if constexpr (KW % 4 == 0) {
@@ -651,10 +650,24 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
           *reinterpret_cast<uint4*>(w0 + i) = *reinterpret_cast<const uint4*>(r0 + i);
           *reinterpret_cast<uint4*>(w1 + i) = *reinterpret_cast<const uint4*>(r1 + i);
         }
+      } else if constexpr (KW % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < KW; i += 2) {
+          *reinterpret_cast<uint2*>(w0 + i) = *reinterpret_cast<const uint2*>(r0 + i);
+          *reinterpret_cast<uint2*>(w1 + i) = *reinterpret_cast<const uint2*>(r1 + i);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < KW; ++i) { w0[i] = r0[i]; w1[i] = r1[i]; }
       }
+      // two chains of MMAs, added up: half the latency
+      float half[2][NT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) half[h][nt][e] = 0.f;
 #pragma unroll
       for (int i = 0; i < KW; ++i) {
         const uint32_t a[2][4] = {{codes2<0>(w0[i]), codes2<0>(w1[i]), codes2<1>(w0[i]), codes2<1>(w1[i])},
@@ -664,53 +677,76 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const uint2 q = C::Q_REGS ? qf[C::Q_REGS ? 2 * i + h : 0] : qf_s[((2 * i + h) * NT + nt) * 32 + lane];
-            mma_bf16(sc[kb][nt], a[h][0], a[h][1], a[h][2], a[h][3], q.x, q.y);
+            mma_bf16(half[h][nt], a[h][0], a[h][1], a[h][2], a[h][3], q.x, q.y);
           }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[kb][nt][e] = half[0][nt][e] + half[1][nt][e];
     }
     // scores; this thread's keys are those of rows g and g + 8 of both groups
-    const bool inner = j0 >= all_from && j0 + STEP - 1 <= first;
     float vscale[2][2], vzero[2][2], top[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) top[nt][i] = m[nt][i];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int key = kb * 16 + key_of_row(g) + 8 * h;
-        const uint32_t kpair = kp[key], vpair = vp[key];
-        const float a = pair_scale(kpair) * scale2, bq = (pair_zero(kpair) - FOUR * pair_scale(kpair)) * scale2;
+        const uint32_t kpair = kp[kb * 16 + 8 * h], vpair = vp[kb * 16 + 8 * h];
+        const float a = pair_scale(kpair) * scale2, bq = fmaf(-ABOVE, a, pair_zero(kpair) * scale2);
         vscale[kb][h] = pair_scale(vpair);
         vzero[kb][h] = pair_zero(vpair);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float x = fmaf(a, sc[kb][nt][2 * h + i], bq * qsum[nt][i]);
-            if (p.softcap > 0.f) x = p.softcap * tanhf(x / (p.softcap * LOG2E)) * LOG2E;
-            if (!inner && (j0 + key > pos[nt][i] || (p.window > 0 && j0 + key <= pos[nt][i] - p.window))) x = -INFINITY;
-            sc[kb][nt][2 * h + i] = x;
-            top[nt][i] = fmaxf(top[nt][i], x);
-          }
+          for (int i = 0; i < 2; ++i) sc[kb][nt][2 * h + i] = fmaf(a, sc[kb][nt][2 * h + i], bq * qsum[nt][i]);
       }
+    if (p.softcap > 0.f) {
+      const float in = 1.f / (p.softcap * LOG2E), out = p.softcap * LOG2E;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[kb][nt][e] = out * tanhf(sc[kb][nt][e] * in);
+    }
+    if (j0 < all_from || j0 + STEP - 1 > first) {
+      // the ends of somebody's range: hidden keys have no score, and nothing of their values
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = j0 + kb * 16 + key_of_row(g) + 8 * h;
+          // a probability of 0 must not meet a NaN, of a slot that is not this request's or of a key that only some columns see:
+          // the pair becomes 0, and who sees the key gets the NaN through its score
+          const bool finite = fabsf(vscale[kb][h]) <= 3.402823466e38f && fabsf(vzero[kb][h]) <= 3.402823466e38f;
+          if (!finite) vscale[kb][h] = vzero[kb][h] = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const bool hidden = j > pos[nt][i] || (p.window > 0 && j <= pos[nt][i] - p.window);
+              if (hidden) sc[kb][nt][2 * h + i] = -INFINITY;
+              else if (!finite) sc[kb][nt][2 * h + i] = __int_as_float(0x7fc00000);
+            }
+        }
+    }
     bool moved = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
-        moved |= top[nt][i] > m[nt][i];
+        top[nt][i] = fmaxf(fmaxf(sc[0][nt][i], sc[0][nt][2 + i]), fmaxf(sc[1][nt][i], sc[1][nt][2 + i]));
+        moved |= top[nt][i] > m[nt][i] + SLACK;
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float f = m[nt][i] == -INFINITY ? 0.f : ex2(m[nt][i] - top[nt][i]);
-          m[nt][i] = top[nt][i];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
+          const float above = fmaxf(top[nt][i], m[nt][i]), f = ex2(m[nt][i] - above);
+          m[nt][i] = above;
           l[nt][i] *= f;
           z[nt][i] *= f;
 #pragma unroll
@@ -724,34 +760,30 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float ps[2];
+          float pr[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float x = sc[kb][nt][2 * h + i];
-            const bool seen = x != -INFINITY;                       // (a NaN stays)
-            const float pr = seen ? ex2(x - m[nt][i]) : 0.f;
-            l[nt][i] += pr;
-            ps[i] = seen ? pr * vscale[kb][h] : 0.f;
-            z[nt][i] += seen ? pr * vzero[kb][h] : 0.f;
+            pr[i] = ex2(sc[kb][nt][2 * h + i] - m[nt][i]);
+            l[nt][i] += pr[i];
+            z[nt][i] = fmaf(pr[i], vzero[kb][h], z[nt][i]);
           }
-          const __nv_bfloat162 two = __floats2bfloat162_rn(ps[0], ps[1]);
+          const __nv_bfloat162 two = __floats2bfloat162_rn(pr[0] * vscale[kb][h], pr[1] * vscale[kb][h]);
           const uint32_t bits = *reinterpret_cast<const uint32_t*>(&two);
-          z[nt][0] = fmaf(-FOUR, pair_scale(bits), z[nt][0]);
-          z[nt][1] = fmaf(-FOUR, pair_zero(bits), z[nt][1]);
+          z[nt][0] = fmaf(-ABOVE, pair_scale(bits), z[nt][0]);
+          z[nt][1] = fmaf(-ABOVE, pair_zero(bits), z[nt][1]);
           pb[nt][h] = transposed(bits);
         }
       // values: 16-bit units g UNITS .. of keys t, t + 4, t + 8, t + 12 of the group
       uint32_t u[4][(UNITS + 1) / 2];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int row = kb * 16 + t + 4 * q;
-        const char* at = vs + row * ROW_BYTES;
-        if constexpr (UNITS == 4) {
-          const uint2 x = *reinterpret_cast<const uint2*>(at + v_piece(row, g >> 1) * 16 + (g & 1) * 8);
-          u[q][0] = x.x; u[q][1] = x.y;
-        } else if constexpr (UNITS == 8) {
-          const uint4 x = *reinterpret_cast<const uint4*>(at + v_piece(row, g) * 16);
+        const char* at = vs + (kb * 16 + t + 4 * q) * ROW_BYTES;
+        if constexpr (UNITS % 8 == 0) {
+          const uint4 x = reinterpret_cast<const uint4*>(at)[g];
           u[q][0] = x.x; u[q][1] = x.y; u[q][2] = x.z; u[q][3] = x.w;
+        } else if constexpr (UNITS % 4 == 0) {
+          const uint2 x = reinterpret_cast<const uint2*>(at)[g];
+          u[q][0] = x.x; u[q][1] = x.y;
         } else if constexpr (UNITS % 2 == 0) {
 #pragma unroll
           for (int i = 0; i < UNITS / 2; ++i) u[q][i] = reinterpret_cast<const uint32_t*>(at)[g * (UNITS / 2) + i];
@@ -774,9 +806,14 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       }
     }
   }
+  if (!ok) {
+    // a wait ran out: the copies that may still be in flight land before their memory is used again or given up
+    for (int i = 0; i < RING; ++i)
+      for (int parity = 0; parity < 2; ++parity)
+        for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(smem_u32(&full[warp][i]), parity); ++w) {}
+  }
 
   // the warps' results meet in shared memory
-  asm volatile("cp.async.wait_group 0;\n" ::);
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][D]
   float* sm_ml = sm_o + MMA_WARPS * C::NC * D;                     // [warp][column][3]
@@ -809,19 +846,17 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   for (int i = threadIdx.x; i < nc * D; i += MMA_WARPS * 32) {
     const int c = i / D, d = i % D, r = c0 + c, head = kvh * G + r % G;
     const size_t row = (size_t)(q_begin + r / G) * p.H + head;
-    float top = -INFINITY;
+    const bool sink = p.splits == 1 && p.sinks != nullptr;
+    const float sink2 = sink ? p.sinks[head] * LOG2E : LOWEST;
+    float top = fmaxf(LOWEST, sink2);
 #pragma unroll
     for (int w = 0; w < MMA_WARPS; ++w) top = fmaxf(top, sm_ml[(w * C::NC + c) * 3]);
-    const bool sink = p.splits == 1 && p.sinks != nullptr;
-    const float sink2 = sink ? p.sinks[head] * LOG2E : -INFINITY;
-    top = fmaxf(top, sink2);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, total = sink ? ex2(sink2 - base) : 0.f;
+    float sum = 0.f, total = sink ? ex2(sink2 - top) : 0.f;
 #pragma unroll
     for (int w = 0; w < MMA_WARPS; ++w) {
       const float* ml = sm_ml + (w * C::NC + c) * 3;
-      const float f = ml[0] == -INFINITY ? 0.f : ex2(ml[0] - base);
-      total += (ml[1] == 0.f ? 0.f : f * ml[1]);
+      const float f = ex2(ml[0] - top);
+      total += f * ml[1];
       sum += f * (sm_o[(w * C::NC + c) * D + d] + ml[2]);
     }
     if (p.splits == 1) {
@@ -839,8 +874,9 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 template <int NT>
 int attend_mma(const Int4Params& p, int max_q_len, cudaStream_t stream) {
   using C = MmaCfg<NT>;
-  const cudaError_t set = cudaFuncSetAttribute(int4_mma_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (set != cudaSuccess) return ts_fail("int4_attention: %s", cudaGetErrorString(set));
+  static SmemSet set;
+  const cudaError_t sized = set.to(int4_mma_kernel<NT>, C::SMEM);
+  if (sized != cudaSuccess) return ts_fail("int4_attention: %s", cudaGetErrorString(sized));
   const int G = p.H / p.Hkv;
   const long long tiles = ((long long)max_q_len * G + C::NC - 1) / C::NC * p.Hkv;
   TS_REQUIRE(tiles <= 65535 && p.B <= 65535, "int4_attention: grid out of range");
@@ -868,6 +904,15 @@ int attend_simt(const Int4Params& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+#ifdef TS_INT4_MMA
+// 1 if a block ever gave up on a wait since the library was loaded (reads device memory: syncs)
+TS_EXPORT int ts_int4_attention_error() {
+  int flag = 0;
+  if (cudaMemcpyFromSymbol(&flag, g_error_flag, sizeof(int)) != cudaSuccess) return -1;
+  return flag;
+}
+#endif
 
 // k, v [T, Hkv, D] (strides in elements, columns contiguous) to the slots of slot_mapping [T] (< 0: skipped; slots are distinct)
 TS_EXPORT int ts_int4_kvwrite(int dtype, const void* k, const void* v, long long k_row, long long k_head, long long v_row, long long v_head,
@@ -930,7 +975,8 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
                   splits, part_o, part_ml};
   if (columns > 0) {
 #ifdef TS_INT4_MMA
-    TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0, "int4_attention: the tensor-core kernel takes bfloat16 queries");
+    TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");
+    TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 15) == 0, "int4_attention: the tensor-core kernel copies runs that begin on 16 bytes");
     if (columns == 8) return attend_mma<1>(p, max_q_len, stream);
 #if TS_HEAD_DIM <= 128
     if (columns == 16) return attend_mma<2>(p, max_q_len, stream);

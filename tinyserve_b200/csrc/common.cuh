@@ -179,6 +179,20 @@ static inline cudaError_t ts_launch_cluster(void (*kernel)(KArgs...), dim3 grid,
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// A kernel's dynamic shared memory, set once per device (the call takes a third of a microsecond, as long as a small launch's other
+// preparations together)
+struct SmemSet {
+  unsigned long long done = 0;
+  template <typename K> cudaError_t to(K kernel, int bytes) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && (done >> device & 1))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device < 64) done |= 1ull << device;
+    return e;
+  }
+};
+
 // distributed shared memory of a cluster: rank, barrier, and a load from a peer block's copy of
 // a shared variable
 __device__ __forceinline__ uint32_t cluster_rank() {

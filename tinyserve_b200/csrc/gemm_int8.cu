@@ -19,7 +19,9 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------ rows to 8 bits
-constexpr int QUANT_THREADS = 256;
+// A row's block has up to 512 threads of eight neighbouring elements a step; up to four steps stay in registers between the search
+// for the largest magnitude and the codes (longer rows are read twice, the second time from the caches).
+constexpr int QUANT_THREADS = 512, QUANT_KEPT = 4;
 
 struct QuantParams {
   const void* x;        // [M, K], leading dimension ldx
@@ -29,15 +31,20 @@ struct QuantParams {
   int K;
 };
 
-__device__ __forceinline__ int code_of(float x, float scale) {
-  return (int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f);
+// round(x / scale) of the quotient rounded to 32 bits.  x times the reciprocal is off by three roundings of at most 127, 2.3e-5: a
+// division is only made where that could matter, next to a half (2 in 10,000), and where the reciprocal could overflow.
+__device__ __forceinline__ int code_of(float x, float scale, float inverse) {
+  float r = x * inverse;
+  if (fabsf(fabsf(r - rintf(r)) - 0.5f) < 1e-4f || !(scale > 1e-30f)) r = __fdiv_rn(x, scale);
+  return (int)fminf(fmaxf(rintf(r), -127.f), 127.f);
 }
 
-// a block a row: the largest magnitude, then the codes (the second read comes from the caches)
-template <typename T>
+// a block a row; KEPT: steps that stay in registers (0: the row is read twice)
+template <typename T, int KEPT>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParams p, bool vec) {
   __shared__ float tops[QUANT_THREADS / 32];
   __shared__ int bads[QUANT_THREADS / 32];
+  const int threads = blockDim.x;
   // The trigger comes behind the wait: what the kernel after this one reads before its own wait (the codes of the weights) is
   // then complete, whoever wrote it.
   pdl_wait();
@@ -48,16 +55,28 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParam
   const int n8 = vec ? p.K / 8 : 0;
   float top = 0.f;
   int bad = 0;
-  for (int i = threadIdx.x; i < n8; i += QUANT_THREADS) {
-    float v[8];
-    load8<T>(x + i * 8, v);
+  float kept[KEPT > 0 ? KEPT : 1][8];
+  auto look = [&](const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       top = fmaxf(top, fabsf(v[e]));
       bad |= !(fabsf(v[e]) <= 3.402823466e38f);
     }
+  };
+  if constexpr (KEPT > 0) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+      if (threadIdx.x + k * threads < n8) load8<T>(x + (threadIdx.x + k * threads) * 8, kept[k]);
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+      if (threadIdx.x + k * threads < n8) look(kept[k]);
+  } else {
+    for (int i = threadIdx.x; i < n8; i += threads) {
+      load8<T>(x + i * 8, kept[0]);
+      look(kept[0]);
+    }
   }
-  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += QUANT_THREADS) {
+  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += threads) {
     const float v = to_f32<T>(x[i]);
     top = fmaxf(top, fabsf(v));
     bad |= !(fabsf(v) <= 3.402823466e38f);
@@ -66,23 +85,31 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParam
   bad = __any_sync(0xffffffffu, bad);
   if ((threadIdx.x & 31) == 0) { tops[threadIdx.x >> 5] = top; bads[threadIdx.x >> 5] = bad; }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < QUANT_THREADS / 32; ++w) { top = fmaxf(top, tops[w]); bad |= bads[w]; }
+  for (int w = 0; w < threads / 32; ++w) { top = fmaxf(top, tops[w]); bad |= bads[w]; }
   const float scale = __fdiv_rn(top, 127.f);
   const bool zero = bad || !(scale > 0.f);
   if (threadIdx.x == 0) p.scales[m] = bad ? __int_as_float(0x7fc00000) : scale;
-  for (int i = threadIdx.x; i < n8; i += QUANT_THREADS) {
-    float v[8];
-    load8<T>(x + i * 8, v);
+  const float inverse = 1.f / scale;
+  auto write = [&](const float (&v)[8], int i) {
     uint32_t w[2] = {0u, 0u};
     if (!zero) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(code_of(v[e], scale) & 255) << (8 * (e & 3));
+      for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(code_of(v[e], scale, inverse) & 255) << (8 * (e & 3));
     }
     *reinterpret_cast<uint2*>(out + i * 8) = make_uint2(w[0], w[1]);
+  };
+  if constexpr (KEPT > 0) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+      if (threadIdx.x + k * threads < n8) write(kept[k], threadIdx.x + k * threads);
+  } else {
+    for (int i = threadIdx.x; i < n8; i += threads) {
+      load8<T>(x + i * 8, kept[0]);
+      write(kept[0], i);
+    }
   }
-  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += QUANT_THREADS)
-    out[i] = zero ? 0 : (signed char)code_of(to_f32<T>(x[i]), scale);
+  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += threads)
+    out[i] = zero ? 0 : (signed char)code_of(to_f32<T>(x[i]), scale, inverse);
 }
 
 // ------------------------------------------------------------------------------------------ the product
@@ -144,7 +171,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int n_tile = blockIdx.x, t_tile = blockIdx.y, split = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int kb_total = (p.K + BK - 1) / BK, per = (kb_total + p.splits - 1) / p.splits;
   const int kb0 = split * per, nkb = max(0, min(kb_total, kb0 + per) - kb0);
 
@@ -289,8 +316,9 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, long long K, l
 
 template <int TILE_T>
 int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p, cudaStream_t stream) {
-  const cudaError_t set = cudaFuncSetAttribute(gemm_i8_kernel<TILE_T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<TILE_T>::SMEM);
-  if (set != cudaSuccess) return ts_fail("gemm_int8: %s", cudaGetErrorString(set));
+  static SmemSet set;
+  const cudaError_t sized = set.to(gemm_i8_kernel<TILE_T>, (int)Cfg<TILE_T>::SMEM);
+  if (sized != cudaSuccess) return ts_fail("gemm_int8: %s", cudaGetErrorString(sized));
   const dim3 grid((p.N + TILE_N - 1) / TILE_N, (p.M + TILE_T - 1) / TILE_T, p.splits);
   const cudaError_t e = ts_launch_cluster(gemm_i8_kernel<TILE_T>, grid, dim3(THREADS), Cfg<TILE_T>::SMEM, stream, dim3(1, 1, p.splits), map_w, map_x, p);
   if (e != cudaSuccess) return ts_fail("gemm_int8 (clusters of %d): %s", p.splits, cudaGetErrorString(e));
@@ -299,13 +327,20 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p
 
 int tile_tokens(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
 
+template <typename T>
+int launch_quantize(const QuantParams& p, bool vec, int M, cudaStream_t stream) {
+  const int n8 = (p.K + 7) / 8, threads = n8 >= QUANT_THREADS ? QUANT_THREADS : (n8 + 31) / 32 * 32;
+  if (!vec || n8 > QUANT_KEPT * threads) TS_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 0>), dim3(M), dim3(vec ? threads : QUANT_THREADS), 0, stream, p, vec);
+  else if (n8 <= threads) TS_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 1>), dim3(M), dim3(threads), 0, stream, p, vec);
+  else TS_LAUNCH("quantize_rows", (quantize_rows_kernel<T, QUANT_KEPT>), dim3(M), dim3(threads), 0, stream, p, vec);
+  return 0;
+}
+
 int quantize(int dtype, const void* x, long long ldx, void* codes, long long ldq, float* scales, int M, int K, cudaStream_t stream) {
   const int e = dtype == TS_F32 ? 4 : 2;
   const bool vec = (((uintptr_t)x | (uintptr_t)(ldx * e)) & 15) == 0 && (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
   const QuantParams p = {x, static_cast<signed char*>(codes), scales, ldx, ldq, K};
-  if (dtype == TS_F32) TS_LAUNCH("quantize_rows", quantize_rows_kernel<float>, dim3(M), dim3(QUANT_THREADS), 0, stream, p, vec);
-  else TS_LAUNCH("quantize_rows", quantize_rows_kernel<bf16>, dim3(M), dim3(QUANT_THREADS), 0, stream, p, vec);
-  return 0;
+  return dtype == TS_F32 ? launch_quantize<float>(p, vec, M, stream) : launch_quantize<bf16>(p, vec, M, stream);
 }
 
 }  // namespace

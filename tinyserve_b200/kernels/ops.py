@@ -2565,21 +2565,67 @@ def delta_rule(q, k, v, gate, logits, bias, rate, state, ctx, num_heads, key_dim
 
 
 # ----------------------------------------------------------------------------- fewer bits
+# (A decoded token's launches take a few microseconds each: the checks below ask a tensor for as little as they need, and the
+# entry points are looked up once, with their argument types.)
+_INT, _LONG, _PTR, _FLOAT = c_int, c_longlong, c_void_p, c_float
+_INT8_ENTRIES = {
+    "ts_quantize_rows": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _INT, _INT, _PTR),
+    "ts_gemm_int8": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _PTR, _LONG, _PTR, _PTR, _INT, _PTR, _LONG, _INT, _INT, _INT, _INT, _INT, _INT, _PTR),
+}
+_INT4_ENTRIES = {
+    "ts_int4_kvwrite": (_INT, _PTR, _PTR, _LONG, _LONG, _LONG, _LONG, _INT, _INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR),
+    "ts_int4_rope_kvwrite": (_INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR, _PTR, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR,
+                             _PTR, _INT, _INT, _PTR),
+    "ts_int4_attention": (_INT, _PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
+                          _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR, _PTR, _INT, _INT, _PTR),
+}
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(unit, name):
+    """(library, entry point) of the 8-bit products (``unit`` 0) or of a head size over a 4-bit cache."""
+    lib = _gemm_int8() if unit == 0 else _attention_int4(unit)
+    fn = getattr(lib, name)
+    fn.argtypes = (_INT8_ENTRIES if unit == 0 else _INT4_ENTRIES)[name]
+    return lib, fn
+
+
+def _here(what, *tensors):
+    """Operands lie on the current device: the launch goes to its current stream, which is returned."""
+    here = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            if not t.is_cuda:
+                raise RuntimeError("kernel operands must be CUDA tensors: there is no CPU path")
+            raise RuntimeError(f"{what}: an operand lies on {t.device}, the current device is cuda:{here}")
+    if here < 0:
+        raise RuntimeError("kernel operands must be CUDA tensors: there is no CPU path")
+    return _STREAM.value if _STREAM is not None else torch._C._cuda_getCurrentRawStream(here)
+
+
+def _launched(lib, code, n):
+    if code != 0:
+        raise RuntimeError(lib.ts_last_error().decode())
+    count_launches(n)
+
+
 class Int8Rows:
     """Rows of a matrix in 8 bits: ``codes`` int8 [R, K] (rows that begin on 16 bytes: a leading dimension that is a multiple
     of 16) and ``scales`` float32 [R]; row r stands for codes[r] * scales[r].  ``quantize_rows`` makes them, for the weights of a
     product as for its tokens: scale = max |row| / 127, code = round(row / scale), halves to even, both in 32 bits."""
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("codes", "scales", "shape", "stride")
     dtype = torch.int8
 
     def __init__(self, codes, scales):
-        if codes.dtype != torch.int8 or codes.dim() != 2 or scales.dtype != torch.float32 or scales.shape != codes.shape[:1]:
+        shape = tuple(codes.shape)
+        if codes.dtype != torch.int8 or len(shape) != 2 or scales.dtype != torch.float32 or tuple(scales.shape) != shape[:1]:
             raise TypeError("Int8Rows: codes are int8 [R, K] and scales float32 [R], got "
-                            f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
-        if (codes.shape[1] > 1 and codes.stride(1) != 1) or codes.stride(0) % 16 or codes.data_ptr() % 16 or not scales.is_contiguous():
+                            f"{codes.dtype} {shape} and {scales.dtype} {tuple(scales.shape)}")
+        row, column = codes.stride()
+        if (shape[1] > 1 and column != 1) or row % 16 or (shape[0] > 1 and row < shape[1]) or codes.data_ptr() % 16 or not scales.is_contiguous():
             raise ValueError("Int8Rows: a row of codes lies in one run that begins on 16 bytes (a leading dimension that is a "
-                             "multiple of 16), and the scales are contiguous")
-        self.codes, self.scales, self.shape = codes, scales, tuple(codes.shape)
+                             "multiple of 16), rows do not overlap, and the scales are contiguous")
+        self.codes, self.scales, self.shape, self.stride = codes, scales, shape, row
 
     @property
     def device(self):
@@ -2594,38 +2640,32 @@ class Int8Rows:
 INT8_MAX_K = 131072
 
 
-def _here(what, *tensors):
-    """Operands lie on the current device: the launch goes to its current stream."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != here):
-            if not t.is_cuda:
-                raise RuntimeError("kernel operands must be CUDA tensors: there is no CPU path")
-            raise RuntimeError(f"{what}: an operand lies on {t.device}, the current device is cuda:{here}")
-
-
 def _quantizable(x, what):
-    if x.dim() != 2 or x.dtype not in _DTYPE:
-        raise TypeError(f"{what}: rows are float32 or bfloat16 [R, K], got {x.dtype} {tuple(x.shape)}")
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    """(rows, K, leading dimension) of an operand that can be brought to 8 bits."""
+    shape = x.shape
+    if len(shape) != 2 or x.dtype not in _DTYPE:
+        raise TypeError(f"{what}: rows are float32 or bfloat16 [R, K], got {x.dtype} {tuple(shape)}")
+    M, K = shape
+    row, column = x.stride()
+    if K > 1 and column != 1:
         raise ValueError(f"{what}: a row lies in one run (stride 1 along K), got strides {x.stride()}")
-    if not 0 < x.shape[1] <= INT8_MAX_K:
-        raise ValueError(f"{what}: K is 1 to {INT8_MAX_K} (sums of products of 8-bit numbers in 32 bits), got {x.shape[1]}")
+    if not 0 < K <= INT8_MAX_K:
+        raise ValueError(f"{what}: K is 1 to {INT8_MAX_K} (sums of products of 8-bit numbers in 32 bits), got {K}")
+    return M, K, row
 
 
 def quantize_rows(x) -> Int8Rows:
     """The rows of x (float32 or bfloat16 [R, K], rows contiguous) in 8 bits.  A row of zeros has scale 0; one that holds an infinity or a NaN
     has scale NaN."""
     x = materialize(x)
-    _quantizable(x, "quantize_rows")
-    _here("quantize_rows", x)
-    M, K = x.shape
-    codes = torch.empty(M, -(-K // 16) * 16, dtype=torch.int8, device=x.device)[:, :K]
+    M, K, ldx = _quantizable(x, "quantize_rows")
+    stream = _here("quantize_rows", x)
+    ld = -(-K // 16) * 16
+    codes = torch.empty(M, ld, dtype=torch.int8, device=x.device)[:, :K]
     scales = torch.empty(M, dtype=torch.float32, device=x.device)
     if M:
-        lib = _gemm_int8()
-        _check(lib, lib.ts_quantize_rows(c_int(_dt(x)), _ptr(x), c_longlong(x.stride(0)), _ptr(codes), c_longlong(codes.stride(0)), _ptr(scales),
-                                         c_int(M), c_int(K), _stream()))
+        lib, fn = _entry(0, "ts_quantize_rows")
+        _launched(lib, fn(_DTYPE[x.dtype], x.data_ptr(), ldx, codes.data_ptr(), ld, scales.data_ptr(), M, K, stream), 1)
     return Int8Rows(codes, scales)
 
 
@@ -2644,34 +2684,38 @@ def _linear_int8(x, weight, bias, out_float32, constant_weight):
         raise TypeError("linear: rows in 8 bits need a weight in 8 bits (quantize_rows)")
     N, K = weight.shape
     given = isinstance(x, Int8Rows)
-    if not given:
-        x = materialize(x)
-        _quantizable(x, "linear")
-    if x.shape[1] != K:
-        raise ValueError(f"linear: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    if given:
+        (M, xk), xt, dtype, rows = x.shape, -1, torch.bfloat16, x.codes
+        if not 0 < K <= INT8_MAX_K:
+            raise ValueError(f"linear: K is 1 to {INT8_MAX_K}, got {K}")
+    else:
+        rows = materialize(x)
+        M, xk, ldx = _quantizable(rows, "linear")
+        dtype = rows.dtype
+        xt = _DTYPE[dtype]
+    if xk != K:
+        raise ValueError(f"linear: x {(M, xk)} does not fit weight {weight.shape}")
     if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in _DTYPE or not bias.is_contiguous()):
         raise ValueError(f"linear: bias {bias.dtype} {tuple(bias.shape)} does not fit {N} outputs (float32 or bfloat16, contiguous)")
-    M = x.shape[0]
-    device = weight.codes.device
-    dtype = torch.float32 if out_float32 else torch.bfloat16 if given else x.dtype
-    _here("linear", x.codes if given else x, weight.codes, weight.scales, x.scales if given else None, bias)
-    out = torch.empty(M, N, dtype=dtype, device=device)
+    if out_float32:
+        dtype = torch.float32
+    codes, scales = weight.codes, weight.scales
+    stream = _here("linear", rows, codes, scales, bias, x.scales if given else None)
+    out = torch.empty(M, N, dtype=dtype, device=codes.device)
     if M == 0 or N == 0:
         return out
     if given:
-        cx, ldcx, sx = c_void_p(x.codes.data_ptr()), x.codes.stride(0), c_void_p(x.scales.data_ptr())
-        xp, ldx, xt = c_void_p(0), 0, -1
+        xp = ldx = 0
+        cx, ldcx, sx = rows.data_ptr(), x.stride, x.scales.data_ptr()
     else:
         ldcx = -(-K // 16) * 16
-        scratch = torch.empty(M * (ldcx + 4), dtype=torch.uint8, device=device)
-        cx, sx = c_void_p(scratch.data_ptr()), c_void_p(scratch.data_ptr() + M * ldcx)
-        xp, ldx, xt = c_void_p(x.data_ptr()), x.stride(0), _DTYPE[x.dtype]
-    lib = _gemm_int8()
-    _check(lib, lib.ts_gemm_int8(
-        c_int(xt), xp, c_longlong(ldx), cx, c_longlong(ldcx), sx, c_void_p(weight.codes.data_ptr()), c_longlong(weight.codes.stride(0)),
-        c_void_p(weight.scales.data_ptr()), _ptr(bias), c_int(_DTYPE[bias.dtype] == 0 if bias is not None else 0), c_void_p(out.data_ptr()),
-        c_longlong(N), c_int(1 if dtype == torch.float32 else 0), c_int(M), c_int(N), c_int(K), c_int(int8_splits(M, N, K)),
-        c_int(1 if constant_weight else 0), _stream()), 1 if given else 2)
+        scratch = torch.empty(M * (ldcx + 4), dtype=torch.uint8, device=codes.device)
+        xp, cx = rows.data_ptr(), scratch.data_ptr()
+        sx = cx + M * ldcx
+    lib, fn = _entry(0, "ts_gemm_int8")
+    _launched(lib, fn(xt, xp, ldx, cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else None,
+                      0 if bias is None or bias.dtype == torch.bfloat16 else 1, out.data_ptr(), N, 1 if dtype == torch.float32 else 0, M, N, K,
+                      int8_splits(M, N, K), 1 if constant_weight else 0, stream), 1 if given else 2)
     return out
 
 
@@ -2682,10 +2726,11 @@ class Int4Pages:
     __slots__ = ("codes", "pairs", "shape")
 
     def __init__(self, codes, pairs):
-        if codes.dtype != torch.uint8 or codes.dim() != 4 or pairs.dtype != torch.bfloat16 or pairs.shape != codes.shape[:3] + (2,):
+        shape = tuple(codes.shape)
+        if codes.dtype != torch.uint8 or len(shape) != 4 or pairs.dtype != torch.bfloat16 or tuple(pairs.shape) != shape[:3] + (2,):
             raise TypeError("Int4Pages: codes are uint8 [pages, heads, slots, D / 2] and pairs bfloat16 [pages, heads, slots, 2], got "
-                            f"{codes.dtype} {tuple(codes.shape)} and {pairs.dtype} {tuple(pairs.shape)}")
-        pages, heads, slots, half = codes.shape
+                            f"{codes.dtype} {shape} and {pairs.dtype} {tuple(pairs.shape)}")
+        pages, heads, slots, half = shape
         if not codes.is_contiguous() or not pairs.is_contiguous() or codes.data_ptr() % (4 if half % 16 else 16) or pairs.data_ptr() % 4:
             raise ValueError("Int4Pages: codes and pairs are contiguous; codes begin on 16 bytes (on 4 where a row is no multiple of 16), pairs on 4")
         self.codes, self.pairs, self.shape = codes, pairs, (pages, heads, slots, 2 * half)
@@ -2695,16 +2740,20 @@ class Int4Pages:
         return self.codes.device
 
 
-def _int4_caches(what, k_cache, v_cache, page):
+def _int4_caches(what, k_cache, v_cache, page=None):
+    """The caches' common shape (pages, heads, page size, D), checked against ``page``."""
     if not isinstance(k_cache, Int4Pages) or not isinstance(v_cache, Int4Pages) or k_cache.shape != v_cache.shape:
         raise TypeError(f"{what}: keys and values are both Int4Pages of one shape")
-    if page != k_cache.shape[2] or page & (page - 1):
-        raise ValueError(f"{what}: pages of {page} tokens on a cache with pages of {k_cache.shape[2]} (a power of two)")
+    size = k_cache.shape[2]
+    if (page is not None and page != size) or size & (size - 1) or size == 0:
+        raise ValueError(f"{what}: pages of {page or size} tokens on a cache with pages of {size} (a power of two)")
+    return k_cache.shape
 
 
 def _int32_row(what, t, name, n):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
-        raise TypeError(f"{what}: {name} is int32 [{n}], contiguous, got {t.dtype} {tuple(t.shape)}")
+    shape = t.shape
+    if t.dtype != torch.int32 or len(shape) != 1 or shape[0] < n or (n > 1 and not t.is_contiguous()):
+        raise TypeError(f"{what}: {name} is int32 [{n}], contiguous, got {t.dtype} {tuple(shape)}")
 
 
 def int4_kvwrite(k, v, k_cache, v_cache, slot_mapping):
@@ -2713,33 +2762,30 @@ def int4_kvwrite(k, v, k_cache, v_cache, slot_mapping):
     bfloat16(min), scale = bfloat16((max - zero) / 15), code = round((x - zero) / scale), halves to even, within 0 and 15; a row with an
     infinity or a NaN gets a pair of NaN."""
     what = "int4_kvwrite"
-    _int4_caches(what, k_cache, v_cache, k_cache.shape[2] if isinstance(k_cache, Int4Pages) else 0)
-    pages, heads, page, D = k_cache.shape
-    for x in (k, v):
-        if x.dim() != 3 or x.dtype not in _DTYPE or x.dtype != k.dtype or tuple(x.shape) != (k.shape[0], heads, D):
-            raise TypeError(f"{what}: keys and values are float32 or bfloat16 [T, {heads}, {D}], got {x.dtype} {tuple(x.shape)}")
-        if x.stride(2) != 1:
-            raise ValueError(f"{what}: a head lies in one run, got strides {x.stride()}")
-    T = k.shape[0]
+    pages, heads, page, D = _int4_caches(what, k_cache, v_cache)
+    shape = tuple(k.shape)
+    if len(shape) != 3 or shape[1:] != (heads, D) or tuple(v.shape) != shape or k.dtype not in _DTYPE or v.dtype != k.dtype:
+        raise TypeError(f"{what}: keys and values are float32 or bfloat16 [T, {heads}, {D}], got {k.dtype} {shape} and {v.dtype} {tuple(v.shape)}")
+    k_row, k_head, k_column = k.stride()
+    v_row, v_head, v_column = v.stride()
+    if k_column != 1 or v_column != 1:
+        raise ValueError(f"{what}: a head lies in one run, got strides {k.stride()} and {v.stride()}")
+    T = shape[0]
     _int32_row(what, slot_mapping, "slot_mapping", T)
-    _here(what, k, v, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping)
-    lib = _attention_int4(D)
-    if T == 0:
-        return
-    _check(lib, lib.ts_int4_kvwrite(
-        c_int(_DTYPE[k.dtype]), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), c_longlong(k.stride(0)), c_longlong(k.stride(1)),
-        c_longlong(v.stride(0)), c_longlong(v.stride(1)), c_int(T), c_int(heads), c_void_p(k_cache.codes.data_ptr()),
-        c_void_p(k_cache.pairs.data_ptr()), c_void_p(v_cache.codes.data_ptr()), c_void_p(v_cache.pairs.data_ptr()),
-        c_void_p(slot_mapping.data_ptr()), c_int(page), c_int(pages), _stream()))
+    stream = _here(what, k, v, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping)
+    lib, fn = _entry(D, "ts_int4_kvwrite")
+    if T:
+        _launched(lib, fn(_DTYPE[k.dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, T, heads, k_cache.codes.data_ptr(),
+                          k_cache.pairs.data_ptr(), v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), slot_mapping.data_ptr(), page, pages, stream), 1)
 
 
 def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary, q_weight, k_weight, eps, k_cache, v_cache, slot_mapping, page_size):
     what = "qk_norm_rope_kvwrite"
     qkv = materialize(qkv)
     H, Hkv, D = num_heads, num_kv_heads, head_dim
-    _int4_caches(what, k_cache, v_cache, page_size)
-    if k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
-        raise TypeError(f"{what}: {Hkv} heads of {D} on a cache of {k_cache.shape[1]} heads of {k_cache.shape[3]}")
+    shape = _int4_caches(what, k_cache, v_cache, page_size)
+    if shape[1] != Hkv or shape[3] != D:
+        raise TypeError(f"{what}: {Hkv} heads of {D} on a cache of {shape[1]} heads of {shape[3]}")
     if qkv.dim() != 2 or qkv.shape[1] != (H + 2 * Hkv) * D or qkv.dtype not in _DTYPE or not qkv.is_contiguous():
         raise ValueError("qkv must be [T, (H + 2 Hkv) * D], contiguous, float32 or bfloat16")
     if (q_weight is None) != (k_weight is None) or (q_weight is not None and q_weight.dtype != k_weight.dtype):
@@ -2747,21 +2793,24 @@ def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary
     T = qkv.shape[0]
     if slot_mapping is not None:
         _int32_row(what, slot_mapping, "slot_mapping", T)
+    rot, cos, sin, interleaved = 0, None, None, 0
     if rotary is not None:
+        rot, cos, sin, interleaved = rotary.rotary_dim, rotary.cos, rotary.sin, 1 if rotary.interleaved else 0
         _int32_row(what, positions, "positions", T)
-    cos, sin = (rotary.cos, rotary.sin) if rotary is not None else (None, None)
-    _here(what, qkv, positions, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping, cos, sin, q_weight, k_weight)
+    stream = _here(what, qkv, positions, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping, cos, sin, q_weight, k_weight)
     q = torch.empty(T, H, D, dtype=qkv.dtype, device=qkv.device)
-    lib = _attention_int4(D)
-    if T == 0:
-        return q
-    _check(lib, lib.ts_int4_rope_kvwrite(
-        c_int(_DTYPE[qkv.dtype]), _ptr(qkv), _ptr(q), _ptr(positions), _ptr(cos), _ptr(sin), c_int(rotary.rotary_dim if rotary is not None else 0),
-        c_int(int(rotary.interleaved) if rotary is not None else 0), _ptr(q_weight), _ptr(k_weight),
-        c_int(_vec_flag(q_weight, qkv.dtype) if q_weight is not None else 0), c_float(eps), c_int(T), c_int(H), c_int(Hkv),
-        _ptr(k_cache.codes), _ptr(k_cache.pairs), _ptr(v_cache.codes), _ptr(v_cache.pairs), _ptr(slot_mapping), c_int(page_size),
-        c_int(k_cache.shape[0]), _stream()))
+    lib, fn = _entry(D, "ts_int4_rope_kvwrite")
+    at = lambda t: t.data_ptr() if t is not None else None
+    if T:
+        _launched(lib, fn(_DTYPE[qkv.dtype], at(qkv), at(q), at(positions), at(cos), at(sin), rot, interleaved, at(q_weight), at(k_weight),
+                          _vec_flag(q_weight, qkv.dtype) if q_weight is not None else 0, eps, T, H, Hkv, at(k_cache.codes), at(k_cache.pairs),
+                          at(v_cache.codes), at(v_cache.pairs), at(slot_mapping), page_size, shape[0], stream), 1)
     return q
+
+
+def int4_attention_error(head_dim: int) -> int:
+    """1 if a block of the tensor-core kernel over a 4-bit cache ever gave up on a wait (synchronises)."""
+    return _attention_int4(head_dim).ts_int4_attention_error()
 
 
 def int4_attention_backend(dtype, head_dim) -> str:
@@ -2782,52 +2831,55 @@ def int4_attention_splits(blocks, max_kv_len):
 
 def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_splits, backend, sinks, softcap):
     what = "paged_attention"
-    _int4_caches(what, k_cache, v_cache, view.page_size)
-    pages, Hkv, page, D = k_cache.shape
-    if q.dim() != 3 or q.dtype not in _DTYPE or q.shape[2] != D or q.shape[1] % Hkv:
-        raise TypeError(f"{what}: queries are float32 or bfloat16 [T, H, {D}] with H a multiple of {Hkv}, got {q.dtype} {tuple(q.shape)}")
-    if q.stride(2) != 1:
+    pages, Hkv, page, D = _int4_caches(what, k_cache, v_cache, view.page_size)
+    shape, dtype = tuple(q.shape), q.dtype
+    if len(shape) != 3 or dtype not in _DTYPE or shape[2] != D or shape[1] % Hkv or shape[1] == 0:
+        raise TypeError(f"{what}: queries are float32 or bfloat16 [T, H, {D}] with H a multiple of {Hkv}, got {dtype} {shape}")
+    q_row, q_head, q_column = q.stride()
+    if q_column != 1:
         raise ValueError(f"{what}: a head lies in one run, got strides {q.stride()}")
-    T, H = q.shape[:2]
-    B = ctx.num_requests
+    T, H, _ = shape
+    G = H // Hkv
+    B, cu_q, kv_lens, table = ctx.num_requests, ctx.cu_q, ctx.kv_lens, view.block_table
     window, softcap = int(window or 0), float(softcap or 0.0)
     if window < 0 or softcap < 0:
         raise ValueError(f"{what}: a window and a soft cap are positive (0: none)")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous()):
+    if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (H,) or not sinks.is_contiguous()):
         raise TypeError(f"{what}: sinks are float32 [heads] on the device")
-    table = view.block_table
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < B or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
+    rows, blocks = table.shape if table.dim() == 2 else (0, 0)
+    table_row, table_column = table.stride() if table.dim() == 2 else (0, 0)
+    if table.dtype != torch.int32 or rows < B or blocks < 1 or (blocks > 1 and table_column != 1):
         raise TypeError(f"{what}: the block table is int32 [requests, blocks], rows contiguous, got {table.dtype} {tuple(table.shape)}")
-    _int32_row(what, ctx.cu_q, "cu_q", B + 1)
-    _int32_row(what, ctx.kv_lens, "kv_lens", B)
-    chosen = int4_attention_backend(q.dtype, D)
-    if backend not in (None, chosen, "simt"):
-        raise ValueError(f"attention backend {backend!r} does not take {q.dtype}, head size {D} and a 4-bit cache")
-    chosen = backend or chosen
-    _here(what, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, table, ctx.cu_q, ctx.kv_lens, sinks)
-    out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
-    lib = _attention_int4(D)
+    _int32_row(what, cu_q, "cu_q", B + 1)
+    _int32_row(what, kv_lens, "kv_lens", B)
+    chosen = int4_attention_backend(dtype, D)
+    if backend is not None:
+        if backend not in (chosen, "simt"):
+            raise ValueError(f"attention backend {backend!r} does not take {dtype}, head size {D} and a 4-bit cache")
+        chosen = backend
+    stream = _here(what, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, table, cu_q, kv_lens, sinks)
+    out = torch.empty(shape, dtype=dtype, device=q.device)
+    lib, fn = _entry(D, "ts_int4_attention")
     if T == 0 or B == 0:
         return out
-    span = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
+    max_q_len, span = ctx.max_q_len, ctx.max_kv_len
+    if window:
+        span = min(span, window)
     columns = 0
     if chosen == "mma":
-        rows = ctx.max_q_len * (H // Hkv)
+        rows = max_q_len * G
         columns = 16 if rows > 8 and D <= 128 else 8
-        if -(-rows // columns) * Hkv > 65535 or B > 65535:
-            columns = 0
+        if -(-rows // columns) * Hkv > 65535 or B > 65535 or page < 4 or (k_cache.pairs.data_ptr() | v_cache.pairs.data_ptr()) % 16:
+            columns = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes it)
     if num_splits is None:
-        num_splits = (int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else
-                      int4_attention_splits(T * Hkv * -(-(H // Hkv) // 8), span))
+        num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
     part_o = part_ml = None
     if num_splits > 1:
-        part_o = torch.empty(T * H * num_splits * D, dtype=torch.float32, device=q.device)
-        part_ml = torch.empty(T * H * num_splits * 2, dtype=torch.float32, device=q.device)
-    _check(lib, lib.ts_int4_attention(
-        c_int(_DTYPE[q.dtype]), c_void_p(q.data_ptr()), c_longlong(q.stride(0)), c_longlong(q.stride(1)), c_void_p(out.data_ptr()),
-        c_void_p(k_cache.codes.data_ptr()), c_void_p(k_cache.pairs.data_ptr()), c_void_p(v_cache.codes.data_ptr()),
-        c_void_p(v_cache.pairs.data_ptr()), c_void_p(table.data_ptr()), c_void_p(ctx.cu_q.data_ptr()), c_void_p(ctx.kv_lens.data_ptr()),
-        c_int(T), c_int(B), c_int(H), c_int(Hkv), c_int(page), c_int(table.shape[1]), c_int(table.stride(0)), c_int(pages), c_float(scale),
-        c_int(window), c_float(softcap), _ptr(sinks), c_int(num_splits), _ptr(part_o), _ptr(part_ml), c_int(ctx.max_q_len),
-        c_int(columns), _stream()), 1 if num_splits == 1 else 2)
+        scratch = torch.empty(T * H * num_splits * (D + 2), dtype=torch.float32, device=q.device)
+        part_o = scratch.data_ptr()
+        part_ml = part_o + 4 * T * H * num_splits * D
+    _launched(lib, fn(_DTYPE[dtype], q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
+                      v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H, Hkv, page,
+                      blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, num_splits, part_o, part_ml,
+                      max_q_len, columns, stream), 1 if num_splits == 1 else 2)
     return out
