@@ -265,8 +265,7 @@ __device__ __forceinline__ int request_of(const int* cu_q, int B, int t) {
   return lo;
 }
 // row of key j of a request in the cache; a page number outside the pool is reported and read as page 0
-__device__ __forceinline__ size_t cache_row(const Int4Params& p, const int* bt, int kvh, int j) {
-  int page = bt[j >> p.page_shift];
+__device__ __forceinline__ size_t cache_row(const Int4Params& p, int page, int kvh, int j) {
   if ((unsigned)page >= (unsigned)p.num_pages) {
     ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_PAGE);
     page = 0;
@@ -325,7 +324,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
   for (int tile = split * per; tile < min(tiles, (split + 1) * per); ++tile) {
     const int j0 = j_lo + tile * SIMT_KEYS, j = j0 + tid, n = min(SIMT_KEYS, j_hi - j0);
     if (tid < n) {
-      const size_t row = cache_row(p, bt, kvh, j);
+      const size_t row = cache_row(p, bt[j >> p.page_shift], kvh, j);
       key_row[tid] = row;
       v_pair[tid] = p.vp[row];
       const uint32_t kpair = p.kp[row];
@@ -460,22 +459,29 @@ __global__ void int4_combine_kernel(Int4Params p) {
 // ------------------------------------------------------------------------------------------ attention on the tensor cores
 // bfloat16 queries.  A block is up to 8 NT columns = (query, head) pairs of one key head, and a range of its keys; every warp walks keys of its
 // own, 32 at a time, through a ring of shared memory that nobody else touches (bulk copies by runs of a page, no block barriers in the loop):
-//   S^T = K Q^T with the keys as the rows of m16n8k16, P^T brought to the next operand's layout by movmatrix, O^T += V^T P^T with the columns
-//   of the values as rows.  A code c enters the tensor core as the bfloat16 number 16 + c, which is one shift and one AND-OR for two
-//   codes (c in the upper mantissa bits under the exponent of 16): no conversion, no multiplication.  Scales and zeros are per
-//   key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.(16 + c)) + (z - 16 s) sum(q), and for values with p' = bfloat16(p s):
-//   sum p v = sum p' (16 + c) + sum (p z - 16 p'), the second a number per column that every column of the output gets.  (p' is rounded
-//   before both sums, so that the 16 cancels exactly.)
+//   S^T = K Q^T with the keys as the rows, P^T brought to the next operand's layout by movmatrix, O^T += V^T P^T with the columns of the
+//   values as rows.  What bounds it is the instructions that unpack codes, so they are few:
+//   K  an AND makes four codes of a word an operand register of 8-bit integers (m16n8k32).  The queries are split for it: a row's elements in
+//      units of 2^-14 of its largest one's power of two, 16 bits, are 256 hi + lo, hi signed and lo not; sums are whole numbers, exact.
+//      (bfloat16 has 8 significant bits: elements down to 2^-7 of the largest keep all of theirs, smaller ones are
+//      rounded to 2^-15 of it, far below what the projection's own rounding left.  Eight-bit floating point would hold a code without
+//      any change, but its mma.sync is made of conversions to 16 bits: 827 instructions a step of 32 keys, as it is 635.)
+//   V  keys run along K there, two of one column side by side, which bytes would need a transposition for: a code enters as the bfloat16
+//      number 16 + c, one shift and one AND-OR for two of them.
+//   Scales and zeros are per key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.c) + z sum(q); for the values, with p' =
+//   bfloat16(p s), sum p v = sum p' (16 + c) + sum p z - 16 sum p'; the last sum is one more MMA, with ones for V, so that the 16 cancels
+//   whatever p' was rounded to.
 constexpr int MMA_WARPS = 8, STEP = 32, RING = 3;
 constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
 constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;   // codes of K and V, pairs of K and V
 constexpr float ABOVE = 16.f;                                      // what a code's bfloat16 is above it
+constexpr int MERGE_ROW = D + 4;                                   // floats of a column's partial result: the four columns of a quad meet other banks
 
 template <int NT> struct MmaCfg {
   static constexpr int NC = 8 * NT;
-  static constexpr int Q_BYTES = (D / 16) * NT * 32 * 8;
+  static constexpr int Q_BYTES = KW * NT * 32 * 16 + NC * 8;       // operands; (factor, sum) of every column
   static constexpr int RING_BYTES = MMA_WARPS * RING * STAGE_BYTES;
-  static constexpr int MERGE_BYTES = MMA_WARPS * NC * (D + 3) * 4;
+  static constexpr int MERGE_BYTES = MMA_WARPS * NC * (MERGE_ROW + 3) * 4;
   static constexpr int SMEM = Q_BYTES + (RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES);
   static constexpr bool Q_REGS = NT == 1 && D <= 128;              // the queries' operands stay in registers
   static constexpr int BLOCKS = Q_REGS ? 2 : 1;
@@ -499,6 +505,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// four codes of a word as bytes: of columns 0, 4, 1, 5 and, shifted, 2, 6, 3, 7
+__device__ __forceinline__ uint32_t codes4(uint32_t word) { return word & 0x0f0f0f0fu; }
+__device__ __forceinline__ void mma_hi(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_lo(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// pairs of 32-bit numbers: one instruction for both
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float x, float y) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ void f2_out(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 // codes number e (0 .. 3) of both halves of a word as two bfloat16 numbers 16 + c
 template <int E>
 __device__ __forceinline__ uint32_t codes2(uint32_t word) {
@@ -511,6 +534,7 @@ __device__ __forceinline__ uint32_t codes2(uint32_t word) {
 // Where a running maximum starts: below every score, and finite, so that nothing subtracts infinities.  It moves only when a score passes it by
 // more than SLACK (a power of two): probabilities up to 2^SLACK do no harm in 32-bit sums, and most steps then rescale nothing.
 constexpr float LOWEST = -3e38f, SLACK = 8.f;
+constexpr uint32_t ONES = 0x3f803f80u;                             // two bfloat16
 // Row r of the 16 that an MMA reads of K is this key of the group: thread t of a quad then finds its columns of V^T (rows 2t, 2t + 1, 2t + 8,
 // 2t + 9) in keys t, t + 4, t + 8, t + 12, and the eight lanes whose reads of K meet read neighbouring keys' halves of a bank line
 __device__ __forceinline__ int key_of_row(int r) { return (r & 8) | (r >> 1 & 3) | (r & 1) << 2; }
@@ -521,7 +545,8 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   extern __shared__ __align__(16) char smem[];
   __shared__ uint64_t full[MMA_WARPS][RING];
   __shared__ volatile int abort_flag;
-  uint2* qf_s = reinterpret_cast<uint2*>(smem);                    // [D / 16][NT][32 lanes]
+  uint4* qf_s = reinterpret_cast<uint4*>(smem);                    // [KW][NT][32 lanes]: high and low bytes of eight columns
+  float2* q_stat = reinterpret_cast<float2*>(smem + KW * NT * 32 * 16);       // [NC]
   char* work = smem + C::Q_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (lane < RING) mbar_init(smem_u32(&full[warp][lane]), 1);
@@ -547,6 +572,11 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   // A step's 32 keys lie in whole or in runs of a page; every run is four copies (codes and pairs of K and V) by a lane of its own.  A run
   // that starts behind the last key is not fetched, and what its place holds is masked.
   const int run_shift = min(p.page_shift, 5), runs = STEP >> run_shift, run_keys = 1 << run_shift;
+  int page_ahead = 0;          // of this lane's run of the step that is fetched next: read a step before it is needed
+  auto look = [&](int s) {
+    const int j = (step0 + s) * STEP + (lane << run_shift);
+    if (s < s_end && lane < runs && j < j_hi) page_ahead = bt[j >> p.page_shift];
+  };
   auto fetch = [&](int s, int stage) {
     const int j = (step0 + s) * STEP + (lane << run_shift);
     const bool mine = lane < runs && j < j_hi;
@@ -555,48 +585,70 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
     if (lane == 0) mbar_expect_tx(bar, n * (STAGE_BYTES >> (5 - run_shift)));
     __syncwarp();
     if (mine) {
-      const size_t row = cache_row(p, bt, kvh, j);
+      const size_t row = cache_row(p, page_ahead, kvh, j);
       const uint32_t at = smem_u32(ring) + stage * STAGE_BYTES, code_bytes = ROW_BYTES << run_shift, first_row = lane << run_shift;
       bulk_copy(at + first_row * ROW_BYTES, reinterpret_cast<const char*>(p.kc) + row * ROW_BYTES, code_bytes, bar);
       bulk_copy(at + (STEP + first_row) * ROW_BYTES, reinterpret_cast<const char*>(p.vc) + row * ROW_BYTES, code_bytes, bar);
       bulk_copy(at + 2 * STEP * ROW_BYTES + first_row * 4, p.kp + row, run_keys * 4, bar);
       bulk_copy(at + 2 * STEP * ROW_BYTES + (STEP + first_row) * 4, p.vp + row, run_keys * 4, bar);
     }
+    look(s + MMA_WARPS);
   };
   const int mine = split * per + warp;
+  look(mine);
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i)
     if (mine + i * MMA_WARPS < s_end) fetch(mine + i * MMA_WARPS, i);
 
-  // the queries as B operands: row (query, head) c, columns 4 (s % 2) .. + 3 of word t KW + s / 2
-  for (int i = threadIdx.x; i < (D / 16) * NT * 32; i += MMA_WARPS * 32) {
-    const int l = i & 31, nt = (i >> 5) % NT, s = (i >> 5) / NT, c = nt * 8 + (l >> 2);
-    uint2 v = make_uint2(0u, 0u);
-    if (c < nc) {
+  // the queries as B operands: a warp makes a column, a lane a word's eight columns: word t KW + i goes to step i, thread t of the column's quad
+  for (int c = warp; c < C::NC; c += MMA_WARPS) {
+    float x[8] = {};
+    if (lane < W && c < nc) {
       const int r = c0 + c;
-      const bf16* src = static_cast<const bf16*>(p.q) + (q_begin + r / G) * p.q_row + (kvh * G + r % G) * p.q_head + ((l & 3) * KW + (s >> 1)) * 8 + 4 * (s & 1);
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-      if (((reinterpret_cast<uintptr_t>(src)) & 7) == 0) v = *reinterpret_cast<const uint2*>(src);
-      else v = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+      const bf16* src = static_cast<const bf16*>(p.q) + (q_begin + r / G) * p.q_row + (kvh * G + r % G) * p.q_head + lane * 8;
+      if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) load8<bf16>(src, x);
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __bfloat162float(src[e]);
+      }
     }
-    qf_s[i] = v;
+    float top = 0.f, sum = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top = fmaxf(top, fabsf(x[e]));
+      sum += x[e];
+      bad |= !(fabsf(x[e]) <= 3.402823466e38f);
+    }
+    top = warp_max(top);
+    sum = warp_sum(sum);
+    bad = __any_sync(0xffffffffu, bad);
+    // the row's largest element goes to 2^14 .. 2^15
+    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -112), 127);
+    const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+    uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+    constexpr int COLUMN[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int whole = bad ? 0 : __float2int_rn(x[COLUMN[e]] * up);
+      hi[e >> 2] |= (uint32_t)(whole >> 8 & 255) << (8 * (e & 3));
+      lo[e >> 2] |= (uint32_t)(whole & 255) << (8 * (e & 3));
+    }
+    if (lane < W) qf_s[((lane % KW) * NT + (c >> 3)) * 32 + (c & 7) * 4 + lane / KW] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+    if (lane == 0) q_stat[c] = make_float2(bad ? __int_as_float(0x7fc00000) : 1.f / up, sum);
   }
   __syncthreads();
-  uint2 qf[C::Q_REGS ? D / 16 : 1];
-  float qsum[NT][2];                                               // of columns 2t and 2t + 1
+  uint4 qf[C::Q_REGS ? KW : 1];
+  F2 factor[NT], qsum[NT];                                         // of columns 2t and 2t + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    float sum = 0.f;
+    if (C::Q_REGS) {
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const uint2 v = qf_s[(s * NT + nt) * 32 + lane];
-      if (C::Q_REGS) qf[C::Q_REGS ? s : 0] = v;
-      sum += pair_scale(v.x) + pair_zero(v.x) + pair_scale(v.y) + pair_zero(v.y);       // (the halves of a word as numbers)
+      for (int i = 0; i < KW; ++i) qf[C::Q_REGS ? i : 0] = qf_s[i * 32 + lane];
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    qsum[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-    qsum[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+    const float2 a = q_stat[nt * 8 + 2 * t], b = q_stat[nt * 8 + 2 * t + 1];
+    factor[nt] = f2(a.x, b.x);
+    qsum[nt] = f2(a.y, b.y);
   }
   int pos[NT][2];
 #pragma unroll
@@ -609,7 +661,8 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   const int all_from = p.window > 0 ? max(0, last - p.window + 1) : 0;       // keys from here to `first` are seen by every column
   const float scale2 = p.scale * LOG2E;
 
-  float o[D / 16][NT][4], m[NT][2], l[NT][2], z[NT][2];
+  float o[D / 16][NT][4], m[NT][2], ps[NT][4];                     // ps: sum p' of columns 2t and 2t + 1 (and the same again)
+  F2 l[NT], z[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -617,7 +670,9 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) { m[nt][i] = LOWEST; l[nt][i] = z[nt][i] = 0.f; }
+    for (int e = 0; e < 4; ++e) ps[nt][e] = 0.f;
+    m[nt][0] = m[nt][1] = LOWEST;
+    l[nt] = z[nt] = f2(0.f, 0.f);
   }
 
   int stage = 0, waits = 0;
@@ -660,45 +715,43 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 #pragma unroll
         for (int i = 0; i < KW; ++i) { w0[i] = r0[i]; w1[i] = r1[i]; }
       }
-      // two chains of MMAs, added up: half the latency
-      float half[2][NT][4];
+      int part[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) half[h][nt][e] = 0.f;
+          for (int e = 0; e < 4; ++e) part[h][nt][e] = 0;
 #pragma unroll
       for (int i = 0; i < KW; ++i) {
-        const uint32_t a[2][4] = {{codes2<0>(w0[i]), codes2<0>(w1[i]), codes2<1>(w0[i]), codes2<1>(w1[i])},
-                                  {codes2<2>(w0[i]), codes2<2>(w1[i]), codes2<3>(w0[i]), codes2<3>(w1[i])}};
+        const uint32_t a0 = codes4(w0[i]), a1 = codes4(w1[i]), a2 = codes4(w0[i] >> 4), a3 = codes4(w1[i] >> 4);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint2 q = C::Q_REGS ? qf[C::Q_REGS ? 2 * i + h : 0] : qf_s[((2 * i + h) * NT + nt) * 32 + lane];
-            mma_bf16(half[h][nt], a[h][0], a[h][1], a[h][2], a[h][3], q.x, q.y);
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 q = C::Q_REGS ? qf[C::Q_REGS ? i : 0] : qf_s[(i * NT + nt) * 32 + lane];
+          mma_hi(part[0][nt], a0, a1, a2, a3, q.x, q.y);
+          mma_lo(part[1][nt], a0, a1, a2, a3, q.z, q.w);
+        }
       }
+      // scores; this thread's keys are those of rows g and g + 8
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t kpair = kp[kb * 16 + 8 * h];
+        const float a = pair_scale(kpair) * scale2, b = pair_zero(kpair) * scale2;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[kb][nt][e] = half[0][nt][e] + half[1][nt][e];
+        for (int nt = 0; nt < NT; ++nt) {
+          const F2 sum = f2((float)(part[0][nt][2 * h] * 256 + part[1][nt][2 * h]), (float)(part[0][nt][2 * h + 1] * 256 + part[1][nt][2 * h + 1]));
+          f2_out(f2_fma(f2(a, a), f2_mul(sum, factor[nt]), f2_mul(f2(b, b), qsum[nt])), sc[kb][nt][2 * h], sc[kb][nt][2 * h + 1]);
+        }
+      }
     }
-    // scores; this thread's keys are those of rows g and g + 8 of both groups
     float vscale[2][2], vzero[2][2], top[NT][2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t kpair = kp[kb * 16 + 8 * h], vpair = vp[kb * 16 + 8 * h];
-        const float a = pair_scale(kpair) * scale2, bq = fmaf(-ABOVE, a, pair_zero(kpair) * scale2);
+        const uint32_t vpair = vp[kb * 16 + 8 * h];
         vscale[kb][h] = pair_scale(vpair);
         vzero[kb][h] = pair_zero(vpair);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) sc[kb][nt][2 * h + i] = fmaf(a, sc[kb][nt][2 * h + i], bq * qsum[nt][i]);
       }
     if (p.softcap > 0.f) {
       const float in = 1.f / (p.softcap * LOG2E), out = p.softcap * LOG2E;
@@ -740,18 +793,23 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
-          const float above = fmaxf(top[nt][i], m[nt][i]), f = ex2(m[nt][i] - above);
+          const float above = fmaxf(top[nt][i], m[nt][i]);
+          f[i] = ex2(m[nt][i] - above);
           m[nt][i] = above;
-          l[nt][i] *= f;
-          z[nt][i] *= f;
+          ps[nt][i] *= f[i];
+          ps[nt][2 + i] *= f[i];
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= f; o[mt][nt][2 + i] *= f; }
+          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= f[i]; o[mt][nt][2 + i] *= f[i]; }
         }
+        l[nt] = f2_mul(l[nt], f2(f[0], f[1]));
+        z[nt] = f2_mul(z[nt], f2(f[0], f[1]));
+      }
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -760,19 +818,19 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float pr[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            pr[i] = ex2(sc[kb][nt][2 * h + i] - m[nt][i]);
-            l[nt][i] += pr[i];
-            z[nt][i] = fmaf(pr[i], vzero[kb][h], z[nt][i]);
-          }
-          const __nv_bfloat162 two = __floats2bfloat162_rn(pr[0] * vscale[kb][h], pr[1] * vscale[kb][h]);
+          const F2 at = f2_add(f2(sc[kb][nt][2 * h], sc[kb][nt][2 * h + 1]), f2(-m[nt][0], -m[nt][1]));
+          float x0, x1;
+          f2_out(at, x0, x1);
+          const F2 pr = f2(ex2(x0), ex2(x1));
+          l[nt] = f2_add(l[nt], pr);
+          z[nt] = f2_fma(pr, f2(vzero[kb][h], vzero[kb][h]), z[nt]);
+          f2_out(f2_mul(pr, f2(vscale[kb][h], vscale[kb][h])), x0, x1);
+          const __nv_bfloat162 two = __floats2bfloat162_rn(x0, x1);
           const uint32_t bits = *reinterpret_cast<const uint32_t*>(&two);
-          z[nt][0] = fmaf(-ABOVE, pair_scale(bits), z[nt][0]);
-          z[nt][1] = fmaf(-ABOVE, pair_zero(bits), z[nt][1]);
           pb[nt][h] = transposed(bits);
         }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_bf16(ps[nt], ONES, ONES, ONES, ONES, pb[nt][0], pb[nt][1]);
       // values: 16-bit units g UNITS .. of keys t, t + 4, t + 8, t + 12 of the group
       uint32_t u[4][(UNITS + 1) / 2];
 #pragma unroll
@@ -815,36 +873,39 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 
   // the warps' results meet in shared memory
   __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][D]
-  float* sm_ml = sm_o + MMA_WARPS * C::NC * D;                     // [warp][column][3]
+  float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][MERGE_ROW]: output column d of lane group g at place (d's number there) * 8 + g
+  float* sm_ml = sm_o + MMA_WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) {
+    float ls[2], zs[2];
+    f2_out(l[nt], ls[0], ls[1]);
+    f2_out(z[nt], zs[0], zs[1]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
-        l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], d);
-        z[nt][i] += __shfl_xor_sync(0xffffffffu, z[nt][i], d);
+        ls[i] += __shfl_xor_sync(0xffffffffu, ls[i], d);
+        zs[i] += __shfl_xor_sync(0xffffffffu, zs[i], d);
       }
       const int c = nt * 8 + 2 * t + i;
       if (g == 0) {
         sm_ml[(warp * C::NC + c) * 3] = m[nt][i];
-        sm_ml[(warp * C::NC + c) * 3 + 1] = l[nt][i];
-        sm_ml[(warp * C::NC + c) * 3 + 2] = z[nt][i];
+        sm_ml[(warp * C::NC + c) * 3 + 1] = ls[i];
+        sm_ml[(warp * C::NC + c) * 3 + 2] = fmaf(-ABOVE, ps[nt][i], zs[i]);
       }
+      float* dst = sm_o + (warp * C::NC + c) * MERGE_ROW + g;
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int unit = g * UNITS + u, d = 8 * (unit >> 1) + (unit & 1);
-        float* dst = sm_o + (warp * C::NC + c) * D + d;
-        dst[0] = o[2 * u][nt][i];
-        dst[2] = o[2 * u][nt][2 + i];
-        dst[4] = o[2 * u + 1][nt][i];
-        dst[6] = o[2 * u + 1][nt][2 + i];
+      for (int mt = 0; mt < D / 16; ++mt) {
+        dst[16 * mt] = o[mt][nt][i];
+        dst[16 * mt + 8] = o[mt][nt][2 + i];
       }
     }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < nc * D; i += MMA_WARPS * 32) {
-    const int c = i / D, d = i % D, r = c0 + c, head = kvh * G + r % G;
+    const int c = i / D, place = i % D, r = c0 + c, head = kvh * G + r % G;
+    // place 8 n + g: nibble n % 4 of unit g UNITS + n / 4
+    const int unit = (place & 7) * UNITS + (place >> 5), d = 8 * (unit >> 1) + (unit & 1) + 2 * (place >> 3 & 3);
     const size_t row = (size_t)(q_begin + r / G) * p.H + head;
     const bool sink = p.splits == 1 && p.sinks != nullptr;
     const float sink2 = sink ? p.sinks[head] * LOG2E : LOWEST;
@@ -857,13 +918,13 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       const float* ml = sm_ml + (w * C::NC + c) * 3;
       const float f = ex2(ml[0] - top);
       total += f * ml[1];
-      sum += f * (sm_o[(w * C::NC + c) * D + d] + ml[2]);
+      sum += f * (sm_o[(w * C::NC + c) * MERGE_ROW + place] + ml[2]);
     }
     if (p.splits == 1) {
       static_cast<bf16*>(p.out)[row * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : sum / total);
     } else {
       p.part_o[(row * p.splits + split) * D + d] = sum;
-      if (d == 0) {
+      if (place == 0) {
         p.part_ml[(row * p.splits + split) * 2] = top;
         p.part_ml[(row * p.splits + split) * 2 + 1] = total;
       }
