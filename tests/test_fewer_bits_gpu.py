@@ -224,7 +224,7 @@ def test_write(dtype, T, Hkv, D, page):
         assert (off <= 0.5 * pair[..., :1].float()[~bad] + (2.0 ** -8 * 3 * top)[:, None] + 1e-30).all()
 
 
-LENGTHS = {"one": [(1, 1)], "decode": [(1, 1), (1, 64), (1, 65), (1, 700)], "long": [(1, 5000)], "portions": [(3, 3), (70, 200), (33, 33)], "mixed": [(1, 300), (40, 100), (1, 1), (0, 17), (129, 129)]}
+LENGTHS = {"wide": [(300, 900), (5, 260), (1, 1000), (64, 64)], "one": [(1, 1)], "decode": [(1, 1), (1, 64), (1, 65), (1, 700)], "long": [(1, 5000)], "portions": [(3, 3), (70, 200), (33, 33)], "mixed": [(1, 300), (40, 100), (1, 1), (0, 17), (129, 129)]}
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -238,7 +238,8 @@ def test_attention(dtype, H, Hkv, D, page, name):
     sinks = torch.randn(H, device="cuda")
     for window, softcap, sink, splits in ((0, 0.0, None, None), (0, 0.0, None, 3), (50, 0.0, sinks, None), (1, 2.0, None, None), (100, 5.0, sinks, 12)):
         want, top, span = attention(q, lengths, ks, vs, D ** -0.5, window, softcap, sink)
-        for backend in {ops.int4_attention_backend(dtype, D), "simt"}:
+        chosen = ops.int4_attention_backend(dtype, D)
+        for backend in {chosen, "simt"} | ({"mma"} if chosen == "tcgen05" else set()):
             out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, window, sinks=sink, softcap=softcap, num_splits=splits, backend=backend)
             assert ((out.double() - want).abs() <= allowed(dtype, want, top, span, D, max(m for _, m in lengths))).all(), (window, softcap, splits, backend)
 

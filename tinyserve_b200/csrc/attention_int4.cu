@@ -251,6 +251,7 @@ struct Int4Params {
   float softcap;
   const float* sinks;                        // [H] or null: one more term exp(sinks[h]) in head h's sum
   int splits;                                // key ranges; > 1: partial results for the combine kernel
+  int most;                                  // > 0: requests with more queries are somebody else's
   float *part_o, *part_ml;                   // [T * H][splits][D], [T * H][splits][2] (maximum in the log2 domain, sum)
 };
 
@@ -440,6 +441,10 @@ __global__ void int4_combine_kernel(Int4Params p) {
   pdl_wait();
   const size_t row = blockIdx.x;
   if ((int)(row / p.H) >= p.cu_q[p.B]) return;
+  if (p.most > 0) {
+    const int b = request_of(p.cu_q, p.B, (int)(row / p.H));
+    if (p.cu_q[b + 1] - p.cu_q[b] > p.most) return;
+  }
   const float* ml = p.part_ml + row * p.splits * 2;
   float m = p.sinks ? p.sinks[row % p.H] * LOG2E : -INFINITY;
   const float sink = m;
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC, b = blockIdx.z;
   const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
   const int nc = min(C::NC, q_len * G - c0);                       // columns of this block
-  if (nc <= 0) return;
+  if (nc <= 0 || (p.most > 0 && q_len > p.most)) return;
   const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
   const int pos0 = kv_len - q_len;                                 // position of the request's first query of this step
   const int* bt = p.block_table + (size_t)b * p.table_stride;
@@ -1019,12 +1024,13 @@ TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const in
 }
 
 // q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
-// steps of 32 up to 256; 16 columns up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.
+// steps of 32 up to 256; 16 columns up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns):
+// requests with more queries than that are left alone.
 TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
                                 const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
                                 int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
                                 int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, int max_q_len,
-                                int columns, cudaStream_t stream) {
+                                int columns, int most, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_attention: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
@@ -1033,7 +1039,7 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
   TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml)), "int4_attention: key ranges need their scratch");
   Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
                   block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
-                  splits, part_o, part_ml};
+                  splits, most, part_o, part_ml};
   if (columns > 0) {
 #ifdef TS_INT4_MMA
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");

@@ -1,0 +1,490 @@
+// Attention of prompt portions over a paged cache in 4 bits, on the 5th-generation tensor cores: bfloat16 queries, head size 64 or 128
+// (-DTS_HEAD_DIM).  The mathematics and the use of tensor memory are those of attention_tcgen05.cu (two tiles of 128 rows = (query, head) of one
+// key head take turns on the tensor core, S = Q K^T, P written over S, O += P V, one softmax thread a row, maxima that move by
+// more than 2^8 only); keys and values come differently.  Four warps make them: a thread reads a key's row of codes (64 bytes at 128
+// columns) and its pair, and writes the row as bfloat16 into the swizzled tile that the tensor core reads: a code becomes the number 16 + c
+// (one shift, one AND-OR for two), minus 16 (exact), times scale plus zero (one rounding to bfloat16, the
+// only one that a cache of whole numbers would not have).  That is about 600 instructions a thread for a tile of 128 keys, on warps that
+// have nothing else to do, while the tensor core takes 2,000 cycles for the tile's four products.  Nothing is expanded in
+// memory: a portion of any length behind a context of any length needs no scratch.
+//
+// A key whose pair is not finite becomes a key of NaN with a value of zeros: who sees it gets NaN, who does not is not touched (its
+// probability of 0 would not survive a NaN in V).
+//
+// 512 threads: warp 0 loads the queries, warp 1 issues, warps 4-7 and 8-11 are the softmax of the two tiles (168 registers), 12-15 make keys and
+// values.  Blocks find their request themselves (a scan over the query offsets), so that no list is cut on the host and a captured graph
+// serves any step of its shape.  Every wait is bounded; a block that gives up raises ts_attention_int4_tcgen05_error.
+#include "tcgen05.cuh"
+
+#ifndef TS_HEAD_DIM
+#error "compile with -DTS_HEAD_DIM=64 or 128"
+#endif
+
+TS_DEFINE_LAST_ERROR()
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr int D = TS_HEAD_DIM;
+static_assert(D == 64 || D == 128, "the tcgen05 prefill kernel takes head sizes 64 and 128");
+constexpr int BM = 128;                      // rows of a query tile
+constexpr int BN = 128;                      // keys of a tile
+constexpr int GROUPS = 2;                    // query tiles of a block
+constexpr int P_PARTS = 2;                   // the probabilities of a key tile are handed over in this many parts
+constexpr int SOFTMAX_WARP0 = 4, MAKER_WARP0 = 12, THREADS = 512;
+constexpr int K_STAGES = 2, V_STAGES = 2;
+constexpr int DCH = D / 64;                  // 64-column chunks of a head
+constexpr int CHUNK_BYTES = 128 * 128;       // 128 rows of 128 bytes
+constexpr int Q_BYTES = DCH * CHUNK_BYTES;
+constexpr int KV_BYTES = DCH * CHUNK_BYTES;  // one of K or V of a tile
+constexpr int TMEM_COLS = 512;               // S_0, S_1: 128 columns each (P_g over the first 64 of S_g); O_0 at 256, O_1 at 384
+constexpr int W4 = D / 32;                   // 16-byte pieces of a row of codes
+constexpr size_t SMEM = 1024 + GROUPS * Q_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 256;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Params {
+  bf16* out;                // [T, H, D]
+  const uint4 *kc, *vc;     // codes
+  const uint32_t *kp, *vp;  // pairs
+  const int* block_table;   // [B, table_stride]
+  const int* cu_q;          // [B + 1]
+  const int* kv_lens;       // [B]
+  int T, B, H, Hkv, page_shift, max_blocks, table_stride, num_pages;
+  int heads_per_tile, queries_per_tile, head_tiles;     // of one query tile
+  int few;                  // requests of up to this many queries are somebody else's
+  int window;
+  const float* sinks;       // [H] or null
+  float scale_log2;
+  float cap2, cap_in;       // a soft cap c > 0: c log2(e) and scale / c; cap2 0: none
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// columns 2 E and 2 E + 1 of a word's eight, as scale * c + zero
+template <int E>
+__device__ __forceinline__ uint32_t values2(uint32_t word, __nv_bfloat162 scale, __nv_bfloat162 zero) {
+  const uint32_t moved = E == 0 ? word << 3 : word >> (4 * E - 3);
+  uint32_t two;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(two) : "r"(moved), "r"(0x00780078u), "r"(0x41804180u));
+  const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&two), __floats2bfloat162_rn(16.f, 16.f));
+  const __nv_bfloat162 v = __hfma2(c, scale, zero);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ bool finite_pair(uint32_t pair) {
+  return (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
+  extern __shared__ char smem_raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* Qs = smem;                               // [GROUPS][Q_BYTES]
+  char* Ks = Qs + GROUPS * Q_BYTES;              // [K_STAGES][KV_BYTES]
+  char* Vs = Ks + K_STAGES * KV_BYTES;           // [V_STAGES][KV_BYTES]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(Vs + V_STAGES * KV_BYTES);
+  uint64_t* q_full = bars;                       // 1
+  uint64_t* k_full = q_full + 1;                 // [K_STAGES] the makers' four warps
+  uint64_t* k_empty = k_full + K_STAGES;         // [K_STAGES] both tiles' scores of the stage's keys are computed
+  uint64_t* v_full = k_empty + K_STAGES;         // [V_STAGES]
+  uint64_t* v_empty = v_full + V_STAGES;         // [V_STAGES] the stage's values are added to both O
+  uint64_t* s_full = v_empty + V_STAGES;         // [GROUPS] S_g holds the scores of a key tile
+  uint64_t* p_full = s_full + GROUPS;            // [GROUPS][P_PARTS] the part of P_g is in tensor memory, O_g is rescaled
+  uint64_t* o_ready = p_full + GROUPS * P_PARTS; // [GROUPS] O_g holds the sum over the key tiles so far
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_ready + GROUPS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(q_full), 1);
+    for (int s = 0; s < K_STAGES; ++s) {
+      mbar_init(smem_u32(&k_full[s]), 4);
+      mbar_init(smem_u32(&k_empty[s]), 1);
+    }
+    for (int s = 0; s < V_STAGES; ++s) {
+      mbar_init(smem_u32(&v_full[s]), 4);
+      mbar_init(smem_u32(&v_empty[s]), 1);
+    }
+    for (int g = 0; g < GROUPS; ++g) {
+      mbar_init(smem_u32(&s_full[g]), 1);
+      for (int h = 0; h < P_PARTS; ++h) mbar_init(smem_u32(&p_full[g * P_PARTS + h]), 4);
+      mbar_init(smem_u32(&o_ready[g]), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                 ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // this block holds all of the SM's tensor memory now: only now may a dependent kernel start
+  pdl_trigger();
+  pdl_wait();
+
+  // block x from the last: the tiles of all requests in a row, the latest queries (the most keys) first
+  const int QPT = p.queries_per_tile, GT = p.heads_per_tile, per_block = GROUPS * QPT;
+  const int G = p.H / p.Hkv;
+  int b = -1, q0 = 0;
+  {
+    int total = 0;
+    for (int at = 0; at < p.B; at += 32) {
+      const int n = at + lane < p.B ? min(p.cu_q[at + lane + 1], p.T) - p.cu_q[at + lane] : 0;
+      total += n > p.few ? (n + per_block - 1) / per_block : 0;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    const int want = total - 1 - (int)blockIdx.x;
+    int before = 0;
+    for (int at = 0; at < p.B && want >= 0 && b < 0; at += 32) {
+      const int n = at + lane < p.B ? min(p.cu_q[at + lane + 1], p.T) - p.cu_q[at + lane] : 0;
+      const int tiles = n > p.few ? (n + per_block - 1) / per_block : 0;
+      int upto = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+      }
+      const uint32_t here = __ballot_sync(0xffffffffu, before + upto > want);
+      if (here != 0) {
+        const int who = __ffs(here) - 1;
+        b = at + who;
+        q0 = (want - before - __shfl_sync(0xffffffffu, upto - tiles, who)) * per_block;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  const int kvh = blockIdx.y / p.head_tiles, head_tile = blockIdx.y % p.head_tiles;
+  const int q_begin = b >= 0 ? p.cu_q[b] : 0, q_len = b >= 0 ? min(p.cu_q[b + 1], p.T) - q_begin : 0;
+  const int kv_len = b >= 0 ? (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift) : 0;
+  const int g0 = head_tile * GT;
+  const int nq_all = max(0, min(per_block, q_len - q0));
+  const int groups = nq_all > QPT ? 2 : 1;       // query tiles of this block that hold queries
+  const int pos0 = kv_len - q_len + q0;
+  const int j_hi = max(0, min(kv_len, pos0 + nq_all));
+  const int j_lo = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+  const int first_tile = j_lo / BN;
+  // (a block whose rows see no key at all still walks one tile, of which nothing is visible)
+  const int n_tiles = nq_all > 0 ? max(1, (j_hi + BN - 1) / BN - first_tile) : 0;
+
+  if (warp < SOFTMAX_WARP0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+    if (warp == 0 && lane == 0 && n_tiles > 0) {
+      // queries: rows (query, head) with the head fastest; one box per 64 columns and query tile
+      const uint32_t qbar = smem_u32(q_full);
+      mbar_expect_tx(qbar, groups * DCH * 64 * 2 * GT * QPT);
+      for (int g = 0; g < groups; ++g)
+        for (int c = 0; c < DCH; ++c)
+          tma_load_3d(smem_u32(Qs + g * Q_BYTES + c * CHUNK_BYTES), &map_q, qbar, c * 64, kvh * G + g0, q_begin + q0 + g * QPT);
+    } else if (warp == 1 && n_tiles > 0 && elect_one()) {
+      constexpr uint32_t idesc_qk = make_idesc(BM, BN, false);
+      constexpr uint32_t idesc_pv = make_idesc(BM, D, true);
+      constexpr int QK_STEPS = D / 16, PV_STEPS = BN / 16 / P_PARTS;
+      const uint64_t q_desc = smem_desc(smem_u32(Qs)), k_desc = smem_desc(smem_u32(Ks));
+      const uint64_t v_desc = smem_desc_mn(smem_u32(Vs), CHUNK_BYTES);
+      // S_g = Q_g K^T of key tile t (the P V of tile g's previous key tile, which reads P_g from S_g's
+      // columns, is in the pipe before it)
+      auto scores = [&](int g, int t) -> bool {
+        const int s = t % K_STAGES;
+        if (!mbar_spin_wait(smem_u32(&k_full[s]), (t / K_STAGES) & 1, abort_flag)) return false;
+        tcgen05_fence_after();
+        const uint64_t qd = q_desc + g * (Q_BYTES >> 4), kd = k_desc + s * (KV_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < QK_STEPS; ++k) {
+          const uint64_t off = ((k / 4) * CHUNK_BYTES + (k % 4) * 32) >> 4;
+          umma(tmem_base + g * BN, qd + off, kd + off, idesc_qk, k > 0 ? 1u : 0u);
+        }
+        tcgen05_commit(smem_u32(&s_full[g]));
+        if (g == groups - 1) tcgen05_commit(smem_u32(&k_empty[s]));
+        return true;
+      };
+      // O_g += P_g V of key tile t, a part of the keys at a time
+      auto values = [&](int g, int t) -> bool {
+        const int s = t % V_STAGES;
+        if (!mbar_spin_wait(smem_u32(&v_full[s]), (t / V_STAGES) & 1, abort_flag)) return false;
+        const uint64_t vd = v_desc + s * (KV_BYTES >> 4);
+        const uint32_t o_addr = tmem_base + 2 * BN + g * 128, p_addr = tmem_base + g * BN;
+#pragma unroll
+        for (int h = 0; h < P_PARTS; ++h) {
+          if (!mbar_spin_wait(smem_u32(&p_full[g * P_PARTS + h]), t & 1, abort_flag)) return false;
+          tcgen05_fence_after();
+#pragma unroll
+          for (int i = 0; i < PV_STEPS; ++i) {
+            const int k = h * PV_STEPS + i;
+            umma_ts(o_addr, p_addr + k * 8, vd + ((k * 16 * 128) >> 4), idesc_pv, t > 0 || k > 0 ? 1u : 0u);
+          }
+        }
+        tcgen05_commit(smem_u32(&o_ready[g]));
+        if (g == groups - 1) tcgen05_commit(smem_u32(&v_empty[s]));
+        return true;
+      };
+      bool ok = mbar_spin_wait(smem_u32(q_full), 0, abort_flag);
+      for (int g = 0; ok && g < groups; ++g) ok = scores(g, 0);
+      for (int t = 0; ok && t < n_tiles; ++t)
+        for (int g = 0; ok && g < groups; ++g) {
+          ok = values(g, t);
+          if (ok && t + 1 < n_tiles) ok = scores(g, t + 1);
+        }
+    }
+  } else if (warp >= MAKER_WARP0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+    // thread r makes row r of every tile
+    const int r = threadIdx.x - MAKER_WARP0 * 32;
+    const int* bt = p.block_table + (size_t)max(b, 0) * p.table_stride;
+    struct Row { uint4 codes[W4]; uint32_t pair; };
+    struct Where { size_t row; bool live; };
+    // the row of the cache that tile t's key r stands in; live: it belongs to the block's range
+    auto find = [&](int t) -> Where {
+      const int j = (first_tile + t) * BN + r;
+      const bool live = t < n_tiles && j >= j_lo && j < j_hi;
+      int page = live ? bt[j >> p.page_shift] : 0;
+      if ((unsigned)page >= (unsigned)p.num_pages) {
+        ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_PAGE);
+        page = 0;
+      }
+      return {(((size_t)page * p.Hkv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1)), live};
+    };
+    auto read = [&](const uint4* codes, const Where& w, Row& row) {
+#pragma unroll
+      for (int i = 0; i < W4; ++i) row.codes[i] = w.live ? codes[w.row * W4 + i] : make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto write = [&](char* tile, const Row& row, uint32_t pair) {
+      const __nv_bfloat162 both = *reinterpret_cast<const __nv_bfloat162*>(&pair);
+      const __nv_bfloat162 scale = __low2bfloat162(both), zero = __high2bfloat162(both);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t w = i % 4 == 0 ? row.codes[i / 4].x : i % 4 == 1 ? row.codes[i / 4].y : i % 4 == 2 ? row.codes[i / 4].z : row.codes[i / 4].w;
+        *reinterpret_cast<uint4*>(tile + (i / 8) * CHUNK_BYTES + r * 128 + (((i % 8) ^ (r & 7)) << 4)) =
+            make_uint4(values2<0>(w, scale, zero), values2<1>(w, scale, zero), values2<2>(w, scale, zero), values2<3>(w, scale, zero));
+      }
+    };
+    constexpr uint32_t NAN_PAIR = 0x7fc07fc0u;
+    // the next tile's keys are on their way while this tile's values are made, and these while its keys are
+    Where at_k = find(0);
+    Row k, v;
+    read(p.kc, at_k, k);
+    uint32_t k_pair = at_k.live ? p.kp[at_k.row] : 0u, v_pair = at_k.live ? p.vp[at_k.row] : 0u;
+    bool ok = true;
+    auto hand_over = [&](uint64_t* full) {
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(full));
+    };
+    auto room = [&](uint64_t* empty, int round) -> bool {
+      const bool got = mbar_wait(smem_u32(empty), (round & 1) ^ 1, abort_flag);
+      return __all_sync(0xffffffffu, got);
+    };
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      read(p.vc, at_k, v);
+      const Where next_k = find(t + 1);
+      ok = room(&k_empty[t % K_STAGES], t / K_STAGES);
+      if (!ok) break;
+      const bool good = finite_pair(k_pair) && finite_pair(v_pair);
+      const uint32_t pair_of_v = good ? v_pair : 0u;
+      write(Ks + (t % K_STAGES) * KV_BYTES, k, good ? k_pair : NAN_PAIR);
+      hand_over(&k_full[t % K_STAGES]);
+      read(p.kc, next_k, k);
+      k_pair = next_k.live ? p.kp[next_k.row] : 0u;
+      v_pair = next_k.live ? p.vp[next_k.row] : 0u;
+      ok = room(&v_empty[t % V_STAGES], t / V_STAGES);
+      if (!ok) break;
+      write(Vs + (t % V_STAGES) * KV_BYTES, v, pair_of_v);
+      hand_over(&v_full[t % V_STAGES]);
+      at_k = next_k;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+    // one thread per row of query tile g
+    const int g = (warp - SOFTMAX_WARP0) >> 2;
+    if (g < groups && n_tiles > 0) {
+      const int q4 = warp & 3;
+      const int r = q4 * 32 + lane;
+      const int qg = q0 + g * QPT;                       // the tile's first query
+      const int nq = min(QPT, q_len - qg);
+      const int n_valid = QPT > 1 ? nq * GT : min(GT, G - g0);
+      const bool valid = r < n_valid;
+      const int qi = QPT > 1 ? r / GT : 0, gg = QPT > 1 ? r % GT : r;
+      const int pos = valid ? kv_len - q_len + qg + qi : -1;
+      const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      const uint32_t lane_addr = static_cast<uint32_t>(q4 * 32) << 16;
+      const uint32_t tmem_s = tmem_base + g * BN, tmem_o = tmem_base + 2 * BN + g * 128;
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int t = 0; t < n_tiles; ++t) {
+        const int j0 = (first_tile + t) * BN;
+        ok = mbar_wait(smem_u32(&s_full[g]), t & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tcgen05_fence_after();
+        const bool all_visible = j0 + BN - 1 <= pos && j0 >= lo;
+        float sv[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_load32_nowait(tmem_s + lane_addr + c, sv + c);
+        tmem_load_wait();
+        float sc = p.scale_log2;
+        if (p.cap2 > 0.f) {
+#pragma unroll
+          for (int e = 0; e < BN; ++e) {
+            const float x = ex2(sv[e] * p.cap_in * (2.f * LOG2E));
+            sv[e] = p.cap2 * (1.f - __fdividef(2.f, x + 1.f));
+          }
+          sc = 1.f;
+        }
+        if (!all_visible) {
+#pragma unroll
+          for (int e = 0; e < BN; ++e) {
+            const int j = j0 + e;
+            if (!(j <= pos && j >= lo)) sv[e] = -INFINITY;
+          }
+        }
+        // the row's maximum, four independent chains
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < BN; e += 4) {
+          mx4[0] = fmaxf(mx4[0], sv[e]);
+          mx4[1] = fmaxf(mx4[1], sv[e + 1]);
+          mx4[2] = fmaxf(mx4[2], sv[e + 2]);
+          mx4[3] = fmaxf(mx4[3], sv[e + 3]);
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        // the reference maximum only moves when the row's maximum has grown by more than 2^8: until then the probabilities are taken
+        // against the old reference and O needs no rescaling
+        const float m_cand = fmaxf(m, mx * sc);
+        const float m_new = (m_cand - m <= 8.f) ? m : m_cand;      // -inf - -inf: moves (to -inf), harmless
+        const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = ex2(m - m_safe);
+        // probabilities -> tensor memory, bfloat16 pairs over the first 64 columns of S_g, handed over in P_PARTS parts
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < P_PARTS; ++h) {
+#pragma unroll
+          for (int c = h * (BN / P_PARTS); c < (h + 1) * (BN / P_PARTS); c += 32) {
+            float packed[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = ex2(fmaf(sv[c + e], sc, -m_safe)), p1 = ex2(fmaf(sv[c + e + 1], sc, -m_safe));        // -inf gives 0
+              sum4[(e / 2) & 3] += p0 + p1;
+              packed[e / 2] = __uint_as_float(pack2(p0, p1));
+            }
+            tmem_store16(tmem_s + lane_addr + c / 2, packed);
+          }
+          if (h == 0 && t > 0 && !__all_sync(0xffffffffu, alpha == 1.f)) {
+            // O_g is rescaled once half of the scores have left their registers, 32 columns at a time
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float v[32];
+              tmem_load32(tmem_o + lane_addr + c, v);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] *= alpha;
+              tmem_store32(tmem_o + lane_addr + c, v);
+            }
+          }
+          tmem_store_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&p_full[g * P_PARTS + h]));
+        }
+        l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        m = m_new;
+      }
+      if (ok) {
+        ok = mbar_wait(smem_u32(&o_ready[g]), (n_tiles - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (ok) {
+        tcgen05_fence_after();
+        float alpha = 1.f;
+        if (p.sinks && valid) {       // (log2 domain, like the running maximum; O is scaled on its way out)
+          const float sk = p.sinks[kvh * G + g0 + gg] * LOG2E;
+          const float m_new = fmaxf(m, sk);
+          alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
+          l = l * alpha + exp2f(sk - m_new);
+        }
+        const float inv = l == 0.f ? 0.f : alpha / l;
+        bf16* dst = p.out + ((size_t)(q_begin + qg + qi) * p.H + kvh * G + g0 + gg) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float v[32];
+          tmem_load32(tmem_o + lane_addr + c, v);
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(dst + c + e) =
+                  make_uint4(pack2(v[e] * inv, v[e + 1] * inv), pack2(v[e + 2] * inv, v[e + 3] * inv),
+                             pack2(v[e + 4] * inv, v[e + 5] * inv), pack2(v[e + 6] * inv, v[e + 7] * inv));
+          }
+        }
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");
+  }
+}
+
+}  // namespace
+
+TS_EXPORT int ts_attention_int4_tcgen05_error() {
+  int flag = 0;
+  if (cudaMemcpyFromSymbol(&flag, g_error_flag, sizeof(int)) != cudaSuccess) return -1;
+  return flag;
+}
+
+// q [T, H, D] (strides in elements, of 16 bytes), out [T, H, D]; codes and pairs as for ts_int4_attention.  Requests of up to `few` queries are left
+// alone.
+TS_EXPORT int ts_int4_attention_tcgen05(const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
+                                        const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
+                                        int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
+                                        int window, float softcap, const float* sinks, int few, cudaStream_t stream) {
+  int shift = 0;
+  while (shift < 20 && (1 << shift) < page_size) ++shift;
+  TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && page_size == 1 << shift && num_pages > 0 && max_blocks > 0 && few >= 0,
+             "int4_attention_tcgen05: %d tokens of %d requests, %d heads on %d, pages of %d", T, B, H, Hkv, page_size);
+  TS_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes) & 15) == 0 && ((uintptr_t)k_pairs | (uintptr_t)v_pairs) % 4 == 0 &&
+                 (q_row * 2) % 16 == 0 && (q_head * 2) % 16 == 0 && q_row > 0 && q_head > 0, "int4_attention_tcgen05: operands must be 16-byte aligned");
+  const int G = H / Hkv;
+  Params p = {};
+  p.out = (bf16*)out; p.kc = (const uint4*)k_codes; p.vc = (const uint4*)v_codes; p.kp = (const uint32_t*)k_pairs; p.vp = (const uint32_t*)v_pairs;
+  p.block_table = block_table; p.cu_q = cu_q; p.kv_lens = kv_lens;
+  p.T = T; p.B = B; p.H = H; p.Hkv = Hkv; p.page_shift = shift; p.max_blocks = max_blocks; p.table_stride = table_stride; p.num_pages = num_pages;
+  p.few = few; p.window = window; p.sinks = sinks;
+  p.scale_log2 = scale * LOG2E;
+  p.cap2 = softcap > 0.f ? softcap * LOG2E : 0.f;
+  p.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+  p.heads_per_tile = G < BM ? G : BM;
+  p.queries_per_tile = G < BM ? BM / G : 1;
+  p.head_tiles = (G + p.heads_per_tile - 1) / p.heads_per_tile;
+  const long long gy = (long long)Hkv * p.head_tiles;
+  TS_REQUIRE(gy <= 65535, "int4_attention_tcgen05: too many head tiles");
+  // every request may end in a block that is not full; one of up to `few` queries has none
+  const int per_block = GROUPS * p.queries_per_tile;
+  const int with_tiles = T / (few + 1) < B ? T / (few + 1) : B;
+  const int blocks = T / per_block + with_tiles;
+  if (blocks == 0) return 0;
+  CUtensorMap mq;
+  {
+    EncodeTiledFn fn = encode_tiled();
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
+    const cuuint64_t strides[2] = {(cuuint64_t)q_head * 2, (cuuint64_t)q_row * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)p.heads_per_tile, (cuuint32_t)p.queries_per_tile}, elem[3] = {1, 1, 1};
+    TS_REQUIRE(fn && fn(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
+               "int4_attention_tcgen05: tensor map of q failed");
+  }
+  static SmemSet set;
+  const cudaError_t sized = set.to(int4_prefill_kernel, (int)SMEM);
+  if (sized != cudaSuccess) return ts_fail("int4_attention_tcgen05: %s", cudaGetErrorString(sized));
+  TS_LAUNCH("int4_attention_tcgen05", int4_prefill_kernel, dim3(blocks, (unsigned)gy), dim3(THREADS), SMEM, stream, mq, p);
+  return 0;
+}

@@ -658,6 +658,10 @@ def _attention_int4(head_dim: int):
     return build.load_unit("attention_int4.cu", {"TS_HEAD_DIM": head_dim})
 
 
+def _attention_int4_tcgen05(head_dim: int):
+    return build.load_unit("attention_int4_tcgen05.cu", {"TS_HEAD_DIM": head_dim})
+
+
 def gemm_int8_error() -> int:
     """1 if a block of the 8-bit product ever gave up on a wait (synchronises)."""
     return _gemm_int8().ts_gemm_int8_error()
@@ -675,6 +679,7 @@ def units_for(head_dims, key_dims=(), delta_dims=()) -> list:
     units += [("attention_tcgen05.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims))
               if d in TCGEN05_HEAD_DIMS]
     units += [("attention_int4.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims))]
+    units += [("attention_int4_tcgen05.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims)) if d in TCGEN05_HEAD_DIMS]
     units += [("linear_attention.cu", {"TS_KEY_DIM": d}) for d in sorted(set(key_dims))]
     units += [("delta_rule.cu", {"TS_KEY_DIM": d}) for d in sorted(set(delta_dims))]
     return units
@@ -2577,14 +2582,16 @@ _INT4_ENTRIES = {
     "ts_int4_rope_kvwrite": (_INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR, _PTR, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR,
                              _PTR, _INT, _INT, _PTR),
     "ts_int4_attention": (_INT, _PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
-                          _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR, _PTR, _INT, _INT, _PTR),
+                          _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR, _PTR, _INT, _INT, _INT, _PTR),
+    "ts_int4_attention_tcgen05": (_PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
+                                  _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR),
 }
 
 
 @functools.lru_cache(maxsize=None)
 def _entry(unit, name):
     """(library, entry point) of the 8-bit products (``unit`` 0) or of a head size over a 4-bit cache."""
-    lib = _gemm_int8() if unit == 0 else _attention_int4(unit)
+    lib = _gemm_int8() if unit == 0 else _attention_int4_tcgen05(unit) if name.endswith("_tcgen05") else _attention_int4(unit)
     fn = getattr(lib, name)
     fn.argtypes = (_INT8_ENTRIES if unit == 0 else _INT4_ENTRIES)[name]
     return lib, fn
@@ -2809,13 +2816,22 @@ def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary
 
 
 def int4_attention_error(head_dim: int) -> int:
-    """1 if a block of the tensor-core kernel over a 4-bit cache ever gave up on a wait (synchronises)."""
-    return _attention_int4(head_dim).ts_int4_attention_error()
+    """1 if a block of the tensor-core kernels over a 4-bit cache ever gave up on a wait (synchronises)."""
+    portions = _attention_int4_tcgen05(head_dim).ts_attention_int4_tcgen05_error() if head_dim in TCGEN05_HEAD_DIMS else 0
+    return _attention_int4(head_dim).ts_int4_attention_error() or portions
 
 
 def int4_attention_backend(dtype, head_dim) -> str:
-    """Which kernel attends over a 4-bit cache: "mma" (tensor cores: bfloat16 heads in steps of 32 up to 256) or "simt"."""
-    return "mma" if dtype == torch.bfloat16 and head_dim % 32 == 0 and head_dim <= 256 else "simt"
+    """Which kernels attend over a 4-bit cache: "mma" (mma.sync: bfloat16 heads in steps of 32 up to 256), "tcgen05" (requests with
+    more queries than ``INT4_DIRECT_ROWS`` rows hold on the tcgen05 kernel, the others as "mma") or "simt" (the 32-bit kernel)."""
+    if dtype != torch.bfloat16 or head_dim % 32 or head_dim > 256:
+        return "simt"
+    return "tcgen05" if head_dim in TCGEN05_HEAD_DIMS else "mma"
+
+
+#: rows (queries x heads of a key head) of a request that one pass of the mma kernel over its keys takes; a request with
+#: more of them goes to the tcgen05 kernel, where there is one
+INT4_DIRECT_ROWS = 16
 
 
 def int4_decode_splits(blocks, max_kv_len):
@@ -2854,7 +2870,7 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     _int32_row(what, kv_lens, "kv_lens", B)
     chosen = int4_attention_backend(dtype, D)
     if backend is not None:
-        if backend not in (chosen, "simt"):
+        if backend not in (chosen, "simt") and (backend, chosen) != ("mma", "tcgen05"):
             raise ValueError(f"attention backend {backend!r} does not take {dtype}, head size {D} and a 4-bit cache")
         chosen = backend
     stream = _here(what, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, table, cu_q, kv_lens, sinks)
@@ -2865,12 +2881,22 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     max_q_len, span = ctx.max_q_len, ctx.max_kv_len
     if window:
         span = min(span, window)
-    columns = 0
-    if chosen == "mma":
+    most = columns = 0
+    if chosen != "simt":
+        few = max(1, INT4_DIRECT_ROWS // G)
+        if chosen == "tcgen05" and max_q_len > few and scale > 0 and (q.data_ptr() | 2 * q_row | 2 * q_head) % 16 == 0 and q_row > 0 and q_head > 0:
+            tc, portions = _entry(D, "ts_int4_attention_tcgen05")
+            _launched(tc, portions(q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
+                                   v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H,
+                                   Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, few,
+                                   stream), 1)
+            if B == 1 or T == B * max_q_len:
+                return out           # (no request has fewer queries than the longest)
+            most = max_q_len = few
         rows = max_q_len * G
         columns = 16 if rows > 8 and D <= 128 else 8
         if -(-rows // columns) * Hkv > 65535 or B > 65535 or page < 4 or (k_cache.pairs.data_ptr() | v_cache.pairs.data_ptr()) % 16:
-            columns = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes it)
+            columns = most = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes everything)
     if num_splits is None:
         num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
     part_o = part_ml = None
@@ -2881,5 +2907,5 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     _launched(lib, fn(_DTYPE[dtype], q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                       v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H, Hkv, page,
                       blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, num_splits, part_o, part_ml,
-                      max_q_len, columns, stream), 1 if num_splits == 1 else 2)
+                      max_q_len, columns, most, stream), 1 if num_splits == 1 else 2)
     return out

@@ -253,6 +253,8 @@ class Attention(Mixer):
     takes_cache_bits = True
 
     def work_tile_queries(self, dtype, page_size):
+        if self.cache_bits:
+            return 0          # (the kernels over a 4-bit cache find their requests on the device)
         return ops.prefill_tile_queries(dtype, self.num_heads * self.maps, self.num_kv_heads * self.maps, self.stored_dim,
                                         page_size)
 
