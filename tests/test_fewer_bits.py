@@ -56,8 +56,8 @@ def test_cuts_along_k_are_never_empty():
     for M in (1, 17, 64, 65, 5000):
         for N in (1, 128, 1000, 4096, 24576):
             for K in (1, 128, 129, 1000, 4096, 12288, 131072):
-                s, slices = ops.int8_splits(M, N, K), -(-K // 128)
-                assert 1 <= s <= 8 and (s - 1) * -(-slices // s) < slices
+                (tile, s), slices = ops.int8_plan(M, N, K), -(-K // 128)
+                assert (tile, s) == (256, 0) or (tile in (16, 32, 64, 128) and 1 <= s <= 8 and (s - 1) * -(-slices // s) < slices)
 
 
 def test_pages_in_4_bits():

@@ -10,6 +10,7 @@
 // One shift and one AND-OR then make a pair of neighbouring columns as two bfloat16 (see `codes2` in the kernels below).
 // Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
 // a token for heads of 128 where bfloat16 takes 256.
+#include "pairs.cuh"
 #include "tcgen05.cuh"
 
 #ifndef TS_HEAD_DIM
@@ -77,6 +78,7 @@ struct RowRange {
   }
 };
 
+__device__ __noinline__ uint32_t divided_code(float y, float scale) { return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(y, scale)), 0.f), 15.f); }
 // a row that its LANES lanes hold, to the slot of its token
 __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)[WORDS][8], RowRange r, int which, int head, int t, int lane) {
   const int slot = p.slot_mapping[t];
@@ -100,12 +102,22 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
       // the quotient rounded to 32 bits decides; the product with the reciprocal is off by 3 roundings of at most 16, so a division is
       // only made next to a half, and where the reciprocal could overflow
       const float inverse = 1.f / scale;
+      float furthest = scale > 1e-30f ? 0.f : 1.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float y = __fsub_rn(x[w][i], zero);
-        float r = y * inverse;
-        if (fabsf(fabsf(r - rintf(r)) - 0.5f) < 1e-4f || !(scale > 1e-30f)) r = __fdiv_rn(y, scale);
-        bits |= (uint32_t)fminf(fmaxf(rintf(r), 0.f), 15.f) << shift_of(i);
+        // (adding 1.5 2^23 rounds to a whole number, halves to even, and leaves it in the low bits)
+        const float r = fminf(fmaxf(__fsub_rn(x[w][i], zero) * inverse, 0.f), 15.f), t = r + 12582912.f;
+        furthest = fmaxf(furthest, fabsf(r - (t - 12582912.f)));
+        bits |= (__float_as_uint(t) & 15u) << shift_of(i);
+      }
+      if (furthest > 0.49995f) {
+        bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float y = __fsub_rn(x[w][i], zero), r = fminf(fmaxf(y * inverse, 0.f), 15.f), t = r + 12582912.f;
+          const bool near = fabsf(r - (t - 12582912.f)) > 0.49995f || !(scale > 1e-30f);
+          bits |= (near ? divided_code(y, scale) : __float_as_uint(t) & 15u) << shift_of(i);
+        }
       }
     }
     (which ? p.vc : p.kc)[at * W + word] = bits;
@@ -520,13 +532,6 @@ __device__ __forceinline__ void mma_lo(int (&c)[4], uint32_t a0, uint32_t a1, ui
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// pairs of 32-bit numbers: one instruction for both
-struct F2 { unsigned long long v; };
-__device__ __forceinline__ F2 f2(float x, float y) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
-__device__ __forceinline__ void f2_out(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 // codes number e (0 .. 3) of both halves of a word as two bfloat16 numbers 16 + c
 template <int E>
 __device__ __forceinline__ uint32_t codes2(uint32_t word) {

@@ -10,6 +10,7 @@
 // slice of K of 128 codes is 128 bytes, one swizzle row, so that shared memory, the TMA boxes and the four MMAs of a slice (32 bytes of
 // K each) are those of 64 bfloat16.  K is cut over the blocks of a cluster, which add their integer sums through distributed shared
 // memory: no scratch, no counters, nothing that two launches could share.
+#include "pairs.cuh"
 #include "tcgen05.cuh"
 
 TS_DEFINE_LAST_ERROR()
@@ -31,20 +32,74 @@ struct QuantParams {
   int K;
 };
 
-// round(x / scale) of the quotient rounded to 32 bits.  x times the reciprocal is off by three roundings of at most 127, 2.3e-5: a
-// division is only made where that could matter, next to a half (2 in 10,000), and where the reciprocal could overflow.
-__device__ __forceinline__ int code_of(float x, float scale, float inverse) {
-  float r = x * inverse;
-  if (fabsf(fabsf(r - rintf(r)) - 0.5f) < 1e-4f || !(scale > 1e-30f)) r = __fdiv_rn(x, scale);
-  return (int)fminf(fmaxf(rintf(r), -127.f), 127.f);
+// Eight neighbouring elements of a row as they lie in memory; `top` keeps the largest magnitude as bits, where an infinity or a NaN is larger than
+// every number.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ __forceinline__ static uint32_t largest(uint32_t top, float x) { return max(top, __float_as_uint(x) & 0x7fffffffu); }
+  __device__ __forceinline__ void look(uint32_t& top) const {
+    top = largest(largest(largest(largest(top, a.x), a.y), a.z), a.w);
+    top = largest(largest(largest(largest(top, b.x), b.y), b.z), b.w);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const { x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w; }
+  __device__ __forceinline__ static uint32_t bits(uint32_t top) { return top; }
+};
+template <> struct Eight<bf16> {
+  uint4 raw;
+  __device__ __forceinline__ void load(const bf16* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void look(uint32_t& top) const {          // (two magnitudes of 16 bits)
+    top = __vmaxu2(__vmaxu2(top, raw.x & 0x7fff7fffu), raw.y & 0x7fff7fffu);
+    top = __vmaxu2(__vmaxu2(top, raw.z & 0x7fff7fffu), raw.w & 0x7fff7fffu);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  __device__ __forceinline__ static uint32_t bits(uint32_t top) { return max(top << 16, top & 0xffff0000u); }
+};
+
+// round(x / scale) of the quotient rounded to 32 bits, as a byte.  x times the reciprocal is off by three roundings of at most 127, 2.3e-5: a
+// division is only made where that could matter, next to a half (1 in 10,000), and where the reciprocal could overflow.  Adding 1.5 2^23
+// rounds to a whole number, halves to even, and leaves it in the low bits.
+constexpr float ROUNDER = 12582912.f;
+__device__ __noinline__ uint32_t divided_code(float x, float scale) {
+  return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f) & 255u;
+}
+__device__ __forceinline__ uint32_t code_of(float x, float scale, float inverse) {
+  const float r = x * inverse, t = r + ROUNDER;
+  return fabsf(r - (t - ROUNDER)) > 0.49995f || !(scale > 1e-30f) ? divided_code(x, scale) : __float_as_uint(t) & 255u;
+}
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inverse) {
+  uint32_t c[8];
+  float furthest = scale > 1e-30f ? 0.f : 1.f;
+  const F2 inv = f2(inverse, inverse), up = f2(ROUNDER, ROUNDER), down = f2(-ROUNDER, -ROUNDER), minus = f2(-1.f, -1.f);
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const F2 r = f2_mul(f2(x[e], x[e + 1]), inv), t = f2_add(r, up), off = f2_fma(f2_add(t, down), minus, r);
+    float o0, o1, t0, t1;
+    f2_out(off, o0, o1);
+    f2_out(t, t0, t1);
+    furthest = fmaxf(furthest, fmaxf(fabsf(o0), fabsf(o1)));
+    c[e] = __float_as_uint(t0);
+    c[e + 1] = __float_as_uint(t1);
+  }
+  if (furthest > 0.49995f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = code_of(x[e], scale, inverse);
+  }
+  // (the low bytes of four words side by side)
+  return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
 }
 
 // a block a row; KEPT: steps that stay in registers (0: the row is read twice)
 template <typename T, int KEPT>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParams p, bool vec) {
-  __shared__ float tops[QUANT_THREADS / 32];
-  __shared__ int bads[QUANT_THREADS / 32];
-  const int threads = blockDim.x;
+  __shared__ uint32_t tops[QUANT_THREADS / 32];
+  const int threads = blockDim.x, warps = threads / 32;
   // The trigger comes behind the wait: what the kernel after this one reads before its own wait (the codes of the weights) is
   // then complete, whoever wrote it.
   pdl_wait();
@@ -53,50 +108,38 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParam
   const T* x = static_cast<const T*>(p.x) + m * p.ldx;
   signed char* out = p.codes + m * p.ldq;
   const int n8 = vec ? p.K / 8 : 0;
-  float top = 0.f;
-  int bad = 0;
-  float kept[KEPT > 0 ? KEPT : 1][8];
-  auto look = [&](const float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      top = fmaxf(top, fabsf(v[e]));
-      bad |= !(fabsf(v[e]) <= 3.402823466e38f);
-    }
-  };
+  uint32_t top = 0;
+  Eight<T> kept[KEPT > 0 ? KEPT : 1];
   if constexpr (KEPT > 0) {
 #pragma unroll
     for (int k = 0; k < KEPT; ++k)
-      if (threadIdx.x + k * threads < n8) load8<T>(x + (threadIdx.x + k * threads) * 8, kept[k]);
+      if (threadIdx.x + k * threads < n8) kept[k].load(x + (threadIdx.x + k * threads) * 8);
 #pragma unroll
     for (int k = 0; k < KEPT; ++k)
-      if (threadIdx.x + k * threads < n8) look(kept[k]);
+      if (threadIdx.x + k * threads < n8) kept[k].look(top);
   } else {
     for (int i = threadIdx.x; i < n8; i += threads) {
-      load8<T>(x + i * 8, kept[0]);
-      look(kept[0]);
+      kept[0].load(x + i * 8);
+      kept[0].look(top);
     }
   }
-  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += threads) {
-    const float v = to_f32<T>(x[i]);
-    top = fmaxf(top, fabsf(v));
-    bad |= !(fabsf(v) <= 3.402823466e38f);
+  top = Eight<T>::bits(top);
+  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += threads) top = Eight<float>::largest(top, to_f32<T>(x[i]));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (warps > 1) {
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, tops[(threadIdx.x & 31) % warps]);
   }
-  top = warp_max(top);
-  bad = __any_sync(0xffffffffu, bad);
-  if ((threadIdx.x & 31) == 0) { tops[threadIdx.x >> 5] = top; bads[threadIdx.x >> 5] = bad; }
-  __syncthreads();
-  for (int w = 0; w < threads / 32; ++w) { top = fmaxf(top, tops[w]); bad |= bads[w]; }
-  const float scale = __fdiv_rn(top, 127.f);
+  const bool bad = top >= 0x7f800000u;
+  const float scale = __fdiv_rn(__uint_as_float(top), 127.f);
   const bool zero = bad || !(scale > 0.f);
   if (threadIdx.x == 0) p.scales[m] = bad ? __int_as_float(0x7fc00000) : scale;
   const float inverse = 1.f / scale;
-  auto write = [&](const float (&v)[8], int i) {
-    uint32_t w[2] = {0u, 0u};
-    if (!zero) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(code_of(v[e], scale, inverse) & 255) << (8 * (e & 3));
-    }
-    *reinterpret_cast<uint2*>(out + i * 8) = make_uint2(w[0], w[1]);
+  auto write = [&](const Eight<T>& at, int i) {
+    float v[8];
+    at.get(v);
+    *reinterpret_cast<uint2*>(out + i * 8) = zero ? make_uint2(0u, 0u) : codes_of(v, scale, inverse);
   };
   if constexpr (KEPT > 0) {
 #pragma unroll
@@ -104,12 +147,11 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParam
       if (threadIdx.x + k * threads < n8) write(kept[k], threadIdx.x + k * threads);
   } else {
     for (int i = threadIdx.x; i < n8; i += threads) {
-      load8<T>(x + i * 8, kept[0]);
+      kept[0].load(x + i * 8);
       write(kept[0], i);
     }
   }
-  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += threads)
-    out[i] = zero ? 0 : (signed char)code_of(to_f32<T>(x[i]), scale, inverse);
+  for (int i = n8 * 8 + threadIdx.x; i < p.K; i += threads) out[i] = zero ? 0 : (signed char)code_of(to_f32<T>(x[i]), scale, inverse);
 }
 
 // ------------------------------------------------------------------------------------------ the product
@@ -141,11 +183,11 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_load8_int(uint32_t addr, int (&v)[8]) {
-  float f[8];
-  tmem_load8(addr, f);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __float_as_int(f[i]);
+// four words of a peer's shared memory, at the place that `own_shared` names in this block's
+__device__ __forceinline__ void cluster_store4(uint32_t own_shared, uint32_t rank, int a, int b, int c, int d) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(own_shared), "r"(rank));
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 template <int TILE_T> struct Cfg {
@@ -154,7 +196,7 @@ template <int TILE_T> struct Cfg {
   static constexpr int STAGES = RING / STAGE_BYTES > 6 ? 6 : RING / STAGE_BYTES;
   static constexpr int TMEM_COLS = TILE_T < 32 ? 32 : TILE_T;
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 256;
-  static_assert(STAGES >= 3 && STAGES * STAGE_BYTES >= TILE_T * TILE_N * 4, "the ring holds the block's sums");
+  static_assert(STAGES >= 3 && STAGES * STAGE_BYTES >= (TILE_T + 4 * MAX_SPLITS) * TILE_N * 4, "the ring holds what the cluster sends");
 };
 
 template <int TILE_T>
@@ -170,7 +212,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int n_tile = blockIdx.x, t_tile = blockIdx.y, split = blockIdx.z;
+  const int t_tile = blockIdx.x, n_tile = blockIdx.y, split = blockIdx.z;          // the blocks that share a weight tile run together
   const int warp = threadIdx.x >> 5;
   const int kb_total = (p.K + BK - 1) / BK, per = (kb_total + p.splits - 1) / p.splits;
   const int kb0 = split * per, nkb = max(0, min(kb_total, kb0 + per) - kb0);
@@ -194,6 +236,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   tcgen05_fence_after();
   pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
+  __shared__ float sx[TILE_T];          // (from global memory, a row's scale was waited for at every store: 5 us of 130 tokens x 1,024 on 4,096 rows)
 
   if (threadIdx.x == 0) {
     // loader: one slice of K per stage
@@ -243,6 +286,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (ok && nkb > 0) tcgen05_commit(smem_u32(accum));
   } else {
     pdl_wait();
+    for (int j = (int)threadIdx.x - 64; j >= 0 && j < TILE_T; j += 64) sx[j] = t_tile * TILE_T + j < p.M ? p.sx[t_tile * TILE_T + j] : 0.f;
   }
   __syncthreads();
 
@@ -255,44 +299,79 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const uint32_t taddr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
   const float sw = n < p.N ? p.sw[n] : 0.f;
   const float bn = p.bias.ptr != nullptr && n < p.N ? p.bias[n] : 0.f;
-  auto put = [&](int m, int sum) {
-    float y = (float)sum * (p.sx[m] * sw) + bn;
-    if (p.out_f32) static_cast<float*>(p.out)[m * p.ldc + n] = y;
-    else static_cast<bf16*>(p.out)[m * p.ldc + n] = __float2bfloat16_rn(y);
+  auto put = [&](int j, int sum) {          // token j of the tile
+    const float y = (float)sum * (sx[j] * sw) + bn;
+    if (p.out_f32) static_cast<float*>(p.out)[(t0 + j) * p.ldc + n] = y;
+    else static_cast<bf16*>(p.out)[(t0 + j) * p.ldc + n] = __float2bfloat16_rn(y);
   };
+  constexpr int COLS = TILE_T < 32 ? TILE_T : 32;           // tokens taken from tensor memory at a time
+  auto take = [&](int c, int (&v)[COLS]) {
+    if (!have) {
+#pragma unroll
+      for (int i = 0; i < COLS; ++i) v[i] = 0;
+    } else if constexpr (COLS == 32) {
+      float f[32];
+      tmem_load32(taddr + c, f);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_int(f[i]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < COLS; h += 8) {
+        float f[8];
+        tmem_load8(taddr + c + h, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[h + i] = __float_as_int(f[i]);
+      }
+    }
+  };
+  const int live = min(TILE_T, p.M - t0);
   if (p.splits == 1) {
 #pragma unroll 1
-    for (int c = 0; c < TILE_T && t0 + c < p.M; c += 8) {
-      int v[8] = {};
-      if (have) tmem_load8_int(taddr + c, v);
+    for (int c = 0; c < live; c += COLS) {
+      int v[COLS];
+      take(c, v);
       if (n < p.N) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t0 + c + i < p.M) put(t0 + c + i, v[i]);
+        for (int i = 0; i < COLS; ++i)
+          if (c + i < live) put(c + i, v[i]);
       }
     }
   } else {
-    // every block of the cluster leaves its sums in its shared memory (the ring is idle); rank r then owns the tokens r, r + splits, ..
-    int* red = reinterpret_cast<int*>(smem);               // [TILE_T][TILE_N]
+    // Once no block of the cluster reads its ring any more, every block sends its sums to the block that owns the token (rank r: `own` tokens
+    // in a row from r own on, a multiple of four), which adds them up from its own shared memory.  (Loads from the peers instead, eight
+    // in flight a thread, take a trip through the cluster for every token: 256 tokens x 4,096 on 4,096 rows 21 us.)
+    const int own = ((live + p.splits - 1) / p.splits + 3) & ~3;
+    const uint32_t box = smem_u32(smem);                    // [sender][weight row][token of mine]
+    cluster_arrive();
+    cluster_wait();
 #pragma unroll 1
-    for (int c = 0; c < TILE_T; c += 8) {
-      int v[8] = {};
-      if (have) tmem_load8_int(taddr + c, v);
+    for (int c = 0; c < live; c += COLS) {
+      int v[COLS];
+      take(c, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) red[(c + i) * TILE_N + threadIdx.x] = v[i];
+      for (int i = 0; i < COLS; i += 4) {
+        const int j = c + i, owner = j / own;
+        if (j < live) cluster_store4(box + ((split * TILE_N + threadIdx.x) * own + j - owner * own) * 4, owner, v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
     }
     cluster_arrive();
     cluster_wait();
-    for (int j = split; j < TILE_T && t0 + j < p.M; j += p.splits) {
-      int sum = 0;
+    const int4* sums = reinterpret_cast<const int4*>(smem);
+    for (int j = 0; j < own && split * own + j < live; j += 4) {
+      int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll
       for (int s = 0; s < MAX_SPLITS; ++s)
-        if (s < p.splits) sum += __float_as_int(cluster_load_f32(reinterpret_cast<const float*>(red) + j * TILE_N + threadIdx.x, s));
-      if (n < p.N) put(t0 + j, sum);
+        if (s < p.splits) {
+          const int4 x = sums[((s * TILE_N + threadIdx.x) * own + j) >> 2];
+          sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+        }
+      if (n < p.N) {
+        const int at = split * own + j, v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at + i < live) put(at + i, v[i]);
+      }
     }
-    // no block leaves while a peer may still read its shared memory
-    cluster_arrive();
-    cluster_wait();
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -319,17 +398,17 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const I8Params& p
   static SmemSet set;
   const cudaError_t sized = set.to(gemm_i8_kernel<TILE_T>, (int)Cfg<TILE_T>::SMEM);
   if (sized != cudaSuccess) return ts_fail("gemm_int8: %s", cudaGetErrorString(sized));
-  const dim3 grid((p.N + TILE_N - 1) / TILE_N, (p.M + TILE_T - 1) / TILE_T, p.splits);
+  const dim3 grid((p.M + TILE_T - 1) / TILE_T, (p.N + TILE_N - 1) / TILE_N, p.splits);
   const cudaError_t e = ts_launch_cluster(gemm_i8_kernel<TILE_T>, grid, dim3(THREADS), Cfg<TILE_T>::SMEM, stream, dim3(1, 1, p.splits), map_w, map_x, p);
   if (e != cudaSuccess) return ts_fail("gemm_int8 (clusters of %d): %s", p.splits, cudaGetErrorString(e));
   return 0;
 }
 
-int tile_tokens(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
-
 template <typename T>
 int launch_quantize(const QuantParams& p, bool vec, int M, cudaStream_t stream) {
-  const int n8 = (p.K + 7) / 8, threads = n8 >= QUANT_THREADS ? QUANT_THREADS : (n8 + 31) / 32 * 32;
+  // many rows: fewer threads with more of a row each (a block is short, and there are enough of them); few rows: as many as there are
+  const int n8 = (p.K + 7) / 8, share = M >= 512 ? (n8 + QUANT_KEPT - 1) / QUANT_KEPT : n8;
+  const int threads = share >= QUANT_THREADS ? QUANT_THREADS : (share + 31) / 32 * 32;
   if (!vec || n8 > QUANT_KEPT * threads) TS_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 0>), dim3(M), dim3(vec ? threads : QUANT_THREADS), 0, stream, p, vec);
   else if (n8 <= threads) TS_LAUNCH("quantize_rows", (quantize_rows_kernel<T, 1>), dim3(M), dim3(threads), 0, stream, p, vec);
   else TS_LAUNCH("quantize_rows", (quantize_rows_kernel<T, QUANT_KEPT>), dim3(M), dim3(threads), 0, stream, p, vec);
@@ -361,15 +440,15 @@ TS_EXPORT int ts_quantize_rows(int dtype, const void* x, long long ldx, void* co
 
 // out [M, N] (ldc; float where out_f32, else bfloat16) from codes and scales of x and w (leading dimensions multiples of 16).
 // x_dtype >= 0: x is a tensor of that type (leading dimension ldx) whose rows are brought to cx, sx first; -1: cx and sx are given.
-// w_constant: nobody that may still run writes w (with x_dtype >= 0 the first launch sees to that).
+// tile_t: tokens of a tile (16, 32, 64 or 128); splits: cuts along K (a cluster of up to 8 blocks).  w_constant: nobody that may still run writes w (with x_dtype >= 0 the first launch sees to that).
 TS_EXPORT int ts_gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, long long ldcx, float* sx, const void* cw, long long ldw,
                            const float* sw, const void* bias, int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K,
-                           int splits, int w_constant, cudaStream_t stream) {
+                           int tile_t, int splits, int w_constant, cudaStream_t stream) {
   TS_REQUIRE(M > 0 && N > 0 && K > 0 && K <= 131072, "gemm_int8: M=%d N=%d K=%d (K up to 131072: the sums are 32-bit integers)", M, N, K);
   TS_REQUIRE((ldcx | ldw) % 16 == 0 && (((uintptr_t)cx | (uintptr_t)cw) & 15) == 0, "gemm_int8: rows of codes begin on 16 bytes");
   TS_REQUIRE(splits >= 1 && splits <= MAX_SPLITS, "gemm_int8: splits out of range");
-  const int tile_t = tile_tokens(M);
-  TS_REQUIRE((M + tile_t - 1) / tile_t <= 65535, "gemm_int8: too many rows");
+  TS_REQUIRE(tile_t == 16 || tile_t == 32 || tile_t == 64 || tile_t == 128, "gemm_int8: tiles of %d tokens", tile_t);
+  TS_REQUIRE((N + TILE_N - 1) / TILE_N <= 65535, "gemm_int8: too many outputs");
   if (x_dtype >= 0) {
     TS_REQUIRE(x_dtype == TS_F32 || x_dtype == TS_BF16, "gemm_int8: unknown dtype %d", x_dtype);
     const int rc = quantize(x_dtype, x, ldx, cx, ldcx, sx, M, K, stream);

@@ -651,6 +651,10 @@ def _gemm_int8():
     return build.load_unit("gemm_int8.cu")
 
 
+def _gemm_int8_pair():
+    return build.load_unit("gemm_int8_pair.cu")
+
+
 def _attention_int4(head_dim: int):
     if head_dim not in SUPPORTED_HEAD_DIMS:
         raise ValueError(f"head size {head_dim} is not supported: attention takes multiples of 16 "
@@ -663,8 +667,8 @@ def _attention_int4_tcgen05(head_dim: int):
 
 
 def gemm_int8_error() -> int:
-    """1 if a block of the 8-bit product ever gave up on a wait (synchronises)."""
-    return _gemm_int8().ts_gemm_int8_error()
+    """1 if a block of the 8-bit products ever gave up on a wait (synchronises)."""
+    return _gemm_int8().ts_gemm_int8_error() or _gemm_int8_pair().ts_gemm_int8_pair_error()
 
 
 def units_for(head_dims, key_dims=(), delta_dims=()) -> list:
@@ -672,7 +676,7 @@ def units_for(head_dims, key_dims=(), delta_dims=()) -> list:
     its matrix-state mixers and these of its delta-rule mixers needs."""
     units = [("elementwise.cu", {}), ("gemm_simt.cu", {}), ("gemm_tcgen05.cu", {}), ("gemm_pair_tcgen05.cu", {}),
              ("gemv_mma.cu", {}), ("sampler.cu", {}), ("latent_moe.cu", {}), ("sequence.cu", {}), ("streams.cu", {}),
-             ("gemm_int8.cu", {})]
+             ("gemm_int8.cu", {}), ("gemm_int8_pair.cu", {})]
     units += [("attention_simt.cu", {"TS_HEAD_DIM": d}) for d in sorted(set(head_dims))]
     units += [("attention_mma.cu", _mma_defines(d)) for d in sorted(set(head_dims))
               if d <= MMA_MAX_HEAD_DIM]
@@ -2575,7 +2579,8 @@ def delta_rule(q, k, v, gate, logits, bias, rate, state, ctx, num_heads, key_dim
 _INT, _LONG, _PTR, _FLOAT = c_int, c_longlong, c_void_p, c_float
 _INT8_ENTRIES = {
     "ts_quantize_rows": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _INT, _INT, _PTR),
-    "ts_gemm_int8": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _PTR, _LONG, _PTR, _PTR, _INT, _PTR, _LONG, _INT, _INT, _INT, _INT, _INT, _INT, _PTR),
+    "ts_gemm_int8": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _PTR, _LONG, _PTR, _PTR, _INT, _PTR, _LONG, _INT, _INT, _INT, _INT, _INT, _INT, _INT, _PTR),
+    "ts_gemm_int8_pair": (_PTR, _LONG, _PTR, _PTR, _LONG, _PTR, _PTR, _INT, _PTR, _LONG, _INT, _INT, _INT, _INT, _INT, _PTR),
 }
 _INT4_ENTRIES = {
     "ts_int4_kvwrite": (_INT, _PTR, _PTR, _LONG, _LONG, _LONG, _LONG, _INT, _INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR),
@@ -2591,7 +2596,7 @@ _INT4_ENTRIES = {
 @functools.lru_cache(maxsize=None)
 def _entry(unit, name):
     """(library, entry point) of the 8-bit products (``unit`` 0) or of a head size over a 4-bit cache."""
-    lib = _gemm_int8() if unit == 0 else _attention_int4_tcgen05(unit) if name.endswith("_tcgen05") else _attention_int4(unit)
+    lib = _gemm_int8_pair() if name == "ts_gemm_int8_pair" else _gemm_int8() if unit == 0 else _attention_int4_tcgen05(unit) if name.endswith("_tcgen05") else _attention_int4(unit)
     fn = getattr(lib, name)
     fn.argtypes = (_INT8_ENTRIES if unit == 0 else _INT4_ENTRIES)[name]
     return lib, fn
@@ -2676,14 +2681,25 @@ def quantize_rows(x) -> Int8Rows:
     return Int8Rows(codes, scales)
 
 
-def int8_splits(M, N, K):
-    """Cuts along K of the 8-bit product: a product with few row tiles fills the places of two blocks an SM, with at
-    least two slices of 128 a cut; the cuts of a tile are a cluster of up to 8 blocks."""
-    tile_t = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
-    tiles = -(-N // 128) * -(-M // tile_t)
-    slices = -(-K // 128)
-    splits = max(1, min(2 * num_sms() // tiles, slices // 2, 8))
-    return -(-slices // -(-slices // splits))           # no cut without a slice
+def int8_plan(M, N, K):
+    """(tokens of a tile, cuts along K) of the 8-bit product; cuts 0: on pairs of SMs (csrc/gemm_int8_pair.cu).
+
+    Up to 64 tokens are one tile.  More are cut into tiles of 64 as long as all tiles have a place (two blocks an SM), else pairs of SMs share
+    wide ones (us, tiles of 64 / pairs: 512 x 12288 on 4096 33.9 / 35.4, 512 x 1024 on 4096 8.1 / 9.4; 400 x 4096 on 6144 25.6 / 17.8, 256 x 4096 on
+    24576 46.5 / 31.9, 2048 x 1024 on 6144 45 / 22.4); up to 128 tokens in one tile of 128 come first there (100 x 4096 on 24576 26.3 / 30.3).
+    K is cut, in powers of two, where the tiles leave more than half of the SMs idle and a cut keeps eight slices of 128 (us, whole / cut: 8 x
+    4096 on 4096 9.2 / 6.4 by four, 32 x 4096 on 6144 10.8 / 8.9 by four, 64 x 12288 on 4096 31 / 17.9 by eight; 96 tiles, 128 x 4096
+    on 6144, 14.2 / 15.7 by two; 8 slices, 1 x 1024 on 4096, 3.7 / 3.9; in sixths 32 x 4096 on 6144 takes 15.4: clusters of six find no place)."""
+    tile_t = 16 if M <= 16 else 32 if M <= 32 else 64
+    row_tiles, slices = -(-N // 128), -(-K // 128)
+    tiles = row_tiles * -(-M // tile_t)
+    if M > 64 and tiles > 2 * num_sms():
+        return (128, 1) if M <= 128 and row_tiles <= 2 * num_sms() else (256, 0)
+    splits = 1
+    if 2 * tiles <= num_sms():
+        while splits < 8 and 2 * splits * tiles <= 2 * num_sms() and slices >= 16 * splits:
+            splits *= 2
+    return tile_t, -(-slices // -(-slices // splits))           # no cut without a slice
 
 
 def _linear_int8(x, weight, bias, out_float32, constant_weight):
@@ -2719,10 +2735,22 @@ def _linear_int8(x, weight, bias, out_float32, constant_weight):
         scratch = torch.empty(M * (ldcx + 4), dtype=torch.uint8, device=codes.device)
         xp, cx = rows.data_ptr(), scratch.data_ptr()
         sx = cx + M * ldcx
+    tile_t, splits = int8_plan(M, N, K)
+    if splits == 0 and N * out.element_size() % 16:
+        tile_t, splits = 128, 1
+    if splits == 0:
+        if not given:
+            lib, fn = _entry(0, "ts_quantize_rows")
+            _launched(lib, fn(xt, xp, ldx, cx, ldcx, sx, M, K, stream), 1)
+        lib, fn = _entry(0, "ts_gemm_int8_pair")
+        _launched(lib, fn(cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else None,
+                          0 if bias is None or bias.dtype == torch.bfloat16 else 1, out.data_ptr(), N, 1 if dtype == torch.float32 else 0, M, N, K,
+                          num_sms() // 2, stream), 1)
+        return out
     lib, fn = _entry(0, "ts_gemm_int8")
     _launched(lib, fn(xt, xp, ldx, cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else None,
                       0 if bias is None or bias.dtype == torch.bfloat16 else 1, out.data_ptr(), N, 1 if dtype == torch.float32 else 0, M, N, K,
-                      int8_splits(M, N, K), 1 if constant_weight else 0, stream), 1 if given else 2)
+                      tile_t, splits, 1 if constant_weight else 0, stream), 1 if given else 2)
     return out
 
 
