@@ -343,17 +343,29 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
       const uint32_t kpair = p.kp[row];
       const float ks = pair_scale(kpair), kz = pair_zero(kpair);
       float acc[SIMT_HEADS] = {};
-#pragma unroll 2
-      for (int w = 0; w < W; ++w) {
-        const uint32_t bits = p.kc[row * W + w];
-        float c[8];
+      constexpr int AHEAD = W % 16 == 0 ? 16 : W % 12 == 0 ? 12 : W % 8 == 0 ? 8 : W % 4 == 0 ? 4 : 2;      // words of the row that are on their way at once
+#pragma unroll 1
+      for (int w0 = 0; w0 < W; w0 += AHEAD) {
+        uint32_t bits[AHEAD];
+        if constexpr (AHEAD % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = (float)((bits >> shift_of(i)) & 15u);
+          for (int w = 0; w < AHEAD; w += 4) *reinterpret_cast<uint4*>(bits + w) = *reinterpret_cast<const uint4*>(p.kc + row * W + w0 + w);
+        } else {
 #pragma unroll
-        for (int h = 0; h < SIMT_HEADS; ++h) {
-          const float4 a = *reinterpret_cast<const float4*>(&qs[h][w * 8]), e = *reinterpret_cast<const float4*>(&qs[h][w * 8 + 4]);
-          acc[h] = fmaf(a.x, c[0], fmaf(a.y, c[1], fmaf(a.z, c[2], fmaf(a.w, c[3], acc[h]))));
-          acc[h] = fmaf(e.x, c[4], fmaf(e.y, c[5], fmaf(e.z, c[6], fmaf(e.w, c[7], acc[h]))));
+          for (int w = 0; w < AHEAD; ++w) bits[w] = p.kc[row * W + w0 + w];
+        }
+#pragma unroll
+        for (int w = 0; w < AHEAD; ++w) {
+          float c[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[i] = (float)((bits[w] >> shift_of(i)) & 15u);
+#pragma unroll
+          for (int h = 0; h < SIMT_HEADS; ++h)
+            if (h < nh) {
+              const float4 a = *reinterpret_cast<const float4*>(&qs[h][(w0 + w) * 8]), e = *reinterpret_cast<const float4*>(&qs[h][(w0 + w) * 8 + 4]);
+              acc[h] = fmaf(a.x, c[0], fmaf(a.y, c[1], fmaf(a.z, c[2], fmaf(a.w, c[3], acc[h]))));
+              acc[h] = fmaf(e.x, c[4], fmaf(e.y, c[5], fmaf(e.z, c[6], fmaf(e.w, c[7], acc[h]))));
+            }
         }
       }
 #pragma unroll
@@ -393,6 +405,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[h][i] *= a;
         }
+#pragma unroll 4
       for (int key = kg; key < n; key += KG) {
         const uint32_t bits = p.vc[key_row[key] * W + word];
         const float vs = pair_scale(v_pair[key]), vz = pair_zero(v_pair[key]);
@@ -495,11 +508,14 @@ constexpr float ABOVE = 16.f;                                      // what a cod
 constexpr int MERGE_ROW = D + 4;                                   // floats of a column's partial result: the four columns of a quad meet other banks
 
 template <int NT> struct MmaCfg {
-  static constexpr int NC = 8 * NT;
+  static constexpr int NC = 8 * NT, MAX_CLUSTER = 8;
   static constexpr int Q_BYTES = KW * NT * 32 * 16 + NC * 8;       // operands; (factor, sum) of every column
   static constexpr int RING_BYTES = MMA_WARPS * RING * STAGE_BYTES;
   static constexpr int MERGE_BYTES = MMA_WARPS * NC * (MERGE_ROW + 3) * 4;
-  static constexpr int SMEM = Q_BYTES + (RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES);
+  static constexpr int WORK_BYTES = RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES;
+  // what the blocks of a cluster send each other: with n of them [sender][column / n rounded up][D + 4]
+  static constexpr int BOX_BYTES = (NC + MAX_CLUSTER) * MERGE_ROW * 4;
+  static constexpr int SMEM = Q_BYTES + WORK_BYTES + BOX_BYTES;
   static constexpr bool Q_REGS = NT == 1 && D <= 128;              // the queries' operands stay in registers
   static constexpr int BLOCKS = Q_REGS ? 2 : 1;
 };
@@ -568,7 +584,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
   const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC, b = blockIdx.z;
   const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
-  const int nc = min(C::NC, q_len * G - c0);                       // columns of this block
+  const int nc = min(C::NC, q_len * G - c0);                       // columns of this block (and of its cluster: they leave together)
   if (nc <= 0 || (p.most > 0 && q_len > p.most)) return;
   const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
   const int pos0 = kv_len - q_len;                                 // position of the request's first query of this step
@@ -885,6 +901,13 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][MERGE_ROW]: output column d of lane group g at place (d's number there) * 8 + g
   float* sm_ml = sm_o + MMA_WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
+  float* box = reinterpret_cast<float*>(work + C::WORK_BYTES);     // (its own memory: a peer may send while this block still reads its ring)
+  const int per_rank = (C::NC + p.splits - 1) / p.splits;
+  auto send = [](uint32_t at, uint32_t rank, float v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+  };
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float ls[2], zs[2];
@@ -932,13 +955,41 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
     }
     if (p.splits == 1) {
       static_cast<bf16*>(p.out)[row * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : sum / total);
-    } else {
+    } else if (p.part_o != nullptr) {
       p.part_o[(row * p.splits + split) * D + d] = sum;
       if (place == 0) {
         p.part_ml[(row * p.splits + split) * 2] = top;
         p.part_ml[(row * p.splits + split) * 2 + 1] = total;
       }
+    } else {
+      // to the block that owns the column (rank c % splits)
+      const int at = split * per_rank + c / p.splits;
+      send(smem_u32(box + at * MERGE_ROW + place), c % p.splits, sum);
+      if (place < 2) send(smem_u32(box + at * MERGE_ROW + D + place), c % p.splits, place == 0 ? top : total);
     }
+  }
+  if (p.splits == 1 || p.part_o != nullptr) return;
+  cluster_arrive();
+  cluster_wait();
+  for (int i = threadIdx.x; i < per_rank * D; i += MMA_WARPS * 32) {
+    const int c = i / D * p.splits + split, place = i % D, r = c0 + c, head = kvh * G + r % G;
+    if (c >= nc) break;
+    const int unit = (place & 7) * UNITS + (place >> 5), d = 8 * (unit >> 1) + (unit & 1) + 2 * (place >> 3 & 3);
+    const float sink2 = p.sinks != nullptr ? p.sinks[head] * LOG2E : LOWEST;
+    float top = fmaxf(LOWEST, sink2);
+#pragma unroll
+    for (int s = 0; s < C::MAX_CLUSTER; ++s)
+      if (s < p.splits) top = fmaxf(top, box[(s * per_rank + i / D) * MERGE_ROW + D]);
+    float sum = 0.f, total = p.sinks != nullptr ? ex2(sink2 - top) : 0.f;
+#pragma unroll
+    for (int s = 0; s < C::MAX_CLUSTER; ++s)
+      if (s < p.splits) {
+        const float* from = box + (s * per_rank + i / D) * MERGE_ROW;
+        const float f = ex2(from[D] - top);
+        sum += f * from[place];
+        total += f * from[D + 1];
+      }
+    static_cast<bf16*>(p.out)[((size_t)(q_begin + r / G) * p.H + head) * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : sum / total);
   }
 }
 
@@ -951,7 +1002,14 @@ int attend_mma(const Int4Params& p, int max_q_len, cudaStream_t stream) {
   const int G = p.H / p.Hkv;
   const long long tiles = ((long long)max_q_len * G + C::NC - 1) / C::NC * p.Hkv;
   TS_REQUIRE(tiles <= 65535 && p.B <= 65535, "int4_attention: grid out of range");
-  TS_LAUNCH("int4_attention", int4_mma_kernel<NT>, dim3(p.splits, (unsigned)tiles, p.B), dim3(MMA_WARPS * 32), C::SMEM, stream, p);
+  const dim3 grid(p.splits, (unsigned)tiles, p.B), block(MMA_WARPS * 32);
+  if (p.splits > 1 && p.part_o == nullptr) {
+    // the key ranges of a tile are a cluster and merge in it
+    const cudaError_t e = ts_launch_cluster(int4_mma_kernel<NT>, grid, block, C::SMEM, stream, dim3(p.splits, 1, 1), p);
+    if (e != cudaSuccess) return ts_fail("int4_attention (clusters of %d): %s", p.splits, cudaGetErrorString(e));
+    return 0;
+  }
+  TS_LAUNCH("int4_attention", int4_mma_kernel<NT>, grid, block, C::SMEM, stream, p);
   if (p.splits > 1)
     TS_LAUNCH("int4_attention (combine)", int4_combine_kernel<bf16>, dim3((unsigned)(p.T * p.H)), dim3(D < 128 ? D : 128), 0, stream, p);
   return 0;
@@ -1028,7 +1086,7 @@ TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const in
   return 0;
 }
 
-// q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
+// q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml, or (with columns, up to 8) merges in clusters.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
 // steps of 32 up to 256; 16 columns up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns):
 // requests with more queries than that are left alone.
 TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
@@ -1041,7 +1099,7 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
              T, B, H, Hkv, page_size);
   TS_REQUIRE((long long)T * H < (1LL << 31), "int4_attention: too many rows");
-  TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml)), "int4_attention: key ranges need their scratch");
+  TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml) || (columns > 0 && splits <= 8 && !part_o)), "int4_attention: key ranges need their scratch");
   Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
                   block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
                   splits, most, part_o, part_ml};

@@ -2862,15 +2862,27 @@ def int4_attention_backend(dtype, head_dim) -> str:
 INT4_DIRECT_ROWS = 16
 
 
+#: key ranges of the tensor-core kernel over a 4-bit cache that merge in a cluster; more of them are merged by a second kernel
+INT4_CLUSTER_SPLITS = 8
+
+
 def int4_decode_splits(blocks, max_kv_len):
-    """Key ranges of the tensor-core kernel over a 4-bit cache: two blocks an SM; a range has a step of 32 keys for each of its
-    eight warps."""
-    return max(1, min(2 * num_sms() // blocks, -(-max_kv_len // 256), 32))
+    """Key ranges of the tensor-core kernel over a 4-bit cache: two blocks an SM, at least 160 keys a range (five of its eight warps
+    have a step of 32), in powers of two as long as they merge in a cluster; and two where the blocks of a ragged batch
+    would not come out even (us: 1 request of 640 keys 7.4 whole, 6.5 in four; 64 of 2,000 to 8,192 112.9 whole, 109.4 in two; 3 of 32,768
+    40.3 in eight, 35.6 in twelve, 39.3 in 24)."""
+    want = min(2 * num_sms() // blocks, max_kv_len // 160, 32)
+    if want > INT4_CLUSTER_SPLITS:
+        return want
+    if want < 2:
+        return 2 if 2 * num_sms() < blocks <= 4 * num_sms() and max_kv_len >= 2048 else 1
+    return 8 if want >= 8 else 4 if want >= 4 else 2
 
 
 def int4_attention_splits(blocks, max_kv_len):
-    """Key ranges of the 32-bit kernel over a 4-bit cache: four blocks an SM, two tiles of 128 keys a range at least."""
-    return max(1, min(-(-4 * num_sms() // blocks), max_kv_len // 256, 32))
+    """Key ranges of the 32-bit kernel over a 4-bit cache: four blocks an SM, a tile of 128 keys a range at least (5 requests of 700 to
+    1,900 keys, 16 heads on 8, us: one range 109, four 34.8, eight 23.4, sixteen 17.8, 32 20.4)."""
+    return max(1, min(-(-4 * num_sms() // blocks), -(-max_kv_len // 128), 32))
 
 
 def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_splits, backend, sinks, softcap):
@@ -2928,12 +2940,13 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     if num_splits is None:
         num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
     part_o = part_ml = None
-    if num_splits > 1:
+    merged = columns > 0 and num_splits <= INT4_CLUSTER_SPLITS          # (in clusters, without scratch)
+    if num_splits > 1 and not merged:
         scratch = torch.empty(T * H * num_splits * (D + 2), dtype=torch.float32, device=q.device)
         part_o = scratch.data_ptr()
         part_ml = part_o + 4 * T * H * num_splits * D
     _launched(lib, fn(_DTYPE[dtype], q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                       v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H, Hkv, page,
                       blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, num_splits, part_o, part_ml,
-                      max_q_len, columns, most, stream), 1 if num_splits == 1 else 2)
+                      max_q_len, columns, most, stream), 1 if num_splits == 1 or merged else 2)
     return out
