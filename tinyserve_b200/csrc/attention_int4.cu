@@ -525,7 +525,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
@@ -540,12 +540,21 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // four codes of a word as bytes: of columns 0, 4, 1, 5 and, shifted, 2, 6, 3, 7
 __device__ __forceinline__ uint32_t codes4(uint32_t word) { return word & 0x0f0f0f0fu; }
+// (the first MMA of a chain adds to zeros that are no registers)
+__device__ __forceinline__ void mma_hi_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+__device__ __forceinline__ void mma_lo_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ void mma_hi(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_lo(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // codes number e (0 .. 3) of both halves of a word as two bfloat16 numbers 16 + c
@@ -598,6 +607,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   // A step's 32 keys lie in whole or in runs of a page; every run is four copies (codes and pairs of K and V) by a lane of its own.  A run
   // that starts behind the last key is not fetched, and what its place holds is masked.
   const int run_shift = min(p.page_shift, 5), runs = STEP >> run_shift, run_keys = 1 << run_shift;
+  const uint32_t ring_at = smem_u32(ring), run_at = lane << run_shift, code_bytes = ROW_BYTES << run_shift, pair_bytes = 4 * run_keys;
   int page_ahead = 0;          // of this lane's run of the step that is fetched next: read a step before it is needed
   auto look = [&](int s) {
     const int j = (step0 + s) * STEP + (lane << run_shift);
@@ -611,12 +621,18 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
     if (lane == 0) mbar_expect_tx(bar, n * (STAGE_BYTES >> (5 - run_shift)));
     __syncwarp();
     if (mine) {
-      const size_t row = cache_row(p, page_ahead, kvh, j);
-      const uint32_t at = smem_u32(ring) + stage * STAGE_BYTES, code_bytes = ROW_BYTES << run_shift, first_row = lane << run_shift;
-      bulk_copy(at + first_row * ROW_BYTES, reinterpret_cast<const char*>(p.kc) + row * ROW_BYTES, code_bytes, bar);
-      bulk_copy(at + (STEP + first_row) * ROW_BYTES, reinterpret_cast<const char*>(p.vc) + row * ROW_BYTES, code_bytes, bar);
-      bulk_copy(at + 2 * STEP * ROW_BYTES + first_row * 4, p.kp + row, run_keys * 4, bar);
-      bulk_copy(at + 2 * STEP * ROW_BYTES + (STEP + first_row) * 4, p.vp + row, run_keys * 4, bar);
+      if ((unsigned)page_ahead >= (unsigned)p.num_pages) {
+        ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_PAGE);
+        page_ahead = 0;
+      }
+      // (a pool of this kernel has fewer than 2^31 rows: one multiplication a copy)
+      const uint32_t row = (((uint32_t)page_ahead * p.Hkv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1));
+      const uint32_t at = ring_at + stage * STAGE_BYTES + run_at * ROW_BYTES, pairs_at = ring_at + stage * STAGE_BYTES + 2 * STEP * ROW_BYTES + run_at * 4;
+      const unsigned long long codes = (unsigned long long)row * ROW_BYTES, pairs = (unsigned long long)row * 4;
+      bulk_copy(at, reinterpret_cast<const char*>(p.kc) + codes, code_bytes, bar);
+      bulk_copy(at + STEP * ROW_BYTES, reinterpret_cast<const char*>(p.vc) + codes, code_bytes, bar);
+      bulk_copy(pairs_at, reinterpret_cast<const char*>(p.kp) + pairs, pair_bytes, bar);
+      bulk_copy(pairs_at + STEP * 4, reinterpret_cast<const char*>(p.vp) + pairs, pair_bytes, bar);
     }
     look(s + MMA_WARPS);
   };
@@ -743,19 +759,18 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       }
       int part[2][NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) part[h][nt][e] = 0;
-#pragma unroll
       for (int i = 0; i < KW; ++i) {
         const uint32_t a0 = codes4(w0[i]), a1 = codes4(w1[i]), a2 = codes4(w0[i] >> 4), a3 = codes4(w1[i] >> 4);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const uint4 q = C::Q_REGS ? qf[C::Q_REGS ? i : 0] : qf_s[(i * NT + nt) * 32 + lane];
-          mma_hi(part[0][nt], a0, a1, a2, a3, q.x, q.y);
-          mma_lo(part[1][nt], a0, a1, a2, a3, q.z, q.w);
+          if (i == 0) {
+            mma_hi_first(part[0][nt], a0, a1, a2, a3, q.x, q.y);
+            mma_lo_first(part[1][nt], a0, a1, a2, a3, q.z, q.w);
+          } else {
+            mma_hi(part[0][nt], a0, a1, a2, a3, q.x, q.y);
+            mma_lo(part[1][nt], a0, a1, a2, a3, q.z, q.w);
+          }
         }
       }
       // scores; this thread's keys are those of rows g and g + 8
@@ -1106,6 +1121,7 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
   if (columns > 0) {
 #ifdef TS_INT4_MMA
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");
+    TS_REQUIRE(((long long)num_pages * Hkv << shift) < (1LL << 31), "int4_attention: the tensor-core kernel takes pools of fewer than 2^31 rows");
     TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 15) == 0, "int4_attention: the tensor-core kernel copies runs that begin on 16 bytes");
     if (columns == 8) return attend_mma<1>(p, max_q_len, stream);
 #if TS_HEAD_DIM <= 128

@@ -2935,7 +2935,8 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
             most = max_q_len = few
         rows = max_q_len * G
         columns = 16 if rows > 8 and D <= 128 else 8
-        if -(-rows // columns) * Hkv > 65535 or B > 65535 or page < 4 or (k_cache.pairs.data_ptr() | v_cache.pairs.data_ptr()) % 16:
+        if -(-rows // columns) * Hkv > 65535 or B > 65535 or page < 4 or pages * Hkv * page >= 2 ** 31 \
+                or (k_cache.pairs.data_ptr() | v_cache.pairs.data_ptr()) % 16:
             columns = most = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes everything)
     if num_splits is None:
         num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
