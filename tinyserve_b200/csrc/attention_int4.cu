@@ -56,32 +56,66 @@ __device__ __forceinline__ void load8_any(const T* p, float (&x)[8], bool vec) {
   }
 }
 
-// What the LANES lanes of a row have of it: minimum, maximum, anything that is not finite
+// What the LANES lanes of a row have of it: minimum, maximum, and whether everything is finite (0 x of an infinity or a NaN is a NaN)
 struct RowRange {
   float lo = INFINITY, hi = -INFINITY;
-  int bad = 0;
+  F2 zeros = f2(0.f, 0.f);
+  bool bad = false;
   __device__ __forceinline__ void add(const float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+    for (int i = 0; i < 8; i += 2) {
+      lo = fminf(fminf(lo, x[i]), x[i + 1]);
+      hi = fmaxf(fmaxf(hi, x[i]), x[i + 1]);
+      zeros = f2_fma(f2(x[i], x[i + 1]), f2(0.f, 0.f), zeros);
     }
   }
   __device__ __forceinline__ void join() {
+    float z0, z1;
+    f2_out(zeros, z0, z1);
+    const uint32_t group = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+    bad = (__ballot_sync(0xffffffffu, !(z0 + z1 == 0.f)) & group) != 0;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      bad |= __shfl_xor_sync(0xffffffffu, bad, o);
     }
   }
 };
 
-__device__ __noinline__ uint32_t divided_code(float y, float scale) { return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(y, scale)), 0.f), 15.f); }
+__device__ __noinline__ float divided_code(float y, float scale) { return fminf(fmaxf(rintf(__fdiv_rn(y, scale)), 0.f), 15.f); }
+
+// eight neighbouring columns as a word of codes.  The quotient rounded to 32 bits decides; the product with the reciprocal is off by 3 roundings of at
+// most 16, so a division is only made next to a half, and where the reciprocal could overflow.  Adding 1.5 2^23 rounds to a whole
+// number, halves to even; four codes 4 bits apart are a sum of exact products below 2^16.
+__device__ __forceinline__ uint32_t word_of(const float (&x)[8], float zero, float scale) {
+  constexpr float ROUNDER = 12582912.f;
+  const float inverse = 1.f / scale;
+  const F2 inv = f2(inverse, inverse), low = f2(-zero, -zero), up = f2(ROUNDER, ROUNDER), down = f2(-ROUNDER, -ROUNDER), minus = f2(-1.f, -1.f);
+  float n[8], furthest = scale > 1e-30f ? 0.f : 1.f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float r0, r1, o0, o1;
+    f2_out(f2_mul(f2_add(f2(x[i], x[i + 1]), low), inv), r0, r1);
+    const F2 r = f2(fminf(fmaxf(r0, 0.f), 15.f), fminf(fmaxf(r1, 0.f), 15.f)), whole = f2_add(f2_add(r, up), down);
+    f2_out(f2_fma(whole, minus, r), o0, o1);
+    furthest = fmaxf(furthest, fmaxf(fabsf(o0), fabsf(o1)));
+    f2_out(whole, n[i], n[i + 1]);
+  }
+  if (furthest > 0.49995f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = __fsub_rn(x[i], zero), r = fminf(fmaxf(y * inverse, 0.f), 15.f);
+      if (fabsf(r - n[i]) > 0.49995f || !(scale > 1e-30f)) n[i] = divided_code(y, scale);
+    }
+  }
+  const F2 four = f2_fma(f2_fma(f2_fma(f2(n[6], n[7]), f2(16.f, 16.f), f2(n[4], n[5])), f2(16.f, 16.f), f2(n[2], n[3])), f2(16.f, 16.f), f2(n[0], n[1]));
+  float even, odd;
+  f2_out(f2_add(four, f2(8388608.f, 8388608.f)), even, odd);          // (2^23: the whole number is the low bits)
+  return __byte_perm(__float_as_uint(even), __float_as_uint(odd), 0x5410);
+}
+
 // a row that its LANES lanes hold, to the slot of its token
-__device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)[WORDS][8], RowRange r, int which, int head, int t, int lane) {
-  const int slot = p.slot_mapping[t];
+__device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)[WORDS][8], const RowRange& r, int which, int head, int slot, int lane) {
   if (slot < 0) return;
   if (slot >= p.slots) {
     if (lane == 0) ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_CACHE_SLOT);
@@ -96,31 +130,7 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
 #pragma unroll
   for (int w = 0; w < WORDS; ++w) {
     const int word = lane + w * LANES;
-    if (word >= W) continue;
-    uint32_t bits = 0;
-    if (!bad && scale > 0.f) {
-      // the quotient rounded to 32 bits decides; the product with the reciprocal is off by 3 roundings of at most 16, so a division is
-      // only made next to a half, and where the reciprocal could overflow
-      const float inverse = 1.f / scale;
-      float furthest = scale > 1e-30f ? 0.f : 1.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // (adding 1.5 2^23 rounds to a whole number, halves to even, and leaves it in the low bits)
-        const float r = fminf(fmaxf(__fsub_rn(x[w][i], zero) * inverse, 0.f), 15.f), t = r + 12582912.f;
-        furthest = fmaxf(furthest, fabsf(r - (t - 12582912.f)));
-        bits |= (__float_as_uint(t) & 15u) << shift_of(i);
-      }
-      if (furthest > 0.49995f) {
-        bits = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = __fsub_rn(x[w][i], zero), r = fminf(fmaxf(y * inverse, 0.f), 15.f), t = r + 12582912.f;
-          const bool near = fabsf(r - (t - 12582912.f)) > 0.49995f || !(scale > 1e-30f);
-          bits |= (near ? divided_code(y, scale) : __float_as_uint(t) & 15u) << shift_of(i);
-        }
-      }
-    }
-    (which ? p.vc : p.kc)[at * W + word] = bits;
+    if (word < W) (which ? p.vc : p.kc)[at * W + word] = !bad && scale > 0.f ? word_of(x[w], zero, scale) : 0u;
   }
   if (lane == 0) {
     const uint32_t s = bad ? 0x7fc0u : (scale > 0.f ? __bfloat16_as_ushort(scale16) : 0u), z = bad ? 0x7fc0u : __bfloat16_as_ushort(zero16);
@@ -128,15 +138,15 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
   }
 }
 
-// LANES lanes bring one row (token, key or value, head) to its slot
+// LANES lanes bring one row (token, key or value, head) to its slot; a block's x is the token
 template <typename T>
 __global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams p, bool vec) {
   pdl_trigger();
   pdl_wait();
-  const long long row = (long long)blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES;
-  const int lane = threadIdx.x % LANES;
-  const bool live = row < 2LL * p.T * p.Hkv;
-  const int head = (int)(row % p.Hkv), which = (int)(row / p.Hkv & 1), t = live ? (int)(row / p.Hkv >> 1) : 0;
+  const int t = blockIdx.x, row = blockIdx.y * (blockDim.x / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const bool live = row < 2 * p.Hkv;
+  const int which = row >= p.Hkv ? 1 : 0, head = row - which * p.Hkv;
+  const int slot = p.slot_mapping[t];
   const T* src = which ? static_cast<const T*>(p.v) + t * p.v_row + head * p.v_head : static_cast<const T*>(p.k) + t * p.k_row + head * p.k_head;
   float x[WORDS][8];
   RowRange r;
@@ -149,7 +159,7 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams
     }
   }
   r.join();
-  if (live) store_row(p, x, r, which, head, t, lane);
+  if (live) store_row(p, x, r, which, head, slot, lane);
 }
 
 // The same behind a fused projection: qkv [T, (H + 2 Hkv) D] -> q [T, H, D] and the cache.  Heads of q and k are divided by their root
@@ -165,25 +175,46 @@ struct RopeParams {
   int has_norm;
   float eps;
   int H;
+  // rows of q, k, v, weights and angles come in eights that begin on 16 bytes (halves of the rotation are whole eights too)
+  bool vec, vec_weights, vec_angles;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteParams p, RopeParams rp, bool vec) {
-  __shared__ float stage[WRITE_THREADS / LANES][D];
+__global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteParams p, RopeParams rp) {
+  __shared__ __align__(16) float stage[WRITE_THREADS / LANES][D];
   pdl_trigger();
+  const int t = blockIdx.x, heads = rp.H + 2 * p.Hkv, head = blockIdx.y * (blockDim.x / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const bool live = head < heads, is_q = head < rp.H, is_v = head >= rp.H + p.Hkv;
+  const bool turned = live && !is_v;
+  // (weights are nobody's output: they are on their way during the wait)
+  float wt[WORDS][8];
+  if (rp.has_norm) {
+    const VecParam w8 = is_q ? rp.qw : rp.kw;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int word = lane + w * LANES;
+      if (turned && word < W) {
+        if (rp.vec_weights) {
+          if (w8.is_f32) load8<float>(static_cast<const float*>(w8.ptr) + word * 8, wt[w]);
+          else load8<bf16>(static_cast<const bf16*>(w8.ptr) + word * 8, wt[w]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) wt[w][i] = w8[word * 8 + i];
+        }
+      }
+    }
+  }
   pdl_wait();
-  const int heads = rp.H + 2 * p.Hkv, lane = threadIdx.x % LANES;
-  const long long row = (long long)blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES;
-  const bool live = row < (long long)p.T * heads;
-  const int t = live ? (int)(row / heads) : 0, head = live ? (int)(row % heads) : 0;
-  const bool is_q = head < rp.H, is_v = head >= rp.H + p.Hkv;
   const T* src = static_cast<const T*>(rp.qkv) + ((size_t)t * heads + head) * D;
+  const int slot = p.slot_mapping != nullptr ? p.slot_mapping[t] : -1;
+  const int half = rp.rot >> 1;
+  const size_t angles = rp.cos != nullptr ? (size_t)rp.positions[t] * half : 0;
   float x[WORDS][8], sum = 0.f;
 #pragma unroll
   for (int w = 0; w < WORDS; ++w) {
     const int word = lane + w * LANES;
     if (live && word < W) {
-      load8_any<T>(src + word * 8, x[w], vec);
+      load8_any<T>(src + word * 8, x[w], rp.vec);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = fmaf(x[w][i], x[w][i], sum);
     }
@@ -192,36 +223,40 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteP
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float rstd = rsqrtf(sum / (float)D + rp.eps);
-    const VecParam wt = is_q ? rp.qw : rp.kw;
 #pragma unroll
     for (int w = 0; w < WORDS; ++w) {
-      const int word = lane + w * LANES;
-      if (live && !is_v && word < W) {
+      if (turned && lane + w * LANES < W) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[w][i] = x[w][i] * rstd * wt[word * 8 + i];
+        for (int i = 0; i < 8; ++i) x[w][i] = x[w][i] * rstd * wt[w][i];
       }
     }
   }
   if (rp.cos != nullptr) {
     float* mine = stage[threadIdx.x / LANES];
-    const int half = rp.rot >> 1;
 #pragma unroll
     for (int w = 0; w < WORDS; ++w) {
       const int word = lane + w * LANES;
-      if (live && !is_v && word < W) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine[word * 8 + i] = x[w][i];
-      }
+      if (turned && word < W) store8<float>(mine + word * 8, x[w]);
     }
     __syncwarp();
-    const size_t angles = live && !is_v ? (size_t)rp.positions[t] * half : 0;
 #pragma unroll
     for (int w = 0; w < WORDS; ++w) {
-      const int word = lane + w * LANES;
-      if (live && !is_v && word < W) {
+      const int word = lane + w * LANES, d0 = word * 8;
+      if (!turned || word >= W || d0 >= rp.rot) continue;
+      if (rp.vec_angles) {
+        // eight columns of one half with the eight of the other
+        const bool first = d0 < half;
+        const int j = first ? d0 : d0 - half;
+        float mate[8], c[8], s[8];
+        load8<float>(mine + (first ? d0 + half : d0 - half), mate);
+        load8<float>(rp.cos + angles + j, c);
+        load8<float>(rp.sin + angles + j, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[w][i] = first ? x[w][i] * c[i] - mate[i] * s[i] : x[w][i] * c[i] + mate[i] * s[i];
+      } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int d = word * 8 + i;
+          const int d = d0 + i;
           if (d >= rp.rot) continue;
           const int j = rp.interleaved ? d >> 1 : (d < half ? d : d - half);
           const bool first = rp.interleaved ? (d & 1) == 0 : d < half;
@@ -239,12 +274,19 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteP
     if (live && word < W) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[w][i] = to_f32<T>(from_f32<T>(x[w][i]));
-      r.add(x[w]);
       if (is_q) store8<T>(static_cast<T*>(rp.q) + ((size_t)t * rp.H + head) * D + word * 8, x[w]);
+      else r.add(x[w]);
     }
   }
   r.join();
-  if (live && !is_q && p.slot_mapping != nullptr) store_row(p, x, r, is_v ? 1 : 0, is_v ? head - rp.H - p.Hkv : head - rp.H, t, lane);
+  if (live && !is_q) store_row(p, x, r, is_v ? 1 : 0, is_v ? head - rp.H - p.Hkv : head - rp.H, slot, lane);
+}
+
+// tokens x groups of a token's rows
+struct RowGrid { dim3 grid, block; };
+RowGrid row_grid(int tokens, int rows) {
+  const int threads = rows * LANES < WRITE_THREADS ? (rows * LANES + 31) / 32 * 32 : WRITE_THREADS;
+  return {dim3(tokens, (rows + threads / LANES - 1) / (threads / LANES)), dim3(threads)};
 }
 
 // ------------------------------------------------------------------------------------------ attention
@@ -1070,10 +1112,10 @@ TS_EXPORT int ts_int4_kvwrite(int dtype, const void* k, const void* v, long long
   const bool vec = ((((uintptr_t)k | (uintptr_t)v) | (uintptr_t)((k_row | k_head | v_row | v_head) * e)) & 15) == 0;
   WriteParams p = {k, v, k_row, k_head, v_row, v_head, (uint32_t*)k_codes, (uint32_t*)v_codes, (uint32_t*)k_pairs, (uint32_t*)v_pairs,
                    slot_mapping, T, Hkv, shift, (long long)num_pages << shift};
-  const long long rows = 2LL * T * Hkv, per = WRITE_THREADS / LANES, blocks = (rows + per - 1) / per;
-  TS_REQUIRE(blocks < (1LL << 31), "int4_kvwrite: too many rows");
-  if (dtype == TS_F32) TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<float>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, vec);
-  else TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<bf16>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, vec);
+  const RowGrid g = row_grid(T, 2 * Hkv);
+  TS_REQUIRE(g.grid.y <= 65535, "int4_kvwrite: too many heads");
+  if (dtype == TS_F32) TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<float>, g.grid, g.block, 0, stream, p, vec);
+  else TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<bf16>, g.grid, g.block, 0, stream, p, vec);
   return 0;
 }
 
@@ -1088,16 +1130,16 @@ TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const in
   TS_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0 && (rot == 0 || (cos && sin && positions)), "int4_rope_kvwrite: a rotation over %d of %d columns", rot, D);
   TS_REQUIRE((q_weight == nullptr) == (k_weight == nullptr), "int4_rope_kvwrite: q and k norm weights come together");
   TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 3) == 0 && ((uintptr_t)q & 15) == 0, "int4_rope_kvwrite: the cache or q is not aligned");
-  const bool vec = ((uintptr_t)qkv & 15) == 0;
   WriteParams p = {};
   p.kc = (uint32_t*)k_codes; p.vc = (uint32_t*)v_codes; p.kp = (uint32_t*)k_pairs; p.vp = (uint32_t*)v_pairs;
   p.slot_mapping = slot_mapping; p.T = T; p.Hkv = Hkv; p.page_shift = shift; p.slots = (long long)num_pages << shift;
   const RopeParams rp = {qkv, q, positions, rot ? cos : nullptr, sin, rot, interleaved, VecParam{q_weight, weight_f32}, VecParam{k_weight, weight_f32},
-                         q_weight != nullptr, eps, H};
-  const long long rows = (long long)T * (H + 2 * Hkv), per = WRITE_THREADS / LANES, blocks = (rows + per - 1) / per;
-  TS_REQUIRE(blocks < (1LL << 31), "int4_rope_kvwrite: too many rows");
-  if (dtype == TS_F32) TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<float>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, rp, vec);
-  else TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<bf16>, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, p, rp, vec);
+                         q_weight != nullptr, eps, H, ((uintptr_t)qkv & 15) == 0, (((uintptr_t)q_weight | (uintptr_t)k_weight) & 15) == 0,
+                         !interleaved && rot % 16 == 0 && (((uintptr_t)cos | (uintptr_t)sin) & 15) == 0};
+  const RowGrid g = row_grid(T, H + 2 * Hkv);
+  TS_REQUIRE(g.grid.y <= 65535, "int4_rope_kvwrite: too many heads");
+  if (dtype == TS_F32) TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<float>, g.grid, g.block, 0, stream, p, rp);
+  else TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<bf16>, g.grid, g.block, 0, stream, p, rp);
   return 0;
 }
 

@@ -320,7 +320,8 @@ class Attention(Mixer):
     def forward(self, h, ctx, call):
         if self.general:
             return self._forward_general(h, ctx, call)
-        qkv = ops.linear(h, self.w["qkv_proj.weight"], self.w.get("qkv_proj.bias"), allow_partials=True, constant_weight=True)
+        # (the kernel in front of a 4-bit cache reads finished rows)
+        qkv = ops.linear(h, self.w["qkv_proj.weight"], self.w.get("qkv_proj.bias"), allow_partials=not self.cache_bits, constant_weight=True)
         cache = ctx.cache(call.cache)
         view = ctx.group(cache.group)
         out = ops.attention_from_qkv(
