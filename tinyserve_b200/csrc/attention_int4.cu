@@ -541,12 +541,13 @@ __global__ void int4_combine_kernel(Int4Params p) {
 //   V  keys run along K there, two of one column side by side, which bytes would need a transposition for: a code enters as the bfloat16
 //      number 16 + c, one shift and one AND-OR for two of them.
 //   Scales and zeros are per key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.c) + z sum(q); for the values, with p' =
-//   bfloat16(p s), sum p v = sum p' (16 + c) + sum p z - 16 sum p'; the last sum is one more MMA, with ones for V, so that the 16 cancels
-//   whatever p' was rounded to.
+//   bfloat16(p s), sum p v = sum p' (c - 8) + sum p (z + 8 s), and sum p' (c - 8) = sum p' (16 + c) - 24 sum p', which is one more MMA, with
+//   ones for V, so that the 24 cancels whatever p' was rounded to.  (Around the middle of the codes the rounding of p' weighs half as much as
+//   around 0: 4,096 keys, relative error of the output before its own rounding 1.4e-3 and 2.5e-3.)
 constexpr int MMA_WARPS = 8, STEP = 32, RING = 3;
 constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
 constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;   // codes of K and V, pairs of K and V
-constexpr float ABOVE = 16.f;                                      // what a code's bfloat16 is above it
+constexpr float MIDDLE = 8.f, ABOVE = 16.f + MIDDLE;               // of the codes; what a code's bfloat16 is above c - MIDDLE
 constexpr int MERGE_ROW = D + 4;                                   // floats of a column's partial result: the four columns of a quad meet other banks
 
 template <int NT> struct MmaCfg {
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       for (int h = 0; h < 2; ++h) {
         const uint32_t vpair = vp[kb * 16 + 8 * h];
         vscale[kb][h] = pair_scale(vpair);
-        vzero[kb][h] = pair_zero(vpair);
+        vzero[kb][h] = fmaf(MIDDLE, pair_scale(vpair), pair_zero(vpair));
       }
     if (p.softcap > 0.f) {
       const float in = 1.f / (p.softcap * LOG2E), out = p.softcap * LOG2E;

@@ -2,11 +2,22 @@
 // (-DTS_HEAD_DIM).  The mathematics and the use of tensor memory are those of attention_tcgen05.cu (two tiles of 128 rows = (query, head) of one
 // key head take turns on the tensor core, S = Q K^T, P written over S, O += P V, one softmax thread a row, maxima that move by
 // more than 2^8 only); keys and values come differently.  Four warps make them: a thread reads a key's row of codes (64 bytes at 128
-// columns) and its pair, and writes the row as bfloat16 into the swizzled tile that the tensor core reads: a code becomes the number 16 + c
-// (one shift, one AND-OR for two), minus 16 (exact), times scale plus zero (one rounding to bfloat16, the
-// only one that a cache of whole numbers would not have).  That is about 600 instructions a thread for a tile of 128 keys, on warps that
-// have nothing else to do, while the tensor core takes 2,000 cycles for the tile's four products.  Nothing is expanded in
-// memory: a portion of any length behind a context of any length needs no scratch.
+// columns) and its pair, and writes the row as 16-bit numbers into the swizzled tile that the tensor core reads: a code becomes the number
+// 1 + c / 16 (one shift, one AND-OR for two codes), times 16 scale, plus zero - 16 scale (rounded once for the row; the value once more).  That is
+// 400 instructions a thread for a tile of 128 keys, while the tensor core takes 2,000 cycles for the tile's four products.
+// Nothing is expanded in memory: a portion of any length behind a context of any length needs no scratch.
+//
+// The 16 bits are those of half precision (11 significant bits, where bfloat16 has 8): the codes' values, the queries and the probabilities lose
+// nothing that shows behind the rounding of the output (2,048 queries over 4,096 keys, 32 heads of 128 on 8, relative error of the output:
+// in bfloat16 4.4e-3, so 1.7e-3, which is that rounding alone; exact codes, with scales and zeros applied to every score and probability, came
+// to 2.3e-3 and took 271 us instead of 131).  Its range is short, so powers of two keep everything inside: one a row for the queries, one a tile for the keys,
+// and one for the values of all tiles so far, with which the sums in tensor memory are rescaled when it grows.  (From the
+// pairs of the tile at hand: a look at all of a block's pairs beforehand took 30 us.)  What lies 2^-26 below the largest loses bits.
+//
+// That portion takes 131 us, 0.79 PFLOP/s.  What bounds it is the softmax warps' path from scores to probabilities (with one matrix instruction a product and
+// tiles made twice only, still 108 us; without its exponentials no less than with them), then the start of a block (22 us for 256 blocks of one
+// tile) and the makers (11 us).  The subtraction of 1024 that an earlier form of the makers had cost 10 us; pairs of 32-bit operations in
+// the softmax save 5; probabilities in one part or in four instead of two took 143 us.
 //
 // A key whose pair is not finite becomes a key of NaN with a value of zeros: who sees it gets NaN, who does not is not touched (its
 // probability of 0 would not survive a NaN in V).
@@ -14,6 +25,9 @@
 // 512 threads: warp 0 loads the queries, warp 1 issues, warps 4-7 and 8-11 are the softmax of the two tiles (168 registers), 12-15 make keys and
 // values.  Blocks find their request themselves (a scan over the query offsets), so that no list is cut on the host and a captured graph
 // serves any step of its shape.  Every wait is bounded; a block that gives up raises ts_attention_int4_tcgen05_error.
+#include <cuda_fp16.h>
+
+#include "pairs.cuh"
 #include "tcgen05.cuh"
 
 #ifndef TS_HEAD_DIM
@@ -39,7 +53,10 @@ constexpr int Q_BYTES = DCH * CHUNK_BYTES;
 constexpr int KV_BYTES = DCH * CHUNK_BYTES;  // one of K or V of a tile
 constexpr int TMEM_COLS = 512;               // S_0, S_1: 128 columns each (P_g over the first 64 of S_g); O_0 at 256, O_1 at 384
 constexpr int W4 = D / 32;                   // 16-byte pieces of a row of codes
-constexpr size_t SMEM = 1024 + GROUPS * Q_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 256;
+constexpr size_t SMEM = 1024 + GROUPS * Q_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 512;
+constexpr int RANGES = 4;                    // tiles whose exponents are kept
+constexpr float P_UP = 7.f;                  // probabilities are written times 2^7: up to 2^15, so that those of long rows stay above 2^-24
+constexpr int HIGHEST = 12;                  // the largest of what is scaled goes to 2^12 .. 2^13 (half precision ends at 65,504)
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
@@ -67,16 +84,26 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// columns 2 E and 2 E + 1 of a word's eight, as scale * c + zero
-template <int E>
-__device__ __forceinline__ uint32_t values2(uint32_t word, __nv_bfloat162 scale, __nv_bfloat162 zero) {
-  const uint32_t moved = E == 0 ? word << 3 : word >> (4 * E - 3);
-  uint32_t two;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(two) : "r"(moved), "r"(0x00780078u), "r"(0x41804180u));
-  const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&two), __floats2bfloat162_rn(16.f, 16.f));
-  const __nv_bfloat162 v = __hfma2(c, scale, zero);
+__device__ __forceinline__ uint32_t halves2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// columns 2 E and 2 E + 1 of a word's eight, as scale * c + zero
+template <int E>
+__device__ __forceinline__ uint32_t values2(uint32_t word, __half2 scale, __half2 zero) {
+  const uint32_t moved = E < 2 ? word << (6 - 4 * E) : word >> (4 * E - 6);
+  uint32_t two;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(two) : "r"(moved), "r"(0x03c003c0u), "r"(0x3c003c00u));
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&two), scale, zero);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// instruction descriptor of kind::f16 with half precision on both sides (make_idesc has bfloat16)
+__host__ __device__ constexpr uint32_t idesc_half(int M, int N, bool b_mn_major) { return make_idesc(M, N, b_mn_major) & ~((1u << 7) | (1u << 10)); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+// the exponent that the largest magnitude (as bits) has; 0 and what is not finite: that of 2^14, which nothing is scaled for
+__device__ __forceinline__ int exponent_of(uint32_t bits) { return bits == 0 || bits >= 0x7f800000u ? HIGHEST : max((int)(bits >> 23) - 127, -100); }
+__device__ __forceinline__ float pair_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float pair_zero(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 __device__ __forceinline__ bool finite_pair(uint32_t pair) {
   return (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
 }
@@ -89,8 +116,13 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
   char* Ks = Qs + GROUPS * Q_BYTES;              // [K_STAGES][KV_BYTES]
   char* Vs = Ks + K_STAGES * KV_BYTES;           // [V_STAGES][KV_BYTES]
   uint64_t* bars = reinterpret_cast<uint64_t*>(Vs + V_STAGES * KV_BYTES);
-  uint64_t* q_full = bars;                       // 1
-  uint64_t* k_full = q_full + 1;                 // [K_STAGES] the makers' four warps
+  uint64_t* q_full = bars;                       // 1: the queries have landed
+  uint64_t* q_ready = q_full + 1;                // the softmax warps: ... and are in half precision
+  uint64_t* seen = q_ready + 1;                  // the makers' four warps have seen the tile's pairs
+  uint64_t* range = seen + 1;                    // [RANGES] the exponents of a tile's keys and values are known (a place is free when it
+                                                 // comes up again: keys four tiles on need the scores of two tiles on, which come
+                                                 // behind the probabilities of one tile on)
+  uint64_t* k_full = range + RANGES;             // [K_STAGES] the makers' four warps
   uint64_t* k_empty = k_full + K_STAGES;         // [K_STAGES] both tiles' scores of the stage's keys are computed
   uint64_t* v_full = k_empty + K_STAGES;         // [V_STAGES]
   uint64_t* v_empty = v_full + V_STAGES;         // [V_STAGES] the stage's values are added to both O
@@ -99,10 +131,15 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
   uint64_t* o_ready = p_full + GROUPS * P_PARTS; // [GROUPS] O_g holds the sum over the key tiles so far
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_ready + GROUPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* largest = tmem_slot + 2;             // [2][8]: largest magnitudes of a tile's keys and values, by maker warp
+  int2* exponents = reinterpret_cast<int2*>(largest + 16);       // [RANGES]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(q_full), 1);
+    mbar_init(smem_u32(q_ready), GROUPS * 4);
+    mbar_init(smem_u32(seen), 4);
+    for (int s = 0; s < RANGES; ++s) mbar_init(smem_u32(&range[s]), 1);
     for (int s = 0; s < K_STAGES; ++s) {
       mbar_init(smem_u32(&k_full[s]), 4);
       mbar_init(smem_u32(&k_empty[s]), 1);
@@ -186,8 +223,8 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         for (int c = 0; c < DCH; ++c)
           tma_load_3d(smem_u32(Qs + g * Q_BYTES + c * CHUNK_BYTES), &map_q, qbar, c * 64, kvh * G + g0, q_begin + q0 + g * QPT);
     } else if (warp == 1 && n_tiles > 0 && elect_one()) {
-      constexpr uint32_t idesc_qk = make_idesc(BM, BN, false);
-      constexpr uint32_t idesc_pv = make_idesc(BM, D, true);
+      constexpr uint32_t idesc_qk = idesc_half(BM, BN, false);
+      constexpr uint32_t idesc_pv = idesc_half(BM, D, true);
       constexpr int QK_STEPS = D / 16, PV_STEPS = BN / 16 / P_PARTS;
       const uint64_t q_desc = smem_desc(smem_u32(Qs)), k_desc = smem_desc(smem_u32(Ks));
       const uint64_t v_desc = smem_desc_mn(smem_u32(Vs), CHUNK_BYTES);
@@ -227,7 +264,8 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         if (g == groups - 1) tcgen05_commit(smem_u32(&v_empty[s]));
         return true;
       };
-      bool ok = mbar_spin_wait(smem_u32(q_full), 0, abort_flag);
+      bool ok = mbar_spin_wait(smem_u32(q_ready), 0, abort_flag);
+      tcgen05_fence_after();
       for (int g = 0; ok && g < groups; ++g) ok = scores(g, 0);
       for (int t = 0; ok && t < n_tiles; ++t)
         for (int g = 0; ok && g < groups; ++g) {
@@ -257,9 +295,9 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
 #pragma unroll
       for (int i = 0; i < W4; ++i) row.codes[i] = w.live ? codes[w.row * W4 + i] : make_uint4(0u, 0u, 0u, 0u);
     };
-    auto write = [&](char* tile, const Row& row, uint32_t pair) {
-      const __nv_bfloat162 both = *reinterpret_cast<const __nv_bfloat162*>(&pair);
-      const __nv_bfloat162 scale = __low2bfloat162(both), zero = __high2bfloat162(both);
+    auto write = [&](char* tile, const Row& row, uint32_t pair, float factor) {
+      const float s16 = 16.f * factor * pair_scale(pair);
+      const __half2 scale = __float2half2_rn(s16), zero = __float2half2_rn(fmaf(pair_zero(pair), factor, -s16));
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         const uint32_t w = i % 4 == 0 ? row.codes[i / 4].x : i % 4 == 1 ? row.codes[i / 4].y : i % 4 == 2 ? row.codes[i / 4].z : row.codes[i / 4].w;
@@ -268,12 +306,19 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       }
     };
     constexpr uint32_t NAN_PAIR = 0x7fc07fc0u;
+    // the largest magnitude that a pair's codes can stand for
+    auto reach = [](uint32_t pair) -> uint32_t {
+      if (!finite_pair(pair)) return 0u;
+      const float zero = pair_zero(pair), end = fmaf(15.f, pair_scale(pair), zero);
+      return min(__float_as_uint(fmaxf(fabsf(zero), fabsf(end))), 0x7f7fffffu);
+    };
+    uint32_t top_v = 0;          // of all tiles so far
+    bool ok = true;
     // the next tile's keys are on their way while this tile's values are made, and these while its keys are
     Where at_k = find(0);
     Row k, v;
     read(p.kc, at_k, k);
     uint32_t k_pair = at_k.live ? p.kp[at_k.row] : 0u, v_pair = at_k.live ? p.vp[at_k.row] : 0u;
-    bool ok = true;
     auto hand_over = [&](uint64_t* full) {
       fence_async_shared();
       __syncwarp();
@@ -286,18 +331,36 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
     for (int t = 0; ok && t < n_tiles; ++t) {
       read(p.vc, at_k, v);
       const Where next_k = find(t + 1);
+      const bool good = finite_pair(k_pair) && finite_pair(v_pair);
+      uint32_t* of_tile = largest + (t & 1) * 8;
+      const uint32_t k_of_warp = __reduce_max_sync(0xffffffffu, reach(k_pair)), v_of_warp = __reduce_max_sync(0xffffffffu, reach(v_pair));
+      if (lane == 0) {
+        of_tile[warp - MAKER_WARP0] = k_of_warp;
+        of_tile[4 + warp - MAKER_WARP0] = v_of_warp;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(seen));
+      ok = mbar_wait(smem_u32(seen), t & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      top_v = max(top_v, max(max(of_tile[4], of_tile[5]), max(of_tile[6], of_tile[7])));
+      const int k_exponent = exponent_of(max(max(of_tile[0], of_tile[1]), max(of_tile[2], of_tile[3]))), v_exponent = exponent_of(top_v);
+      const float k_factor = power_of_two(HIGHEST - k_exponent), v_factor = power_of_two(HIGHEST - v_exponent);
       ok = room(&k_empty[t % K_STAGES], t / K_STAGES);
       if (!ok) break;
-      const bool good = finite_pair(k_pair) && finite_pair(v_pair);
+      if (r == 0) {
+        exponents[t % RANGES] = make_int2(k_exponent, v_exponent);
+        mbar_arrive(smem_u32(&range[t % RANGES]));
+      }
       const uint32_t pair_of_v = good ? v_pair : 0u;
-      write(Ks + (t % K_STAGES) * KV_BYTES, k, good ? k_pair : NAN_PAIR);
+      write(Ks + (t % K_STAGES) * KV_BYTES, k, good ? k_pair : NAN_PAIR, k_factor);
       hand_over(&k_full[t % K_STAGES]);
       read(p.kc, next_k, k);
       k_pair = next_k.live ? p.kp[next_k.row] : 0u;
       v_pair = next_k.live ? p.vp[next_k.row] : 0u;
       ok = room(&v_empty[t % V_STAGES], t / V_STAGES);
       if (!ok) break;
-      write(Vs + (t % V_STAGES) * KV_BYTES, v, pair_of_v);
+      write(Vs + (t % V_STAGES) * KV_BYTES, v, pair_of_v, v_factor);
       hand_over(&v_full[t % V_STAGES]);
       at_k = next_k;
     }
@@ -305,6 +368,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
     // one thread per row of query tile g
     const int g = (warp - SOFTMAX_WARP0) >> 2;
+    if (g >= groups && lane == 0) mbar_arrive(smem_u32(q_ready));
     if (g < groups && n_tiles > 0) {
       const int q4 = warp & 3;
       const int r = q4 * 32 + lane;
@@ -318,23 +382,49 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       const uint32_t lane_addr = static_cast<uint32_t>(q4 * 32) << 16;
       const uint32_t tmem_s = tmem_base + g * BN, tmem_o = tmem_base + 2 * BN + g * 128;
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int t = 0; t < n_tiles; ++t) {
+      bool ok = mbar_wait(smem_u32(q_full), 0, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      // this thread's row of queries in half precision, its largest element at 2^14 .. 2^15 (rows behind the last are whatever lay there)
+      char* mine = Qs + g * Q_BYTES + r * 128;
+      auto unit = [&](int u) { return reinterpret_cast<uint4*>(mine + (u / 8) * CHUNK_BYTES + (((u % 8) ^ (r & 7)) << 4)); };
+      uint32_t top = 0;
+#pragma unroll
+      for (int u = 0; u < D / 8; ++u) {
+        const uint4 x = *unit(u);
+        top = __vmaxu2(__vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+      }
+      const int q_exponent = exponent_of(max(top << 16, top & 0xffff0000u));
+      const float up = power_of_two(HIGHEST - q_exponent);
+#pragma unroll 4
+      for (int u = 0; u < D / 8; ++u) {
+        const uint4 x = *unit(u);
+        auto both = [&](uint32_t w) { return halves2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); };
+        *unit(u) = make_uint4(both(x.x), both(x.y), both(x.z), both(x.w));
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(q_ready));
+      const float down = power_of_two(q_exponent - HIGHEST);           // of this row's scores
+      int v_exponent = 0;
+      for (int t = 0; ok && t < n_tiles; ++t) {
         const int j0 = (first_tile + t) * BN;
-        ok = mbar_wait(smem_u32(&s_full[g]), t & 1, abort_flag);
+        ok = mbar_wait(smem_u32(&range[t % RANGES]), (t / RANGES) & 1, abort_flag) && mbar_wait(smem_u32(&s_full[g]), t & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tcgen05_fence_after();
+        const int2 of_tile = exponents[t % RANGES];
+        const float k_down = down * power_of_two(of_tile.x - HIGHEST), grown = t > 0 ? power_of_two(v_exponent - of_tile.y) : 1.f;
+        v_exponent = of_tile.y;
         const bool all_visible = j0 + BN - 1 <= pos && j0 >= lo;
         float sv[BN];
 #pragma unroll
         for (int c = 0; c < BN; c += 32) tmem_load32_nowait(tmem_s + lane_addr + c, sv + c);
         tmem_load_wait();
-        float sc = p.scale_log2;
+        float sc = p.scale_log2 * k_down;
         if (p.cap2 > 0.f) {
 #pragma unroll
           for (int e = 0; e < BN; ++e) {
-            const float x = ex2(sv[e] * p.cap_in * (2.f * LOG2E));
+            const float x = ex2(sv[e] * (p.cap_in * k_down * (2.f * LOG2E)));
             sv[e] = p.cap2 * (1.f - __fdividef(2.f, x + 1.f));
           }
           sc = 1.f;
@@ -361,9 +451,10 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         const float m_cand = fmaxf(m, mx * sc);
         const float m_new = (m_cand - m <= 8.f) ? m : m_cand;      // -inf - -inf: moves (to -inf), harmless
         const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = ex2(m - m_safe);
-        // probabilities -> tensor memory, bfloat16 pairs over the first 64 columns of S_g, handed over in P_PARTS parts
-        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        const float alpha = ex2(m - m_safe), from = m_safe - P_UP;
+        // probabilities -> tensor memory, pairs of half precision over the first 64 columns of S_g, handed over in P_PARTS parts
+        F2 sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+        const F2 sc2 = f2(sc, sc), from2 = f2(-from, -from);
 #pragma unroll
         for (int h = 0; h < P_PARTS; ++h) {
 #pragma unroll
@@ -371,20 +462,23 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
             float packed[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float p0 = ex2(fmaf(sv[c + e], sc, -m_safe)), p1 = ex2(fmaf(sv[c + e + 1], sc, -m_safe));        // -inf gives 0
-              sum4[(e / 2) & 3] += p0 + p1;
-              packed[e / 2] = __uint_as_float(pack2(p0, p1));
+              float p0, p1;
+              f2_out(f2_fma(f2(sv[c + e], sv[c + e + 1]), sc2, from2), p0, p1);
+              p0 = ex2(p0);        // -inf gives 0
+              p1 = ex2(p1);
+              sum2[(e / 2) & 1] = f2_add(sum2[(e / 2) & 1], f2(p0, p1));
+              packed[e / 2] = __uint_as_float(halves2(p0, p1));
             }
             tmem_store16(tmem_s + lane_addr + c / 2, packed);
           }
-          if (h == 0 && t > 0 && !__all_sync(0xffffffffu, alpha == 1.f)) {
+          if (h == 0 && t > 0 && !__all_sync(0xffffffffu, alpha * grown == 1.f)) {
             // O_g is rescaled once half of the scores have left their registers, 32 columns at a time
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               float v[32];
               tmem_load32(tmem_o + lane_addr + c, v);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] *= alpha;
+              for (int e = 0; e < 32; ++e) v[e] *= alpha * grown;
               tmem_store32(tmem_o + lane_addr + c, v);
             }
           }
@@ -393,7 +487,9 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&p_full[g * P_PARTS + h]));
         }
-        l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        float sum_a, sum_b;
+        f2_out(f2_add(sum2[0], sum2[1]), sum_a, sum_b);
+        l = l * alpha + (sum_a + sum_b);
         m = m_new;
       }
       if (ok) {
@@ -407,9 +503,9 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
           const float sk = p.sinks[kvh * G + g0 + gg] * LOG2E;
           const float m_new = fmaxf(m, sk);
           alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
-          l = l * alpha + exp2f(sk - m_new);
+          l = l * alpha + exp2f(sk - m_new + P_UP);
         }
-        const float inv = l == 0.f ? 0.f : alpha / l;
+        const float inv = l == 0.f ? 0.f : alpha / l * power_of_two(v_exponent - HIGHEST);
         bf16* dst = p.out + ((size_t)(q_begin + qg + qi) * p.H + kvh * G + g0 + gg) * D;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
