@@ -181,7 +181,8 @@ def attention(q, lengths, ks, vs, scale, window=0, softcap=0.0, sinks=None):
 def allowed(dtype, want, top, span, D, keys):
     """32 bits, sums in any order, additions that cut off (two half steps): a score of D products is off by 2 (D + 8) half steps of its
     terms' sum, a probability by twice that, a sum over the keys by two a key of terms up to twice the range.  bfloat16: the
-    probabilities (times their value's scale) and the result are rounded."""
+    probabilities (times their value's scale) and the result are rounded to at least its bits; what queries as 16-bit integers (2^-16 of a row's largest element
+    each) and keys in half precision (2^-11) add to a score is, for these inputs, below a quarter of that."""
     t = 2.0 ** -24 * (4 * (D + 8) * top + 4 * (keys + 64)) * span
     return t if dtype == torch.float32 else t + 2.0 ** -8 * span + HALF[dtype] * want.abs()
 
@@ -302,3 +303,109 @@ def test_pages_outside_the_pool_are_reported():
             ops.raise_on_device_error()
     finally:
         words_[:] = 0
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("q_size,k_size,v_size", [(1e12, 1e-12, 1e25), (1e-12, 1e12, 1e-25), (1.0, 1.0, 1e-36), (1e-30, 1e30, 1e30)])
+@pytest.mark.parametrize("grows", [0.0, 0.02, -0.02])
+def test_attention_of_any_magnitude(D, page, q_size, k_size, v_size, grows):
+    """Magnitudes that no 16-bit format but bfloat16 holds, and values that grow or shrink 2^10 over a request: a row is as exact as the
+    largest value that it sees (two roundings to bfloat16 of what it adds, and the result's)."""
+    from tinyserve_b200.kernels import ops
+    lengths = [(500, 500), (1, 450), (40, 300)]
+    ctx, view, kc, vc, ks, vs = batch(lengths, 2, D, page, torch.bfloat16)
+    # powers of two: the codes stay, the pairs are exact
+    k_by, v_by = 2.0 ** round(math.log2(k_size)), 2.0 ** round(math.log2(v_size))
+    kc.pairs.mul_(k_by)
+    ks = [x * k_by for x in ks]
+    q = (torch.randn(ctx.num_tokens, 8, D, generator=torch.Generator().manual_seed(9)) * q_size).bfloat16().cuda()
+    bound = []
+    for b, (n, m) in enumerate(lengths):
+        by = v_by * torch.exp2((torch.arange(m) * grows).round()).double().cuda()
+        at = view.block_table[b].long()[torch.arange(m) // page], torch.arange(m) % page
+        vc.pairs[at[0], :, at[1]] = (vc.pairs[at[0], :, at[1]].double() * by[:, None, None]).bfloat16()
+        vs[b] = vs[b] * by[:, None, None]
+        bound.append(vs[b].abs().amax((1, 2)).cummax(0).values[m - n:])
+    bound = torch.cat(bound)[:, None, None]
+    scale = D ** -0.5 * 0.5 / (q_size * k_by)
+    want, _, _ = attention(q, lengths, ks, vs, scale)
+    for backend in ("tcgen05", "mma", "simt"):
+        out = ops.paged_attention(q, kc, vc, view, ctx, scale, backend=backend)
+        assert ((out.double() - want).abs() <= 2 * 2.0 ** -8 * bound + HALF[torch.bfloat16] * want.abs()).all(), backend
+
+
+@pytest.mark.parametrize("H,Hkv", [(8, 2), (4, 4)])
+def test_a_captured_step_serves_other_lengths(H, Hkv):
+    """Write and attention captured for requests of one length, replayed for others of as many tokens: offsets, lengths, tables and slots
+    are read on the device, the host's numbers are bounds."""
+    from tinyserve_b200.kernels import ops
+    D, page, T = 128, 16, 66
+    ctx, view, kc, vc, _, _ = batch([(33, 400), (33, 400)], Hkv, D, page, torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(T, h, D, generator=g, device="cuda").bfloat16() for h in (H, Hkv, Hkv))
+    slots = torch.full((T,), -1, dtype=torch.int32, device="cuda")
+
+    def step():
+        ops.int4_kvwrite(k, v, kc, vc, slots)
+        return ops.paged_attention(q, kc, vc, view, ctx, 0.1)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for lengths in ([(33, 200), (33, 400)], [(1, 7), (65, 400)], [(64, 399), (2, 2)], [(66, 66), (0, 0)], [(5, 100), (30, 30)]):
+        ctx.cu_q.copy_(torch.tensor([0, lengths[0][0], lengths[0][0] + lengths[1][0]], dtype=torch.int32))
+        ctx.kv_lens.copy_(torch.tensor([m for _, m in lengths], dtype=torch.int32))
+        at = [view.block_table[b, j // page].item() * page + j % page for b, (n, m) in enumerate(lengths) for j in range(m - n, m)]
+        slots.fill_(-1)
+        slots[:len(at)] = torch.tensor(at, dtype=torch.int32)
+        out.fill_(-7)
+        graph.replay()
+        replayed = out.clone()
+        dense = [[values(c).transpose(1, 2)[view.block_table[b].long()].flatten(0, 1)[:m] for b, (_, m) in enumerate(lengths)] for c in (kc, vc)]
+        want, top, span = attention(q[:len(at)], lengths, dense[0], dense[1], 0.1)
+        assert ((replayed[:len(at)].double() - want).abs() <= allowed(torch.bfloat16, want, top, span, D, 400)).all(), lengths
+        assert torch.equal(step()[:len(at)], replayed[:len(at)])
+
+
+def test_calls_on_two_streams_at_once():
+    """Products and attention of two streams side by side give what they give alone, bit by bit."""
+    from tinyserve_b200.kernels import ops
+    rows = rows_of(4096, 2048)
+    xs = [torch.randn(m, 2048, generator=torch.Generator().manual_seed(m)).bfloat16().cuda() for m in (3, 40, 700)]
+    cases = [batch(lengths, 2, 128, 16, torch.bfloat16, seed=i) for i, lengths in enumerate(([(1, 9000), (1, 50)], [(70, 700)], [(1, 30)] * 9))]
+    qs = [torch.randn(c[0].num_tokens, 8, 128, generator=torch.Generator().manual_seed(i)).bfloat16().cuda() for i, c in enumerate(cases)]
+
+    def run():
+        return [ops.linear(x, rows) for x in xs] + [ops.paged_attention(q, c[2], c[3], c[1], c[0], 0.1) for q, c in zip(qs, cases)]
+
+    alone = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for results in got:
+        assert all(torch.equal(a, b) for a, b in zip(results, alone))
+
+
+def test_a_captured_product_serves_other_inputs():
+    from tinyserve_b200.kernels import ops
+    rows, bias = rows_of(515, 1040), torch.randn(515, device="cuda")
+    for M in (1, 20, 130):
+        x = torch.randn(M, 1040, device="cuda").bfloat16()
+        ops.linear(x, rows, bias)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.linear(x, rows, bias)
+        for seed in range(3):
+            x.copy_(torch.randn(M, 1040, generator=torch.Generator().manual_seed(seed)).bfloat16())
+            if seed == 2:
+                x[M // 2] = math.nan
+            graph.replay()
+            assert torch.equal(out.nan_to_num(7.0), ops.linear(x, rows, bias).nan_to_num(7.0))

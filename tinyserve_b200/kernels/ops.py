@@ -2924,14 +2924,16 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     most = columns = 0
     if chosen != "simt":
         few = max(1, INT4_DIRECT_ROWS // G)
+        # (requests of one length, it seems: the portions' kernel takes them all, whatever the offsets on the device hold)
+        alike = B == 1 or T == B * max_q_len
         if chosen == "tcgen05" and max_q_len > few and scale > 0 and (q.data_ptr() | 2 * q_row | 2 * q_head) % 16 == 0 and q_row > 0 and q_head > 0:
             tc, portions = _entry(D, "ts_int4_attention_tcgen05")
             _launched(tc, portions(q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                                    v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H,
-                                   Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, few,
-                                   stream), 1)
-            if B == 1 or T == B * max_q_len:
-                return out           # (no request has fewer queries than the longest)
+                                   Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None,
+                                   0 if alike else few, stream), 1)
+            if alike:
+                return out
             most = max_q_len = few
         rows = max_q_len * G
         columns = 16 if rows > 8 and D <= 128 else 8
