@@ -306,6 +306,7 @@ struct Int4Params {
   const float* sinks;                        // [H] or null: one more term exp(sinks[h]) in head h's sum
   int splits;                                // key ranges; > 1: partial results for the combine kernel
   int most;                                  // > 0: requests with more queries are somebody else's
+  int ordered;                               // != 0: blocks take the requests by length, the longest first
   float *part_o, *part_ml;                   // [T * H][splits][D], [T * H][splits][2] (maximum in the log2 domain, sum)
 };
 
@@ -544,6 +545,11 @@ __global__ void int4_combine_kernel(Int4Params p) {
 //   bfloat16(p s), sum p v = sum p' (c - 8) + sum p (z + 8 s), and sum p' (c - 8) = sum p' (16 + c) - 24 sum p', which is one more MMA, with
 //   ones for V, so that the 24 cancels whatever p' was rounded to.  (Around the middle of the codes the rounding of p' weighs half as much as
 //   around 0: 4,096 keys, relative error of the output before its own rounding 1.4e-3 and 2.5e-3.)
+// Values of 2^110 and more may overflow these sums, as probabilities reach 2^8 in them.
+// 64 requests of 2,000 to 8,192 keys, 32 heads of 128 on 8 (366 MB): 87 us, 4.2 TB/s; fetching alone takes 62.  The integer pipe is busiest (two thirds of its
+// rate while a block walks), then the fixed 5 us of a block, of which an SM holds two.  Requests in the order of their numbers instead of by length:
+// 108 us, for the blocks that come last run alone.  Shifts as multiplications on the other pipe 91 and 99 us, three blocks an SM
+// with 80 registers a thread 123.
 constexpr int MMA_WARPS = 8, STEP = 32, RING = 3;
 constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
 constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;   // codes of K and V, pairs of K and V
@@ -617,6 +623,23 @@ constexpr uint32_t ONES = 0x3f803f80u;                             // two bfloat
 // 2t + 9) in keys t, t + 4, t + 8, t + 12, and the eight lanes whose reads of K meet read neighbouring keys' halves of a bank line
 __device__ __forceinline__ int key_of_row(int r) { return (r & 8) | (r >> 1 & 3) | (r & 1) << 2; }
 
+// The request with the n-th longest cache, for up to 256 of them (a thread each); `lens` is 256 integers of shared memory.  Blocks come in
+// the order of their index, and a long one that comes last runs alone.
+__device__ __forceinline__ int nth_longest(const Int4Params& p, int n, int* lens) {
+  const int i = threadIdx.x, len = i < p.B ? p.kv_lens[i] : -1;
+  lens[i] = len;
+  __syncthreads();
+  int before = 0;
+  for (int j = 0; j < p.B; j += 4) {
+    const int4 x = *reinterpret_cast<const int4*>(lens + j);
+    before += (x.x > len || (x.x == len && j < i)) + (x.y > len || (x.y == len && j + 1 < i)) + (x.z > len || (x.z == len && j + 2 < i)) + (x.w > len || (x.w == len && j + 3 < i));
+  }
+  __syncthreads();
+  if (i < p.B && before == n) lens[0] = i;
+  __syncthreads();
+  return lens[0];
+}
+
 template <int NT>
 __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_kernel(Int4Params p) {
   using C = MmaCfg<NT>;
@@ -634,10 +657,14 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   pdl_trigger();
   pdl_wait();
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
-  const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC, b = blockIdx.z;
+  const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC;
+  const int b = p.ordered ? nth_longest(p, blockIdx.z, reinterpret_cast<int*>(work)) : blockIdx.z;
+  if (p.ordered) __syncthreads();                                  // (its memory is the ring's)
   const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
   const int nc = min(C::NC, q_len * G - c0);                       // columns of this block (and of its cluster: they leave together)
   if (nc <= 0 || (p.most > 0 && q_len > p.most)) return;
+  const bool clustered = p.splits > 1 && p.part_o == nullptr;
+  if (clustered) cluster_arrive();                                 // this block runs: peers may write to its memory
   const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
   const int pos0 = kv_len - q_len;                                 // position of the request's first query of this step
   const int* bt = p.block_table + (size_t)b * p.table_stride;
@@ -647,20 +674,23 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   const int s_end = min(steps, (split + 1) * per);
 
   char* ring = work + warp * RING * STAGE_BYTES;
-  // A step's 32 keys lie in whole or in runs of a page; every run is four copies (codes and pairs of K and V) by a lane of its own.  A run
-  // that starts behind the last key is not fetched, and what its place holds is masked.
-  const int run_shift = min(p.page_shift, 5), runs = STEP >> run_shift, run_keys = 1 << run_shift;
-  const uint32_t ring_at = smem_u32(ring), run_at = lane << run_shift, code_bytes = ROW_BYTES << run_shift, pair_bytes = 4 * run_keys;
+  // A step's 32 keys lie in whole or in runs of a page; every run is four copies (codes of K and V, pairs of K and V), each by a lane of its
+  // own: eight runs of four keys are all 32 lanes.  A run that starts behind the last key is not fetched, and what its place holds is masked.
+  const int run_shift = min(p.page_shift, 5), run = lane >> 2 << run_shift;
+  const char* base = reinterpret_cast<const char*>(lane & 2 ? (lane & 1 ? p.vp : p.kp) : (lane & 1 ? p.vc : p.kc));
+  const uint32_t row_bytes = lane & 2 ? 4 : ROW_BYTES, run_bytes = row_bytes << run_shift;
+  const uint32_t run_at = smem_u32(ring) + (lane & 2 ? 2 * STEP * ROW_BYTES : 0) + ((lane & 1) * STEP + run) * row_bytes;
+  const int last_run = run < STEP ? j_hi - run : 0;                // a step that starts in front of it has keys for this lane
   int page_ahead = 0;          // of this lane's run of the step that is fetched next: read a step before it is needed
   auto look = [&](int s) {
-    const int j = (step0 + s) * STEP + (lane << run_shift);
-    if (s < s_end && lane < runs && j < j_hi) page_ahead = bt[j >> p.page_shift];
+    const int j = (step0 + s) * STEP;
+    if (s < s_end && j < last_run) page_ahead = bt[(j + run) >> p.page_shift];
   };
   auto fetch = [&](int s, int stage) {
-    const int j = (step0 + s) * STEP + (lane << run_shift);
-    const bool mine = lane < runs && j < j_hi;
+    const int j = (step0 + s) * STEP;
+    const bool mine = j < last_run;
     const uint32_t bar = smem_u32(&full[warp][stage]);
-    const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
+    const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine)) >> 2;
     if (lane == 0) mbar_expect_tx(bar, n * (STAGE_BYTES >> (5 - run_shift)));
     __syncwarp();
     if (mine) {
@@ -669,13 +699,8 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
         page_ahead = 0;
       }
       // (a pool of this kernel has fewer than 2^31 rows: one multiplication a copy)
-      const uint32_t row = (((uint32_t)page_ahead * p.Hkv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1));
-      const uint32_t at = ring_at + stage * STAGE_BYTES + run_at * ROW_BYTES, pairs_at = ring_at + stage * STAGE_BYTES + 2 * STEP * ROW_BYTES + run_at * 4;
-      const unsigned long long codes = (unsigned long long)row * ROW_BYTES, pairs = (unsigned long long)row * 4;
-      bulk_copy(at, reinterpret_cast<const char*>(p.kc) + codes, code_bytes, bar);
-      bulk_copy(at + STEP * ROW_BYTES, reinterpret_cast<const char*>(p.vc) + codes, code_bytes, bar);
-      bulk_copy(pairs_at, reinterpret_cast<const char*>(p.kp) + pairs, pair_bytes, bar);
-      bulk_copy(pairs_at + STEP * 4, reinterpret_cast<const char*>(p.vp) + pairs, pair_bytes, bar);
+      const uint32_t row = (((uint32_t)page_ahead * p.Hkv + kvh) << p.page_shift) + ((j + run) & ((1 << p.page_shift) - 1));
+      bulk_copy(run_at + stage * STAGE_BYTES, base + (unsigned long long)row * row_bytes, run_bytes, bar);
     }
     look(s + MMA_WARPS);
   };
@@ -956,6 +981,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   }
 
   // the warps' results meet in shared memory
+  if (clustered) cluster_wait();                                   // (all peers run)
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][MERGE_ROW]: output column d of lane group g at place (d's number there) * 8 + g
   float* sm_ml = sm_o + MMA_WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
@@ -1026,7 +1052,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       if (place < 2) send(smem_u32(box + at * MERGE_ROW + D + place), c % p.splits, place == 0 ? top : total);
     }
   }
-  if (p.splits == 1 || p.part_o != nullptr) return;
+  if (!clustered) return;
   cluster_arrive();
   cluster_wait();
   for (int i = threadIdx.x; i < per_rank * D; i += MMA_WARPS * 32) {
@@ -1052,7 +1078,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
 }
 
 template <int NT>
-int attend_mma(const Int4Params& p, int max_q_len, cudaStream_t stream) {
+int attend_mma(Int4Params p, int max_q_len, cudaStream_t stream) {
   using C = MmaCfg<NT>;
   static SmemSet set;
   const cudaError_t sized = set.to(int4_mma_kernel<NT>, C::SMEM);
@@ -1061,6 +1087,8 @@ int attend_mma(const Int4Params& p, int max_q_len, cudaStream_t stream) {
   const long long tiles = ((long long)max_q_len * G + C::NC - 1) / C::NC * p.Hkv;
   TS_REQUIRE(tiles <= 65535 && p.B <= 65535, "int4_attention: grid out of range");
   const dim3 grid(p.splits, (unsigned)tiles, p.B), block(MMA_WARPS * 32);
+  // (when everything runs at once, on 148 SMs, order is no use)
+  p.ordered = p.B > 1 && p.B <= MMA_WARPS * 32 && tiles * p.splits * p.B > (long long)C::BLOCKS * 148;
   if (p.splits > 1 && p.part_o == nullptr) {
     // the key ranges of a tile are a cluster and merge in it
     const cudaError_t e = ts_launch_cluster(int4_mma_kernel<NT>, grid, block, C::SMEM, stream, dim3(p.splits, 1, 1), p);
@@ -1160,7 +1188,7 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
   TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml) || (columns > 0 && splits <= 8 && !part_o)), "int4_attention: key ranges need their scratch");
   Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
                   block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
-                  splits, most, part_o, part_ml};
+                  splits, most, 0, part_o, part_ml};
   if (columns > 0) {
 #ifdef TS_INT4_MMA
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");

@@ -2846,7 +2846,7 @@ def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary
 def int4_attention_error(head_dim: int) -> int:
     """1 if a block of the tensor-core kernels over a 4-bit cache ever gave up on a wait (synchronises)."""
     portions = _attention_int4_tcgen05(head_dim).ts_attention_int4_tcgen05_error() if head_dim in TCGEN05_HEAD_DIMS else 0
-    return _attention_int4(head_dim).ts_int4_attention_error() or portions
+    return (_attention_int4(head_dim).ts_int4_attention_error() if int4_attention_backend(torch.bfloat16, head_dim) != "simt" else 0) or portions
 
 
 def int4_attention_backend(dtype, head_dim) -> str:
@@ -2868,14 +2868,15 @@ INT4_CLUSTER_SPLITS = 8
 
 def int4_decode_splits(blocks, max_kv_len):
     """Key ranges of the tensor-core kernel over a 4-bit cache: two blocks an SM, at least 160 keys a range (five of its eight warps
-    have a step of 32), in powers of two as long as they merge in a cluster; and two where the blocks of a ragged batch
-    would not come out even (us: 1 request of 640 keys 7.4 whole, 6.5 in four; 64 of 2,000 to 8,192 112.9 whole, 109.4 in two; 3 of 32,768
-    40.3 in eight, 35.6 in twelve, 39.3 in 24)."""
+    have a step of 32), in powers of two as long as they merge in a cluster, in more than that behind 2,048 keys a range; and two where long requests
+    would otherwise leave SMs idle that shorter ones had (8 key heads, 2,000 to 8,192 keys, us whole / in two / four / eight / twelve: 4 requests 40.6 / 24.4 /
+    19.2 / 14.1 / 19.0; 8 43.6 / 30.8 / 21.5 / 25.4 / 27.9; 20 59.5 / 39.4 / 45.8; 32 68.4 / 51.4 / 67.2, of 8,000 to 8,192 71.8 / 80.7; 64 82.9 /
+    98.1 / 132.6; 3 of 32,768 174 / 91 / 63.5 / 40.7 / 35.7)."""
     want = min(2 * num_sms() // blocks, max_kv_len // 160, 32)
-    if want > INT4_CLUSTER_SPLITS:
+    if want > INT4_CLUSTER_SPLITS and max_kv_len > INT4_CLUSTER_SPLITS * 2048:
         return want
     if want < 2:
-        return 2 if 2 * num_sms() < blocks <= 4 * num_sms() and max_kv_len >= 2048 else 1
+        return 2 if blocks <= 2 * num_sms() and max_kv_len >= 2048 else 1
     return 8 if want >= 8 else 4 if want >= 4 else 2
 
 
