@@ -60,6 +60,18 @@ def test_cuts_along_k_are_never_empty():
                 assert (tile, s) == (256, 0) or (tile in (16, 32, 64, 128) and 1 <= s <= 8 and (s - 1) * -(-slices // s) < slices)
 
 
+def test_how_keys_are_cut():
+    from tinyserve_b200.kernels import ops
+    for blocks in (1, 8, 24, 64, 100, 150, 296, 297, 740, 741, 10 ** 6):
+        for keys in (0, 1, 160, 2047, 2048, 32768, 10 ** 6):
+            splits = ops.int4_decode_splits(blocks, keys)
+            assert 1 <= splits <= 32 and (splits == 1 or (splits * 160 <= keys and splits * blocks <= 4 * ops.num_sms()))
+            assert splits in (1, 2, 4, 8) or splits > ops.INT4_CLUSTER_SPLITS
+            assert 1 <= ops.int4_attention_splits(blocks, keys) <= 32
+            for D in (32, 128, 160):
+                assert ops.int4_decode_warps(blocks, splits, D) == (4 if splits == 1 and D <= 128 and blocks > 740 else 8)
+
+
 def test_pages_in_4_bits():
     from tinyserve_b200.kernels import ops
     with pytest.raises(TypeError, match="uint8"):

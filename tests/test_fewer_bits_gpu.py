@@ -409,3 +409,33 @@ def test_a_captured_product_serves_other_inputs():
                 x[M // 2] = math.nan
             graph.replay()
             assert torch.equal(out.nan_to_num(7.0), ops.linear(x, rows, bias).nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("B,Hkv,D,page,window", [(40, 8, 64, 16, 0), (100, 8, 32, 4, 0), (100, 8, 128, 16, 40), (190, 4, 64, 8, 0), (257, 3, 64, 16, 0), (300, 1, 128, 32, 0), (33, 9, 96, 64, 0)])
+def test_attention_of_many_requests(B, Hkv, D, page, window):
+    """More blocks than run at once: long requests first, blocks of four warps; two of equal length, one without keys, padding rows behind the last."""
+    from tinyserve_b200.kernels import ops
+    g = torch.Generator().manual_seed(B)
+    lengths = [(1, int(m)) for m in torch.randint(1, 400, (B,), generator=g)]
+    lengths[3], lengths[7], lengths[B // 2] = (1, 900), (1, 900), (0, 12)
+    ctx, view, kc, vc, ks, vs = batch(lengths, Hkv, D, page, torch.bfloat16)
+    q = torch.randn(B + 5, 2 * Hkv, D, generator=g).bfloat16().cuda()
+    out = ops.paged_attention(q, kc, vc, view, ctx, 0.1, window)[:B - 1]
+    want, top, span = attention(q[:B - 1], lengths, ks, vs, 0.1, window)
+    assert ((out.double() - want).abs() <= allowed(torch.bfloat16, want, top, span, D, 900)).all()
+    assert ops.int4_attention_error(D) == 0 and ops.int4_attention_error(48) == 0
+
+
+def test_products_that_follow_a_product():
+    """Int8Rows as the weight of a gated, an activated and a joint product: the plain product, then what follows it."""
+    from tinyserve_b200.kernels import ops
+    for M in (1, 40, 300):
+        x = torch.randn(M, 512, generator=torch.Generator().manual_seed(M)).bfloat16().cuda()
+        rows, other = rows_of(768, 512), rows_of(256, 512, 1)
+        y = ops.linear(x, rows)
+        assert torch.equal(ops.gated_linear(x, rows), ops.gated_activation(y, "silu"))
+        assert torch.equal(ops.activated_linear(x, rows, "gelu_tanh" if "gelu_tanh" in ops.PLAIN_ACTIVATIONS else sorted(ops.PLAIN_ACTIVATIONS)[0]),
+                           ops.plain_activation_(y.clone(), "gelu_tanh" if "gelu_tanh" in ops.PLAIN_ACTIVATIONS else sorted(ops.PLAIN_ACTIVATIONS)[0]))
+        # rows of one row, of none, and a row read again and again
+        assert torch.equal(ops.linear(x[:1].expand(3, -1), other), ops.linear(x[:1], other).expand(3, -1))
+        assert ops.linear(x[:0], other).shape == (0, 256) and ops.quantize_rows(x[:0]).codes.shape == (0, 512)

@@ -550,23 +550,23 @@ __global__ void int4_combine_kernel(Int4Params p) {
 // rate while a block walks), then the fixed 5 us of a block, of which an SM holds two.  Requests in the order of their numbers instead of by length:
 // 108 us, for the blocks that come last run alone.  Shifts as multiplications on the other pipe 91 and 99 us, three blocks an SM
 // with 80 registers a thread 123.
-constexpr int MMA_WARPS = 8, STEP = 32, RING = 3;
+constexpr int STEP = 32, RING = 3;
 constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
 constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;   // codes of K and V, pairs of K and V
 constexpr float MIDDLE = 8.f, ABOVE = 16.f + MIDDLE;               // of the codes; what a code's bfloat16 is above c - MIDDLE
 constexpr int MERGE_ROW = D + 4;                                   // floats of a column's partial result: the four columns of a quad meet other banks
 
-template <int NT> struct MmaCfg {
+template <int NT, int WARPS> struct MmaCfg {
   static constexpr int NC = 8 * NT, MAX_CLUSTER = 8;
   static constexpr int Q_BYTES = KW * NT * 32 * 16 + NC * 8;       // operands; (factor, sum) of every column
-  static constexpr int RING_BYTES = MMA_WARPS * RING * STAGE_BYTES;
-  static constexpr int MERGE_BYTES = MMA_WARPS * NC * (MERGE_ROW + 3) * 4;
+  static constexpr int RING_BYTES = WARPS * RING * STAGE_BYTES;
+  static constexpr int MERGE_BYTES = WARPS * NC * (MERGE_ROW + 3) * 4;
   static constexpr int WORK_BYTES = RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES;
   // what the blocks of a cluster send each other: with n of them [sender][column / n rounded up][D + 4]
-  static constexpr int BOX_BYTES = (NC + MAX_CLUSTER) * MERGE_ROW * 4;
+  static constexpr int BOX_BYTES = WARPS == 8 ? (NC + MAX_CLUSTER) * MERGE_ROW * 4 : 0;
   static constexpr int SMEM = Q_BYTES + WORK_BYTES + BOX_BYTES;
   static constexpr bool Q_REGS = NT == 1 && D <= 128;              // the queries' operands stay in registers
-  static constexpr int BLOCKS = Q_REGS ? 2 : 1;
+  static constexpr int BLOCKS = Q_REGS ? 16 / WARPS : 1;          // of an SM
 };
 
 // bytes (a multiple of 16) of global memory to shared memory, counted by a barrier
@@ -623,28 +623,38 @@ constexpr uint32_t ONES = 0x3f803f80u;                             // two bfloat
 // 2t + 9) in keys t, t + 4, t + 8, t + 12, and the eight lanes whose reads of K meet read neighbouring keys' halves of a bank line
 __device__ __forceinline__ int key_of_row(int r) { return (r & 8) | (r >> 1 & 3) | (r & 1) << 2; }
 
-// The request with the n-th longest cache, for up to 256 of them (a thread each); `lens` is 256 integers of shared memory.  Blocks come in
-// the order of their index, and a long one that comes last runs alone.
+// The request with the n-th longest cache, of up to 256; `lens` is as many integers of shared memory.  Blocks come in the order of their
+// index, and a long one that comes last runs alone.
+constexpr int MAX_ORDERED = 256;
+template <int THREADS>
 __device__ __forceinline__ int nth_longest(const Int4Params& p, int n, int* lens) {
-  const int i = threadIdx.x, len = i < p.B ? p.kv_lens[i] : -1;
-  lens[i] = len;
+#pragma unroll
+  for (int i = threadIdx.x; i < MAX_ORDERED; i += THREADS) lens[i] = i < p.B ? p.kv_lens[i] : -1;
   __syncthreads();
-  int before = 0;
-  for (int j = 0; j < p.B; j += 4) {
-    const int4 x = *reinterpret_cast<const int4*>(lens + j);
-    before += (x.x > len || (x.x == len && j < i)) + (x.y > len || (x.y == len && j + 1 < i)) + (x.z > len || (x.z == len && j + 2 < i)) + (x.w > len || (x.w == len && j + 3 < i));
+  int found = -1;
+#pragma unroll
+  for (int i = threadIdx.x; i < MAX_ORDERED; i += THREADS) {
+    const int len = lens[i];
+    int before = 0;
+    if (i < p.B) {
+      for (int j = 0; j < p.B; j += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(lens + j);
+        before += (x.x > len || (x.x == len && j < i)) + (x.y > len || (x.y == len && j + 1 < i)) + (x.z > len || (x.z == len && j + 2 < i)) + (x.w > len || (x.w == len && j + 3 < i));
+      }
+      if (before == n) found = i;
+    }
   }
   __syncthreads();
-  if (i < p.B && before == n) lens[0] = i;
+  if (found >= 0) lens[0] = found;
   __syncthreads();
   return lens[0];
 }
 
-template <int NT>
-__global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_kernel(Int4Params p) {
-  using C = MmaCfg<NT>;
+template <int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mma_kernel(Int4Params p) {
+  using C = MmaCfg<NT, WARPS>;
   extern __shared__ __align__(16) char smem[];
-  __shared__ uint64_t full[MMA_WARPS][RING];
+  __shared__ uint64_t full[WARPS][RING];
   __shared__ volatile int abort_flag;
   uint4* qf_s = reinterpret_cast<uint4*>(smem);                    // [KW][NT][32 lanes]: high and low bytes of eight columns
   float2* q_stat = reinterpret_cast<float2*>(smem + KW * NT * 32 * 16);       // [NC]
@@ -658,12 +668,12 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   pdl_wait();
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
   const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC;
-  const int b = p.ordered ? nth_longest(p, blockIdx.z, reinterpret_cast<int*>(work)) : blockIdx.z;
+  const int b = p.ordered ? nth_longest<WARPS * 32>(p, blockIdx.z, reinterpret_cast<int*>(work)) : blockIdx.z;
   if (p.ordered) __syncthreads();                                  // (its memory is the ring's)
   const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
   const int nc = min(C::NC, q_len * G - c0);                       // columns of this block (and of its cluster: they leave together)
   if (nc <= 0 || (p.most > 0 && q_len > p.most)) return;
-  const bool clustered = p.splits > 1 && p.part_o == nullptr;
+  const bool clustered = WARPS == 8 && p.splits > 1 && p.part_o == nullptr;
   if (clustered) cluster_arrive();                                 // this block runs: peers may write to its memory
   const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
   const int pos0 = kv_len - q_len;                                 // position of the request's first query of this step
@@ -702,16 +712,16 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
       const uint32_t row = (((uint32_t)page_ahead * p.Hkv + kvh) << p.page_shift) + ((j + run) & ((1 << p.page_shift) - 1));
       bulk_copy(run_at + stage * STAGE_BYTES, base + (unsigned long long)row * row_bytes, run_bytes, bar);
     }
-    look(s + MMA_WARPS);
+    look(s + WARPS);
   };
   const int mine = split * per + warp;
   look(mine);
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i)
-    if (mine + i * MMA_WARPS < s_end) fetch(mine + i * MMA_WARPS, i);
+    if (mine + i * WARPS < s_end) fetch(mine + i * WARPS, i);
 
   // the queries as B operands: a warp makes a column, a lane a word's eight columns: word t KW + i goes to step i, thread t of the column's quad
-  for (int c = warp; c < C::NC; c += MMA_WARPS) {
+  for (int c = warp; c < C::NC; c += WARPS) {
     float x[8] = {};
     if (lane < W && c < nc) {
       const int r = c0 + c;
@@ -788,12 +798,12 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   int stage = 0, waits = 0;
   bool ok = true;
 #pragma unroll 1
-  for (int s = mine; s < s_end; s += MMA_WARPS) {
+  for (int s = mine; s < s_end; s += WARPS) {
     ok = mbar_wait(smem_u32(&full[warp][stage]), waits & 1, &abort_flag);
     ok = __all_sync(0xffffffffu, ok);          // (and everybody has read what the stage before this one held)
     if (!ok) break;
     {
-      const int ahead = s + (RING - 1) * MMA_WARPS;
+      const int ahead = s + (RING - 1) * WARPS;
       if (ahead < s_end) fetch(ahead, stage == 0 ? RING - 1 : stage - 1);
     }
     const char* ks = ring + stage * STAGE_BYTES;
@@ -984,7 +994,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   if (clustered) cluster_wait();                                   // (all peers run)
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(work);                    // [warp][column][MERGE_ROW]: output column d of lane group g at place (d's number there) * 8 + g
-  float* sm_ml = sm_o + MMA_WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
+  float* sm_ml = sm_o + WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
   float* box = reinterpret_cast<float*>(work + C::WORK_BYTES);     // (its own memory: a peer may send while this block still reads its ring)
   const int per_rank = (C::NC + p.splits - 1) / p.splits;
   auto send = [](uint32_t at, uint32_t rank, float v) {
@@ -1019,7 +1029,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nc * D; i += MMA_WARPS * 32) {
+  for (int i = threadIdx.x; i < nc * D; i += WARPS * 32) {
     const int c = i / D, place = i % D, r = c0 + c, head = kvh * G + r % G;
     // place 8 n + g: nibble n % 4 of unit g UNITS + n / 4
     const int unit = (place & 7) * UNITS + (place >> 5), d = 8 * (unit >> 1) + (unit & 1) + 2 * (place >> 3 & 3);
@@ -1028,10 +1038,10 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
     const float sink2 = sink ? p.sinks[head] * LOG2E : LOWEST;
     float top = fmaxf(LOWEST, sink2);
 #pragma unroll
-    for (int w = 0; w < MMA_WARPS; ++w) top = fmaxf(top, sm_ml[(w * C::NC + c) * 3]);
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_ml[(w * C::NC + c) * 3]);
     float sum = 0.f, total = sink ? ex2(sink2 - top) : 0.f;
 #pragma unroll
-    for (int w = 0; w < MMA_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const float* ml = sm_ml + (w * C::NC + c) * 3;
       const float f = ex2(ml[0] - top);
       total += f * ml[1];
@@ -1055,7 +1065,7 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   if (!clustered) return;
   cluster_arrive();
   cluster_wait();
-  for (int i = threadIdx.x; i < per_rank * D; i += MMA_WARPS * 32) {
+  for (int i = threadIdx.x; i < per_rank * D; i += WARPS * 32) {
     const int c = i / D * p.splits + split, place = i % D, r = c0 + c, head = kvh * G + r % G;
     if (c >= nc) break;
     const int unit = (place & 7) * UNITS + (place >> 5), d = 8 * (unit >> 1) + (unit & 1) + 2 * (place >> 3 & 3);
@@ -1077,25 +1087,25 @@ __global__ void __launch_bounds__(MMA_WARPS * 32, MmaCfg<NT>::BLOCKS) int4_mma_k
   }
 }
 
-template <int NT>
+template <int NT, int WARPS>
 int attend_mma(Int4Params p, int max_q_len, cudaStream_t stream) {
-  using C = MmaCfg<NT>;
+  using C = MmaCfg<NT, WARPS>;
   static SmemSet set;
-  const cudaError_t sized = set.to(int4_mma_kernel<NT>, C::SMEM);
+  const cudaError_t sized = set.to(int4_mma_kernel<NT, WARPS>, C::SMEM);
   if (sized != cudaSuccess) return ts_fail("int4_attention: %s", cudaGetErrorString(sized));
   const int G = p.H / p.Hkv;
   const long long tiles = ((long long)max_q_len * G + C::NC - 1) / C::NC * p.Hkv;
   TS_REQUIRE(tiles <= 65535 && p.B <= 65535, "int4_attention: grid out of range");
-  const dim3 grid(p.splits, (unsigned)tiles, p.B), block(MMA_WARPS * 32);
+  const dim3 grid(p.splits, (unsigned)tiles, p.B), block(WARPS * 32);
   // (when everything runs at once, on 148 SMs, order is no use)
-  p.ordered = p.B > 1 && p.B <= MMA_WARPS * 32 && tiles * p.splits * p.B > (long long)C::BLOCKS * 148;
+  p.ordered = p.B > 1 && p.B <= MAX_ORDERED && tiles * p.splits * p.B > (long long)C::BLOCKS * 148;
   if (p.splits > 1 && p.part_o == nullptr) {
     // the key ranges of a tile are a cluster and merge in it
-    const cudaError_t e = ts_launch_cluster(int4_mma_kernel<NT>, grid, block, C::SMEM, stream, dim3(p.splits, 1, 1), p);
+    const cudaError_t e = ts_launch_cluster(int4_mma_kernel<NT, WARPS>, grid, block, C::SMEM, stream, dim3(p.splits, 1, 1), p);
     if (e != cudaSuccess) return ts_fail("int4_attention (clusters of %d): %s", p.splits, cudaGetErrorString(e));
     return 0;
   }
-  TS_LAUNCH("int4_attention", int4_mma_kernel<NT>, grid, block, C::SMEM, stream, p);
+  TS_LAUNCH("int4_attention", int4_mma_kernel<NT, WARPS>, grid, block, C::SMEM, stream, p);
   if (p.splits > 1)
     TS_LAUNCH("int4_attention (combine)", int4_combine_kernel<bf16>, dim3((unsigned)(p.T * p.H)), dim3(D < 128 ? D : 128), 0, stream, p);
   return 0;
@@ -1173,13 +1183,13 @@ TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const in
 }
 
 // q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml, or (with columns, up to 8) merges in clusters.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
-// steps of 32 up to 256; 16 columns up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns):
+// steps of 32 up to 256; 16 columns up to 128) with 8 warps a block, or 4 (8 columns, one key range, heads up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns):
 // requests with more queries than that are left alone.
 TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
                                 const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
                                 int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
                                 int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, int max_q_len,
-                                int columns, int most, cudaStream_t stream) {
+                                int columns, int warps, int most, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_attention: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
@@ -1194,12 +1204,13 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");
     TS_REQUIRE(((long long)num_pages * Hkv << shift) < (1LL << 31), "int4_attention: the tensor-core kernel takes pools of fewer than 2^31 rows");
     TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 15) == 0, "int4_attention: the tensor-core kernel copies runs that begin on 16 bytes");
-    if (columns == 8) return attend_mma<1>(p, max_q_len, stream);
+    if (columns == 8 && warps == 8) return attend_mma<1, 8>(p, max_q_len, stream);
 #if TS_HEAD_DIM <= 128
-    if (columns == 16) return attend_mma<2>(p, max_q_len, stream);
+    if (columns == 8 && warps == 4 && splits == 1) return attend_mma<1, 4>(p, max_q_len, stream);
+    if (columns == 16 && warps == 8) return attend_mma<2, 8>(p, max_q_len, stream);
 #endif
 #endif
-    return ts_fail("int4_attention: no tensor-core kernel for heads of %d and %d columns", D, columns);
+    return ts_fail("int4_attention: no tensor-core kernel for heads of %d, %d columns and %d warps", D, columns, warps);
   }
   return dtype == TS_F32 ? attend_simt<float>(p, stream) : attend_simt<bf16>(p, stream);
 }

@@ -2587,7 +2587,7 @@ _INT4_ENTRIES = {
     "ts_int4_rope_kvwrite": (_INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR, _PTR, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR,
                              _PTR, _INT, _INT, _PTR),
     "ts_int4_attention": (_INT, _PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
-                          _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR, _PTR, _INT, _INT, _INT, _PTR),
+                          _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR, _PTR, _INT, _INT, _INT, _INT, _PTR),
     "ts_int4_attention_tcgen05": (_PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
                                   _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR),
 }
@@ -2880,6 +2880,14 @@ def int4_decode_splits(blocks, max_kv_len):
     return 8 if want >= 8 else 4 if want >= 4 else 2
 
 
+def int4_decode_warps(blocks, splits, head_dim):
+    """Warps of a block of the tensor-core kernel over a 4-bit cache: four, of which an SM holds four blocks, where there are more blocks than it
+    holds by a quarter (a block's start and end then hide behind three others); else eight, two blocks an SM, which come out more even
+    (8 key heads, us by eight / four: 300 requests of 100 to 2,000 keys 115 / 102, 200 92.7 / 77; 100 of 500 to 4,000 71 / 69; 128 of 2,000 to
+    8,192 155 / 154, 90 115 / 128, 64 87 / 125; 64 of 100 to 1,500 24.5 / 28.4)."""
+    return 4 if blocks > 5 * num_sms() and splits == 1 and head_dim <= 128 else 8
+
+
 def int4_attention_splits(blocks, max_kv_len):
     """Key ranges of the 32-bit kernel over a 4-bit cache: four blocks an SM, a tile of 128 keys a range at least (5 requests of 700 to
     1,900 keys, 16 heads on 8, us: one range 109, four 34.8, eight 23.4, sixteen 17.8, 32 20.4)."""
@@ -2943,6 +2951,7 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
             columns = most = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes everything)
     if num_splits is None:
         num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
+    warps = int4_decode_warps(B * Hkv * -(-rows // columns), num_splits, D) if columns == 8 else 8
     part_o = part_ml = None
     merged = columns > 0 and num_splits <= INT4_CLUSTER_SPLITS          # (in clusters, without scratch)
     if num_splits > 1 and not merged:
@@ -2952,5 +2961,5 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     _launched(lib, fn(_DTYPE[dtype], q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                       v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H, Hkv, page,
                       blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, num_splits, part_o, part_ml,
-                      max_q_len, columns, most, stream), 1 if num_splits == 1 or merged else 2)
+                      max_q_len, columns, warps, most, stream), 1 if num_splits == 1 or merged else 2)
     return out
