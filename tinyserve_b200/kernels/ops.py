@@ -2604,14 +2604,14 @@ def _entry(unit, name):
 
 def _here(what, *tensors):
     """Operands lie on the current device: the launch goes to its current stream, which is returned."""
-    here = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else -1
+    here = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.get_device() != here:
-            if not t.is_cuda:
+        if t is not None and (t.get_device() != here or here < 0):
+            if not t.is_cuda or here < 0:
                 raise RuntimeError("kernel operands must be CUDA tensors: there is no CPU path")
-            raise RuntimeError(f"{what}: an operand lies on {t.device}, the current device is cuda:{here}")
-    if here < 0:
-        raise RuntimeError("kernel operands must be CUDA tensors: there is no CPU path")
+            raise RuntimeError(f"{what}: operands lie on {t.device} and on cuda:{here}")
+    if here != torch._C._cuda_getDevice():          # (there is a CUDA tensor: the runtime is up)
+        raise RuntimeError(f"{what}: the operands lie on cuda:{here}, the current device is cuda:{torch.cuda.current_device()}")
     return _STREAM.value if _STREAM is not None else torch._C._cuda_getCurrentRawStream(here)
 
 
