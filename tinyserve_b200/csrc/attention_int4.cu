@@ -10,6 +10,7 @@
 // One shift and one AND-OR then make a pair of neighbouring columns as two bfloat16 (see `codes2` in the kernels below).
 // Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
 // a token for heads of 128 where bfloat16 takes 256.
+#include "entry.cuh"
 #include "pairs.cuh"
 #include "tcgen05.cuh"
 
@@ -1140,9 +1141,9 @@ TS_EXPORT int ts_int4_attention_error() {
 #endif
 
 // k, v [T, Hkv, D] (strides in elements, columns contiguous) to the slots of slot_mapping [T] (< 0: skipped; slots are distinct)
-TS_EXPORT int ts_int4_kvwrite(int dtype, const void* k, const void* v, long long k_row, long long k_head, long long v_row, long long v_head,
-                              int T, int Hkv, void* k_codes, void* k_pairs, void* v_codes, void* v_pairs, const int* slot_mapping,
-                              int page_size, int num_pages, cudaStream_t stream) {
+static int int4_kvwrite(int dtype, const void* k, const void* v, long long k_row, long long k_head, long long v_row, long long v_head,
+                        int T, int Hkv, void* k_codes, void* k_pairs, void* v_codes, void* v_pairs, const int* slot_mapping,
+                        int page_size, int num_pages, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_kvwrite: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && Hkv > 0 && shift >= 0 && num_pages > 0, "int4_kvwrite: %d tokens, %d heads, pages of %d", T, Hkv, page_size);
@@ -1157,12 +1158,13 @@ TS_EXPORT int ts_int4_kvwrite(int dtype, const void* k, const void* v, long long
   else TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<bf16>, g.grid, g.block, 0, stream, p, vec);
   return 0;
 }
+TS_ENTRY(int4_kvwrite)
 
 // qkv [T, (H + 2 Hkv) D] contiguous -> q [T, H, D] and, with a slot_mapping, the cache; see RopeParams.  rot 0: no rotation, q_weight null: no norm.
-TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const int* positions, const float* cos, const float* sin, int rot,
-                                   int interleaved, const void* q_weight, const void* k_weight, int weight_f32, float eps, int T, int H, int Hkv,
-                                   void* k_codes, void* k_pairs, void* v_codes, void* v_pairs, const int* slot_mapping, int page_size,
-                                   int num_pages, cudaStream_t stream) {
+static int int4_rope_kvwrite(int dtype, const void* qkv, void* q, const int* positions, const float* cos, const float* sin, int rot,
+                             int interleaved, const void* q_weight, const void* k_weight, int weight_f32, float eps, int T, int H, int Hkv,
+                             void* k_codes, void* k_pairs, void* v_codes, void* v_pairs, const int* slot_mapping, int page_size,
+                             int num_pages, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_rope_kvwrite: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && H > 0 && Hkv > 0 && shift >= 0 && num_pages > 0, "int4_rope_kvwrite: %d tokens, %d and %d heads, pages of %d", T, H, Hkv, page_size);
@@ -1181,15 +1183,16 @@ TS_EXPORT int ts_int4_rope_kvwrite(int dtype, const void* qkv, void* q, const in
   else TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<bf16>, g.grid, g.block, 0, stream, p, rp);
   return 0;
 }
+TS_ENTRY(int4_rope_kvwrite)
 
 // q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml, or (with columns, up to 8) merges in clusters.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
 // steps of 32 up to 256; 16 columns up to 128) with 8 warps a block, or 4 (8 columns, one key range, heads up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns):
 // requests with more queries than that are left alone.
-TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
-                                const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
-                                int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
-                                int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, int max_q_len,
-                                int columns, int warps, int most, cudaStream_t stream) {
+static int int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
+                          const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
+                          int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
+                          int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, int max_q_len,
+                          int columns, int warps, int most, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_attention: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
@@ -1214,3 +1217,4 @@ TS_EXPORT int ts_int4_attention(int dtype, const void* q, long long q_row, long 
   }
   return dtype == TS_F32 ? attend_simt<float>(p, stream) : attend_simt<bf16>(p, stream);
 }
+TS_ENTRY(int4_attention)

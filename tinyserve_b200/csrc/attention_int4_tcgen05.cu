@@ -27,6 +27,7 @@
 // serves any step of its shape.  Every wait is bounded; a block that gives up raises ts_attention_int4_tcgen05_error.
 #include <cuda_fp16.h>
 
+#include "entry.cuh"
 #include "pairs.cuh"
 #include "tcgen05.cuh"
 
@@ -539,10 +540,10 @@ TS_EXPORT int ts_attention_int4_tcgen05_error() {
 
 // q [T, H, D] (strides in elements, of 16 bytes), out [T, H, D]; codes and pairs as for ts_int4_attention.  Requests of up to `few` queries are left
 // alone.
-TS_EXPORT int ts_int4_attention_tcgen05(const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
-                                        const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
-                                        int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
-                                        int window, float softcap, const float* sinks, int few, cudaStream_t stream) {
+static int int4_attention_tcgen05(const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
+                                  const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
+                                  int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
+                                  int window, float softcap, const float* sinks, int few, cudaStream_t stream) {
   int shift = 0;
   while (shift < 20 && (1 << shift) < page_size) ++shift;
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && page_size == 1 << shift && num_pages > 0 && max_blocks > 0 && few >= 0,
@@ -584,3 +585,4 @@ TS_EXPORT int ts_int4_attention_tcgen05(const void* q, long long q_row, long lon
   TS_LAUNCH("int4_attention_tcgen05", int4_prefill_kernel, dim3(blocks, (unsigned)gy), dim3(THREADS), SMEM, stream, mq, p);
   return 0;
 }
+TS_ENTRY(int4_attention_tcgen05)

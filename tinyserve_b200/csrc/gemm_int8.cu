@@ -14,6 +14,7 @@
 // For few tokens the bytes of W bound it: 8 tokens x 4,096 on 24,576 rows take 18.9 us with the rows' codes (101 MB, 5.3 TB/s), 64 x 12,288 on 4,096 rows
 // 17.9 (50 MB, cut by eight); the smallest calls are launches (1 x 1,024 on 4,096 rows 5.4 us, both kernels).  A single launch that makes the
 // rows' codes in every block's loader was slower (1 x 1,024: 7.4 us): every block waits for the whole row before its first MMA.
+#include "entry.cuh"
 #include "pairs.cuh"
 #include "tcgen05.cuh"
 
@@ -436,18 +437,19 @@ TS_EXPORT int ts_gemm_int8_error() {
 }
 
 // codes [M, K] (leading dimension ldq) and scales [M] of the rows of x [M, K] (ldx)
-TS_EXPORT int ts_quantize_rows(int dtype, const void* x, long long ldx, void* codes, long long ldq, float* scales, int M, int K, cudaStream_t stream) {
+static int quantize_rows(int dtype, const void* x, long long ldx, void* codes, long long ldq, float* scales, int M, int K, cudaStream_t stream) {
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "quantize_rows: unknown dtype %d", dtype);
   TS_REQUIRE(M > 0 && K > 0, "quantize_rows: empty operand");
   return quantize(dtype, x, ldx, codes, ldq, scales, M, K, stream);
 }
+TS_ENTRY(quantize_rows)
 
 // out [M, N] (ldc; float where out_f32, else bfloat16) from codes and scales of x and w (leading dimensions multiples of 16).
 // x_dtype >= 0: x is a tensor of that type (leading dimension ldx) whose rows are brought to cx, sx first; -1: cx and sx are given.
 // tile_t: tokens of a tile (16, 32, 64 or 128); splits: cuts along K (a cluster of up to 8 blocks).  w_constant: nobody that may still run writes w (with x_dtype >= 0 the first launch sees to that).
-TS_EXPORT int ts_gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, long long ldcx, float* sx, const void* cw, long long ldw,
-                           const float* sw, const void* bias, int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K,
-                           int tile_t, int splits, int w_constant, cudaStream_t stream) {
+static int gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, long long ldcx, float* sx, const void* cw, long long ldw,
+                     const float* sw, const void* bias, int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K,
+                     int tile_t, int splits, int w_constant, cudaStream_t stream) {
   TS_REQUIRE(M > 0 && N > 0 && K > 0 && K <= 131072, "gemm_int8: M=%d N=%d K=%d (K up to 131072: the sums are 32-bit integers)", M, N, K);
   TS_REQUIRE((ldcx | ldw) % 16 == 0 && (((uintptr_t)cx | (uintptr_t)cw) & 15) == 0, "gemm_int8: rows of codes begin on 16 bytes");
   TS_REQUIRE(splits >= 1 && splits <= MAX_SPLITS, "gemm_int8: splits out of range");
@@ -468,3 +470,4 @@ TS_EXPORT int ts_gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, 
     default: return launch<128>(map_w, map_x, p, stream);
   }
 }
+TS_ENTRY(gemm_int8)

@@ -11,6 +11,7 @@
 //
 // The epilogue scales a row's sums by sx[m] sw[n] in 32 bits and reaches global memory through tiles of 128 rows x 128 bytes in shared memory, so that
 // stores cover whole lines.  Every wait is bounded; a block that gives up tells its partner.
+#include "entry.cuh"
 #include "tcgen05.cuh"
 
 TS_DEFINE_LAST_ERROR()
@@ -308,8 +309,8 @@ TS_EXPORT int ts_gemm_int8_pair_error() {
 
 // out [M, N] (ldc; float where out_f32, else bfloat16; rows of whole 16 bytes) from codes and scales of x and w (leading dimensions multiples of 16).
 // pairs: SM pairs of the device.
-TS_EXPORT int ts_gemm_int8_pair(const void* cx, long long ldcx, const float* sx, const void* cw, long long ldw, const float* sw, const void* bias,
-                                int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K, int pairs, cudaStream_t stream) {
+static int gemm_int8_pair(const void* cx, long long ldcx, const float* sx, const void* cw, long long ldw, const float* sw, const void* bias,
+                          int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K, int pairs, cudaStream_t stream) {
   TS_REQUIRE(M > 0 && N > 0 && K > 0 && K <= 131072 && pairs > 0, "gemm_int8_pair: M=%d N=%d K=%d (K up to 131072: the sums are 32-bit integers)", M, N, K);
   TS_REQUIRE((ldcx | ldw) % 16 == 0 && (((uintptr_t)cx | (uintptr_t)cw) & 15) == 0, "gemm_int8_pair: rows of codes begin on 16 bytes");
   const int e = out_f32 ? 4 : 2;
@@ -322,3 +323,4 @@ TS_EXPORT int ts_gemm_int8_pair(const void* cx, long long ldcx, const float* sx,
   p.slices = (K + BK - 1) / BK;
   return launch(mx, mw, p, pairs, stream);
 }
+TS_ENTRY(gemm_int8_pair)

@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 
 import torch
@@ -2575,22 +2576,10 @@ def delta_rule(q, k, v, gate, logits, bias, rate, state, ctx, num_heads, key_dim
 
 # ----------------------------------------------------------------------------- fewer bits
 # (A decoded token's launches take a few microseconds each: the checks below ask a tensor for as little as they need, and the
-# entry points are looked up once, with their argument types.)
-_INT, _LONG, _PTR, _FLOAT = c_int, c_longlong, c_void_p, c_float
-_INT8_ENTRIES = {
-    "ts_quantize_rows": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _INT, _INT, _PTR),
-    "ts_gemm_int8": (_INT, _PTR, _LONG, _PTR, _LONG, _PTR, _PTR, _LONG, _PTR, _PTR, _INT, _PTR, _LONG, _INT, _INT, _INT, _INT, _INT, _INT, _INT, _PTR),
-    "ts_gemm_int8_pair": (_PTR, _LONG, _PTR, _PTR, _LONG, _PTR, _PTR, _INT, _PTR, _LONG, _INT, _INT, _INT, _INT, _INT, _PTR),
-}
-_INT4_ENTRIES = {
-    "ts_int4_kvwrite": (_INT, _PTR, _PTR, _LONG, _LONG, _LONG, _LONG, _INT, _INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR),
-    "ts_int4_rope_kvwrite": (_INT, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _PTR, _PTR, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR,
-                             _PTR, _INT, _INT, _PTR),
-    "ts_int4_attention": (_INT, _PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
-                          _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR, _PTR, _INT, _INT, _INT, _INT, _PTR),
-    "ts_int4_attention_tcgen05": (_PTR, _LONG, _LONG, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _INT, _INT, _INT, _INT, _INT,
-                                  _INT, _FLOAT, _INT, _FLOAT, _PTR, _INT, _PTR),
-}
+# entry points are looked up once.)
+# Their arguments go in one run of 64-bit fields, "q" an integer or a pointer, "d" a float (csrc/entry.cuh).
+_INT8_ENTRIES = {"ts_quantize_rows": "9q", "ts_gemm_int8": "21q", "ts_gemm_int8_pair": "16q"}
+_INT4_ENTRIES = {"ts_int4_kvwrite": "17q", "ts_int4_rope_kvwrite": "11qd11q", "ts_int4_attention": "20qdqd9q", "ts_int4_attention_tcgen05": "19qdqd3q"}
 
 
 @functools.lru_cache(maxsize=None)
@@ -2598,8 +2587,10 @@ def _entry(unit, name):
     """(library, entry point) of the 8-bit products (``unit`` 0) or of a head size over a 4-bit cache."""
     lib = _gemm_int8_pair() if name == "ts_gemm_int8_pair" else _gemm_int8() if unit == 0 else _attention_int4_tcgen05(unit) if name.endswith("_tcgen05") else _attention_int4(unit)
     fn = getattr(lib, name)
-    fn.argtypes = (_INT8_ENTRIES if unit == 0 else _INT4_ENTRIES)[name]
-    return lib, fn
+    fn.argtypes = (c_void_p, c_int)
+    fields = struct.Struct("=" + (_INT8_ENTRIES if unit == 0 else _INT4_ENTRIES)[name])
+    pack, n = fields.pack, fields.size // 8
+    return lib, lambda *args: fn(pack(*args), n)
 
 
 def _here(what, *tensors):
@@ -2612,7 +2603,7 @@ def _here(what, *tensors):
             raise RuntimeError(f"{what}: operands lie on {t.device} and on cuda:{here}")
     if here != torch._C._cuda_getDevice():          # (there is a CUDA tensor: the runtime is up)
         raise RuntimeError(f"{what}: the operands lie on cuda:{here}, the current device is cuda:{torch.cuda.current_device()}")
-    return _STREAM.value if _STREAM is not None else torch._C._cuda_getCurrentRawStream(here)
+    return (_STREAM.value or 0) if _STREAM is not None else torch._C._cuda_getCurrentRawStream(here)
 
 
 def _launched(lib, code, n):
@@ -2743,12 +2734,12 @@ def _linear_int8(x, weight, bias, out_float32, constant_weight):
             lib, fn = _entry(0, "ts_quantize_rows")
             _launched(lib, fn(xt, xp, ldx, cx, ldcx, sx, M, K, stream), 1)
         lib, fn = _entry(0, "ts_gemm_int8_pair")
-        _launched(lib, fn(cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else None,
+        _launched(lib, fn(cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else 0,
                           0 if bias is None or bias.dtype == torch.bfloat16 else 1, out.data_ptr(), N, 1 if dtype == torch.float32 else 0, M, N, K,
                           num_sms() // 2, stream), 1)
         return out
     lib, fn = _entry(0, "ts_gemm_int8")
-    _launched(lib, fn(xt, xp, ldx, cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else None,
+    _launched(lib, fn(xt, xp, ldx, cx, ldcx, sx, codes.data_ptr(), weight.stride, scales.data_ptr(), bias.data_ptr() if bias is not None else 0,
                       0 if bias is None or bias.dtype == torch.bfloat16 else 1, out.data_ptr(), N, 1 if dtype == torch.float32 else 0, M, N, K,
                       tile_t, splits, 1 if constant_weight else 0, stream), 1 if given else 2)
     return out
@@ -2835,7 +2826,7 @@ def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary
     stream = _here(what, qkv, positions, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping, cos, sin, q_weight, k_weight)
     q = torch.empty(T, H, D, dtype=qkv.dtype, device=qkv.device)
     lib, fn = _entry(D, "ts_int4_rope_kvwrite")
-    at = lambda t: t.data_ptr() if t is not None else None
+    at = lambda t: t.data_ptr() if t is not None else 0
     if T:
         _launched(lib, fn(_DTYPE[qkv.dtype], at(qkv), at(q), at(positions), at(cos), at(sin), rot, interleaved, at(q_weight), at(k_weight),
                           _vec_flag(q_weight, qkv.dtype) if q_weight is not None else 0, eps, T, H, Hkv, at(k_cache.codes), at(k_cache.pairs),
@@ -2939,7 +2930,7 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
             tc, portions = _entry(D, "ts_int4_attention_tcgen05")
             _launched(tc, portions(q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                                    v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H,
-                                   Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None,
+                                   Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else 0,
                                    0 if alike else few, stream), 1)
             if alike:
                 return out
@@ -2952,7 +2943,7 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
     if num_splits is None:
         num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
     warps = int4_decode_warps(B * Hkv * -(-rows // columns), num_splits, D) if columns == 8 else 8
-    part_o = part_ml = None
+    part_o = part_ml = 0
     merged = columns > 0 and num_splits <= INT4_CLUSTER_SPLITS          # (in clusters, without scratch)
     if num_splits > 1 and not merged:
         scratch = torch.empty(T * H * num_splits * (D + 2), dtype=torch.float32, device=q.device)
@@ -2960,6 +2951,6 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         part_ml = part_o + 4 * T * H * num_splits * D
     _launched(lib, fn(_DTYPE[dtype], q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                       v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H, Hkv, page,
-                      blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else None, num_splits, part_o, part_ml,
+                      blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else 0, num_splits, part_o, part_ml,
                       max_q_len, columns, warps, most, stream), 1 if num_splits == 1 or merged else 2)
     return out
