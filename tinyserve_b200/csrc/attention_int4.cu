@@ -306,9 +306,10 @@ struct Int4Params {
   float softcap;
   const float* sinks;                        // [H] or null: one more term exp(sinks[h]) in head h's sum
   int splits;                                // key ranges; > 1: partial results for the combine kernel
+  float unit;                                // powers of two in a unit of the partial results' maxima
   int most;                                  // > 0: requests with more queries are somebody else's
   int ordered;                               // != 0: blocks take the requests by length, the longest first
-  float *part_o, *part_ml;                   // [T * H][splits][D], [T * H][splits][2] (maximum in the log2 domain, sum)
+  float *part_o, *part_ml;                   // [T * H][splits][D], [T * H][splits][2] (maximum, sum)
 };
 
 // the request that row t belongs to: the first b with cu_q[b + 1] > t (requests may be empty), -1 behind the last
@@ -331,9 +332,16 @@ __device__ __forceinline__ size_t cache_row(const Int4Params& p, int page, int k
 }
 __device__ __forceinline__ float capped(const Int4Params& p, float s) { return p.softcap > 0.f ? p.softcap * tanhf(s / p.softcap) : s; }
 
+// code i of a word as the 32-bit number 2^23 + c (adding or subtracting whole numbers to it is exact)
+constexpr float CODE_BASE = 8388608.f;
+__device__ __forceinline__ float code_above(uint32_t word, int i) { return __uint_as_float(0x4b000000u | (word >> shift_of(i) & 15u)); }
+
 // The 32-bit form (and head sizes that the tensor-core kernel does not take): a block is one token's heads of one key head, up to eight
 // at a time, and a range of its keys.  A thread makes the scores of one key of a tile of 128 for all its heads, so that a
 // row of codes is read once; for P V a thread holds eight columns of all heads and walks every KG-th key.
+// With a pair (s, z) of the key, q.k = s sum q (c - 8) + (z + 8 s) sum q: around the middle of the codes the two terms are small and little of
+// them cancels.  Scores are exponentiated as 2^((score - maximum) log2 e): rounding the product instead of the score
+// costs nothing where the score is large.
 constexpr int SIMT_THREADS = 128, SIMT_KEYS = 128, SIMT_HEADS = 8, KG = SIMT_THREADS / W;
 
 template <typename T>
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
       key_row[tid] = row;
       v_pair[tid] = p.vp[row];
       const uint32_t kpair = p.kp[row];
-      const float ks = pair_scale(kpair), kz = pair_zero(kpair);
+      const float ks = pair_scale(kpair), kz = fmaf(8.f, ks, pair_zero(kpair));
       float acc[SIMT_HEADS] = {};
       constexpr int AHEAD = W % 16 == 0 ? 16 : W % 12 == 0 ? 12 : W % 8 == 0 ? 8 : W % 4 == 0 ? 4 : 2;      // words of the row that are on their way at once
 #pragma unroll 1
@@ -402,18 +410,17 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
         for (int w = 0; w < AHEAD; ++w) {
           float c[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) c[i] = (float)((bits[w] >> shift_of(i)) & 15u);
+          for (int i = 0; i < 8; ++i) c[i] = code_above(bits[w], i) - (CODE_BASE + 8.f);
 #pragma unroll
           for (int h = 0; h < SIMT_HEADS; ++h)
             if (h < nh) {
               const float4 a = *reinterpret_cast<const float4*>(&qs[h][(w0 + w) * 8]), e = *reinterpret_cast<const float4*>(&qs[h][(w0 + w) * 8 + 4]);
-              acc[h] = fmaf(a.x, c[0], fmaf(a.y, c[1], fmaf(a.z, c[2], fmaf(a.w, c[3], acc[h]))));
-              acc[h] = fmaf(e.x, c[4], fmaf(e.y, c[5], fmaf(e.z, c[6], fmaf(e.w, c[7], acc[h]))));
+              acc[h] += fmaf(a.x, c[0], fmaf(a.y, c[1], fmaf(a.z, c[2], a.w * c[3]))) + fmaf(e.x, c[4], fmaf(e.y, c[5], fmaf(e.z, c[6], e.w * c[7])));
             }
         }
       }
 #pragma unroll
-      for (int h = 0; h < SIMT_HEADS; ++h) prob[h][tid] = capped(p, fmaf(ks, acc[h], kz * qsum[h]) * p.scale) * LOG2E;
+      for (int h = 0; h < SIMT_HEADS; ++h) prob[h][tid] = capped(p, fmaf(ks, acc[h], kz * qsum[h]) * p.scale);
     }
     __syncthreads();
     for (int h = warp; h < nh; h += 4) {
@@ -428,13 +435,13 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
       const float base = m == -INFINITY ? 0.f : m;          // (every score -infinity or NaN: nothing to subtract)
 #pragma unroll
       for (int i = 0; i < SIMT_KEYS / 32; ++i) {
-        s[i] = exp2f(s[i] - base);
+        s[i] = exp2f((s[i] - base) * LOG2E);
         sum += s[i];
         prob[h][lane + 32 * i] = s[i];
       }
       sum = warp_sum(sum);
       if (lane == 0) {
-        const float a = exp2f(before - base);
+        const float a = exp2f((before - base) * LOG2E);
         alpha[h] = a;
         ml[h][0] = m;
         ml[h][1] = ml[h][1] * a + sum;
@@ -455,7 +462,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
         const float vs = pair_scale(v_pair[key]), vz = pair_zero(v_pair[key]);
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf((float)((bits >> shift_of(i)) & 15u), vs, vz);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(code_above(bits, i) - CODE_BASE, vs, vz);
 #pragma unroll
         for (int h = 0; h < SIMT_HEADS; ++h)
           if (h < nh) {
@@ -482,9 +489,9 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
     const size_t row = (size_t)t * p.H + h0 + h;
     float m = ml[h][0], l = ml[h][1], a = 1.f;
     if (p.splits == 1 && p.sinks != nullptr) {
-      const float sink = p.sinks[h0 + h] * LOG2E, top = fmaxf(m, sink);
-      a = m == -INFINITY ? 0.f : exp2f(m - top);
-      l = l * a + exp2f(sink - top);
+      const float sink = p.sinks[h0 + h], top = fmaxf(m, sink);
+      a = m == -INFINITY ? 0.f : exp2f((m - top) * LOG2E);
+      l = l * a + exp2f((sink - top) * LOG2E);
     }
     for (int d = tid; d < D; d += SIMT_THREADS) {
       float sum = 0.f;
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
   }
 }
 
-// out[row] = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the key ranges of a row (token, head)
+// out[row] = sum_s f_s o_s / sum_s f_s l_s with f_s = 2^((m_s - m) unit) over the key ranges of a row (token, head)
 template <typename T>
 __global__ void int4_combine_kernel(Int4Params p) {
   pdl_trigger();
@@ -515,15 +522,15 @@ __global__ void int4_combine_kernel(Int4Params p) {
     if (p.cu_q[b + 1] - p.cu_q[b] > p.most) return;
   }
   const float* ml = p.part_ml + row * p.splits * 2;
-  float m = p.sinks ? p.sinks[row % p.H] * LOG2E : -INFINITY;
+  float m = p.sinks ? p.sinks[row % p.H] * (LOG2E / p.unit) : -INFINITY;
   const float sink = m;
   for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[2 * s]);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = p.sinks ? exp2f(sink - base) : 0.f;
-  for (int s = 0; s < p.splits; ++s) l += exp2f(ml[2 * s] - base) * ml[2 * s + 1];
+  float l = p.sinks ? exp2f((sink - base) * p.unit) : 0.f;
+  for (int s = 0; s < p.splits; ++s) l += exp2f((ml[2 * s] - base) * p.unit) * ml[2 * s + 1];
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
     float sum = 0.f;
-    for (int s = 0; s < p.splits; ++s) sum += exp2f(ml[2 * s] - base) * p.part_o[(row * p.splits + s) * D + d];
+    for (int s = 0; s < p.splits; ++s) sum += exp2f((ml[2 * s] - base) * p.unit) * p.part_o[(row * p.splits + s) * D + d];
     static_cast<T*>(p.out)[row * D + d] = from_f32<T>(l == 0.f ? 0.f : sum / l);
   }
 }
@@ -1201,7 +1208,7 @@ static int int4_attention(int dtype, const void* q, long long q_row, long long q
   TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml) || (columns > 0 && splits <= 8 && !part_o)), "int4_attention: key ranges need their scratch");
   Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
                   block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
-                  splits, most, 0, part_o, part_ml};
+                  splits, columns > 0 ? 1.f : LOG2E, most, 0, part_o, part_ml};
   if (columns > 0) {
 #ifdef TS_INT4_MMA
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");
