@@ -11,7 +11,7 @@
 // Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
 // a token for heads of 128 where bfloat16 takes 256.
 #include "entry.cuh"
-#include "pairs.cuh"
+#include "rounding.cuh"
 #include "tcgen05.cuh"
 
 #ifndef TS_HEAD_DIM
@@ -57,59 +57,54 @@ __device__ __forceinline__ void load8_any(const T* p, float (&x)[8], bool vec) {
   }
 }
 
-// What the LANES lanes of a row have of it: minimum, maximum, and whether everything is finite (0 x of an infinity or a NaN is a NaN)
+// The least and the largest element of a row that LANES lanes have; a NaN if there is one
+__device__ __forceinline__ float least(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float largest(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 struct RowRange {
   float lo = INFINITY, hi = -INFINITY;
-  F2 zeros = f2(0.f, 0.f);
-  bool bad = false;
   __device__ __forceinline__ void add(const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      lo = fminf(fminf(lo, x[i]), x[i + 1]);
-      hi = fmaxf(fmaxf(hi, x[i]), x[i + 1]);
-      zeros = f2_fma(f2(x[i], x[i + 1]), f2(0.f, 0.f), zeros);
+      lo = least(least(lo, x[i]), x[i + 1]);
+      hi = largest(largest(hi, x[i]), x[i + 1]);
     }
   }
   __device__ __forceinline__ void join() {
-    float z0, z1;
-    f2_out(zeros, z0, z1);
-    const uint32_t group = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
-    bad = (__ballot_sync(0xffffffffu, !(z0 + z1 == 0.f)) & group) != 0;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = least(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = largest(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
   }
 };
 
 __device__ __noinline__ float divided_code(float y, float scale) { return fminf(fmaxf(rintf(__fdiv_rn(y, scale)), 0.f), 15.f); }
 
-// eight neighbouring columns as a word of codes.  The quotient rounded to 32 bits decides; the product with the reciprocal is off by 3 roundings of at
-// most 16, so a division is only made next to a half, and where the reciprocal could overflow.  Adding 1.5 2^23 rounds to a whole
-// number, halves to even; four codes 4 bits apart are a sum of exact products below 2^16.
-__device__ __forceinline__ uint32_t word_of(const float (&x)[8], float zero, float scale) {
+// eight neighbouring columns as a word of codes.  The quotient rounded to 32 bits decides; a division is only made where the reciprocal could
+// overflow.  Adding 1.5 2^23 rounds to a whole number, halves to even; four codes 4 bits apart are a sum of exact products below 2^16.
+__device__ __forceinline__ uint32_t word_of(const float (&x)[8], float zero, float scale, bool outside) {
   constexpr float ROUNDER = 12582912.f;
   const float inverse = 1.f / scale;
-  const F2 inv = f2(inverse, inverse), low = f2(-zero, -zero), up = f2(ROUNDER, ROUNDER), down = f2(-ROUNDER, -ROUNDER), minus = f2(-1.f, -1.f);
-  float n[8], furthest = scale > 1e-30f ? 0.f : 1.f;
+  const F2 inv = f2(inverse, inverse), minus = f2(-scale, -scale), low = f2(-zero, -zero), up = f2(ROUNDER, ROUNDER), down = f2(-ROUNDER, -ROUNDER);
+  F2 n[4];
+  if (scale > 1e-30f) {
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    float r0, r1, o0, o1;
-    f2_out(f2_mul(f2_add(f2(x[i], x[i + 1]), low), inv), r0, r1);
-    const F2 r = f2(fminf(fmaxf(r0, 0.f), 15.f), fminf(fmaxf(r1, 0.f), 15.f)), whole = f2_add(f2_add(r, up), down);
-    f2_out(f2_fma(whole, minus, r), o0, o1);
-    furthest = fmaxf(furthest, fmaxf(fabsf(o0), fabsf(o1)));
-    f2_out(whole, n[i], n[i + 1]);
-  }
-  if (furthest > 0.49995f) {
+    for (int i = 0; i < 4; ++i) n[i] = f2_quotient(f2_add(f2(x[2 * i], x[2 * i + 1]), low), minus, inv);
+    if (outside) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __fsub_rn(x[i], zero), r = fminf(fmaxf(y * inverse, 0.f), 15.f);
-      if (fabsf(r - n[i]) > 0.49995f || !(scale > 1e-30f)) n[i] = divided_code(y, scale);
+      for (int i = 0; i < 4; ++i) {
+        float r0, r1;
+        f2_out(n[i], r0, r1);
+        n[i] = f2(fminf(fmaxf(r0, 0.f), 15.f), fminf(fmaxf(r1, 0.f), 15.f));
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = f2_add(f2_add(n[i], up), down);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = f2(divided_code(__fsub_rn(x[2 * i], zero), scale), divided_code(__fsub_rn(x[2 * i + 1], zero), scale));
   }
-  const F2 four = f2_fma(f2_fma(f2_fma(f2(n[6], n[7]), f2(16.f, 16.f), f2(n[4], n[5])), f2(16.f, 16.f), f2(n[2], n[3])), f2(16.f, 16.f), f2(n[0], n[1]));
+  const F2 step = f2(16.f, 16.f), four = f2_fma(f2_fma(f2_fma(n[3], step, n[2]), step, n[1]), step, n[0]);
   float even, odd;
   f2_out(f2_add(four, f2(8388608.f, 8388608.f)), even, odd);          // (2^23: the whole number is the low bits)
   return __byte_perm(__float_as_uint(even), __float_as_uint(odd), 0x5410);
@@ -126,12 +121,15 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
   const float zero = __bfloat162float(zero16);
   const bf16 scale16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(r.hi, zero), 15.f));
   const float scale = __bfloat162float(scale16);
-  const bool bad = r.bad || !(fabsf(scale) <= 3.402823466e38f) || !(fabsf(zero) <= 3.402823466e38f);
+  // (an infinity or a NaN in the row is one of its ends, and then the pair is not finite)
+  const bool bad = !(fabsf(scale) <= 3.402823466e38f) || !(fabsf(zero) <= 3.402823466e38f);
+  // the pair's rounding may leave ends of the row outside the codes: rarely, so that only such rows are clamped
+  const bool outside = !(__fsub_rn(r.lo, zero) >= -0.4f * scale && __fsub_rn(r.hi, zero) <= 15.4f * scale);
   const size_t at = (((size_t)(slot >> p.page_shift) * p.Hkv + head) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
 #pragma unroll
   for (int w = 0; w < WORDS; ++w) {
     const int word = lane + w * LANES;
-    if (word < W) (which ? p.vc : p.kc)[at * W + word] = !bad && scale > 0.f ? word_of(x[w], zero, scale) : 0u;
+    if (word < W) (which ? p.vc : p.kc)[at * W + word] = !bad && scale > 0.f ? word_of(x[w], zero, scale, outside) : 0u;
   }
   if (lane == 0) {
     const uint32_t s = bad ? 0x7fc0u : (scale > 0.f ? __bfloat16_as_ushort(scale16) : 0u), z = bad ? 0x7fc0u : __bfloat16_as_ushort(zero16);

@@ -15,7 +15,7 @@
 // 17.9 (50 MB, cut by eight); the smallest calls are launches (1 x 1,024 on 4,096 rows 5.4 us, both kernels).  A single launch that makes the
 // rows' codes in every block's loader was slower (1 x 1,024: 7.4 us): every block waits for the whole row before its first MMA.
 #include "entry.cuh"
-#include "pairs.cuh"
+#include "rounding.cuh"
 #include "tcgen05.cuh"
 
 TS_DEFINE_LAST_ERROR()
@@ -66,34 +66,32 @@ template <> struct Eight<bf16> {
   __device__ __forceinline__ static uint32_t bits(uint32_t top) { return max(top << 16, top & 0xffff0000u); }
 };
 
-// round(x / scale) of the quotient rounded to 32 bits, as a byte.  x times the reciprocal is off by three roundings of at most 127, 2.3e-5: a
-// division is only made where that could matter, next to a half (1 in 10,000), and where the reciprocal could overflow.  Adding 1.5 2^23
-// rounds to a whole number, halves to even, and leaves it in the low bits.
+// round(x / scale) of the quotient rounded to 32 bits, as a byte; a division is only made where the reciprocal could overflow.  Adding
+// 1.5 2^23 rounds to a whole number, halves to even, and leaves it in the low bits.
 constexpr float ROUNDER = 12582912.f;
 __device__ __noinline__ uint32_t divided_code(float x, float scale) {
   return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f) & 255u;
 }
 __device__ __forceinline__ uint32_t code_of(float x, float scale, float inverse) {
-  const float r = x * inverse, t = r + ROUNDER;
-  return fabsf(r - (t - ROUNDER)) > 0.49995f || !(scale > 1e-30f) ? divided_code(x, scale) : __float_as_uint(t) & 255u;
+  if (!(scale > 1e-30f)) return divided_code(x, scale);
+  float t, unused;
+  f2_out(f2_quotient(f2(x, 0.f), f2(-scale, -scale), f2(inverse, inverse)), t, unused);
+  return __float_as_uint(t + ROUNDER) & 255u;
 }
 __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inverse) {
   uint32_t c[8];
-  float furthest = scale > 1e-30f ? 0.f : 1.f;
-  const F2 inv = f2(inverse, inverse), up = f2(ROUNDER, ROUNDER), down = f2(-ROUNDER, -ROUNDER), minus = f2(-1.f, -1.f);
+  if (scale > 1e-30f) {
+    const F2 inv = f2(inverse, inverse), minus = f2(-scale, -scale), up = f2(ROUNDER, ROUNDER);
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const F2 r = f2_mul(f2(x[e], x[e + 1]), inv), t = f2_add(r, up), off = f2_fma(f2_add(t, down), minus, r);
-    float o0, o1, t0, t1;
-    f2_out(off, o0, o1);
-    f2_out(t, t0, t1);
-    furthest = fmaxf(furthest, fmaxf(fabsf(o0), fabsf(o1)));
-    c[e] = __float_as_uint(t0);
-    c[e + 1] = __float_as_uint(t1);
-  }
-  if (furthest > 0.49995f) {
+    for (int e = 0; e < 8; e += 2) {
+      float t0, t1;
+      f2_out(f2_add(f2_quotient(f2(x[e], x[e + 1]), minus, inv), up), t0, t1);
+      c[e] = __float_as_uint(t0);
+      c[e + 1] = __float_as_uint(t1);
+    }
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = code_of(x[e], scale, inverse);
+    for (int e = 0; e < 8; ++e) c[e] = divided_code(x[e], scale);
   }
   // (the low bytes of four words side by side)
   return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
