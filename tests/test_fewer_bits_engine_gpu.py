@@ -80,12 +80,14 @@ def test_mixed_steps(model, dtype, graphs, page, tmp_path):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("H,Hkv,D,rot,inter,norm", [(4, 2, 128, 128, False, True), (3, 1, 96, 64, False, True), (2, 2, 16, 16, True, False), (5, 5, 512, 0, False, True),
                                                     (6, 2, 64, 32, True, True)])
-def test_norm_rotation_and_write_in_one(dtype, H, Hkv, D, rot, inter, norm):
+@pytest.mark.parametrize("T", [9, 300])
+def test_norm_rotation_and_write_in_one(dtype, H, Hkv, D, rot, inter, norm, T):
     """The kernel that norms, turns and writes against the ones that do it to a cache of whole numbers, and then its codes."""
     from types import SimpleNamespace as NS
     from tinyserve_b200.kernels import ops
     from tinyserve_b200.parts.rotary import Rotary
-    T, page = 9, 8
+    page = 8
+    pages = T // page + 1
     g = torch.Generator().manual_seed(D + H)
     qkv = torch.randn(T, (H + 2 * Hkv) * D, generator=g).to(dtype).cuda()
     positions = torch.randint(0, 900, (T,), generator=g).int().cuda()
@@ -94,11 +96,11 @@ def test_norm_rotation_and_write_in_one(dtype, H, Hkv, D, rot, inter, norm):
         cos, sin = Rotary.tables(rot, 1e4, 1000)
         rotary = NS(cos=cos.cuda(), sin=sin.cuda(), rotary_dim=rot, interleaved=inter)
     qw, kw = ((1 + 0.1 * torch.randn(D, generator=g)).to(dtype).cuda() for _ in range(2)) if norm else (None, None)
-    slots = torch.randperm(2 * page, generator=g)[:T].int()
+    slots = torch.randperm(pages * page, generator=g)[:T].int()
     slots[3] = -1
     slots = slots.cuda()
-    plain_caches = [torch.zeros(2, Hkv, page, D, dtype=dtype, device="cuda") for _ in range(2)]
-    caches = [ops.Int4Pages(torch.zeros(2, Hkv, page, D // 2, dtype=torch.uint8, device="cuda"), torch.zeros(2, Hkv, page, 2, dtype=torch.bfloat16, device="cuda")) for _ in range(2)]
+    plain_caches = [torch.zeros(pages, Hkv, page, D, dtype=dtype, device="cuda") for _ in range(2)]
+    caches = [ops.Int4Pages(torch.zeros(pages, Hkv, page, D // 2, dtype=torch.uint8, device="cuda"), torch.zeros(pages, Hkv, page, 2, dtype=torch.bfloat16, device="cuda")) for _ in range(2)]
     args = (qkv, positions, H, Hkv, D, rotary, qw, kw, 1e-6)
     q0 = ops.qk_norm_rope_kvwrite(*args, *plain_caches, slots, page)
     q1 = ops.qk_norm_rope_kvwrite(*args, *caches, slots, page)
@@ -112,9 +114,9 @@ def test_norm_rotation_and_write_in_one(dtype, H, Hkv, D, rot, inter, norm):
         # half a step, the pair's own rounding, and what the rows may differ by
         off = (got - whole.double()).abs()
         assert (off <= 0.5 * packed.pairs[..., :1].double() + (3 * 2.0 ** -8 + 2 * half) * whole.double().abs().amax(-1, keepdim=True) + 1e-30).all()
-    written = torch.zeros(2 * page, dtype=torch.bool)
+    written = torch.zeros(pages * page, dtype=torch.bool)
     written[slots[slots >= 0].long().cpu()] = True
-    assert not caches[0].pairs.transpose(1, 2).reshape(2 * page, -1)[(~written).cuda()].any()
+    assert not caches[0].pairs.transpose(1, 2).reshape(pages * page, -1)[(~written).cuda()].any()
     before = [c.codes.clone() for c in caches]
     ops.qk_norm_rope_kvwrite(*args, *caches, None, page)
     assert all(torch.equal(a, c.codes) for a, c in zip(before, caches))

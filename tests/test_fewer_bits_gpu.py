@@ -188,7 +188,8 @@ def allowed(dtype, want, top, span, D, keys):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("T,Hkv,D,page", [(1, 1, 16, 1), (3, 2, 96, 16), (7, 8, 128, 64), (33, 3, 64, 4), (2, 1, 512, 32), (5, 2, 256, 8)])
+@pytest.mark.parametrize("T,Hkv,D,page", [(1, 1, 16, 1), (3, 2, 96, 16), (7, 8, 128, 64), (33, 3, 64, 4), (2, 1, 512, 32), (5, 2, 256, 8),
+                                           (300, 2, 128, 64), (257, 3, 64, 16), (256, 1, 512, 32), (259, 5, 96, 1), (300, 1, 16, 8), (256, 2, 160, 16)])
 def test_write(dtype, T, Hkv, D, page):
     from tinyserve_b200.kernels import ops
     g = torch.Generator().manual_seed(T + D)

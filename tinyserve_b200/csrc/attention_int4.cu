@@ -43,8 +43,13 @@ struct WriteParams {
   int T, Hkv, page_shift;
   long long slots;                           // of the pool
 };
-constexpr int LANES = W >= 32 ? 32 : (W > 16 ? 32 : (W > 8 ? 16 : (W > 4 ? 8 : (W > 2 ? 4 : 2))));    // a row's lanes: a power of two
-constexpr int WORDS = (W + LANES - 1) / LANES;                                                        // words of a lane
+// a row's lanes, a power of two: of a word each for few tokens, of two for many, where a division and a reduction serve twice as much (8 heads
+// of 128, 4,095 tokens 10.3 us by words, 7.4 by two, 7.3 by four; 64 tokens 1.7 / 1.8 / 2.6; with norm and rotation of 32 heads too, 2,048 tokens 20.9 /
+// 17.3 / 20.2, 64 tokens 2.6 / 2.9 / 3.8)
+constexpr int FEW_LANES = W > 16 ? 32 : (W > 8 ? 16 : (W > 4 ? 8 : (W > 2 ? 4 : 2)));
+constexpr int MANY_LANES = W > 32 ? 32 : (W > 16 ? 16 : (W > 8 ? 8 : (W > 4 ? 4 : 2)));
+constexpr int MANY_TOKENS = 256;
+__host__ __device__ constexpr int words_of(int lanes) { return (W + lanes - 1) / lanes; }            // words of a lane
 constexpr int WRITE_THREADS = 128;
 
 template <typename T>
@@ -60,6 +65,7 @@ __device__ __forceinline__ void load8_any(const T* p, float (&x)[8], bool vec) {
 // The least and the largest element of a row that LANES lanes have; a NaN if there is one
 __device__ __forceinline__ float least(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float largest(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+template <int LANES>
 struct RowRange {
   float lo = INFINITY, hi = -INFINITY;
   __device__ __forceinline__ void add(const float (&x)[8]) {
@@ -111,7 +117,8 @@ __device__ __forceinline__ uint32_t word_of(const float (&x)[8], float zero, flo
 }
 
 // a row that its LANES lanes hold, to the slot of its token
-__device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)[WORDS][8], const RowRange& r, int which, int head, int slot, int lane) {
+template <int LANES>
+__device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)[words_of(LANES)][8], const RowRange<LANES>& r, int which, int head, int slot, int lane) {
   if (slot < 0) return;
   if (slot >= p.slots) {
     if (lane == 0) ts_raise_status(TS_STATUS_BOUNDS, TS_BAD_CACHE_SLOT);
@@ -127,7 +134,7 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
   const bool outside = !(__fsub_rn(r.lo, zero) >= -0.4f * scale && __fsub_rn(r.hi, zero) <= 15.4f * scale);
   const size_t at = (((size_t)(slot >> p.page_shift) * p.Hkv + head) << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
 #pragma unroll
-  for (int w = 0; w < WORDS; ++w) {
+  for (int w = 0; w < words_of(LANES); ++w) {
     const int word = lane + w * LANES;
     if (word < W) (which ? p.vc : p.kc)[at * W + word] = !bad && scale > 0.f ? word_of(x[w], zero, scale, outside) : 0u;
   }
@@ -138,8 +145,9 @@ __device__ __forceinline__ void store_row(const WriteParams& p, const float (&x)
 }
 
 // LANES lanes bring one row (token, key or value, head) to its slot; a block's x is the token
-template <typename T>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams p, bool vec) {
+  constexpr int WORDS = words_of(LANES);
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x, row = blockIdx.y * (blockDim.x / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
@@ -148,7 +156,7 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_kvwrite_kernel(WriteParams
   const int slot = p.slot_mapping[t];
   const T* src = which ? static_cast<const T*>(p.v) + t * p.v_row + head * p.v_head : static_cast<const T*>(p.k) + t * p.k_row + head * p.k_head;
   float x[WORDS][8];
-  RowRange r;
+  RowRange<LANES> r;
 #pragma unroll
   for (int w = 0; w < WORDS; ++w) {
     const int word = lane + w * LANES;
@@ -178,8 +186,9 @@ struct RopeParams {
   bool vec, vec_weights, vec_angles;
 };
 
-template <typename T>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteParams p, RopeParams rp) {
+  constexpr int WORDS = words_of(LANES);
   __shared__ __align__(16) float stage[WRITE_THREADS / LANES][D];
   pdl_trigger();
   const int t = blockIdx.x, heads = rp.H + 2 * p.Hkv, head = blockIdx.y * (blockDim.x / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
@@ -266,7 +275,7 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteP
       }
     }
   }
-  RowRange r;
+  RowRange<LANES> r;
 #pragma unroll
   for (int w = 0; w < WORDS; ++w) {
     const int word = lane + w * LANES;
@@ -283,9 +292,23 @@ __global__ void __launch_bounds__(WRITE_THREADS) int4_rope_kvwrite_kernel(WriteP
 
 // tokens x groups of a token's rows
 struct RowGrid { dim3 grid, block; };
-RowGrid row_grid(int tokens, int rows) {
-  const int threads = rows * LANES < WRITE_THREADS ? (rows * LANES + 31) / 32 * 32 : WRITE_THREADS;
-  return {dim3(tokens, (rows + threads / LANES - 1) / (threads / LANES)), dim3(threads)};
+RowGrid row_grid(int tokens, int rows, int lanes) {
+  const int threads = rows * lanes < WRITE_THREADS ? (rows * lanes + 31) / 32 * 32 : WRITE_THREADS;
+  return {dim3(tokens, (rows + threads / lanes - 1) / (threads / lanes)), dim3(threads)};
+}
+template <typename T, int LANES>
+int launch_write(const WriteParams& p, bool vec, cudaStream_t stream) {
+  const RowGrid g = row_grid(p.T, 2 * p.Hkv, LANES);
+  TS_REQUIRE(g.grid.y <= 65535, "int4_kvwrite: too many heads");
+  TS_LAUNCH("int4_kvwrite", (int4_kvwrite_kernel<T, LANES>), g.grid, g.block, 0, stream, p, vec);
+  return 0;
+}
+template <typename T, int LANES>
+int launch_rope_write(const WriteParams& p, const RopeParams& rp, cudaStream_t stream) {
+  const RowGrid g = row_grid(p.T, rp.H + 2 * p.Hkv, LANES);
+  TS_REQUIRE(g.grid.y <= 65535, "int4_rope_kvwrite: too many heads");
+  TS_LAUNCH("int4_rope_kvwrite", (int4_rope_kvwrite_kernel<T, LANES>), g.grid, g.block, 0, stream, p, rp);
+  return 0;
 }
 
 // ------------------------------------------------------------------------------------------ attention
@@ -1157,11 +1180,8 @@ static int int4_kvwrite(int dtype, const void* k, const void* v, long long k_row
   const bool vec = ((((uintptr_t)k | (uintptr_t)v) | (uintptr_t)((k_row | k_head | v_row | v_head) * e)) & 15) == 0;
   WriteParams p = {k, v, k_row, k_head, v_row, v_head, (uint32_t*)k_codes, (uint32_t*)v_codes, (uint32_t*)k_pairs, (uint32_t*)v_pairs,
                    slot_mapping, T, Hkv, shift, (long long)num_pages << shift};
-  const RowGrid g = row_grid(T, 2 * Hkv);
-  TS_REQUIRE(g.grid.y <= 65535, "int4_kvwrite: too many heads");
-  if (dtype == TS_F32) TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<float>, g.grid, g.block, 0, stream, p, vec);
-  else TS_LAUNCH("int4_kvwrite", int4_kvwrite_kernel<bf16>, g.grid, g.block, 0, stream, p, vec);
-  return 0;
+  if (dtype == TS_F32) return T < MANY_TOKENS ? launch_write<float, FEW_LANES>(p, vec, stream) : launch_write<float, MANY_LANES>(p, vec, stream);
+  return T < MANY_TOKENS ? launch_write<bf16, FEW_LANES>(p, vec, stream) : launch_write<bf16, MANY_LANES>(p, vec, stream);
 }
 TS_ENTRY(int4_kvwrite)
 
@@ -1182,11 +1202,8 @@ static int int4_rope_kvwrite(int dtype, const void* qkv, void* q, const int* pos
   const RopeParams rp = {qkv, q, positions, rot ? cos : nullptr, sin, rot, interleaved, VecParam{q_weight, weight_f32}, VecParam{k_weight, weight_f32},
                          q_weight != nullptr, eps, H, ((uintptr_t)qkv & 15) == 0, (((uintptr_t)q_weight | (uintptr_t)k_weight) & 15) == 0,
                          !interleaved && rot % 16 == 0 && (((uintptr_t)cos | (uintptr_t)sin) & 15) == 0};
-  const RowGrid g = row_grid(T, H + 2 * Hkv);
-  TS_REQUIRE(g.grid.y <= 65535, "int4_rope_kvwrite: too many heads");
-  if (dtype == TS_F32) TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<float>, g.grid, g.block, 0, stream, p, rp);
-  else TS_LAUNCH("int4_rope_kvwrite", int4_rope_kvwrite_kernel<bf16>, g.grid, g.block, 0, stream, p, rp);
-  return 0;
+  if (dtype == TS_F32) return T < MANY_TOKENS ? launch_rope_write<float, FEW_LANES>(p, rp, stream) : launch_rope_write<float, MANY_LANES>(p, rp, stream);
+  return T < MANY_TOKENS ? launch_rope_write<bf16, FEW_LANES>(p, rp, stream) : launch_rope_write<bf16, MANY_LANES>(p, rp, stream);
 }
 TS_ENTRY(int4_rope_kvwrite)
 
