@@ -166,25 +166,28 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // this block holds all of the SM's tensor memory now: only now may a dependent kernel start
-  pdl_trigger();
+  // This block holds all of the SM's tensor memory now: only now may a dependent kernel start.  And only behind the wait: the kernel for the short
+  // requests of the same step then finds complete what came before this one.
   pdl_wait();
+  pdl_trigger();
 
   // block x from the last: the tiles of all requests in a row, the latest queries (the most keys) first
   const int QPT = p.queries_per_tile, GT = p.heads_per_tile, per_block = GROUPS * QPT;
   const int G = p.H / p.Hkv;
-  int b = -1, q0 = 0;
+  int b = -1, q0 = 0, q_begin = 0, q_len = 0, held = 0;
   {
     int total = 0;
     for (int at = 0; at < p.B; at += 32) {
       const int n = at + lane < p.B ? min(p.cu_q[at + lane + 1], p.T) - p.cu_q[at + lane] : 0;
+      if (at + lane < p.B) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.kv_lens + at + lane));
       total += n > p.few ? (n + per_block - 1) / per_block : 0;
     }
     total = __reduce_add_sync(0xffffffffu, total);
     const int want = total - 1 - (int)blockIdx.x;
     int before = 0;
     for (int at = 0; at < p.B && want >= 0 && b < 0; at += 32) {
-      const int n = at + lane < p.B ? min(p.cu_q[at + lane + 1], p.T) - p.cu_q[at + lane] : 0;
+      const int from = at + lane < p.B ? p.cu_q[at + lane] : 0, n = at + lane < p.B ? min(p.cu_q[at + lane + 1], p.T) - from : 0;
+      const int kv = at + lane < p.B ? p.kv_lens[at + lane] : 0;
       const int tiles = n > p.few ? (n + per_block - 1) / per_block : 0;
       int upto = tiles;
 #pragma unroll
@@ -197,13 +200,15 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         const int who = __ffs(here) - 1;
         b = at + who;
         q0 = (want - before - __shfl_sync(0xffffffffu, upto - tiles, who)) * per_block;
+        q_begin = __shfl_sync(0xffffffffu, from, who);
+        q_len = __shfl_sync(0xffffffffu, n, who);
+        held = __shfl_sync(0xffffffffu, kv, who);
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
   const int kvh = blockIdx.y / p.head_tiles, head_tile = blockIdx.y % p.head_tiles;
-  const int q_begin = b >= 0 ? p.cu_q[b] : 0, q_len = b >= 0 ? min(p.cu_q[b + 1], p.T) - q_begin : 0;
-  const int kv_len = b >= 0 ? (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift) : 0;
+  const int kv_len = (int)min((long long)held, (long long)p.max_blocks << p.page_shift);
   const int g0 = head_tile * GT;
   const int nq_all = max(0, min(per_block, q_len - q0));
   const int groups = nq_all > QPT ? 2 : 1;       // query tiles of this block that hold queries
@@ -568,7 +573,7 @@ static int int4_attention_tcgen05(const void* q, long long q_row, long long q_he
   const int per_block = GROUPS * p.queries_per_tile;
   const int with_tiles = T / (few + 1) < B ? T / (few + 1) : B;
   const int blocks = T / per_block + with_tiles;
-  if (blocks == 0) return 0;
+  TS_REQUIRE(blocks > 0, "int4_attention_tcgen05: %d tokens hold no request of more than %d queries", T, few);
   CUtensorMap mq;
   {
     EncodeTiledFn fn = encode_tiled();

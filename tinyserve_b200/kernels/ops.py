@@ -2926,7 +2926,7 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         few = max(1, INT4_DIRECT_ROWS // G)
         # (requests of one length, it seems: the portions' kernel takes them all, whatever the offsets on the device hold)
         alike = B == 1 or T == B * max_q_len
-        if chosen == "tcgen05" and max_q_len > few and scale > 0 and (q.data_ptr() | 2 * q_row | 2 * q_head) % 16 == 0 and q_row > 0 and q_head > 0:
+        if chosen == "tcgen05" and max_q_len > few and (alike or T > few) and scale > 0 and (q.data_ptr() | 2 * q_row | 2 * q_head) % 16 == 0 and q_row > 0 and q_head > 0:
             tc, portions = _entry(D, "ts_int4_attention_tcgen05")
             _launched(tc, portions(q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
                                    v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H,
@@ -2936,13 +2936,15 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
                 return out
             most = max_q_len = few
         rows = max_q_len * G
-        columns = 16 if rows > 8 and D <= 128 else 8
+        # (beside portions most of the short requests bring one query: 64 of them over 800 keys beside 448 queries 68 us by 16 columns, 58 by 8)
+        columns = 16 if rows > 8 and D <= 128 and not most else 8
+        tiles = B * Hkv * (1 if most else -(-rows // columns))
         if -(-rows // columns) * Hkv > 65535 or B > 65535 or page < 4 or pages * Hkv * page >= 2 ** 31 \
                 or (k_cache.pairs.data_ptr() | v_cache.pairs.data_ptr()) % 16:
             columns = most = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes everything)
     if num_splits is None:
-        num_splits = int4_decode_splits(B * Hkv * -(-rows // columns), span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
-    warps = int4_decode_warps(B * Hkv * -(-rows // columns), num_splits, D) if columns == 8 else 8
+        num_splits = int4_decode_splits(tiles, span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
+    warps = int4_decode_warps(tiles, num_splits, D) if columns == 8 else 8
     part_o = part_ml = 0
     merged = columns > 0 and num_splits <= INT4_CLUSTER_SPLITS          # (in clusters, without scratch)
     if num_splits > 1 and not merged:
