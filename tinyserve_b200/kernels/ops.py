@@ -2621,7 +2621,7 @@ class Int8Rows:
 
     def __init__(self, codes, scales):
         shape = tuple(codes.shape)
-        if codes.dtype != torch.int8 or len(shape) != 2 or scales.dtype != torch.float32 or tuple(scales.shape) != shape[:1]:
+        if codes.dtype != torch.int8 or len(shape) != 2 or scales.dtype != torch.float32 or scales.shape != shape[:1]:
             raise TypeError("Int8Rows: codes are int8 [R, K] and scales float32 [R], got "
                             f"{codes.dtype} {shape} and {scales.dtype} {tuple(scales.shape)}")
         row, column = codes.stride()
@@ -2752,10 +2752,10 @@ class Int4Pages:
     __slots__ = ("codes", "pairs", "shape")
 
     def __init__(self, codes, pairs):
-        shape = tuple(codes.shape)
-        if codes.dtype != torch.uint8 or len(shape) != 4 or pairs.dtype != torch.bfloat16 or tuple(pairs.shape) != shape[:3] + (2,):
+        shape = codes.shape
+        if codes.dtype != torch.uint8 or len(shape) != 4 or pairs.dtype != torch.bfloat16 or pairs.shape != (*shape[:3], 2):
             raise TypeError("Int4Pages: codes are uint8 [pages, heads, slots, D / 2] and pairs bfloat16 [pages, heads, slots, 2], got "
-                            f"{codes.dtype} {shape} and {pairs.dtype} {tuple(pairs.shape)}")
+                            f"{codes.dtype} {tuple(shape)} and {pairs.dtype} {tuple(pairs.shape)}")
         pages, heads, slots, half = shape
         if not codes.is_contiguous() or not pairs.is_contiguous() or codes.data_ptr() % (4 if half % 16 else 16) or pairs.data_ptr() % 4:
             raise ValueError("Int4Pages: codes and pairs are contiguous; codes begin on 16 bytes (on 4 where a row is no multiple of 16), pairs on 4")
@@ -2777,9 +2777,8 @@ def _int4_caches(what, k_cache, v_cache, page=None):
 
 
 def _int32_row(what, t, name, n):
-    shape = t.shape
-    if t.dtype != torch.int32 or len(shape) != 1 or shape[0] < n or (n > 1 and not t.is_contiguous()):
-        raise TypeError(f"{what}: {name} is int32 [{n}], contiguous, got {t.dtype} {tuple(shape)}")
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
+        raise TypeError(f"{what}: {name} is int32 [{n}], contiguous, got {t.dtype} {tuple(t.shape)}")
 
 
 def int4_kvwrite(k, v, k_cache, v_cache, slot_mapping):
@@ -2789,20 +2788,21 @@ def int4_kvwrite(k, v, k_cache, v_cache, slot_mapping):
     infinity or a NaN gets a pair of NaN."""
     what = "int4_kvwrite"
     pages, heads, page, D = _int4_caches(what, k_cache, v_cache)
-    shape = tuple(k.shape)
-    if len(shape) != 3 or shape[1:] != (heads, D) or tuple(v.shape) != shape or k.dtype not in _DTYPE or v.dtype != k.dtype:
-        raise TypeError(f"{what}: keys and values are float32 or bfloat16 [T, {heads}, {D}], got {k.dtype} {shape} and {v.dtype} {tuple(v.shape)}")
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or shape[1:] != (heads, D) or v.shape != shape or dtype not in _DTYPE or v.dtype != dtype:
+        raise TypeError(f"{what}: keys and values are float32 or bfloat16 [T, {heads}, {D}], got {dtype} {tuple(shape)} and {v.dtype} {tuple(v.shape)}")
     k_row, k_head, k_column = k.stride()
     v_row, v_head, v_column = v.stride()
     if k_column != 1 or v_column != 1:
         raise ValueError(f"{what}: a head lies in one run, got strides {k.stride()} and {v.stride()}")
     T = shape[0]
     _int32_row(what, slot_mapping, "slot_mapping", T)
-    stream = _here(what, k, v, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, slot_mapping)
+    k_codes, k_pairs, v_codes, v_pairs = k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs
+    stream = _here(what, k, v, k_codes, k_pairs, v_codes, v_pairs, slot_mapping)
     lib, fn = _entry(D, "ts_int4_kvwrite")
     if T:
-        _launched(lib, fn(_DTYPE[k.dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, T, heads, k_cache.codes.data_ptr(),
-                          k_cache.pairs.data_ptr(), v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), slot_mapping.data_ptr(), page, pages, stream), 1)
+        _launched(lib, fn(_DTYPE[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, T, heads, k_codes.data_ptr(), k_pairs.data_ptr(),
+                          v_codes.data_ptr(), v_pairs.data_ptr(), slot_mapping.data_ptr(), page, pages, stream), 1)
 
 
 def _int4_rope_kvwrite(qkv, positions, num_heads, num_kv_heads, head_dim, rotary, q_weight, k_weight, eps, k_cache, v_cache, slot_mapping, page_size):
@@ -2888,13 +2888,13 @@ def int4_attention_splits(blocks, max_kv_len):
 def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_splits, backend, sinks, softcap):
     what = "paged_attention"
     pages, Hkv, page, D = _int4_caches(what, k_cache, v_cache, view.page_size)
-    shape, dtype = tuple(q.shape), q.dtype
+    shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or dtype not in _DTYPE or shape[2] != D or shape[1] % Hkv or shape[1] == 0:
-        raise TypeError(f"{what}: queries are float32 or bfloat16 [T, H, {D}] with H a multiple of {Hkv}, got {dtype} {shape}")
+        raise TypeError(f"{what}: queries are float32 or bfloat16 [T, H, {D}] with H a multiple of {Hkv}, got {dtype} {tuple(shape)}")
+    T, H, _ = shape
     q_row, q_head, q_column = q.stride()
     if q_column != 1:
         raise ValueError(f"{what}: a head lies in one run, got strides {q.stride()}")
-    T, H, _ = shape
     G = H // Hkv
     B, cu_q, kv_lens, table = ctx.num_requests, ctx.cu_q, ctx.kv_lens, view.block_table
     window, softcap = int(window or 0), float(softcap or 0.0)
@@ -2902,10 +2902,11 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         raise ValueError(f"{what}: a window and a soft cap are positive (0: none)")
     if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (H,) or not sinks.is_contiguous()):
         raise TypeError(f"{what}: sinks are float32 [heads] on the device")
-    rows, blocks = table.shape if table.dim() == 2 else (0, 0)
-    table_row, table_column = table.stride() if table.dim() == 2 else (0, 0)
-    if table.dtype != torch.int32 or rows < B or blocks < 1 or (blocks > 1 and table_column != 1):
-        raise TypeError(f"{what}: the block table is int32 [requests, blocks], rows contiguous, got {table.dtype} {tuple(table.shape)}")
+    table_shape = table.shape
+    rows, blocks = table_shape if len(table_shape) == 2 else (0, 0)
+    table_row, table_column = table.stride() if blocks else (0, 0)
+    if rows < B or blocks < 1 or (blocks > 1 and table_column != 1) or table.dtype != torch.int32:
+        raise TypeError(f"{what}: the block table is int32 [requests, blocks], rows contiguous, got {table.dtype} {tuple(table_shape)}")
     _int32_row(what, cu_q, "cu_q", B + 1)
     _int32_row(what, kv_lens, "kv_lens", B)
     chosen = int4_attention_backend(dtype, D)
@@ -2913,25 +2914,27 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         if backend not in (chosen, "simt") and (backend, chosen) != ("mma", "tcgen05"):
             raise ValueError(f"attention backend {backend!r} does not take {dtype}, head size {D} and a 4-bit cache")
         chosen = backend
-    stream = _here(what, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, table, cu_q, kv_lens, sinks)
-    out = torch.empty(shape, dtype=dtype, device=q.device)
+    k_codes, k_pairs, v_codes, v_pairs = k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs
+    stream = _here(what, q, k_codes, k_pairs, v_codes, v_pairs, table, cu_q, kv_lens, sinks)
+    out = torch.empty(T, H, D, dtype=dtype, device=q.device)
     lib, fn = _entry(D, "ts_int4_attention")
     if T == 0 or B == 0:
         return out
     max_q_len, span = ctx.max_q_len, ctx.max_kv_len
     if window:
         span = min(span, window)
+    kp, vp = k_pairs.data_ptr(), v_pairs.data_ptr()
+    # (what both kernels for a step get)
+    operands = (q.data_ptr(), q_row, q_head, out.data_ptr(), k_codes.data_ptr(), kp, v_codes.data_ptr(), vp, table.data_ptr(), cu_q.data_ptr(),
+                kv_lens.data_ptr(), T, B, H, Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else 0)
     most = columns = 0
     if chosen != "simt":
         few = max(1, INT4_DIRECT_ROWS // G)
         # (requests of one length, it seems: the portions' kernel takes them all, whatever the offsets on the device hold)
         alike = B == 1 or T == B * max_q_len
-        if chosen == "tcgen05" and max_q_len > few and (alike or T > few) and scale > 0 and (q.data_ptr() | 2 * q_row | 2 * q_head) % 16 == 0 and q_row > 0 and q_head > 0:
+        if chosen == "tcgen05" and max_q_len > few and (alike or T > few) and scale > 0 and (operands[0] | 2 * q_row | 2 * q_head) % 16 == 0 and q_row > 0 and q_head > 0:
             tc, portions = _entry(D, "ts_int4_attention_tcgen05")
-            _launched(tc, portions(q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
-                                   v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H,
-                                   Hkv, page, blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else 0,
-                                   0 if alike else few, stream), 1)
+            _launched(tc, portions(*operands, 0 if alike else few, stream), 1)
             if alike:
                 return out
             most = max_q_len = few
@@ -2940,7 +2943,7 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         columns = 16 if rows > 8 and D <= 128 and not most else 8
         tiles = B * Hkv * (1 if most else -(-rows // columns))
         if -(-rows // columns) * Hkv > 65535 or B > 65535 or page < 4 or pages * Hkv * page >= 2 ** 31 \
-                or (k_cache.pairs.data_ptr() | v_cache.pairs.data_ptr()) % 16:
+                or (kp | vp) % 16:
             columns = most = 0          # (a grid or a run of a page that the kernel has no form for: the 32-bit kernel takes everything)
     if num_splits is None:
         num_splits = int4_decode_splits(tiles, span) if columns else int4_attention_splits(T * Hkv * -(-G // 8), span)
@@ -2951,8 +2954,5 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         scratch = torch.empty(T * H * num_splits * (D + 2), dtype=torch.float32, device=q.device)
         part_o = scratch.data_ptr()
         part_ml = part_o + 4 * T * H * num_splits * D
-    _launched(lib, fn(_DTYPE[dtype], q.data_ptr(), q_row, q_head, out.data_ptr(), k_cache.codes.data_ptr(), k_cache.pairs.data_ptr(),
-                      v_cache.codes.data_ptr(), v_cache.pairs.data_ptr(), table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), T, B, H, Hkv, page,
-                      blocks, table_row, pages, scale, window, softcap, sinks.data_ptr() if sinks is not None else 0, num_splits, part_o, part_ml,
-                      max_q_len, columns, warps, most, stream), 1 if num_splits == 1 or merged else 2)
+    _launched(lib, fn(_DTYPE[dtype], *operands, num_splits, part_o, part_ml, max_q_len, columns, warps, most, stream), 1 if num_splits == 1 or merged else 2)
     return out
