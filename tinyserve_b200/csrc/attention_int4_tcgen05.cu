@@ -17,7 +17,8 @@
 // That portion takes 131 us, 0.79 PFLOP/s.  What bounds it is the softmax warps' path from scores to probabilities (with one matrix instruction a product and
 // tiles made twice only, still 108 us; without its exponentials no less than with them), then the start of a block (22 us for 256 blocks of one
 // tile) and the makers (11 us).  The subtraction of 1024 that an earlier form of the makers had cost 10 us; pairs of 32-bit operations in
-// the softmax save 5; probabilities in one part or in four instead of two took 143 us.
+// the softmax save 5; probabilities in one part or in four instead of two took 143 us,
+// steps of 64 keys with the scores of two steps in tensor memory 168 (a step's waits and fences weigh more than what they overlap).
 //
 // A key whose pair is not finite becomes a key of NaN with a value of zeros: who sees it gets NaN, who does not is not touched (its
 // probability of 0 would not survive a NaN in V).
