@@ -14,11 +14,13 @@
 // and one for the values of all tiles so far, with which the sums in tensor memory are rescaled when it grows.  (From the
 // pairs of the tile at hand: a look at all of a block's pairs beforehand took 30 us.)  What lies 2^-26 below the largest loses bits.
 //
-// That portion takes 131 us, 0.79 PFLOP/s.  What bounds it is the softmax warps' path from scores to probabilities (with one matrix instruction a product and
-// tiles made twice only, still 108 us; without its exponentials no less than with them), then the start of a block (22 us for 256 blocks of one
-// tile) and the makers (11 us).  The subtraction of 1024 that an earlier form of the makers had cost 10 us; pairs of 32-bit operations in
+// That portion takes 131 us, 0.79 PFLOP/s.  What bounds it is the chain of a query tile's steps: 2,000 cycles from its scores to its last
+// probabilities, 900 until the issuing thread has put P V and the next scores in the pipe, 600 until these are seen, with the other tile's chain beside
+// it (with one matrix instruction a product, tiles made twice only and hardly any softmax still 88 us).  Then come the start of a block (22 us for
+// 256 blocks of one tile) and the makers (11 us).  The subtraction of 1024 that an earlier form of the makers had cost 10 us; pairs of 32-bit operations in
 // the softmax save 5; probabilities in one part or in four instead of two took 143 us,
-// steps of 64 keys with the scores of two steps in tensor memory 168 (a step's waits and fences weigh more than what they overlap).
+// steps of 64 keys with the scores of two steps in tensor memory 168, two softmax threads a row 217 (what they wait for one another
+// weighs more than what overlaps).
 //
 // A key whose pair is not finite becomes a key of NaN with a value of zeros: who sees it gets NaN, who does not is not touched (its
 // probability of 0 would not survive a NaN in V).
