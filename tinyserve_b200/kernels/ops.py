@@ -2748,7 +2748,8 @@ def _linear_int8(x, weight, bias, out_float32, constant_weight):
 class Int4Pages:
     """One of the caches (keys or values) in 4 bits: ``codes`` uint8 [pages, kv heads, slots, D / 2] and ``pairs`` bfloat16 [pages, kv
     heads, slots, 2], both contiguous.  A head of a token with pair (scale, zero) stands for zero + code * scale; eight codes fill a
-    32-bit word, even columns in its lower half, odd ones in its upper half, the first in the lowest bits.  ``int4_kvwrite`` fills it."""
+    32-bit word, even columns in its lower half, odd ones in its upper half, the first in the lowest bits.  ``int4_kvwrite`` fills it.
+    (Attention sums values in 32 bits before it divides: magnitudes up to 2^100 are safe.)"""
     __slots__ = ("codes", "pairs", "shape")
 
     def __init__(self, codes, pairs):
