@@ -440,3 +440,34 @@ def test_products_that_follow_a_product():
         # rows of one row, of none, and a row read again and again
         assert torch.equal(ops.linear(x[:1].expand(3, -1), other), ops.linear(x[:1], other).expand(3, -1))
         assert ops.linear(x[:0], other).shape == (0, 256) and ops.quantize_rows(x[:0]).codes.shape == (0, 512)
+
+
+@pytest.mark.parametrize("D", [64, 128, 160, 256])
+@pytest.mark.parametrize("lengths", [[(1, 3000), (1, 70)], [(200, 700)], [(4, 1500), (1, 20), (90, 300)]])
+def test_attention_is_as_exact_as_its_rounding(D, lengths):
+    """bfloat16: inside, everything is rounded to 11 bits or more, an eighth of the result's half step.  Roots of sums of squares:
+    eight such roundings a term make 1.06 of what rounding the exact result makes."""
+    from tinyserve_b200.kernels import ops
+    ctx, view, kc, vc, ks, vs = batch(lengths, 2, D, 16, torch.bfloat16)
+    q = torch.randn(ctx.num_tokens, 8, D, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    want, _, _ = attention(q, lengths, ks, vs, D ** -0.5)
+    rounding = (want.bfloat16().double() - want).norm()
+    for splits in (None, 1, 9):
+        assert (ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, num_splits=splits).double() - want).norm() <= 1.06 * rounding
+
+
+def test_what_no_query_sees_does_not_matter():
+    """Slots behind a request's last token, in its last page, hold enormous scales, infinities and NaN."""
+    from tinyserve_b200.kernels import ops
+    lengths = [(1, 37), (1, 300), (70, 90), (3, 200)]
+    ctx, view, kc, vc, ks, vs = batch(lengths, 2, 128, 64, torch.bfloat16)
+    q = torch.randn(ctx.num_tokens, 8, 128, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    clean = [ops.paged_attention(q, kc, vc, view, ctx, 0.1, window, num_splits=sp) for window in (0, 50) for sp in (None, 3)]
+    for bad in (3e38, math.inf, -math.inf, 1e-38):
+        for b, (_, m) in enumerate(lengths):
+            page = int(view.block_table[b, (m - 1) // 64])
+            for c in (kc, vc):
+                c.pairs[page, :, (m - 1) % 64 + 1:] = bad
+                c.codes[page, :, (m - 1) % 64 + 1:] = 0x77
+        again = [ops.paged_attention(q, kc, vc, view, ctx, 0.1, window, num_splits=sp) for window in (0, 50) for sp in (None, 3)]
+        assert all(torch.equal(a, b) for a, b in zip(clean, again)), bad

@@ -10,6 +10,8 @@
 // One shift and one AND-OR then make a pair of neighbouring columns as two bfloat16 (see `codes2` in the kernels below).
 // Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
 // a token for heads of 128 where bfloat16 takes 256.
+#include <cuda_fp16.h>
+
 #include "entry.cuh"
 #include "rounding.cuh"
 #include "tcgen05.cuh"
@@ -569,14 +571,15 @@ __global__ void int4_combine_kernel(Int4Params p) {
 //      (bfloat16 has 8 significant bits: elements down to 2^-7 of the largest keep all of theirs, smaller ones are
 //      rounded to 2^-15 of it, far below what the projection's own rounding left.  Eight-bit floating point would hold a code without
 //      any change, but its mma.sync is made of conversions to 16 bits: 827 instructions a step of 32 keys, as it is 635.)
-//   V  keys run along K there, two of one column side by side, which bytes would need a transposition for: a code enters as the bfloat16
-//      number 16 + c, one shift and one AND-OR for two of them.
+//   V  keys run along K there, two of one column side by side, which bytes would need a transposition for: a code enters as the number
+//      16 + c in half precision, one shift and one AND-OR for two of them.
 //   Scales and zeros are per key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.c) + z sum(q); for the values, with p' =
-//   bfloat16(p s), sum p v = sum p' (c - 8) + sum p (z + 8 s), and sum p' (c - 8) = sum p' (16 + c) - 24 sum p', which is one more MMA, with
-//   ones for V, so that the 24 cancels whatever p' was rounded to.  (Around the middle of the codes the rounding of p' weighs half as much as
-//   around 0: 4,096 keys, relative error of the output before its own rounding 1.4e-3 and 2.5e-3.)
+//   half(p s), sum p v = sum p' (c - 8) + sum p (z + 8 s), and sum p' (c - 8) = sum p' (16 + c) - 24 sum p', which is one more MMA, with
+//   ones for V, so that the 24 cancels whatever p' was rounded to.  A power of two for each warp keeps p' within half precision: it follows the
+//   largest scale so far, as the maximum follows the scores.  (64 requests of 2,000 to 8,192 keys, relative error of the output, of which its
+//   own rounding makes 1.7e-3: with p' in bfloat16 2.3e-3, around code 0 instead of 8 3.3e-3.)
 // Values of 2^110 and more may overflow these sums, as probabilities reach 2^8 in them.
-// 64 requests of 2,000 to 8,192 keys, 32 heads of 128 on 8 (366 MB): 87 us, 4.2 TB/s; fetching alone takes 62.  The integer pipe is busiest (two thirds of its
+// 64 requests of 2,000 to 8,192 keys, 32 heads of 128 on 8 (366 MB): 89 us, 4.1 TB/s; fetching alone takes 62.  The integer pipe is busiest (two thirds of its
 // rate while a block walks), then the fixed 5 us of a block, of which an SM holds two.  Requests in the order of their numbers instead of by length:
 // 108 us, for the blocks that come last run alone.  Shifts as multiplications on the other pipe 91 and 99 us, three blocks an SM
 // with 80 registers a thread 123.
@@ -603,8 +606,8 @@ template <int NT, int WARPS> struct MmaCfg {
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+__device__ __forceinline__ void mma_half(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
@@ -636,19 +639,19 @@ __device__ __forceinline__ void mma_lo(int (&c)[4], uint32_t a0, uint32_t a1, ui
   asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// codes number e (0 .. 3) of both halves of a word as two bfloat16 numbers 16 + c
+// codes number e (0 .. 3) of both halves of a word as two numbers 16 + c in half precision
 template <int E>
 __device__ __forceinline__ uint32_t codes2(uint32_t word) {
-  const uint32_t moved = E == 0 ? word << 3 : word >> (4 * E - 3);
+  const uint32_t moved = E < 2 ? word << (6 - 4 * E) : word >> (4 * E - 6);
   uint32_t two;
   // (written out: the compiler makes two instructions of an AND and an OR with constants, and these pipes bound the kernel)
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(two) : "r"(moved), "r"(0x00780078u), "r"(0x41804180u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(two) : "r"(moved), "r"(0x03c003c0u), "r"(0x4c004c00u));
   return two;
 }
 // Where a running maximum starts: below every score, and finite, so that nothing subtracts infinities.  It moves only when a score passes it by
 // more than SLACK (a power of two): probabilities up to 2^SLACK do no harm in 32-bit sums, and most steps then rescale nothing.
 constexpr float LOWEST = -3e38f, SLACK = 8.f;
-constexpr uint32_t ONES = 0x3f803f80u;                             // two bfloat16
+constexpr uint32_t ONES = 0x3c003c00u;                             // two in half precision
 // Row r of the 16 that an MMA reads of K is this key of the group: thread t of a quad then finds its columns of V^T (rows 2t, 2t + 1, 2t + 8,
 // 2t + 9) in keys t, t + 4, t + 8, t + 12, and the eight lanes whose reads of K meet read neighbouring keys' halves of a bank line
 __device__ __forceinline__ int key_of_row(int r) { return (r & 8) | (r >> 1 & 3) | (r & 1) << 2; }
@@ -820,6 +823,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
 
   float o[D / 16][NT][4], m[NT][2], ps[NT][4];                     // ps: sum p' of columns 2t and 2t + 1 (and the same again)
   F2 l[NT], z[NT];
+  // the values' scales are multiplied by `unit`, which brings the largest so far to 2^6 .. 2^7; one of `bound` and more moves it
+  float unit = 1.f, bound = 0.f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -928,7 +933,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
           // a probability of 0 must not meet a NaN, of a slot that is not this request's or of a key that only some columns see:
           // the pair becomes 0, and who sees the key gets the NaN through its score
           const bool finite = fabsf(vscale[kb][h]) <= 3.402823466e38f && fabsf(vzero[kb][h]) <= 3.402823466e38f;
-          if (!finite) vscale[kb][h] = vzero[kb][h] = 0.f;
+          // (and a scale that nobody sees must not set the unit)
+          if (!finite || j >= j_hi || j < j_lo) vscale[kb][h] = vzero[kb][h] = 0.f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -939,7 +945,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
             }
         }
     }
-    bool moved = false;
+    float widest = fmaxf(fmaxf(fabsf(vscale[0][0]), fabsf(vscale[0][1])), fmaxf(fabsf(vscale[1][0]), fabsf(vscale[1][1])));
+    bool moved = widest >= bound && widest > 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -948,6 +955,16 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
         moved |= top[nt][i] > m[nt][i] + SLACK;
       }
     if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, d));
+      float shrink = 1.f;
+      if (widest >= bound && widest > 0.f) {
+        const int e = min(max((int)(__float_as_uint(widest) >> 23) - 127, -100), 127);
+        const float to = __uint_as_float((uint32_t)(6 - e + 127) << 23);
+        shrink = bound > 0.f ? to / unit : 0.f;          // (nothing was added before the first)
+        unit = to;
+        bound = __uint_as_float((uint32_t)(e + 1 + 127) << 23);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
@@ -958,10 +975,11 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
           const float above = fmaxf(top[nt][i], m[nt][i]);
           f[i] = ex2(m[nt][i] - above);
           m[nt][i] = above;
-          ps[nt][i] *= f[i];
-          ps[nt][2 + i] *= f[i];
+          const float both = f[i] * shrink;
+          ps[nt][i] *= both;
+          ps[nt][2 + i] *= both;
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= f[i]; o[mt][nt][2 + i] *= f[i]; }
+          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= both; o[mt][nt][2 + i] *= both; }
         }
         l[nt] = f2_mul(l[nt], f2(f[0], f[1]));
         z[nt] = f2_mul(z[nt], f2(f[0], f[1]));
@@ -980,13 +998,14 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
           const F2 pr = f2(ex2(x0), ex2(x1));
           l[nt] = f2_add(l[nt], pr);
           z[nt] = f2_fma(pr, f2(vzero[kb][h], vzero[kb][h]), z[nt]);
-          f2_out(f2_mul(pr, f2(vscale[kb][h], vscale[kb][h])), x0, x1);
-          const __nv_bfloat162 two = __floats2bfloat162_rn(x0, x1);
+          const float scaled = vscale[kb][h] * unit;
+          f2_out(f2_mul(pr, f2(scaled, scaled)), x0, x1);
+          const __half2 two = __floats2half2_rn(x0, x1);
           const uint32_t bits = *reinterpret_cast<const uint32_t*>(&two);
           pb[nt][h] = transposed(bits);
         }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_bf16(ps[nt], ONES, ONES, ONES, ONES, pb[nt][0], pb[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) mma_half(ps[nt], ONES, ONES, ONES, ONES, pb[nt][0], pb[nt][1]);
       // values: 16-bit units g UNITS .. of keys t, t + 4, t + 8, t + 12 of the group
       uint32_t u[4][(UNITS + 1) / 2];
 #pragma unroll
@@ -1014,8 +1033,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
         const uint32_t x0 = __byte_perm(u[0][i / 2], u[1][i / 2], i % 2 ? 0x7632 : 0x5410), x1 = __byte_perm(u[2][i / 2], u[3][i / 2], i % 2 ? 0x7632 : 0x5410);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(o[2 * i][nt], codes2<0>(x0), codes2<1>(x0), codes2<0>(x1), codes2<1>(x1), pb[nt][0], pb[nt][1]);
-          mma_bf16(o[2 * i + 1][nt], codes2<2>(x0), codes2<3>(x0), codes2<2>(x1), codes2<3>(x1), pb[nt][0], pb[nt][1]);
+          mma_half(o[2 * i][nt], codes2<0>(x0), codes2<1>(x0), codes2<0>(x1), codes2<1>(x1), pb[nt][0], pb[nt][1]);
+          mma_half(o[2 * i + 1][nt], codes2<2>(x0), codes2<3>(x0), codes2<2>(x1), codes2<3>(x1), pb[nt][0], pb[nt][1]);
         }
       }
     }
@@ -1034,6 +1053,7 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
   float* sm_ml = sm_o + WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
   float* box = reinterpret_cast<float*>(work + C::WORK_BYTES);     // (its own memory: a peer may send while this block still reads its ring)
   const int per_rank = (C::NC + p.splits - 1) / p.splits;
+  const float back = 1.f / unit;
   auto send = [](uint32_t at, uint32_t rank, float v) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
@@ -1055,13 +1075,13 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
       if (g == 0) {
         sm_ml[(warp * C::NC + c) * 3] = m[nt][i];
         sm_ml[(warp * C::NC + c) * 3 + 1] = ls[i];
-        sm_ml[(warp * C::NC + c) * 3 + 2] = fmaf(-ABOVE, ps[nt][i], zs[i]);
+        sm_ml[(warp * C::NC + c) * 3 + 2] = fmaf(-ABOVE * back, ps[nt][i], zs[i]);
       }
       float* dst = sm_o + (warp * C::NC + c) * MERGE_ROW + g;
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt) {
-        dst[16 * mt] = o[mt][nt][i];
-        dst[16 * mt + 8] = o[mt][nt][2 + i];
+        dst[16 * mt] = o[mt][nt][i] * back;
+        dst[16 * mt + 8] = o[mt][nt][2 + i] * back;
       }
     }
   }
