@@ -2849,8 +2849,8 @@ def int4_attention_backend(dtype, head_dim) -> str:
     return "tcgen05" if head_dim in TCGEN05_HEAD_DIMS else "mma"
 
 
-#: rows (queries x heads of a key head) of a request that one pass of the mma kernel over its keys takes; a request with
-#: more of them goes to the tcgen05 kernel, where there is one
+#: rows (queries x heads of a key head) up to which a request goes to the mma kernel; one with more of them goes to the
+#: tcgen05 kernel, where there is one
 INT4_DIRECT_ROWS = 16
 
 
