@@ -471,3 +471,26 @@ def test_what_no_query_sees_does_not_matter():
                 c.codes[page, :, (m - 1) % 64 + 1:] = 0x77
         again = [ops.paged_attention(q, kc, vc, view, ctx, 0.1, window, num_splits=sp) for window in (0, 50) for sp in (None, 3)]
         assert all(torch.equal(a, b) for a, b in zip(clean, again)), bad
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [5, 300])
+@pytest.mark.parametrize("D,first", [(128, 1), (64, 3), (96, 8), (512, 5)])
+def test_write_and_attention_of_rows_that_begin_anywhere(dtype, T, D, first):
+    """Heads that begin on any element and lie any number of elements apart: what their contiguous copies give, bit by bit."""
+    from tinyserve_b200.kernels import ops
+    g = torch.Generator().manual_seed(D)
+    k, v = (torch.randn(T, 2, D + 11, generator=g).to(dtype).cuda()[:, :, first:first + D] for _ in range(2))
+    q = torch.randn(T, 4, D + 13, generator=g).to(dtype).cuda()[:, :, first:first + D]
+    slots = torch.randperm(320, generator=g)[:T].int().cuda()
+    caches = [[empty_cache(20, 2, 16, D) for _ in range(2)] for _ in range(2)]
+    ops.int4_kvwrite(k, v, *caches[0], slots)
+    ops.int4_kvwrite(k.contiguous(), v.contiguous(), *caches[1], slots)
+    for a, b in zip(*caches):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.pairs.view(torch.int16), b.pairs.view(torch.int16))
+    ctx, view, kc, vc, _, _ = batch([(T, T + 40)], 2, D, 16, dtype)
+    # (the kernel for long portions takes rows that begin on 16 bytes only: one kernel for both sides here, the usual choice below)
+    one = "mma" if dtype == torch.bfloat16 and D in (64, 128) else None
+    assert torch.equal(ops.paged_attention(q, kc, vc, view, ctx, 0.1, backend=one), ops.paged_attention(q.contiguous(), kc, vc, view, ctx, 0.1, backend=one))
+    want = ops.paged_attention(q.contiguous(), kc, vc, view, ctx, 0.1).double()
+    assert (ops.paged_attention(q, kc, vc, view, ctx, 0.1).double() - want).norm() <= (2.0 ** -7 if dtype == torch.bfloat16 else 0.0) * want.norm()
