@@ -12,7 +12,7 @@
 // memory: no scratch, no counters, nothing that two launches could share.
 //
 // For few tokens the bytes of W bound it: 8 tokens x 4,096 on 24,576 rows take 18.9 us with the rows' codes (101 MB, 5.3 TB/s), 64 x 12,288 on 4,096 rows
-// 17.9 (50 MB, cut by eight); the smallest calls are launches (1 x 1,024 on 4,096 rows 5.4 us, both kernels).  A single launch that makes the
+// 15.9 (50 MB, cut by eight); the smallest calls are launches (1 x 1,024 on 4,096 rows 5.4 us, both kernels).  A single launch that makes the
 // rows' codes in every block's loader was slower (1 x 1,024: 7.4 us): every block waits for the whole row before its first MMA.
 #include "entry.cuh"
 #include "rounding.cuh"
@@ -344,7 +344,8 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     // in a row from r own on, a multiple of four), which adds them up from its own shared memory.  (Loads from the peers instead, eight
     // in flight a thread, take a trip through the cluster for every token: 256 tokens x 4,096 on 4,096 rows 21 us.)
     const int own = ((live + p.splits - 1) / p.splits + 3) & ~3;
-    const uint32_t box = smem_u32(smem);                    // [sender][weight row][token of mine]
+    const uint32_t box = smem_u32(smem);                    // [sender][four tokens of mine][weight row][token]: a warp's stores are one run
+    // (by weight row first, 64 x 12,288 on 4,096 rows took 17.7 us instead of 13.9)
     cluster_arrive();
     cluster_wait();
 #pragma unroll 1
@@ -354,7 +355,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int i = 0; i < COLS; i += 4) {
         const int j = c + i, owner = j / own;
-        if (j < live) cluster_store4(box + ((split * TILE_N + threadIdx.x) * own + j - owner * own) * 4, owner, v[i], v[i + 1], v[i + 2], v[i + 3]);
+        if (j < live) cluster_store4(box + ((split * own + j - owner * own) * (TILE_N / 4) + threadIdx.x) * 16, owner, v[i], v[i + 1], v[i + 2], v[i + 3]);
       }
     }
     cluster_arrive();
@@ -365,7 +366,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int s = 0; s < MAX_SPLITS; ++s)
         if (s < p.splits) {
-          const int4 x = sums[((s * TILE_N + threadIdx.x) * own + j) >> 2];
+          const int4 x = sums[(s * own + j) * (TILE_N / 4) + threadIdx.x];
           sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
         }
       if (n < p.N) {

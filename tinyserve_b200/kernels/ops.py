@@ -2679,15 +2679,17 @@ def int8_plan(M, N, K):
     wide ones (us, tiles of 64 / pairs: 512 x 12288 on 4096 33.9 / 35.4, 512 x 1024 on 4096 8.1 / 9.4; 400 x 4096 on 6144 25.6 / 17.8, 256 x 4096 on
     24576 46.5 / 31.9, 2048 x 1024 on 6144 45 / 22.4); up to 128 tokens in one tile of 128 come first there (100 x 4096 on 24576 26.3 / 30.3).
     K is cut, in powers of two, where the tiles leave more than half of the SMs idle and a cut keeps eight slices of 128 (us, whole / cut: 8 x
-    4096 on 4096 9.2 / 6.4 by four, 32 x 4096 on 6144 10.8 / 8.9 by four, 64 x 12288 on 4096 31 / 17.9 by eight; 96 tiles, 128 x 4096
-    on 6144, 14.2 / 15.7 by two; 8 slices, 1 x 1024 on 4096, 3.7 / 3.9; in sixths 32 x 4096 on 6144 takes 15.4: clusters of six find no place)."""
+    4096 on 4096 9.2 / 6.3 by four, 32 x 4096 on 6144 10.8 / 8.2 by four, 64 x 12288 on 4096 31 / 13.9 by eight; 8 slices, 1 x 1024 on 4096, 3.7 /
+    3.9; in sixths 32 x 4096 on 6144 takes 15.4: clusters of six find no place), and with tiles of 64, whose sums a cut reads from tensor memory in half the
+    time, where every SM has one tile and K 32 slices (128 x 4096 on 6144 14.3 / 12.9 by two, 256 x 4096 on 4096 14.0 / 12.8, 64 x 4096 on 12288 15.8 /
+    15.4; 8 x 4096 on 12288 11.2 / 11.6, 256 x 2048 on 4096 9.7 / 10.7)."""
     tile_t = 16 if M <= 16 else 32 if M <= 32 else 64
     row_tiles, slices = -(-N // 128), -(-K // 128)
     tiles = row_tiles * -(-M // tile_t)
     if M > 64 and tiles > 2 * num_sms():
         return (128, 1) if M <= 128 and row_tiles <= 2 * num_sms() else (256, 0)
     splits = 1
-    if 2 * tiles <= num_sms():
+    if 2 * tiles <= num_sms() or (tile_t == 64 and slices >= 32 and tiles <= num_sms()):
         while splits < 8 and 2 * splits * tiles <= 2 * num_sms() and slices >= 16 * splits:
             splits *= 2
     return tile_t, -(-slices // -(-slices // splits))           # no cut without a slice
