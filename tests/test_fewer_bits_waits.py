@@ -1,0 +1,26 @@
+"""What the kernels of the 8-bit products and the 4-bit cache wait for, looked for in their text: a missing wait shows on the device now and
+then only."""
+import re
+
+import pytest
+
+from test_kernel_sources import kernels
+
+FILES = ("attention_int4.cu", "attention_int4_tcgen05.cu", "gemm_int8.cu", "gemm_int8_pair.cu")
+OURS = sorted(name for name in kernels() if name[0] in FILES)
+
+
+def test_the_kernels_are_found():
+    assert {k for _, k in OURS} >= {"quantize_rows_kernel", "gemm_i8_kernel", "gemm_i8_pair_kernel", "int4_kvwrite_kernel", "int4_rope_kvwrite_kernel",
+                                    "int4_attend_kernel", "int4_combine_kernel", "int4_mma_kernel", "int4_prefill_kernel"}
+
+
+@pytest.mark.parametrize("name", [n for n in OURS if n[1] != "gemm_i8_kernel"])
+def test_every_thread_waits_before_it_reads(name):
+    """One wait, of every block and under no condition, before anything that a predecessor may have written is read.  (The 8-bit product
+    fetches constant weights before its wait, see below; a norm's weights are nobody's output.)"""
+    body = kernels()[name][1]
+    assert body.count("pdl_wait();") == 1
+    before = body[:body.index("pdl_wait();")]
+    assert re.search(r"[;}]\s*$", before) and before.count("{") - before.count("}") == 1
+    assert not re.search(r"p\.(q|k|v|x|kc|vc|kp|vp|cu_q|kv_lens|block_table|slot_mapping|sx|sw)\b|rp\.(qkv|positions)\b", before)

@@ -331,7 +331,6 @@ struct Int4Params {
   int splits;                                // key ranges; > 1: partial results for the combine kernel
   float unit;                                // powers of two in a unit of the partial results' maxima
   int most;                                  // > 0: requests with more queries are somebody else's
-  int beside;                                // != 0: the kernel before this one has the same inputs: it runs on while this one does
   int ordered;                               // != 0: blocks take the requests by length, the longest first
   float *part_o, *part_ml;                   // [T * H][splits][D], [T * H][splits][2] (maximum, sum)
 };
@@ -698,21 +697,16 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
   asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   __syncthreads();
   pdl_trigger();
-  // Behind the portions' kernel, which starts its dependents when its own inputs are complete and all of its blocks run, there is nothing to wait
-  // for before the work, only, so that who waits for this kernel waits for that one too, before the end: in one block, which holds its place.
-  if (!p.beside) pdl_wait();
-  // (64 requests over 800 keys beside a portion of 448: 58 us one kernel behind the other, 47 so; with every block waiting at its end, 58)
-  const bool lasts = p.beside && blockIdx.x + blockIdx.y + blockIdx.z == 0;
+  // Beside portions (`most`) too: that this kernel's inputs were complete when the portions' kernel began does not make them visible here; only
+  // this grid's own wait does.  (64 requests over 800 keys behind a portion of 448: 58 us; 47 without the wait.)
+  pdl_wait();
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
   const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC;
   const int b = p.ordered ? nth_longest<WARPS * 32>(p, blockIdx.z, reinterpret_cast<int*>(work)) : blockIdx.z;
   if (p.ordered) __syncthreads();                                  // (its memory is the ring's)
   const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
   const int nc = min(C::NC, q_len * G - c0);                       // columns of this block (and of its cluster: they leave together)
-  if (nc <= 0 || (p.most > 0 && q_len > p.most)) {
-    if (lasts) pdl_wait();
-    return;
-  }
+  if (nc <= 0 || (p.most > 0 && q_len > p.most)) return;
   const bool clustered = WARPS == 8 && p.splits > 1 && p.part_o == nullptr;
   if (clustered) cluster_arrive();                                 // this block runs: peers may write to its memory
   const int kv_len = (int)min((long long)p.kv_lens[b], (long long)p.max_blocks << p.page_shift);
@@ -1119,10 +1113,7 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
       if (place < 2) send(smem_u32(box + at * MERGE_ROW + D + place), c % p.splits, place == 0 ? top : total);
     }
   }
-  if (!clustered) {
-    if (lasts) pdl_wait();
-    return;
-  }
+  if (!clustered) return;
   cluster_arrive();
   cluster_wait();
   for (int i = threadIdx.x; i < per_rank * D; i += WARPS * 32) {
@@ -1145,7 +1136,6 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
       }
     static_cast<bf16*>(p.out)[((size_t)(q_begin + r / G) * p.H + head) * D + d] = __float2bfloat16_rn(total == 0.f ? 0.f : sum / total);
   }
-  if (lasts) pdl_wait();
 }
 
 template <int NT, int WARPS>
@@ -1240,8 +1230,8 @@ static int int4_rope_kvwrite(int dtype, const void* qkv, void* q, const int* pos
 TS_ENTRY(int4_rope_kvwrite)
 
 // q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml, or (with columns, up to 8) merges in clusters.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
-// steps of 32 up to 256; 16 columns up to 128) with 8 warps a block, or 4 (8 columns, one key range, heads up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns, right behind ts_int4_attention_tcgen05 of the same step):
-// requests with more queries than that are left alone.
+// steps of 32 up to 256; 16 columns up to 128) with 8 warps a block, or 4 (8 columns, one key range, heads up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns, for a step
+// whose longer requests ts_int4_attention_tcgen05 has taken): requests with more queries than that are left alone.
 static int int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
                           const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
                           int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
@@ -1255,7 +1245,7 @@ static int int4_attention(int dtype, const void* q, long long q_row, long long q
   TS_REQUIRE(splits >= 1 && (splits == 1 || (part_o && part_ml) || (columns > 0 && splits <= 8 && !part_o)), "int4_attention: key ranges need their scratch");
   Int4Params p = {q, q_row, q_head, out, (const uint32_t*)k_codes, (const uint32_t*)v_codes, (const uint32_t*)k_pairs, (const uint32_t*)v_pairs,
                   block_table, cu_q, kv_lens, T, B, H, Hkv, shift, max_blocks, table_stride, num_pages, scale, window, softcap, sinks,
-                  splits, columns > 0 ? 1.f : LOG2E, most, most > 0, 0, part_o, part_ml};
+                  splits, columns > 0 ? 1.f : LOG2E, most, 0, part_o, part_ml};
   if (columns > 0) {
 #ifdef TS_INT4_MMA
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");

@@ -169,8 +169,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // This block holds all of the SM's tensor memory now: only now may a dependent kernel start.  And only behind the wait: the kernel for the short
-  // requests of the same step then finds complete what came before this one.
+  // This block holds all of the SM's tensor memory now: only now may a dependent kernel start.
   pdl_wait();
   pdl_trigger();
 
