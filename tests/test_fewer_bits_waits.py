@@ -24,3 +24,16 @@ def test_every_thread_waits_before_it_reads(name):
     before = body[:body.index("pdl_wait();")]
     assert re.search(r"[;}]\s*$", before) and before.count("{") - before.count("}") == 1
     assert not re.search(r"p\.(q|k|v|x|kc|vc|kp|vp|cu_q|kv_lens|block_table|slot_mapping|sx|sw)\b|rp\.(qkv|positions)\b", before)
+
+
+def test_codes_of_weights_are_fetched_early_only_where_they_are_constant():
+    """What stands between the kernel that made a weight's codes and the product (the rows' codes, say) does not make them visible to the
+    product: only the caller's word that they are constant lets it read them before its wait."""
+    from test_kernel_sources import CSRC
+    with open(f"{CSRC}/gemm_int8.cu") as fh:
+        text = re.sub(r"//[^\n]*", "", fh.read())
+    body = kernels()[("gemm_int8.cu", "gemm_i8_kernel")][1]
+    loader = body[body.index("if (threadIdx.x == 0) {", body.index("pdl_trigger")):]
+    assert loader.index("if (!p.w_ready) pdl_wait();") < loader.index("tma_load_2d") < loader.index("    pdl_wait();\n") < loader.index("&map_x")
+    made = re.search(r"I8Params p = \{([^;]*)\};", text).group(1)
+    assert made.split(",")[-1].strip() == "w_constant"

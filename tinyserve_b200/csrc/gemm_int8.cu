@@ -103,8 +103,6 @@ template <typename T, int KEPT>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(QuantParams p, bool vec) {
   __shared__ uint32_t tops[QUANT_THREADS / 32];
   const int threads = blockDim.x, warps = threads / 32;
-  // The trigger comes behind the wait: what the kernel after this one reads before its own wait (the codes of the weights) is
-  // then complete, whoever wrote it.
   pdl_wait();
   pdl_trigger();
   const size_t m = blockIdx.x;
@@ -445,7 +443,8 @@ TS_ENTRY(quantize_rows)
 
 // out [M, N] (ldc; float where out_f32, else bfloat16) from codes and scales of x and w (leading dimensions multiples of 16).
 // x_dtype >= 0: x is a tensor of that type (leading dimension ldx) whose rows are brought to cx, sx first; -1: cx and sx are given.
-// tile_t: tokens of a tile (16, 32, 64 or 128); splits: cuts along K (a cluster of up to 8 blocks).  w_constant: nobody that may still run writes w (with x_dtype >= 0 the first launch sees to that).
+// tile_t: tokens of a tile (16, 32, 64 or 128); splits: cuts along K (a cluster of up to 8 blocks).  w_constant: nobody that may still run writes w, whose first
+// codes are then fetched before the product's dependency wait.
 static int gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, long long ldcx, float* sx, const void* cw, long long ldw,
                      const float* sw, const void* bias, int bias_f32, void* out, long long ldc, int out_f32, int M, int N, int K,
                      int tile_t, int splits, int w_constant, cudaStream_t stream) {
@@ -461,7 +460,7 @@ static int gemm_int8(int x_dtype, const void* x, long long ldx, void* cx, long l
   }
   CUtensorMap map_w, map_x;
   TS_REQUIRE(make_map(&map_w, cw, N, K, ldw, TILE_N) && make_map(&map_x, cx, M, K, ldcx, tile_t), "gemm_int8: cuTensorMapEncodeTiled failed");
-  const I8Params p = {out, sx, sw, VecParam{bias, bias_f32}, ldc, M, N, K, splits, out_f32, x_dtype >= 0 || w_constant};
+  const I8Params p = {out, sx, sw, VecParam{bias, bias_f32}, ldc, M, N, K, splits, out_f32, w_constant};
   switch (tile_t) {
     case 16: return launch<16>(map_w, map_x, p, stream);
     case 32: return launch<32>(map_w, map_x, p, stream);

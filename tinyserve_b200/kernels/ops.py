@@ -1276,8 +1276,8 @@ def linear(x, weight, bias=None, out_float32=False, allow_partials=False, allow_
     x may be the ScaledRows that add_rmsnorm returned.
     ``weight`` may be an ``Int8Rows``: the rows of x are then brought to 8 bits too (or x is an Int8Rows already), and the
     result is a plain tensor of x's type (of bfloat16 for an Int8Rows), or float32 with ``out_float32``.
-    ``constant_weight``: no kernel that may still run writes ``weight`` (a model's weights).  A float32 product
-    then fetches its first tiles of it while the kernels before it still run; without, the weight may be the
+    ``constant_weight``: no kernel that may still run writes ``weight`` (a model's weights).  A float32 product, or
+    one over ``Int8Rows``, then fetches its first tiles of it while the kernels before it still run; without, the weight may be the
     result of the product before.  The bfloat16 products of this package always fetch them so: a
     bfloat16 weight that was computed on the device needs a synchronisation before its first product."""
     scale = None
