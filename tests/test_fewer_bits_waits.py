@@ -37,3 +37,10 @@ def test_codes_of_weights_are_fetched_early_only_where_they_are_constant():
     assert loader.index("if (!p.w_ready) pdl_wait();") < loader.index("tma_load_2d") < loader.index("    pdl_wait();\n") < loader.index("&map_x")
     made = re.search(r"I8Params p = \{([^;]*)\};", text).group(1)
     assert made.split(",")[-1].strip() == "w_constant"
+
+
+def test_bulk_copies_come_behind_the_ranking_of_requests():
+    """The ranking uses the ring's memory by ordinary stores; a copy by the other proxy into the same bytes needs a fence, then a barrier."""
+    body = re.sub(r"\s+", " ", kernels()[("attention_int4.cu", "int4_mma_kernel")][1])
+    between = body[body.index("nth_longest<"):body.index("bulk_copy(")]
+    assert "if (p.ordered) { fence_async_shared(); __syncthreads(); }" in between

@@ -703,7 +703,11 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
   const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC;
   const int b = p.ordered ? nth_longest<WARPS * 32>(p, blockIdx.z, reinterpret_cast<int*>(work)) : blockIdx.z;
-  if (p.ordered) __syncthreads();                                  // (its memory is the ring's)
+  if (p.ordered) {
+    // (its memory is the ring's: bulk copies come behind ordinary stores and loads there)
+    fence_async_shared();
+    __syncthreads();
+  }
   const int q_begin = p.cu_q[b], q_len = min(p.cu_q[b + 1], p.T) - q_begin;
   const int nc = min(C::NC, q_len * G - c0);                       // columns of this block (and of its cluster: they leave together)
   if (nc <= 0 || (p.most > 0 && q_len > p.most)) return;
