@@ -44,3 +44,13 @@ def test_bulk_copies_come_behind_the_ranking_of_requests():
     body = re.sub(r"\s+", " ", kernels()[("attention_int4.cu", "int4_mma_kernel")][1])
     between = body[body.index("nth_longest<"):body.index("bulk_copy(")]
     assert "if (p.ordered) { fence_async_shared(); __syncthreads(); }" in between
+
+
+def test_what_a_launch_keeps_for_its_device_is_atomic():
+    """Calls through ctypes run side by side on several host threads: the word that says which devices a kernel is set up for is shared."""
+    from test_kernel_sources import CSRC
+    with open(f"{CSRC}/common.cuh") as fh:
+        text = fh.read()
+    struct = re.search(r"struct SmemSet \{(.*?)\n\};", text, re.S).group(1)
+    assert "std::atomic<unsigned long long> done{0};" in struct and "done.fetch_or(" in struct
+    assert not re.search(r"\bdone\s*(\||=)", struct)

@@ -4,6 +4,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -180,15 +181,15 @@ static inline cudaError_t ts_launch_cluster(void (*kernel)(KArgs...), dim3 grid,
 }
 
 // A kernel's dynamic shared memory, set once per device (the call takes a third of a microsecond, as long as a small launch's other
-// preparations together)
+// preparations together).  Several host threads may launch at once: two may set it, which does no harm.
 struct SmemSet {
-  unsigned long long done = 0;
+  std::atomic<unsigned long long> done{0};
   template <typename K> cudaError_t to(K kernel, int bytes) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess || (device < 64 && (done >> device & 1))) return e;
+    if (e != cudaSuccess || (device < 64 && (done.load(std::memory_order_acquire) >> device & 1))) return e;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && device < 64) done |= 1ull << device;
+    if (e == cudaSuccess && device < 64) done.fetch_or(1ull << device, std::memory_order_release);
     return e;
   }
 };
