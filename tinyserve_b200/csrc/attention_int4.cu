@@ -1143,7 +1143,7 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
 }
 
 template <int NT, int WARPS>
-int attend_mma(Int4Params p, int max_q_len, cudaStream_t stream) {
+int attend_mma(Int4Params p, int max_q_len, int sms, cudaStream_t stream) {
   using C = MmaCfg<NT, WARPS>;
   static SmemSet set;
   const cudaError_t sized = set.to(int4_mma_kernel<NT, WARPS>, C::SMEM);
@@ -1152,8 +1152,8 @@ int attend_mma(Int4Params p, int max_q_len, cudaStream_t stream) {
   const long long tiles = ((long long)max_q_len * G + C::NC - 1) / C::NC * p.Hkv;
   TS_REQUIRE(tiles <= 65535 && p.B <= 65535, "int4_attention: grid out of range");
   const dim3 grid(p.splits, (unsigned)tiles, p.B), block(WARPS * 32);
-  // (when everything runs at once, on 148 SMs, order is no use)
-  p.ordered = p.B > 1 && p.B <= MAX_ORDERED && tiles * p.splits * p.B > (long long)C::BLOCKS * 148;
+  // (when everything runs at once, order is no use)
+  p.ordered = p.B > 1 && p.B <= MAX_ORDERED && tiles * p.splits * p.B > (long long)C::BLOCKS * sms;
   if (p.splits > 1 && p.part_o == nullptr) {
     // the key ranges of a tile are a cluster and merge in it
     const cudaError_t e = ts_launch_cluster(int4_mma_kernel<NT, WARPS>, grid, block, C::SMEM, stream, dim3(p.splits, 1, 1), p);
@@ -1235,12 +1235,13 @@ TS_ENTRY(int4_rope_kvwrite)
 
 // q, out [T, H, D]; see Int4Params.  splits > 1 needs part_o and part_ml, or (with columns, up to 8) merges in clusters.  columns 8 or 16: the tensor-core kernel (bfloat16, heads in
 // steps of 32 up to 256; 16 columns up to 128) with 8 warps a block, or 4 (8 columns, one key range, heads up to 128), whose grid covers max_q_len queries a request; 0: the 32-bit kernel.  most > 0 (with columns, for a step
-// whose longer requests ts_int4_attention_tcgen05 has taken): requests with more queries than that are left alone.
+// whose longer requests ts_int4_attention_tcgen05 has taken): requests with more queries than that are left alone.  sms: multiprocessors
+// of the device.
 static int int4_attention(int dtype, const void* q, long long q_row, long long q_head, void* out, const void* k_codes, const void* k_pairs,
                           const void* v_codes, const void* v_pairs, const int* block_table, const int* cu_q, const int* kv_lens,
                           int T, int B, int H, int Hkv, int page_size, int max_blocks, int table_stride, int num_pages, float scale,
                           int window, float softcap, const float* sinks, int splits, float* part_o, float* part_ml, int max_q_len,
-                          int columns, int warps, int most, cudaStream_t stream) {
+                          int columns, int warps, int most, int sms, cudaStream_t stream) {
   const int shift = shift_of_page(page_size);
   TS_REQUIRE(dtype == TS_F32 || dtype == TS_BF16, "int4_attention: unknown dtype %d", dtype);
   TS_REQUIRE(T > 0 && B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && shift >= 0 && num_pages > 0 && max_blocks > 0, "int4_attention: %d tokens of %d requests, %d heads on %d, pages of %d",
@@ -1255,10 +1256,10 @@ static int int4_attention(int dtype, const void* q, long long q_row, long long q
     TS_REQUIRE(dtype == TS_BF16 && max_q_len > 0 && page_size >= 4, "int4_attention: the tensor-core kernel takes bfloat16 queries and pages of 4 and more");
     TS_REQUIRE(((long long)num_pages * Hkv << shift) < (1LL << 31), "int4_attention: the tensor-core kernel takes pools of fewer than 2^31 rows");
     TS_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_pairs | (uintptr_t)v_pairs) & 15) == 0, "int4_attention: the tensor-core kernel copies runs that begin on 16 bytes");
-    if (columns == 8 && warps == 8) return attend_mma<1, 8>(p, max_q_len, stream);
+    if (columns == 8 && warps == 8) return attend_mma<1, 8>(p, max_q_len, sms, stream);
 #if TS_HEAD_DIM <= 128
-    if (columns == 8 && warps == 4 && splits == 1) return attend_mma<1, 4>(p, max_q_len, stream);
-    if (columns == 16 && warps == 8) return attend_mma<2, 8>(p, max_q_len, stream);
+    if (columns == 8 && warps == 4 && splits == 1) return attend_mma<1, 4>(p, max_q_len, sms, stream);
+    if (columns == 16 && warps == 8) return attend_mma<2, 8>(p, max_q_len, sms, stream);
 #endif
 #endif
     return ts_fail("int4_attention: no tensor-core kernel for heads of %d, %d columns and %d warps", D, columns, warps);

@@ -2579,7 +2579,7 @@ def delta_rule(q, k, v, gate, logits, bias, rate, state, ctx, num_heads, key_dim
 # entry points are looked up once.)
 # Their arguments go in one run of 64-bit fields, "q" an integer or a pointer, "d" a float (csrc/entry.cuh).
 _INT8_ENTRIES = {"ts_quantize_rows": "9q", "ts_gemm_int8": "21q", "ts_gemm_int8_pair": "16q"}
-_INT4_ENTRIES = {"ts_int4_kvwrite": "17q", "ts_int4_rope_kvwrite": "11qd11q", "ts_int4_attention": "20qdqd9q", "ts_int4_attention_tcgen05": "19qdqd3q"}
+_INT4_ENTRIES = {"ts_int4_kvwrite": "17q", "ts_int4_rope_kvwrite": "11qd11q", "ts_int4_attention": "20qdqd10q", "ts_int4_attention_tcgen05": "19qdqd3q"}
 
 
 @functools.lru_cache(maxsize=None)
@@ -2957,5 +2957,6 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         scratch = torch.empty(T * H * num_splits * (D + 2), dtype=torch.float32, device=q.device)
         part_o = scratch.data_ptr()
         part_ml = part_o + 4 * T * H * num_splits * D
-    _launched(lib, fn(_DTYPE[dtype], *operands, num_splits, part_o, part_ml, max_q_len, columns, warps, most, stream), 1 if num_splits == 1 or merged else 2)
+    _launched(lib, fn(_DTYPE[dtype], *operands, num_splits, part_o, part_ml, max_q_len, columns, warps, most, num_sms(), stream),
+              1 if num_splits == 1 or merged else 2)
     return out
