@@ -41,3 +41,15 @@ def test_the_device_is_asked_for_its_multiprocessors(calls, monkeypatch):
         ops.struct.pack("=" + ops._INT4_ENTRIES[name], *fields)          # (as many as the entry point takes)
     with open(f"{ops.build.CSRC}/attention_int4.cu") as fh:
         assert "148" not in fh.read().split("int attend_mma(")[1].split("\n}")[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [[(1, 30), (1, 5)], [(70, 70), (3, 0)]])
+def test_a_window_longer_than_the_table_is_none(calls, dtype, lengths):
+    """Kernels take a window as a 32-bit integer and subtract it from positions: 2^32 + 5 would be 5, and 2^31 - 1 wraps behind a
+    position below zero (a row of a request with fewer keys than queries)."""
+    table = 16 * max(-(-m // 16) for _, m in lengths)
+    for window, want in ((0, 0), (5, 5), (table - 1, table - 1), (table, 0), (2 ** 31 - 1, 0), (2 ** 31, 0), (2 ** 32 + 5, 0), (2 ** 70, 0)):
+        attend(lengths, dtype=dtype, window=window)
+        assert calls and all(fields[{"ts_int4_attention": 21, "ts_int4_attention_tcgen05": 20}[name]] == want for name, fields in calls), window
+        calls.clear()

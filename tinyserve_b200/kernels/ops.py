@@ -2912,6 +2912,8 @@ def _paged_attention_int4(q, k_cache, v_cache, view, ctx, scale, window, num_spl
         raise TypeError(f"{what}: the block table is int32 [requests, blocks], rows contiguous, got {table.dtype} {tuple(table_shape)}")
     _int32_row(what, cu_q, "cu_q", B + 1)
     _int32_row(what, kv_lens, "kv_lens", B)
+    if window >= blocks * page:
+        window = 0          # (as long as the table: every key is within it, and kernels subtract it from positions in 32 bits)
     chosen = int4_attention_backend(dtype, D)
     if backend is not None:
         if backend not in (chosen, "simt") and (backend, chosen) != ("mma", "tcgen05"):
