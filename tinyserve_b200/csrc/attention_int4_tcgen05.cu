@@ -32,6 +32,7 @@
 
 #include "entry.cuh"
 #include "pairs.cuh"
+#include "softcap.cuh"
 #include "tcgen05.cuh"
 
 #ifndef TS_HEAD_DIM
@@ -430,10 +431,29 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         tmem_load_wait();
         float sc = p.scale_log2 * k_down;
         if (p.cap2 > 0.f) {
+          if (!all_visible) {
+            // (a key that the row does not see has no say in how the others are capped)
 #pragma unroll
-          for (int e = 0; e < BN; ++e) {
-            const float x = ex2(sv[e] * (p.cap_in * k_down * (2.f * LOG2E)));
-            sv[e] = p.cap2 * (1.f - __fdividef(2.f, x + 1.f));
+            for (int e = 0; e < BN; ++e)
+              if (j0 + e > pos || j0 + e < lo) sv[e] = 0.f;
+          }
+          // the usual case: every score of the row's tile is small against the cap
+          const float w = p.cap_in * k_down;
+          float big = 0.f;
+#pragma unroll
+          for (int e = 0; e < BN; ++e) big = fmaxf(big, fabsf(sv[e]));
+          if (big * w <= TANH_SMALL) {
+#pragma unroll
+            for (int e = 0; e < BN; ++e) {
+              const float x = sv[e] * w, t = x * x;
+              sv[e] = p.cap2 * x * fmaf(fmaf(fmaf(fmaf(TANH_P4, t, TANH_P3), t, TANH_P2), t, TANH_P1), t, TANH_P0);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < BN; ++e) {
+              const float x = ex2(sv[e] * (w * (2.f * LOG2E)));
+              sv[e] = p.cap2 * (1.f - __fdividef(2.f, x + 1.f));
+            }
           }
           sc = 1.f;
         }

@@ -30,6 +30,7 @@
 // kernel may start, so that no block of a successor can sit on columns that this kernel still needs.
 // Row maxima and sums never leave their thread, so there are no shuffles.  Every mbarrier wait is
 // bounded (tcgen05.cuh); a block that gives up raises ts_attention_tcgen05_error.
+#include "softcap.cuh"
 #include "tcgen05.cuh"
 
 #ifndef TS_HEAD_DIM
@@ -318,11 +319,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           float big = 0.f;
 #pragma unroll
           for (int e = 0; e < BN; ++e) big = fmaxf(big, fabsf(sv[e]));
-          if (big * p.cap_in <= 0.75f) {
+          if (big * p.cap_in <= TANH_SMALL) {
             const float w2 = p.cap_in * p.cap_in;
-            const float k0 = 9.999994059e-01f * p.scale_log2, k1 = -3.332809286e-01f * p.scale_log2 * w2,
-                        k2 = 1.325760377e-01f * p.scale_log2 * w2 * w2, k3 = -5.001763221e-02f * p.scale_log2 * w2 * w2 * w2,
-                        k4 = 1.289561170e-02f * p.scale_log2 * w2 * w2 * w2 * w2;
+            const float k0 = TANH_P0 * p.scale_log2, k1 = TANH_P1 * p.scale_log2 * w2, k2 = TANH_P2 * p.scale_log2 * w2 * w2,
+                        k3 = TANH_P3 * p.scale_log2 * w2 * w2 * w2, k4 = TANH_P4 * p.scale_log2 * w2 * w2 * w2 * w2;
 #pragma unroll
             for (int e = 0; e < BN; ++e) {
               const float t = sv[e] * sv[e];
