@@ -33,3 +33,24 @@ def test_a_soft_cap_keeps_scores_far_below_it(D, softcap):
         for backend in ("tcgen05", "mma", "simt"):
             out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, window, softcap=softcap, backend=backend)
             assert (out.double() - want).norm() <= AS_EXACT_AS_ITS_ROUNDING * rounding, backend
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [48, 64, 128])
+def test_a_sink_of_minus_infinity_is_none(dtype, D):
+    """exp(-infinity) adds nothing to a head's sum; a row without keys stays zero."""
+    from tinyserve_b200.kernels import ops
+    lengths = [(70, 60), (40, 300), (1, 0), (1, 9)]
+    ctx, view, kc, vc, ks, vs = batch(lengths, 2, D, 16, dtype)
+    q = queries(ctx.num_tokens, 8, D, dtype)
+    sinks = torch.randn(8, generator=torch.Generator().manual_seed(1)).cuda()
+    some = torch.where(torch.arange(8, device="cuda") % 3 == 0, -math.inf, sinks)
+    chosen = ops.int4_attention_backend(dtype, D)
+    for backend in {chosen, "simt"} | ({"mma"} if chosen == "tcgen05" else set()):
+        for splits in (1, 3, None):
+            attend = lambda s: ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, sinks=s, num_splits=splits, backend=backend)
+            without, with_sinks, got = attend(None), attend(sinks), attend(some)
+            assert not without[:10].any() and not without[110].any()
+            # (none of these heads' sums holds another term: the same operations, but for a factor of 1)
+            none = some.isinf()
+            assert torch.equal(got[:, none], without[:, none]) and torch.equal(got[:, ~none], with_sinks[:, ~none]), (backend, splits)

@@ -512,9 +512,9 @@ __global__ void __launch_bounds__(SIMT_THREADS) int4_attend_kernel(Int4Params p)
     const size_t row = (size_t)t * p.H + h0 + h;
     float m = ml[h][0], l = ml[h][1], a = 1.f;
     if (p.splits == 1 && p.sinks != nullptr) {
-      const float sink = p.sinks[h0 + h], top = fmaxf(m, sink);
-      a = m == -INFINITY ? 0.f : exp2f((m - top) * LOG2E);
-      l = l * a + exp2f((sink - top) * LOG2E);
+      const float sink = p.sinks[h0 + h], top = fmaxf(m, sink), from = top == -INFINITY ? 0.f : top;          // (neither keys nor a sink)
+      a = exp2f((m - from) * LOG2E);
+      l = l * a + exp2f((sink - from) * LOG2E);
     }
     for (int d = tid; d < D; d += SIMT_THREADS) {
       float sum = 0.f;

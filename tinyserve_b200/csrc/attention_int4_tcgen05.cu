@@ -529,9 +529,9 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         float alpha = 1.f;
         if (p.sinks && valid) {       // (log2 domain, like the running maximum; O is scaled on its way out)
           const float sk = p.sinks[kvh * G + g0 + gg] * LOG2E;
-          const float m_new = fmaxf(m, sk);
-          alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
-          l = l * alpha + exp2f(sk - m_new + P_UP);
+          const float top = fmaxf(m, sk), from = top == -INFINITY ? 0.f : top;          // (neither keys nor a sink)
+          alpha = exp2f(m - from);
+          l = l * alpha + exp2f(sk - from + P_UP);
         }
         const float inv = l == 0.f ? 0.f : alpha / l * power_of_two(v_exponent - HIGHEST);
         bf16* dst = p.out + ((size_t)(q_begin + qg + qi) * p.H + kvh * G + g0 + gg) * D;
