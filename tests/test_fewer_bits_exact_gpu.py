@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_fewer_bits_gpu import attention, batch
+from test_fewer_bits_gpu import attention, batch, values
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,79 @@ def test_a_sink_of_minus_infinity_is_none(dtype, D):
             # (none of these heads' sums holds another term: the same operations, but for a factor of 1)
             none = some.isinf()
             assert torch.equal(got[:, none], without[:, none]) and torch.equal(got[:, ~none], with_sinks[:, ~none]), (backend, splits)
+
+
+def dense(ctx, view, cache):
+    """What the cached rows of every request stand for, in 64 bits."""
+    x = values(cache).transpose(1, 2).flatten(0, 1)
+    kv, page = ctx.kv_lens.tolist(), view.page_size
+    at = [view.block_table[b].long()[torch.arange(m) // page] * page + (torch.arange(m) % page).cuda() for b, m in enumerate(kv)]
+    return [x[a] for a in at]
+
+
+def scale_row(view, cache, b, j, by):
+    """Key j of request b times a power of two."""
+    page = int(view.block_table[b, j // view.page_size])
+    cache.pairs[page, :, j % view.page_size] = (cache.pairs[page, :, j % view.page_size].double() * by).bfloat16()
+
+
+# how much larger than the other values (and keys) a row may be: the kernel for long portions has one range of half precision for all
+# values that a block reads, the others one for every row and what it sees
+LARGER = {"mma": (2.0 ** 12, 2.0 ** 20, 2.0 ** 40, 2.0 ** 90), "simt": (2.0 ** 20, 2.0 ** 90), "tcgen05": (2.0 ** 12, 2.0 ** 20)}
+
+
+@pytest.mark.parametrize("backend", sorted(LARGER))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[(1, 1000), (3, 300), (1, 40)], [(1, 9000)] * 2, [(40, 700), (2, 64)]])
+@pytest.mark.parametrize("where", [0, 37, -1])
+def test_a_huge_value_of_no_weight(backend, D, lengths, where):
+    """A key that every query gives a probability of nothing, with values far larger than the others': the others keep their bits."""
+    from tinyserve_b200.kernels import ops
+    ctx, view, kc, vc, _, _ = batch(lengths, 2, D, 16, torch.bfloat16)
+    q = queries(ctx.num_tokens, 8, D).abs()
+    for b, (n, m) in enumerate(lengths):
+        j = where % m
+        page = int(view.block_table[b, j // 16])
+        kc.codes[page, :, j % 16] = 0
+        kc.pairs[page, :, j % 16] = torch.tensor([0.0, -16.0], dtype=torch.bfloat16, device="cuda")          # scores of -16 sum |q| / sqrt(D): below -70
+    for by in LARGER[backend]:
+        pairs = vc.pairs.clone()
+        for b, (n, m) in enumerate(lengths):
+            scale_row(view, vc, b, where % m, by)
+        ks, vs = dense(ctx, view, kc), dense(ctx, view, vc)
+        want, _, _ = attention(q, lengths, ks, vs, D ** -0.5)
+        out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, backend=backend)
+        vc.pairs.copy_(pairs)
+        at = 0
+        for n, m in lengths:
+            rows = slice(at, at + n)
+            at += n
+            rounding = (want[rows].bfloat16().double() - want[rows]).norm()
+            assert (out[rows].double() - want[rows]).norm() <= AS_EXACT_AS_ITS_ROUNDING * rounding, (by, n, m)
+
+
+@pytest.mark.parametrize("backend", sorted(LARGER))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[(3, 300), (2, 33)], [(40, 700), (4, 40)], [(130, 200)]])
+@pytest.mark.parametrize("window", [0, 7])
+def test_a_huge_key_that_only_later_queries_see(backend, D, lengths, window):
+    """The last key of every request, and its value, are far larger than the others: the queries before it give what they gave."""
+    from tinyserve_b200.kernels import ops
+    ctx, view, kc, vc, _, _ = batch(lengths, 2, D, 16, torch.bfloat16)
+    q = queries(ctx.num_tokens, 8, D)
+    attend = lambda: ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, window, backend=backend)
+    earlier = torch.cat([torch.arange(n) < n - 1 for n, _ in lengths]).cuda()
+    clean = attend()[earlier]
+    want, _, _ = attention(q, lengths, dense(ctx, view, kc), dense(ctx, view, vc), D ** -0.5, window)
+    want = want[earlier]
+    rounding = (want.bfloat16().double() - want).norm()
+    assert (clean.double() - want).norm() <= AS_EXACT_AS_ITS_ROUNDING * rounding
+    for by in LARGER[backend]:
+        pairs = kc.pairs.clone(), vc.pairs.clone()
+        for b, (_, m) in enumerate(lengths):
+            scale_row(view, kc, b, m - 1, by)
+            scale_row(view, vc, b, m - 1, by)
+        out = attend()[earlier]
+        kc.pairs.copy_(pairs[0])
+        vc.pairs.copy_(pairs[1])
+        assert (out.double() - want).norm() <= AS_EXACT_AS_ITS_ROUNDING * rounding, by

@@ -574,8 +574,9 @@ __global__ void int4_combine_kernel(Int4Params p) {
 //      16 + c in half precision, one shift and one AND-OR for two of them.
 //   Scales and zeros are per key, so they stay outside: with a pair (s, z) of the key, q.k = s (q.c) + z sum(q); for the values, with p' =
 //   half(p s), sum p v = sum p' (c - 8) + sum p (z + 8 s), and sum p' (c - 8) = sum p' (16 + c) - 24 sum p', which is one more MMA, with
-//   ones for V, so that the 24 cancels whatever p' was rounded to.  A power of two for each warp keeps p' within half precision: it follows the
-//   largest scale so far, as the maximum follows the scores.  (64 requests of 2,000 to 8,192 keys, relative error of the output, of which its
+//   ones for V, so that the 24 cancels whatever p' was rounded to.  A factor for each column keeps p' within half precision: it follows the column's
+//   largest p s so far, as the maximum follows the scores.  (Not the largest s: a key that has no weight, or that the column does not see, must not
+//   push the others out of the format's range, whatever its values are.)  (64 requests of 2,000 to 8,192 keys, relative error of the output, of which its
 //   own rounding makes 1.7e-3: with p' in bfloat16 2.3e-3, around code 0 instead of 8 3.3e-3.)
 // Values of 2^110 and more may overflow these sums, as probabilities reach 2^8 in them.
 // 64 requests of 2,000 to 8,192 keys, 32 heads of 128 on 8 (366 MB): 89 us, 4.1 TB/s; fetching alone takes 62.  The integer pipe is busiest (two thirds of its
@@ -619,6 +620,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // four codes of a word as bytes: of columns 0, 4, 1, 5 and, shifted, 2, 6, 3, 7
 __device__ __forceinline__ uint32_t codes4(uint32_t word) { return word & 0x0f0f0f0fu; }
 // (the first MMA of a chain adds to zeros that are no registers)
@@ -650,6 +656,7 @@ __device__ __forceinline__ uint32_t codes2(uint32_t word) {
 // Where a running maximum starts: below every score, and finite, so that nothing subtracts infinities.  It moves only when a score passes it by
 // more than SLACK (a power of two): probabilities up to 2^SLACK do no harm in 32-bit sums, and most steps then rescale nothing.
 constexpr float LOWEST = -3e38f, SLACK = 8.f;
+constexpr float UNIT = 6.f, MAX_UNIT = 112.f;                      // 2^(UNIT + SLACK) is within half precision; p <= 2^SLACK times 2^MAX_UNIT within 32 bits
 constexpr uint32_t ONES = 0x3c003c00u;                             // two in half precision
 // Row r of the 16 that an MMA reads of K is this key of the group: thread t of a quad then finds its columns of V^T (rows 2t, 2t + 1, 2t + 8,
 // 2t + 9) in keys t, t + 4, t + 8, t + 12, and the eight lanes whose reads of K meet read neighbouring keys' halves of a bank line
@@ -821,8 +828,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
 
   float o[D / 16][NT][4], m[NT][2], ps[NT][4];                     // ps: sum p' of columns 2t and 2t + 1 (and the same again)
   F2 l[NT], z[NT];
-  // the values' scales are multiplied by `unit`, which brings the largest so far to 2^6 .. 2^7; one of `bound` and more moves it
-  float unit = 1.f, bound = 0.f;
+  // a column's largest log2(p s) + m so far, which moves as m does, and the factor that brings p s there to 2^UNIT
+  float top_v[NT][2], unit[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -831,7 +838,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) ps[nt][e] = 0.f;
-    m[nt][0] = m[nt][1] = LOWEST;
+    m[nt][0] = m[nt][1] = top_v[nt][0] = top_v[nt][1] = LOWEST;
+    unit[nt][0] = unit[nt][1] = 1.f;
     l[nt] = z[nt] = f2(0.f, 0.f);
   }
 
@@ -943,41 +951,44 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
             }
         }
     }
-    float widest = fmaxf(fmaxf(fabsf(vscale[0][0]), fabsf(vscale[0][1])), fmaxf(fabsf(vscale[1][0]), fabsf(vscale[1][1])));
-    bool moved = widest >= bound && widest > 0.f;
+    // (every key's score against the largest scale of the four: seldom more than a step's own, and the step that moves looks closely)
+    const float widest = lg2(fmaxf(fmaxf(fabsf(vscale[0][0]), fabsf(vscale[0][1])), fmaxf(fabsf(vscale[1][0]), fabsf(vscale[1][1]))));
+    bool moved = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         top[nt][i] = fmaxf(fmaxf(sc[0][nt][i], sc[0][nt][2 + i]), fmaxf(sc[1][nt][i], sc[1][nt][2 + i]));
-        moved |= top[nt][i] > m[nt][i] + SLACK;
+        moved |= top[nt][i] > m[nt][i] + SLACK || top[nt][i] + widest > top_v[nt][i] + SLACK;
       }
     if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, d));
-      float shrink = 1.f;
-      if (widest >= bound && widest > 0.f) {
-        const int e = min(max((int)(__float_as_uint(widest) >> 23) - 127, -100), 127);
-        const float to = __uint_as_float((uint32_t)(6 - e + 127) << 23);
-        shrink = bound > 0.f ? to / unit : 0.f;          // (nothing was added before the first)
-        unit = to;
-        bound = __uint_as_float((uint32_t)(e + 1 + 127) << 23);
-      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          float wide = LOWEST;
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
-          const float above = fmaxf(top[nt][i], m[nt][i]);
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) wide = fmaxf(wide, sc[kb][nt][2 * h + i] + lg2(fabsf(vscale[kb][h])));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
+            wide = fmaxf(wide, __shfl_xor_sync(0xffffffffu, wide, d));
+          }
+          const float above = fmaxf(top[nt][i], m[nt][i]), above_v = fmaxf(wide, top_v[nt][i]);
+          // (where there was no scale but 0, o is 0)
+          const float was = fminf(m[nt][i] - top_v[nt][i] + UNIT, MAX_UNIT), is = fminf(above - above_v + UNIT, MAX_UNIT);
+          const float f_v = ex2(m[nt][i] - above + (is - was));
           f[i] = ex2(m[nt][i] - above);
           m[nt][i] = above;
-          const float both = f[i] * shrink;
-          ps[nt][i] *= both;
-          ps[nt][2 + i] *= both;
+          top_v[nt][i] = above_v;
+          unit[nt][i] = ex2(is);
+          ps[nt][i] *= f_v;
+          ps[nt][2 + i] *= f_v;
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= both; o[mt][nt][2 + i] *= both; }
+          for (int mt = 0; mt < D / 16; ++mt) { o[mt][nt][i] *= f_v; o[mt][nt][2 + i] *= f_v; }
         }
         l[nt] = f2_mul(l[nt], f2(f[0], f[1]));
         z[nt] = f2_mul(z[nt], f2(f[0], f[1]));
@@ -996,8 +1007,7 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
           const F2 pr = f2(ex2(x0), ex2(x1));
           l[nt] = f2_add(l[nt], pr);
           z[nt] = f2_fma(pr, f2(vzero[kb][h], vzero[kb][h]), z[nt]);
-          const float scaled = vscale[kb][h] * unit;
-          f2_out(f2_mul(pr, f2(scaled, scaled)), x0, x1);
+          f2_out(f2_mul(f2_mul(pr, f2(unit[nt][0], unit[nt][1])), f2(vscale[kb][h], vscale[kb][h])), x0, x1);
           const __half2 two = __floats2half2_rn(x0, x1);
           const uint32_t bits = *reinterpret_cast<const uint32_t*>(&two);
           pb[nt][h] = transposed(bits);
@@ -1051,7 +1061,6 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
   float* sm_ml = sm_o + WARPS * C::NC * MERGE_ROW;             // [warp][column][3]
   float* box = reinterpret_cast<float*>(work + C::WORK_BYTES);     // (its own memory: a peer may send while this block still reads its ring)
   const int per_rank = (C::NC + p.splits - 1) / p.splits;
-  const float back = 1.f / unit;
   auto send = [](uint32_t at, uint32_t rank, float v) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
@@ -1070,6 +1079,7 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
         zs[i] += __shfl_xor_sync(0xffffffffu, zs[i], d);
       }
       const int c = nt * 8 + 2 * t + i;
+      const float back = 1.f / unit[nt][i];
       if (g == 0) {
         sm_ml[(warp * C::NC + c) * 3] = m[nt][i];
         sm_ml[(warp * C::NC + c) * 3 + 1] = ls[i];

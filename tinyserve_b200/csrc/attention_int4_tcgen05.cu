@@ -12,7 +12,8 @@
 // in bfloat16 4.4e-3, so 1.7e-3, which is that rounding alone; exact codes, with scales and zeros applied to every score and probability, came
 // to 2.3e-3 and took 271 us instead of 131).  Its range is short, so powers of two keep everything inside: one a row for the queries, one a tile for the keys,
 // and one for the values of all tiles so far, with which the sums in tensor memory are rescaled when it grows.  (From the
-// pairs of the tile at hand: a look at all of a block's pairs beforehand took 30 us.)  What lies 2^-26 below the largest loses bits.
+// pairs of the tile at hand: a look at all of a block's pairs beforehand took 30 us.)  What lies 2^-26 below the largest that the
+// block reads, seen by a row or not, loses bits.
 //
 // That portion takes 131 us, 0.79 PFLOP/s.  What bounds it is the chain of a query tile's steps: 2,000 cycles from its scores to its last
 // probabilities, 900 until the issuing thread has put P V and the next scores in the pipe, 600 until these are seen, with the other tile's chain beside
