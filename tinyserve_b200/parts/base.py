@@ -99,9 +99,6 @@ class CacheSpec:
         if len(set(names)) != len(names) or any(t.heads <= 0 or t.width <= 0 for t in self.tensors):
             raise ValueError(f"cache tensors need distinct names and positive sizes: {self.tensors}")
 
-    def elements_per_token(self) -> int:
-        return sum(t.heads * t.width for t in self.tensors)
-
     def bytes_per_token(self, element_size: int) -> int:
         return sum(t.bytes_per_token(element_size) for t in self.tensors)
 
