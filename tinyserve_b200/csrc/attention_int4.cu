@@ -7,7 +7,7 @@
 // 32-bit number, gets a pair of NaN: whoever attends to it gets NaN, as from a cache of whole numbers.
 //
 // Eight codes fill a 32-bit word: even columns in its lower half, odd ones in its upper half, the first in the lowest bits.
-// One shift and one AND-OR then make a pair of neighbouring columns as two bfloat16 (see `codes2` in the kernels below).
+// One shift and one AND-OR then make a pair of neighbouring columns as two numbers in half precision (see `codes2` below).
 // Codes [page, kv head, slot, D / 2] bytes, pairs [page, kv head, slot, 2]: one head's share of a page is one run of memory, 68 bytes
 // a token for heads of 128 where bfloat16 takes 256.
 #include <cuda_fp16.h>
@@ -586,7 +586,7 @@ __global__ void int4_combine_kernel(Int4Params p) {
 constexpr int STEP = 32, RING = 3;
 constexpr int ROW_BYTES = D / 2, KW = D / 32, UNITS = D / 32;      // words of K a thread holds of a row; 16-bit units of V
 constexpr int STAGE_BYTES = 2 * STEP * ROW_BYTES + 2 * STEP * 4;   // codes of K and V, pairs of K and V
-constexpr float MIDDLE = 8.f, ABOVE = 16.f + MIDDLE;               // of the codes; what a code's bfloat16 is above c - MIDDLE
+constexpr float MIDDLE = 8.f, ABOVE = 16.f + MIDDLE;               // of the codes; what a code's number 16 + c is above c - MIDDLE
 constexpr int MERGE_ROW = D + 4;                                   // floats of a column's partial result: the four columns of a quad meet other banks
 
 template <int NT, int WARPS> struct MmaCfg {

@@ -106,7 +106,7 @@ __device__ __forceinline__ uint32_t values2(uint32_t word, __half2 scale, __half
 // instruction descriptor of kind::f16 with half precision on both sides (make_idesc has bfloat16)
 __host__ __device__ constexpr uint32_t idesc_half(int M, int N, bool b_mn_major) { return make_idesc(M, N, b_mn_major) & ~((1u << 7) | (1u << 10)); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
-// the exponent that the largest magnitude (as bits) has; 0 and what is not finite: that of 2^14, which nothing is scaled for
+// the exponent that the largest magnitude (as bits) has; for 0 and what is not finite HIGHEST, so that nothing is scaled for them
 __device__ __forceinline__ int exponent_of(uint32_t bits) { return bits == 0 || bits >= 0x7f800000u ? HIGHEST : max((int)(bits >> 23) - 127, -100); }
 __device__ __forceinline__ float pair_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pair_zero(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
@@ -394,7 +394,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       float m = -INFINITY, l = 0.f;
       bool ok = mbar_wait(smem_u32(q_full), 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-      // this thread's row of queries in half precision, its largest element at 2^14 .. 2^15 (rows behind the last are whatever lay there)
+      // this thread's row of queries in half precision, its largest element at 2^12 .. 2^13 (rows behind the last are whatever lay there)
       char* mine = Qs + g * Q_BYTES + r * 128;
       auto unit = [&](int u) { return reinterpret_cast<uint4*>(mine + (u / 8) * CHUNK_BYTES + (((u % 8) ^ (r & 7)) << 4)); };
       uint32_t top = 0;
