@@ -30,8 +30,9 @@ class EngineConfig:
     # debug pass: check every index buffer of every step on the host before it is uploaded, and
     # again on the device before the kernels run (the stand-in for a memory checker)
     check_indices: bool = None
-    # "auto": the matrices that only products read are held in ``dtype``; "int8": in 8-bit integers with a scale per output channel
-    # (the rows they meet are brought to 8 bits too, a scale per token)
+    # "auto": all weights are held in ``dtype``; "int8": the projections of attention and of dense feed-forwards in 8-bit integers with a
+    # scale per output channel (the rows they meet are brought to 8 bits too, a scale per token).  Everything else stays in ``dtype``:
+    # embeddings and the vocabulary projection, experts and their routers, latent and linear attention.
     weight_dtype: str = "auto"
     # "auto": keys and values are cached in ``dtype``; "int4": in 4 bits with a scale and a zero per head of a token
     kv_cache_dtype: str = "auto"

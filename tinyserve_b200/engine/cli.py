@@ -42,7 +42,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--no-cuda-graphs", action="store_true")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
-    ap.add_argument("--weight-dtype", choices=WEIGHT_DTYPES, default="auto", help="int8: products in 8-bit integers, a scale per output channel and per token")
+    ap.add_argument("--weight-dtype", choices=WEIGHT_DTYPES, default="auto", help="int8: the projections of attention and of dense feed-forwards in 8-bit integers, a scale per output channel and per token")
     ap.add_argument("--kv-cache-dtype", choices=KV_CACHE_DTYPES, default="auto", help="int4: keys and values in 4 bits, a scale and a zero per head of a token")
     ap.add_argument("--block-size", type=int, default=0, help="tokens per cache page (0: 64 from 2,048 tokens of context on, else 16)")
     ap.add_argument("--num-blocks", type=int, default=0, help="cache pages per group (0: from memory)")

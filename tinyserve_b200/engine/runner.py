@@ -24,7 +24,7 @@ from ..cache.manager import CacheError, CacheManager, GroupSpec
 from ..config.engine_config import EngineConfig
 from ..config.registry import load_model_config
 from ..kernels import ops
-from ..weights import fill_random_on_device, load_weights
+from ..weights import check_weight_dtype, fill_random_on_device, load_weights
 from ..parts.model import build_model
 from .batch import GroupView, StepContext, StepEntry
 
@@ -92,7 +92,8 @@ class ModelRunner:
         self.kernel_launches = 0
         self.last_upload_bytes = 0
         if verbose:
-            print(f"[tinyserve_b200] weights {self.weight_bytes / 2**30:.2f} GiB, "
+            in8 = f" ({100 * check_weight_dtype(self.model, cfg.weight_dtype):.0f} % of the parameters in 8 bits)" if cfg.weight_dtype == "int8" else ""
+            print(f"[tinyserve_b200] weights {self.weight_bytes / 2**30:.2f} GiB{in8}, "
                   f"{self.num_pages - 1} pages of {self.page_size} tokens per cache group "
                   f"({len(groups)} group(s))", flush=True)
 

@@ -15,6 +15,7 @@ serve.py:1397-1403).  ``lm_head.weight`` in a checkpoint of a tied model is igno
 as it has no home there either (serve.py:1385-1387)."""
 from __future__ import annotations
 
+import math
 import os
 import re
 from dataclasses import dataclass
@@ -128,6 +129,16 @@ def check_checkpoint(model, index, duplicates=()):
     return expected
 
 
+def check_weight_dtype(model, weight_dtype: str) -> float:
+    """The share of the model's parameters that ``weight_dtype`` changes; one that changes nothing is refused."""
+    sizes = [(math.prod(spec.shape), spec.int8) for part in model.named_parts() for spec in part.param_specs().values()]
+    share = sum(n for n, int8 in sizes if int8) / max(1, sum(n for n, _ in sizes)) if weight_dtype == "int8" else 0.0
+    if weight_dtype == "int8" and share == 0.0:
+        raise ValueError("no matrix of the model can be held in 8 bits: only the projections of attention and of dense feed-forwards are, "
+                         "and it has none")
+    return share
+
+
 def held(spec: ParamSpec, tensor, weight_dtype: str):
     """A parameter as the engine holds it: with ``weight_dtype`` "int8" the matrices that only products read are brought to 8
     bits, row by row.  Returns (what the part binds, its bytes)."""
@@ -139,6 +150,7 @@ def held(spec: ParamSpec, tensor, weight_dtype: str):
 
 def load_weights(model, model_dir: str, dtype: torch.dtype, device, weight_dtype: str = "auto") -> int:
     """Fill every part of ``model`` from ``model_dir``; returns the bytes placed.  ``weight_dtype``: see ``held``."""
+    check_weight_dtype(model, weight_dtype)
     index, duplicates = _index_folder(model_dir)
     expected = check_checkpoint(model, index, duplicates)
     by_param = {}

@@ -13,7 +13,7 @@ import os
 import torch
 from safetensors.torch import save_file
 
-from .loader import expected_tensors, held
+from .loader import check_weight_dtype, expected_tensors, held
 
 _STORE = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
@@ -68,6 +68,7 @@ def write_random_model(config, out_dir: str, seed: int = 0, store_dtype: str = "
 
 def fill_random_on_device(model, dtype: torch.dtype, device, seed: int = 0, weight_dtype: str = "auto") -> int:
     """Give every part of ``model`` random tensors made on ``device``; returns bytes.  ``weight_dtype``: as for ``load_weights``."""
+    check_weight_dtype(model, weight_dtype)
     gen = torch.Generator(device=device)
     gen.manual_seed(int(seed))
     total = 0
