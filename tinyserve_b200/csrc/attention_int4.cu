@@ -579,7 +579,7 @@ __global__ void int4_combine_kernel(Int4Params p) {
 //   push the others out of the format's range, whatever its values are.)  (64 requests of 2,000 to 8,192 keys, relative error of the output, of which its
 //   own rounding makes 1.7e-3: with p' in bfloat16 2.3e-3, around code 0 instead of 8 3.3e-3.)
 // Values of 2^110 and more may overflow these sums, as probabilities reach 2^8 in them.
-// 64 requests of 2,000 to 8,192 keys, 32 heads of 128 on 8 (366 MB): 89 us, 4.1 TB/s; fetching alone takes 62.  The integer pipe is busiest (two thirds of its
+// 64 requests of 2,000 to 8,192 keys, 32 heads of 128 on 8 (366 MB): 90 us, 4.1 TB/s; fetching alone takes 62.  The integer pipe is busiest (two thirds of its
 // rate while a block walks), then the fixed 5 us of a block, of which an SM holds two.  Requests in the order of their numbers instead of by length:
 // 108 us, for the blocks that come last run alone.  Shifts as multiplications on the other pipe 91 and 99 us, three blocks an SM
 // with 80 registers a thread 123.
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
   __syncthreads();
   pdl_trigger();
   // Beside portions (`most`) too: that this kernel's inputs were complete when the portions' kernel began does not make them visible here; only
-  // this grid's own wait does.  (64 requests over 800 keys behind a portion of 448: 58 us; 47 without the wait.)
+  // this grid's own wait does.  (64 requests over 800 keys beside a portion of 448: 60 us; 47 without the wait.)
   pdl_wait();
   const int G = p.H / p.Hkv, split = blockIdx.x, col_tiles = gridDim.y / p.Hkv;
   const int kvh = blockIdx.y / col_tiles, c0 = blockIdx.y % col_tiles * C::NC;
