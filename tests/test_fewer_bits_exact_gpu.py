@@ -70,9 +70,8 @@ def scale_row(view, cache, b, j, by):
     cache.pairs[page, :, j % view.page_size] = (cache.pairs[page, :, j % view.page_size].double() * by).bfloat16()
 
 
-# how much larger than the other values (and keys) a row may be: the kernel for long portions has one range of half precision for all
-# values that a block reads, the others one for every row and what it sees
-LARGER = {"mma": (2.0 ** 12, 2.0 ** 20, 2.0 ** 40, 2.0 ** 90), "simt": (2.0 ** 20, 2.0 ** 90), "tcgen05": (2.0 ** 12, 2.0 ** 20)}
+# how much larger than the other values (and keys) a row may be: below and above what half precision holds beside them
+LARGER = {backend: (2.0 ** 12, 2.0 ** 20, 2.0 ** 23, 2.0 ** 25, 2.0 ** 40, 2.0 ** 90) for backend in ("mma", "simt", "tcgen05")}
 
 
 @pytest.mark.parametrize("backend", sorted(LARGER))
@@ -130,3 +129,35 @@ def test_a_huge_key_that_only_later_queries_see(backend, D, lengths, window):
         kc.pairs.copy_(pairs[0])
         vc.pairs.copy_(pairs[1])
         assert (out.double() - want).norm() <= AS_EXACT_AS_ITS_ROUNDING * rounding, by
+
+
+@pytest.mark.parametrize("D,H,Hkv", [(64, 14, 2), (128, 8, 2), (128, 3, 3), (64, 130, 1)])
+@pytest.mark.parametrize("lengths", [[(200, 700), (64, 64), (1, 90)], [(130, 100)], [(17, 3000), (40, 41)]])
+def test_portions_whose_keys_and_values_are_far_apart(D, H, Hkv, lengths):
+    """Values from 2^-40 to 2^40 of what they were, and some keys at 2^-30: with windows, sinks and soft caps, rows without keys, NaN that some rows see."""
+    from tinyserve_b200.kernels import ops
+    ctx, view, kc, vc, _, _ = batch(lengths, Hkv, D, 16, torch.bfloat16)
+    g = torch.Generator().manual_seed(D)
+    by = torch.randint(-40, 41, vc.pairs.shape[:3], generator=g).cuda()
+    vc.pairs.copy_(torch.ldexp(vc.pairs.float(), by[..., None]).bfloat16())
+    kc.pairs.copy_(torch.ldexp(kc.pairs.float(), torch.where(by % 7 == 0, -30, 0)[..., None]).bfloat16())
+    q = queries(ctx.num_tokens, H, D)
+    sinks = torch.randn(H, generator=g).cuda()
+    for window, softcap, sink in ((0, 0.0, None), (50, 0.0, sinks), (0, 2.0, None), (7, 1e5, sinks)):
+        want, _, _ = attention(q, lengths, dense(ctx, view, kc), dense(ctx, view, vc), D ** -0.5, window, softcap, sink)
+        out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5, window, softcap=softcap, sinks=sink)
+        # (32 bits inside: every element is off by its rounding, and by the sums' share of the largest term)
+        rounding = (want.bfloat16().double() - want).norm(dim=(1, 2))
+        assert ((out.double() - want).norm(dim=(1, 2)) <= AS_EXACT_AS_ITS_ROUNDING * rounding + 2.0 ** -16 * want.norm(dim=(1, 2))).all(), (window, softcap)
+    clean = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5)
+    n, m = lengths[0]
+    j = min(m, n) // 2 + max(m - n, 0)                       # the queries of the first request from here on see it
+    for cache in (kc, vc):
+        keep = cache.pairs.clone()
+        cache.pairs[int(view.block_table[0, j // 16]), :, j % 16] = math.nan
+        out = ops.paged_attention(q, kc, vc, view, ctx, D ** -0.5)
+        cache.pairs.copy_(keep)
+        sees = torch.arange(ctx.num_tokens, device="cuda") + (m - n) >= j
+        sees[n:] = False
+        assert out[sees].isnan().all() and torch.equal(out[~sees], clean[~sees])
+    assert ops.int4_attention_error(D) == 0

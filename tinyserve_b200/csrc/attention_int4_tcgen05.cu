@@ -12,10 +12,12 @@
 // in bfloat16 4.4e-3, so 1.7e-3, which is that rounding alone; exact codes, with scales and zeros applied to every score and probability, came
 // to 2.3e-3 and took 271 us instead of 131).  Its range is short, so powers of two keep everything inside: one a row for the queries, one a tile for the keys,
 // and one for the values of all tiles so far, with which the sums in tensor memory are rescaled when it grows.  (From the
-// pairs of the tile at hand: a look at all of a block's pairs beforehand took 30 us.)  What lies 2^-26 below the largest that the
-// block reads, seen by a row or not, loses bits.
+// pairs of the tile at hand: a look at all of a block's pairs beforehand took 30 us.)  Half precision holds 2^26 that way: where the
+// keys of a tile or the values of a block lie further apart than 2^24, whoever sees them, the makers say so and the block's rows are made again in 32
+// bits, by one warp each.  (That takes 35 ms for the portion above, and no model's cache is like that; without it, a key that only later queries see
+// could take the bits of the others' values.  Looking for it costs 1 us of 131.)
 //
-// That portion takes 131 us, 0.79 PFLOP/s.  What bounds it is the chain of a query tile's steps: 2,000 cycles from its scores to its last
+// That portion takes 132 us, 0.78 PFLOP/s.  What bounds it is the chain of a query tile's steps: 2,000 cycles from its scores to its last
 // probabilities, 900 until the issuing thread has put P V and the next scores in the pipe, 600 until these are seen, with the other tile's chain beside
 // it (with one matrix instruction a product, tiles made twice only and hardly any softmax still 88 us).  Then come the start of a block (22 us for
 // 256 blocks of one tile) and the makers (11 us).  The subtraction of 1024 that an earlier form of the makers had cost 10 us; pairs of 32-bit operations in
@@ -110,15 +112,82 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 __device__ __forceinline__ int exponent_of(uint32_t bits) { return bits == 0 || bits >= 0x7f800000u ? HIGHEST : max((int)(bits >> 23) - 127, -100); }
 __device__ __forceinline__ float pair_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pair_zero(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+constexpr int WIDEST = 24;                   // powers of two between the largest and the least magnitude that half precision is trusted with
+// `least`: a magnitude but 0, as bits, less one (so that 0, all ones, is never the least)
+__device__ __forceinline__ bool too_wide(int exponent, uint32_t least) { return exponent + 127 - (int)(least >> 23) > WIDEST; }
 __device__ __forceinline__ bool finite_pair(uint32_t pair) {
   return (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
+}
+
+// A row (query, head) by one warp in 32 bits, for the blocks whose keys or values are too far apart for half precision (see `wide`): what a row does
+// not see, or gives no weight, must not cost the others their bits.  Lanes are 32 keys for the scores, and D / 32 columns each for their sum.
+__device__ __noinline__ void whole_row(const Params& p, const char* q_tile, int r, float q_down, const int* bt, int kvh, int from, int pos, float sink, bf16* out, int lane) {
+  constexpr int W = D / 8, SHARE = 32 / W, CPL = D / 32;          // words of a row, lanes of a word, columns of a lane
+  const uint32_t* kc = reinterpret_cast<const uint32_t*>(p.kc);
+  const uint32_t* vc = reinterpret_cast<const uint32_t*>(p.vc);
+  auto unit = [&](int u) { return *reinterpret_cast<const uint4*>(q_tile + r * 128 + (u / 8) * CHUNK_BYTES + (((u % 8) ^ (r & 7)) << 4)); };
+  auto halves = [](uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); };
+  float o[CPL] = {}, m = -INFINITY, l = 0.f;
+  for (int j0 = from; j0 <= pos; j0 += 32) {
+    const int j = j0 + lane;
+    const bool seen = j <= pos;
+    int page = seen ? bt[j >> p.page_shift] : 0;
+    if ((unsigned)page >= (unsigned)p.num_pages) page = 0;          // (reported when the tile was made)
+    const size_t row = (((size_t)page * p.Hkv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1));
+    const uint32_t k_pair = seen ? p.kp[row] : 0u, v_pair = seen ? p.vp[row] : 0u;
+    float dot = 0.f, sum = 0.f;
+#pragma unroll 4
+    for (int u = 0; u < W; ++u) {
+      const uint4 q8 = unit(u);
+      const uint32_t w = seen ? kc[row * W + u] : 0u;
+      const uint32_t q2[4] = {q8.x, q8.y, q8.z, q8.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = halves(q2[e]);
+        dot = fmaf(x.x, (float)(int)(w >> (4 * e) & 15u) - 8.f, fmaf(x.y, (float)(int)(w >> (4 * e + 16) & 15u) - 8.f, dot));
+        sum += x.x + x.y;
+      }
+    }
+    const float ks = pair_scale(k_pair);
+    float s = fmaf(ks, dot * q_down, fmaf(8.f, ks, pair_zero(k_pair)) * (sum * q_down));
+    s = p.cap2 > 0.f ? p.cap2 * tanhf(s * p.cap_in) : s * p.scale_log2;
+    if (!finite_pair(k_pair) || !finite_pair(v_pair)) s = __int_as_float(0x7fc00000);
+    if (!seen) s = -INFINITY;
+    float top = s;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new, alpha = exp2f(m - base), weight = exp2f(s - base);
+    float total = weight;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    l = fmaf(l, alpha, total);
+    m = m_new;
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) o[e] *= alpha;
+    // (a key behind the row's last has weight 0, pair 0 and stands in page 0; a pair that is not finite made the weight a NaN, which l has)
+#pragma unroll 8
+    for (int k = 0; k < 32; ++k) {
+      const float w = __shfl_sync(0xffffffffu, weight, k);
+      const uint32_t pair = __shfl_sync(0xffffffffu, v_pair, k), word = vc[__shfl_sync(0xffffffffu, (unsigned long long)row, k) * W + lane / SHARE];
+      const float vs = finite_pair(pair) ? pair_scale(pair) : 0.f, vz = finite_pair(pair) ? pair_zero(pair) : 0.f;
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) {
+        const int i = lane % SHARE * CPL + e;
+        o[e] = fmaf(w, fmaf((float)(int)(word >> ((i >> 1) * 4 + (i & 1) * 16) & 15u), vs, vz), o[e]);
+      }
+    }
+  }
+  const float sink2 = sink * LOG2E, m_new = fmaxf(m, sink2), base = m_new == -INFINITY ? 0.f : m_new, alpha = exp2f(m - base);
+  l = fmaf(l, alpha, exp2f(sink2 - base));
+#pragma unroll
+  for (int e = 0; e < CPL; ++e) out[lane * CPL + e] = __float2bfloat16_rn(l == 0.f ? 0.f : o[e] * alpha / l);
 }
 
 // CAPPED: with a soft cap, whose code in the loop would cost the calls without one (2,048 queries over 4,096 keys 130.5 us, in one kernel
 // for both 133; with a cap 270)
 template <bool CAPPED>
 __global__ void __launch_bounds__(THREADS, 1)
-int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
+int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Params p) {
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* Qs = smem;                               // [GROUPS][Q_BYTES]
@@ -142,6 +211,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* largest = tmem_slot + 2;             // [2][8]: largest magnitudes of a tile's keys and values, by maker warp
   int2* exponents = reinterpret_cast<int2*>(largest + 16);       // [RANGES]
+  volatile int* wide = reinterpret_cast<volatile int*>(exponents + RANGES);      // a tile's keys, or the values so far, are too far apart for half precision
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -162,7 +232,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       for (int h = 0; h < P_PARTS; ++h) mbar_init(smem_u32(&p_full[g * P_PARTS + h]), 4);
       mbar_init(smem_u32(&o_ready[g]), 1);
     }
-    *abort_flag = 0;
+    *abort_flag = *wide = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {
@@ -325,7 +395,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       const float zero = pair_zero(pair), end = fmaf(15.f, pair_scale(pair), zero);
       return min(__float_as_uint(fmaxf(fabsf(zero), fabsf(end))), 0x7f7fffffu);
     };
-    uint32_t top_v = 0;          // of all tiles so far
+    uint32_t top_v = 0, least_v = ~0u;          // of all tiles so far: the block's largest, this thread's least
     bool ok = true;
     // the next tile's keys are on their way while this tile's values are made, and these while its keys are
     Where at_k = find(0);
@@ -346,7 +416,8 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       const Where next_k = find(t + 1);
       const bool good = finite_pair(k_pair) && finite_pair(v_pair);
       uint32_t* of_tile = largest + (t & 1) * 8;
-      const uint32_t k_of_warp = __reduce_max_sync(0xffffffffu, reach(k_pair)), v_of_warp = __reduce_max_sync(0xffffffffu, reach(v_pair));
+      const uint32_t k_reach = reach(k_pair), v_reach = reach(v_pair);
+      const uint32_t k_of_warp = __reduce_max_sync(0xffffffffu, k_reach), v_of_warp = __reduce_max_sync(0xffffffffu, v_reach);
       if (lane == 0) {
         of_tile[warp - MAKER_WARP0] = k_of_warp;
         of_tile[4 + warp - MAKER_WARP0] = v_of_warp;
@@ -358,6 +429,8 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
       if (!ok) break;
       top_v = max(top_v, max(max(of_tile[4], of_tile[5]), max(of_tile[6], of_tile[7])));
       const int k_exponent = exponent_of(max(max(of_tile[0], of_tile[1]), max(of_tile[2], of_tile[3]))), v_exponent = exponent_of(top_v);
+      least_v = min(least_v, v_reach - 1u);
+      if (too_wide(k_exponent, k_reach - 1u) || too_wide(v_exponent, least_v)) *wide = 1;          // (before the values are handed over)
       const float k_factor = power_of_two(HIGHEST - k_exponent), v_factor = power_of_two(HIGHEST - v_exponent);
       ok = room(&k_empty[t % K_STAGES], t / K_STAGES);
       if (!ok) break;
@@ -525,10 +598,21 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, Params p) {
         m = m_new;
       }
       if (ok) {
-        ok = mbar_wait(smem_u32(&o_ready[g]), (n_tiles - 1) & 1, abort_flag);
+        // (the values' barrier for what the makers say in `wide`)
+        ok = mbar_wait(smem_u32(&o_ready[g]), (n_tiles - 1) & 1, abort_flag) && mbar_wait(smem_u32(&v_full[(n_tiles - 1) % V_STAGES]), (n_tiles - 1) / V_STAGES & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
       }
-      if (ok) {
+      if (ok && *wide) {
+        // row by row
+        for (int i = 0; i < 32; ++i) {
+          const int at = __shfl_sync(0xffffffffu, pos, i), from = __shfl_sync(0xffffffffu, lo, i);
+          const int head = kvh * G + g0 + __shfl_sync(0xffffffffu, gg, i), token = q_begin + qg + __shfl_sync(0xffffffffu, qi, i);
+          const float q_down = __shfl_sync(0xffffffffu, down, i);
+          if (__shfl_sync(0xffffffffu, (int)valid, i))
+            whole_row(p, Qs + g * Q_BYTES, q4 * 32 + i, q_down, p.block_table + (size_t)b * p.table_stride, kvh, from, at,
+                      p.sinks != nullptr ? p.sinks[head] : -INFINITY, p.out + ((size_t)token * p.H + head) * D, lane);
+        }
+      } else if (ok) {
         tcgen05_fence_after();
         float alpha = 1.f;
         if (p.sinks && valid) {       // (log2 domain, like the running maximum; O is scaled on its way out)

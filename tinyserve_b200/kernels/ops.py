@@ -2751,9 +2751,8 @@ class Int4Pages:
     """One of the caches (keys or values) in 4 bits: ``codes`` uint8 [pages, kv heads, slots, D / 2] and ``pairs`` bfloat16 [pages, kv
     heads, slots, 2], both contiguous.  A head of a token with pair (scale, zero) stands for zero + code * scale; eight codes fill a
     32-bit word, even columns in its lower half, odd ones in its upper half, the first in the lowest bits.  ``int4_kvwrite`` fills it.
-    Attention sums values in 32 bits before it divides: magnitudes up to 2^100 are safe.  Prompt portions in bfloat16 with heads of 64 or 128
-    hold the values of a request in half precision around one power of two, keys likewise 128 at a time: those that lie more than
-    2^24 below the largest of them lose bits.  The other kernels have no such limit."""
+    Attention sums values in 32 bits before it divides: magnitudes up to 2^100 are safe.  (Prompt portions in bfloat16 with heads of 64 or 128
+    become some hundred times slower where the values of a request, or 128 keys in a row, lie more than 2^24 apart.)"""
     __slots__ = ("codes", "pairs", "shape")
 
     def __init__(self, codes, pairs):
