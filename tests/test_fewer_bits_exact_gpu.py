@@ -161,3 +161,25 @@ def test_portions_whose_keys_and_values_are_far_apart(D, H, Hkv, lengths):
         sees[n:] = False
         assert out[sees].isnan().all() and torch.equal(out[~sees], clean[~sees])
     assert ops.int4_attention_error(D) == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", range(8, 30))
+@pytest.mark.parametrize("step", [1, 2, 7, 8, 16])
+def test_maxima_a_few_steps_of_32_bits_apart(D, power, step):
+    """Scores of 1.5 2^power in the first tile of keys, a few powers of two above them in the next: whatever 32 bits make of the difference, all
+    values are the same, and so is the result."""
+    from tinyserve_b200.kernels import ops
+    n, m, page = 32, 256, 16
+    ctx, view, kc, vc, _, _ = batch([(n, m)], 1, D, page, torch.bfloat16)
+    for cache, values_of in ((kc, None), (vc, 3.0)):
+        cache.codes.zero_()
+        cache.pairs[..., 0], cache.pairs[..., 1] = 1.0, values_of or 0.0
+    for j in range(m):
+        word = 1 | j // 128 << 16          # column 0: 1; column 1: 0 in the first tile, 1 in the second
+        kc.codes[int(view.block_table[0, j // page]), 0, j % page, :4] = torch.tensor([word & 255, 0, word >> 16, 0], dtype=torch.uint8)
+    q = torch.zeros(n, 4, D, device="cuda", dtype=torch.bfloat16)
+    q[..., 0], q[..., 1] = 1.5 * 2.0 ** power, step
+    for backend in ("tcgen05", "mma", "simt"):
+        out = ops.paged_attention(q, kc, vc, view, ctx, math.log(2.0), backend=backend)
+        assert (out.float() - 3.0).abs().max() <= 3.0 * 2.0 ** -8, backend

@@ -64,6 +64,9 @@ constexpr int W4 = D / 32;                   // 16-byte pieces of a row of codes
 constexpr size_t SMEM = 1024 + GROUPS * Q_BYTES + (K_STAGES + V_STAGES) * KV_BYTES + 512;
 constexpr int RANGES = 4;                    // tiles whose exponents are kept
 constexpr float P_UP = 7.f;                  // probabilities are written times 2^7: up to 2^15, so that those of long rows stay above 2^-24
+// scores up to this many powers of two: beyond, score * scale - maximum in one rounding is off by the half step that the maximum was rounded by,
+// which as a power of two passes half precision, and in the end 32 bits
+constexpr float FAR = 65536.f;
 constexpr int HIGHEST = 12;                  // the largest of what is scaled goes to 2^12 .. 2^13 (half precision ends at 65,504)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -119,8 +122,8 @@ __device__ __forceinline__ bool finite_pair(uint32_t pair) {
   return (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
 }
 
-// A row (query, head) by one warp in 32 bits, for the blocks whose keys or values are too far apart for half precision (see `wide`): what a row does
-// not see, or gives no weight, must not cost the others their bits.  Lanes are 32 keys for the scores, and D / 32 columns each for their sum.
+// A row (query, head) by one warp in 32 bits, for the blocks whose keys or values are too far apart for half precision (see `wide`; what a row does
+// not see, or gives no weight, must not cost the others their bits) and for scores beyond FAR.  Lanes are 32 keys for the scores, and D / 32 columns each for their sum.
 __device__ __noinline__ void whole_row(const Params& p, const char* q_tile, int r, float q_down, const int* bt, int kvh, int from, int pos, float sink, bf16* out, int lane) {
   constexpr int W = D / 8, SHARE = 32 / W, CPL = D / 32;          // words of a row, lanes of a word, columns of a lane
   const uint32_t* kc = reinterpret_cast<const uint32_t*>(p.kc);
@@ -468,6 +471,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const uint32_t lane_addr = static_cast<uint32_t>(q4 * 32) << 16;
       const uint32_t tmem_s = tmem_base + g * BN, tmem_o = tmem_base + 2 * BN + g * 128;
       float m = -INFINITY, l = 0.f;
+      bool far = false;
       bool ok = mbar_wait(smem_u32(q_full), 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       // this thread's row of queries in half precision, its largest element at 2^12 .. 2^13 (rows behind the last are whatever lay there)
@@ -556,6 +560,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const float m_cand = fmaxf(m, mx * sc);
         const float m_new = (m_cand - m <= 8.f) ? m : m_cand;      // -inf - -inf: moves (to -inf), harmless
         const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+        far |= fabsf(m_safe) > FAR;
         const float alpha = ex2(m - m_safe), from = m_safe - P_UP;
         // probabilities -> tensor memory, pairs of half precision over the first 64 columns of S_g, handed over in P_PARTS parts
         F2 sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
@@ -602,7 +607,7 @@ int4_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         ok = mbar_wait(smem_u32(&o_ready[g]), (n_tiles - 1) & 1, abort_flag) && mbar_wait(smem_u32(&v_full[(n_tiles - 1) % V_STAGES]), (n_tiles - 1) / V_STAGES & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
       }
-      if (ok && *wide) {
+      if (ok && (__any_sync(0xffffffffu, far) || *wide)) {
         // row by row
         for (int i = 0; i < 32; ++i) {
           const int at = __shfl_sync(0xffffffffu, pos, i), from = __shfl_sync(0xffffffffu, lo, i);
