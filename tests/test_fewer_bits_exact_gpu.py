@@ -183,3 +183,32 @@ def test_maxima_a_few_steps_of_32_bits_apart(D, power, step):
     for backend in ("tcgen05", "mma", "simt"):
         out = ops.paged_attention(q, kc, vc, view, ctx, math.log(2.0), backend=backend)
         assert (out.float() - 3.0).abs().max() <= 3.0 * 2.0 ** -8, backend
+
+
+@pytest.mark.parametrize("backend", sorted(LARGER))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1e3, 1e4, 1e5, 1e6, 1e8, 1e10, 1e20])
+@pytest.mark.parametrize("spread", [3, 20])
+def test_scores_of_any_size(backend, D, size, spread):
+    """Scores so large that one key has all of the weight, whose values may be far smaller or larger than the others': a row is that key's values.
+    (Rows whose two best scores are within 2^-10 of the largest are left out: 32 bits may take either.)"""
+    from tinyserve_b200.kernels import ops
+    lengths = [(1, 900), (3, 300), (70, 200)]
+    ctx, view, kc, vc, _, _ = batch(lengths, 2, D, 16, torch.bfloat16)
+    by = torch.randint(-spread, spread + 1, vc.pairs.shape[:3], generator=torch.Generator().manual_seed(D)).cuda()
+    vc.pairs.copy_(torch.ldexp(vc.pairs.float(), by[..., None]).bfloat16())
+    q = queries(ctx.num_tokens, 8, D)
+    scale, ks, vs = D ** -0.5 * size, dense(ctx, view, kc), dense(ctx, view, vc)
+    out, at, checked = ops.paged_attention(q, kc, vc, view, ctx, scale, backend=backend).double(), 0, 0
+    for (n, m), k, v in zip(lengths, ks, vs):
+        scores = torch.einsum("thd,jhd->thj", q[at:at + n].double(), k.repeat_interleave(4, 1)) * scale
+        scores = scores.masked_fill(torch.arange(m, device="cuda") > torch.arange(m - n, m, device="cuda")[:, None, None], -math.inf)
+        best = scores.topk(2, -1)
+        clear = (best.values[..., 0] - best.values[..., 1] > 2.0 ** -10 * scores.nan_to_num(neginf=0.0).abs().amax(-1)) & (best.values[..., 0] - best.values[..., 1] > 60)
+        want = v.repeat_interleave(4, 1)[best.indices[..., 0], torch.arange(8, device="cuda")]
+        # (the least of 2^41 between two values' scales has a weight of e^-60 against it)
+        off = (out[at:at + n] - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * want.abs().amax(-1, keepdim=True)
+        assert (off | ~clear[..., None]).all(), (n, m)
+        checked += int(clear.sum())
+        at += n
+    assert checked > 300

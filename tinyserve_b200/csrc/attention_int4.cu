@@ -828,7 +828,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
 
   float o[D / 16][NT][4], m[NT][2], ps[NT][4];                     // ps: sum p' of columns 2t and 2t + 1 (and the same again)
   F2 l[NT], z[NT];
-  // a column's largest log2(p s) + m so far, which moves as m does, and the factor that brings p s there to 2^UNIT
+  // a column's largest log2(p s) so far, which moves as m does, and the factor that brings p s there to 2^UNIT.  (Against m and not by
+  // itself: beside scores of 10^8 a sum would have no bits left for the scale.)
   float top_v[NT][2], unit[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -959,7 +960,8 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         top[nt][i] = fmaxf(fmaxf(sc[0][nt][i], sc[0][nt][2 + i]), fmaxf(sc[1][nt][i], sc[1][nt][2 + i]));
-        moved |= top[nt][i] > m[nt][i] + SLACK || top[nt][i] + widest > top_v[nt][i] + SLACK;
+        const float above = top[nt][i] - m[nt][i];
+        moved |= above > SLACK || above + widest > top_v[nt][i] + SLACK;
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -967,23 +969,23 @@ __global__ void __launch_bounds__(WARPS * 32, MmaCfg<NT, WARPS>::BLOCKS) int4_mm
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
+          const float above = fmaxf(top[nt][i], m[nt][i]), shift = m[nt][i] - above;
           float wide = LOWEST;
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) wide = fmaxf(wide, sc[kb][nt][2 * h + i] + lg2(fabsf(vscale[kb][h])));
+            for (int h = 0; h < 2; ++h) wide = fmaxf(wide, sc[kb][nt][2 * h + i] - above + lg2(fabsf(vscale[kb][h])));
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
-            wide = fmaxf(wide, __shfl_xor_sync(0xffffffffu, wide, d));
-          }
-          const float above = fmaxf(top[nt][i], m[nt][i]), above_v = fmaxf(wide, top_v[nt][i]);
+          for (int d = 4; d < 32; d <<= 1) wide = fmaxf(wide, __shfl_xor_sync(0xffffffffu, wide, d));
+          wide = fmaxf(wide, top_v[nt][i] + shift);
           // (where there was no scale but 0, o is 0)
-          const float was = fminf(m[nt][i] - top_v[nt][i] + UNIT, MAX_UNIT), is = fminf(above - above_v + UNIT, MAX_UNIT);
-          const float f_v = ex2(m[nt][i] - above + (is - was));
-          f[i] = ex2(m[nt][i] - above);
+          const float was = fminf(UNIT - top_v[nt][i], MAX_UNIT), is = fminf(UNIT - wide, MAX_UNIT);
+          const float f_v = ex2(shift + (is - was));
+          f[i] = ex2(shift);
           m[nt][i] = above;
-          top_v[nt][i] = above_v;
+          top_v[nt][i] = wide;
           unit[nt][i] = ex2(is);
           ps[nt][i] *= f_v;
           ps[nt][2 + i] *= f_v;
