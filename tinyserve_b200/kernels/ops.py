@@ -2752,7 +2752,7 @@ class Int4Pages:
     heads, slots, 2], both contiguous.  A head of a token with pair (scale, zero) stands for zero + code * scale; eight codes fill a
     32-bit word, even columns in its lower half, odd ones in its upper half, the first in the lowest bits.  ``int4_kvwrite`` fills it.
     Attention sums values in 32 bits before it divides: magnitudes up to 2^100 are safe.  (Prompt portions in bfloat16 with heads of 64 or 128
-    become some hundred times slower where the values of a request, or 128 keys in a row, lie more than 2^24 apart.)"""
+    become some hundred times slower where the values of a request, or 128 keys in a row, lie more than 2^24 apart, or scores pass 2^16.)"""
     __slots__ = ("codes", "pairs", "shape")
 
     def __init__(self, codes, pairs):
