@@ -38,3 +38,25 @@ def test_a_model_without_any_is_refused(tmp_path):
     for make in (lambda: fill_random_on_device(model, torch.float32, "cpu", 0, "int8"), lambda: load_weights(model, str(tmp_path), torch.float32, "cpu", "int8")):
         with pytest.raises(ValueError, match="no matrix of the model can be held in 8 bits"):
             make()
+
+
+def test_weights_are_complete_before_the_first_product(tmp_path, monkeypatch):
+    """Both ways of filling a model end with a synchronisation of its device: products over constant weights do not wait for who made them."""
+    from helpers import make_model_dir, tiny_config
+    from tinyserve_b200.parts.model import build_model
+    from tinyserve_b200.weights import fill_random_on_device, load_weights, loader, random_init
+    seen = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: seen.append(("device", str(device))))
+    loader.settle("cuda:0")
+    loader.settle(torch.device("cpu"))
+    assert seen == [("device", "cuda:0")]
+    bound = []
+    for module in (loader, random_init):
+        monkeypatch.setattr(module, "settle", lambda device: seen.append(("settled", len(bound))))
+    model = build_model(tiny_config("A"))
+    for part in model.named_parts():
+        monkeypatch.setattr(part, "bind", lambda tensors, part=part: bound.append(part))
+    n = sum(1 for _ in model.named_parts())
+    fill_random_on_device(model, torch.float32, "cpu")
+    load_weights(model, make_model_dir(tmp_path, "A"), torch.float32, "cpu")
+    assert seen[1:] == [("settled", n), ("settled", 2 * n)]

@@ -148,6 +148,13 @@ def held(spec: ParamSpec, tensor, weight_dtype: str):
     return tensor, tensor.numel() * tensor.element_size()
 
 
+def settle(device) -> None:
+    """What was placed on ``device`` is complete when this returns: products fetch weights ahead of their wait for the kernels before
+    them, and some weights are results of kernels (codes of 8 bits, interleaved rows)."""
+    if torch.device(device).type == "cuda":
+        torch.cuda.synchronize(device)
+
+
 def load_weights(model, model_dir: str, dtype: torch.dtype, device, weight_dtype: str = "auto") -> int:
     """Fill every part of ``model`` from ``model_dir``; returns the bytes placed.  ``weight_dtype``: see ``held``."""
     check_weight_dtype(model, weight_dtype)
@@ -182,4 +189,5 @@ def load_weights(model, model_dir: str, dtype: torch.dtype, device, weight_dtype
     for part in model.named_parts():
         if id(part) not in tensors:
             part.bind({})
+    settle(device)
     return total

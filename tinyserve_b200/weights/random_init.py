@@ -13,7 +13,7 @@ import os
 import torch
 from safetensors.torch import save_file
 
-from .loader import check_weight_dtype, expected_tensors, held
+from .loader import check_weight_dtype, expected_tensors, held, settle
 
 _STORE = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
@@ -82,4 +82,5 @@ def fill_random_on_device(model, dtype: torch.dtype, device, seed: int = 0, weig
             bound[local], size = held(spec, value, weight_dtype)
             total += size
         part.bind(bound)
+    settle(device)
     return total
